@@ -405,6 +405,117 @@ int iq_prefill_attention_tokens(const void *q, const void *k, const void *v, int
                                 void *stream);
 
 /*
+ * iq_prefill_attention_tokens that also writes lse f32 [Hq, lse_sh] (NULL:
+ * not written): lse[hq][t] = log of the sum over the keys that token t sees of
+ * exp(scale q.k), which iq_prefill_weights reads.  Needs scale > 0.
+ */
+int iq_prefill_attention_lse(const void *q, const void *k, const void *v, int dtype, int64_t q_st, int64_t q_sh,
+                             int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, const int32_t *cu_seqlens,
+                             int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t Hq, int64_t H,
+                             int64_t head_dim, float scale, void *out, int64_t o_st, int64_t o_sh, int out_dtype,
+                             float *lse, int64_t lse_sh, void *stream);
+
+/*
+ * The softmax weight each key receives, summed over queries and over the
+ * query heads of its KV head: out f32 [H, out_sh], out[h][t] = sum over the
+ * queries i >= t of t's sequence and the heads g of h of
+ * exp(scale q_gi.k_t - lse_gi).  window > 0: over the last `window` queries of
+ * each sequence; window == 0: over all, with the lse of
+ * iq_prefill_attention_lse (with a window the lse may be NULL: it is computed
+ * from the workspace).  q [tokens, Hq, 128], k [tokens, H, 128], sequences and
+ * strides as iq_prefill_attention (head size 128; q token stride below 2^25).
+ * Tokens of no sequence are not written.  workspace: f32,
+ * iq_prefill_weights_floats elements, 16-byte aligned.
+ */
+int64_t iq_prefill_weights_floats(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t window,
+                                  int have_lse);
+
+int iq_prefill_weights(const void *q, const void *k, int dtype, int64_t q_st, int64_t q_sh, int64_t k_st,
+                       int64_t k_sh, const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, int64_t tokens,
+                       int64_t Hq, int64_t H, int64_t window, float scale, const float *lse, int64_t lse_sh,
+                       float *workspace, int64_t workspace_floats, float *out, int64_t out_sh, void *stream);
+
+/*
+ * ---------------------------------------------------------------- exact pages
+ * A pool of exact (unpacked) rows: key and value [pages, heads, block_tokens,
+ * 128] of bf16 or f16 (element strides of page, head and row, multiples of 8;
+ * 16-byte aligned; row strides below 2^24), block_tokens in {16, 32, 64, 128,
+ * 256}, and optionally (both or neither) weights f32 and positions i32
+ * [pages, heads, block_tokens], contiguous: the attention weight each row has
+ * accumulated and its position in the sequence.  Cache row r of sequence s is
+ * row r % block_tokens of pool page tables[s * bt_stride + r / block_tokens]
+ * (i32; bt_cols entries).  Rows of an id outside the pool are neither read nor
+ * written.  No counterpart in the reference.
+ */
+typedef struct iq_dense_pages {
+    uint64_t key, value, weights, positions;
+    int64_t k_sp, k_sh, k_st, v_sp, v_sh, v_st;
+    int64_t pages, heads, block_tokens;
+} iq_dense_pages;
+
+/*
+ * Writes rows of token-major k / v [tokens, heads, 128] (element strides;
+ * 16-byte aligned rows; sequences [cu_seqlens[i], cu_seqlens[i + 1]), none
+ * longer than max_seqlen) into the pages: row t of sequence i to cache row
+ * start[i] + t (start NULL: 0) of every head.  With keep i32 [n_seq, heads,
+ * kept] head h takes only the rows keep[i][h][j], to cache row start[i] + j
+ * (entries outside the sequence are skipped).  Beside row t go its weight
+ * weights[h * w_stride + cu_seqlens[i] + t] (NULL: 0) and its position
+ * positions[i] + t (positions NULL: start[i] + t).
+ */
+int iq_dense_write(const void *k, const void *v, int dtype, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                   const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, const int32_t *start,
+                   const int32_t *positions, const float *weights, int64_t w_stride, const int32_t *keep,
+                   int64_t kept, const iq_dense_pages *pages, const int32_t *tables, int64_t bt_stride,
+                   int64_t bt_cols, void *stream);
+
+/*
+ * The rows a budget keeps of each sequence and head: the first `sink` and the
+ * last `recent` rows, then by weight (weights f32, row t of sequence i and
+ * head h at h * w_stride + cu_seqlens[i] + t), ties to the lowest row, NaN
+ * last.  keep i32 [n_seq, H, budget]: ascending rows within the sequence, -1
+ * behind the last.
+ */
+int iq_select_rows(const float *weights, int64_t w_stride, int64_t H, const int32_t *cu_seqlens, int64_t n_seq,
+                   int64_t max_seqlen, int64_t budget, int64_t sink, int64_t recent, int32_t *keep, void *stream);
+
+/*
+ * Cuts every head of every sequence of more than `budget` rows back to
+ * `budget`, in place: kept are the rows at positions below `sink` or from
+ * seen[i] - recent on, then by weight, ties to the lowest cache row, NaN last.
+ * The evicted cache rows below `budget` take, in order, the kept rows from
+ * `budget` on (key, value, weight and position); all other rows stay as they
+ * are.  lengths i32: rows each sequence holds (at most max_tokens are
+ * considered); new_lengths i32: min(lengths, budget).  workspace: i32,
+ * iq_dense_evict_ints elements.  No page may belong to two sequences.
+ */
+int64_t iq_dense_evict_ints(int64_t H, int64_t n_seq, int64_t max_tokens, int64_t budget);
+
+int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
+                   const int32_t *lengths, const int32_t *seen, int64_t n_seq, int64_t max_tokens, int64_t budget,
+                   int64_t sink, int64_t recent, int32_t *new_lengths, int32_t *workspace, int64_t workspace_ints,
+                   void *stream);
+
+/*
+ * One token's attention per sequence over its first lengths[i] cache rows (at
+ * most max_tokens): q [n_seq, Hq, 128] of the pages' dtype (element strides,
+ * 16-byte aligned rows), Hq a multiple of heads with at most 16 query heads
+ * per KV head; out [n_seq, Hq, 128] of out_dtype (unit channel stride).  fp32
+ * logits, softmax and accumulation; softmax weights rounded to the pages'
+ * dtype before P.V.  A sequence without a row to read gives zeros.  With
+ * accumulate != 0 each row's weights, summed over the query heads of its KV
+ * head, are added to pages->weights (in an order that is only not fixed for a
+ * page that two sequences share).  workspace: f32, iq_dense_workspace_floats
+ * elements, 16-byte aligned, used by one call at a time.
+ */
+int64_t iq_dense_workspace_floats(int64_t Hq, int64_t H, int64_t n_seq, int64_t max_tokens, int accumulate);
+
+int iq_dense_decode(const void *q, int dtype, int64_t q_ss, int64_t q_sh, int64_t Hq, int64_t n_seq,
+                    const iq_dense_pages *pages, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
+                    const int32_t *lengths, int64_t max_tokens, float scale, int accumulate, float *workspace,
+                    int64_t workspace_floats, void *out, int64_t o_ss, int64_t o_sh, int out_dtype, void *stream);
+
+/*
  * Dense tail append of a cache layer.  buf holds [2 (keys, values), H,
  * capacity, D] elements of elem_bytes (element strides buf_kv, buf_h,
  * buf_t); k / v hold n_new (<= 64) rows per head (element strides: head,

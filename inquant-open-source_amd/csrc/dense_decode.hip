@@ -1,0 +1,353 @@
+// One token's attention over exact pages (gfx950), split over the rows and
+// joined, with the rows' accumulated weights on request.
+//
+// For sequence s, KV head h and the G query heads g that share it,
+//   o_g = sum_r p_gr v_r,  p_gr = exp(c q_g.k_r - lse_g),
+//   weights[r] += sum_g p_gr.
+// Each workgroup takes one (KV head, partition of the rows, sequence) with a
+// running maximum and sum per query head, and leaves the unnormalized output
+// with (max, sum); a second launch joins the partitions.  The weights need the
+// joined lse, so the first launch also leaves the logits (4 bytes per row and
+// query head against 512 read per row and KV head).
+#include "dense_common.h"
+
+namespace {
+
+constexpr int D = 128;
+constexpr int NW = 4, NT = 64 * NW;
+constexpr int WT = 64;                       // rows per wavefront and step
+constexpr int PT = WT * NW;                  // rows per workgroup and step
+constexpr float LOG2E = 1.44269504088896341f;
+
+struct DecodeArgs {
+    DensePool pool;
+    const uint16_t *q;
+    int64_t q_ss, q_sh;
+    const int32_t *lengths;
+    int32_t max_tokens, span, parts, G, Hq;  // span: rows per partition, a multiple of PT
+    float c_log2;
+    Partials part;                           // [n * Hq, parts] rows
+    float *logits;                           // [n * Hq, l_stride] in log2 units, or null
+    int64_t l_stride;
+    void *out;
+    int64_t o_ss, o_sh;
+    int odt;
+};
+
+// V rows of a step in LDS: 256 bytes each, the 16-byte chunk c of row r at
+// slot c ^ 4 (r % 4) ^ 2 (r / 4 % 2), so that the transposed reads of 32 lanes
+// (two groups of four rows, 32 bytes each) hit 64 distinct banks.
+struct __attribute__((aligned(16))) DecodeSmem {
+    union {
+        uint16_t v[NW][WT * D];
+        float o[NW][16][D + 4];
+    };
+    float m[NW][16], l[NW][16];
+};
+
+// ds_read_b64_tr_b16: when lane s of 16 reads row K0 + s / 4, channels
+// c0 + 4 (s % 4) .. + 3, lane i receives channel c0 + i of rows K0 .. K0 + 3.
+typedef short gv16x4 __attribute__((__vector_size__(4 * sizeof(short))));
+__device__ __forceinline__ u32x2 tr_read(const uint16_t *p)
+{
+    const gv16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) gv16x4 *)(__attribute__((address_space(3))) uint16_t *)p);
+    return __builtin_bit_cast(u32x2, v);
+}
+
+template <bool F16>
+__global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
+{
+    __shared__ DecodeSmem sm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4;
+    const int h = blockIdx.x, part = blockIdx.y, seq = blockIdx.z;
+    const int have = a.lengths[seq], len = have < a.max_tokens ? have : a.max_tokens;
+    const int t0 = part * a.span;
+    if (t0 >= len) return;                   // uniform; the join does not read this partition
+    const int end = t0 + a.span < len ? t0 + a.span : len;
+    const DensePool &p = a.pool;
+    u32x4 qb[4];                             // B operand: column c16 = query head, channels 32 d + 8 g4 .. + 7
+    {
+        const int g = c16 < a.G ? c16 : 0;
+        const uint16_t *qp = a.q + seq * a.q_ss + (int64_t)(h * a.G + g) * a.q_sh + 8 * g4;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) qb[d] = ld16(qp + 32 * d);
+    }
+    float m_run = NEG_INF, l_run = 0.0f;     // of column c16; l_run: this lane's rows
+    f32x4 acc[8];                            // O^T rows 16 cb + 4 g4 + i (channels), column c16
+#pragma unroll
+    for (int cb = 0; cb < 8; ++cb) acc[cb] = f32x4{0, 0, 0, 0};
+    const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&sm.v[wave][0];
+    const int32_t *table = p.tables + seq * p.bt_stride;
+    for (int c0 = t0 + WT * wave; c0 < end; c0 += PT) {
+        const uint16_t *kt[4], *vt[4];       // first row of each 16-row tile
+        int last[4];                         // its last live row; -1: none, its page is not in the pool
+        u32x4 kf[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            // a tile past the end reads the tile of the last row again (masked)
+            const int want = c0 + 16 * t, tb = want < len ? want : (len - 1) & ~15;
+            const int id = table[tb >> p.shift];
+            const bool ok = id >= 0 && id < p.pages;
+            const int64_t page = ok ? id : 0;
+            const int row = tb & (p.B - 1);
+            kt[t] = p.key + page * p.k_sp + h * p.k_sh + row * p.k_st;
+            vt[t] = p.value + page * p.v_sp + h * p.v_sh + row * p.v_st;
+            const int rest = len - 1 - tb;
+            last[t] = rest < 15 ? rest : 15;
+            const int r = c16 < last[t] ? c16 : last[t];
+            const uint32_t off = (uint32_t)(r * (int)p.k_st + 8 * g4) * 2;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) kf[t][d] = ldnt_at<u32x4>(kt[t], off + 64 * d);
+            if (!ok || want >= len) last[t] = -1;
+        }
+        // the reads of the previous step's rows are done before theirs are overwritten
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = i >> 2, rl = 4 * (i & 3) + g4;
+            const int lim = len - 1 - (c0 + 16 * t < len ? c0 + 16 * t : (len - 1) & ~15);
+            const int r = rl < lim ? rl : lim;
+            const int chunk = c16 ^ (4 * (rl & 3)) ^ (2 * ((rl >> 2) & 1));
+            lds_load16(vt[t], (uint32_t)(r * (int)p.v_st + 8 * chunk) * 2, lds_v + (uint32_t)(4 * i * D * 2));
+        }
+        f32x4 sc[4];                         // S^T rows 16 t + 4 g4 + i (cache rows), column c16
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sc[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) sc[t] = mma32<F16>(kf[t][d], qb[d], sc[t]);
+        float cmax = NEG_INF;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[t][i] = 4 * g4 + i <= last[t] ? sc[t][i] * a.c_log2 : NEG_INF;
+                cmax = fmaxf(cmax, sc[t][i]);
+            }
+        if (a.logits && c16 < a.G) {
+            float *lp = a.logits + (int64_t)(seq * a.Hq + h * a.G + c16) * a.l_stride + c0 + 4 * g4;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (c0 + 16 * t < len) *(f32x4 *)(lp + 16 * t) = sc[t];
+        }
+        cmax = xmax16(cmax);
+        const float m_new = fmaxf(m_run, cmax), m_use = m_new == NEG_INF ? 0.0f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+        float lsum = 0.0f;
+        u32x4 pb[2];                         // B operand: rows 16 (2 m) + 4 g4 + i, then 16 (2 m + 1) + 4 g4 + i
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = __builtin_amdgcn_exp2f(sc[t][i] - m_use);
+                lsum += w[i];
+            }
+            pb[t >> 1][2 * (t & 1)] = pack2<F16>(w[0], w[1]);
+            pb[t >> 1][2 * (t & 1) + 1] = pack2<F16>(w[2], w[3]);
+        }
+        l_run = fmaf(l_run, alpha, lsum);
+        m_run = m_new;
+#pragma unroll
+        for (int cb = 0; cb < 8; ++cb) acc[cb] *= alpha;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wavefront's V rows have landed
+        const uint16_t *sv = sm.v[wave];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int cb = 0; cb < 8; ++cb) {
+                const int r = 32 * m + 4 * g4 + (c16 >> 2);
+                const int slot = (2 * cb + ((c16 & 3) >> 1)) ^ (4 * (c16 >> 2)) ^ (2 * (g4 & 1));
+                const u32x2 lo = tr_read(sv + r * D + 8 * slot + 4 * (c16 & 1));
+                const u32x2 hi = tr_read(sv + (r + 16) * D + 8 * slot + 4 * (c16 & 1));
+                acc[cb] = mma32<F16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pb[m], acc[cb]);
+            }
+    }
+    l_run = xsum16(l_run);
+    // the wavefront's own V rows have been read: its outputs take their place
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int cb = 0; cb < 8; ++cb) *(f32x4 *)&sm.o[wave][c16][16 * cb + 4 * g4] = acc[cb];
+    if (g4 == 0) {
+        sm.m[wave][c16] = m_run;
+        sm.l[wave][c16] = l_run;
+    }
+    __syncthreads();
+    for (int i = tid; i < 32 * a.G; i += NT) {
+        const int g = i >> 5, c = 4 * (i & 31);
+        float M = NEG_INF;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm.m[w][g]);
+        const float use = M == NEG_INF ? 0.0f : M;
+        float L = 0.0f;
+        f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = __builtin_amdgcn_exp2f(sm.m[w][g] - use);
+            L = fmaf(f, sm.l[w][g], L);
+            const f32x4 x = *(const f32x4 *)&sm.o[w][g][c];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+        }
+        const int64_t row = ((int64_t)seq * a.Hq + h * a.G + g) * a.parts + part;
+        *(f32x4 *)(a.part.o + row * D + c) = o;
+        if (c == 0) a.part.ml[row] = f32x2{M, L};
+    }
+}
+
+// Joins the partitions.  The first n * Hq workgroups write an output row each;
+// the others add the weights of JW rows of a (sequence, KV head).
+constexpr int JW = 1024;
+
+struct JoinSmem {
+    float o[8][D];
+    float m[8], l[8];
+    float lse[16];
+};
+
+__global__ __launch_bounds__(NT) void dense_join(DecodeArgs a, int n)
+{
+    __shared__ JoinSmem sm;
+    const int tid = threadIdx.x, rows = n * a.Hq;
+    if ((int)blockIdx.x < rows) {
+        const int seq = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
+        const int have = a.lengths[seq], len = have < a.max_tokens ? have : a.max_tokens;
+        const int live = len > 0 ? (len + a.span - 1) / a.span : 0;
+        const int64_t base = (int64_t)blockIdx.x * a.parts;
+        const int grp = tid >> 5, c = 4 * (tid & 31);
+        float M = NEG_INF, L = 0.0f;
+        f32x4 o = {0, 0, 0, 0};
+        for (int p = grp; p < live; p += 8) {
+            const f32x2 ml = a.part.ml[base + p];
+            const f32x4 x = *(const f32x4 *)(a.part.o + (base + p) * D + c);
+            const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
+            const float f0 = __builtin_amdgcn_exp2f(M - use), f1 = __builtin_amdgcn_exp2f(ml[0] - use);
+            L = L * f0 + ml[1] * f1;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + x[e] * f1;
+            M = m;
+        }
+        *(f32x4 *)&sm.o[grp][c] = o;
+        if (c == 0) {
+            sm.m[grp] = M;
+            sm.l[grp] = L;
+        }
+        __syncthreads();
+        if (tid >= D) return;
+        float mx = NEG_INF;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sm.m[i]);
+        const float use = mx == NEG_INF ? 0.0f : mx;
+        float sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = __builtin_amdgcn_exp2f(sm.m[i] - use);
+            sum = fmaf(f, sm.l[i], sum);
+            v = fmaf(f, sm.o[i][tid], v);
+        }
+        // a sequence without a live row attends to nothing: zeros
+        iq_store_as(a.out, seq * a.o_ss + hq * a.o_sh + tid, sum == 0.0f ? 0.0f : v / sum, a.odt);
+        return;
+    }
+    const int chunks = (a.max_tokens + JW - 1) / JW;
+    const int item = (int)blockIdx.x - rows, H = a.pool.H;
+    const int chunk = item % chunks, h = item / chunks % H, seq = item / chunks / H;
+    const int have = a.lengths[seq], len = have < a.max_tokens ? have : a.max_tokens;
+    if (chunk * JW >= len) return;
+    const int live = (len + a.span - 1) / a.span;
+    const int64_t q0 = (int64_t)seq * a.Hq + h * a.G;
+    for (int g = tid >> 6; g < a.G; g += NW) {
+        float M = NEG_INF, L = 0.0f;
+        for (int p = tid & 63; p < live; p += 64) M = fmaxf(M, a.part.ml[(q0 + g) * a.parts + p][0]);
+#pragma unroll
+        for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+        const float use = M == NEG_INF ? 0.0f : M;
+        for (int p = tid & 63; p < live; p += 64) {
+            const f32x2 ml = a.part.ml[(q0 + g) * a.parts + p];
+            L = fmaf(__builtin_amdgcn_exp2f(ml[0] - use), ml[1], L);
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
+        if ((tid & 63) == 0) sm.lse[g] = L == 0.0f ? __builtin_inff() : use + __builtin_amdgcn_logf(L);
+    }
+    __syncthreads();
+    const int r0 = chunk * JW + 4 * tid;
+    if (r0 >= len) return;
+    f32x4 w = {0, 0, 0, 0};
+    for (int g = 0; g < a.G; ++g) {
+        const f32x4 s = *(const f32x4 *)(a.logits + (q0 + g) * a.l_stride + r0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(s[e] - sm.lse[g]);
+    }
+    const int64_t page = dense_page(a.pool, seq, r0);
+    if (page < 0) return;
+    // added in memory, so that sequences that share a page lose no weight
+    float *at = a.pool.weights + (page * H + h) * a.pool.B + (r0 & (a.pool.B - 1));
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r0 + e < len) unsafeAtomicAdd(at + e, w[e]);
+}
+
+struct Split {
+    int64_t span, parts, logits, floats;     // floats: the whole workspace
+};
+
+Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t max_tokens, bool accumulate)
+{
+    const int64_t steps = (max_tokens + PT - 1) / PT;
+    const int64_t per = (n * H * steps + 2047) / 2048;
+    Split s;
+    s.span = PT * (per > 0 ? per : 1);
+    s.parts = (max_tokens + s.span - 1) / s.span;
+    s.logits = accumulate ? (max_tokens + 63) / 64 * 64 : 0;
+    s.floats = n * Hq * (s.parts * (D + 2) + s.logits);
+    return s;
+}
+
+}  // namespace
+
+extern "C" int64_t iq_dense_workspace_floats(int64_t Hq, int64_t H, int64_t n_seq, int64_t max_tokens, int accumulate)
+{
+    return split_of(Hq, H, n_seq, max_tokens, accumulate != 0).floats;
+}
+
+extern "C" int iq_dense_decode(const void *q, int dtype, int64_t q_ss, int64_t q_sh, int64_t Hq, int64_t n_seq,
+                               const iq_dense_pages *pages, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
+                               const int32_t *lengths, int64_t max_tokens, float scale, int accumulate,
+                               float *workspace, int64_t workspace_floats, void *out, int64_t o_ss, int64_t o_sh,
+                               int out_dtype, void *stream)
+{
+    DensePool pool;
+    if (const int e = dense_pool("iq_dense_decode", pages, dtype, tables, bt_stride, bt_cols, n_seq, pool)) return e;
+    IQ_CHECK_ARG(q && lengths && out, "iq_dense_decode: null pointer");
+    IQ_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_ss | q_sh) % 8 == 0, "iq_dense_decode: query rows must be 16-byte aligned");
+    IQ_CHECK_ARG(Hq >= 1 && Hq % pool.H == 0 && Hq / pool.H <= 16, "iq_dense_decode: heads %lld / %d", (long long)Hq,
+                 pool.H);
+    IQ_CHECK_ARG(out_dtype >= IQ_F32 && out_dtype <= IQ_F16, "iq_dense_decode: bad output dtype");
+    IQ_CHECK_ARG(max_tokens >= 0 && max_tokens <= bt_cols * pool.B && max_tokens <= 0x3fffffff,
+                 "iq_dense_decode: max_tokens past the block tables");
+    IQ_CHECK_ARG(!accumulate || pool.weights, "iq_dense_decode: pages without weights");
+    if (n_seq == 0) return IQ_OK;
+    const Split s = split_of(Hq, pool.H, n_seq, max_tokens, accumulate != 0);
+    IQ_CHECK_ARG(s.floats == 0 || (workspace && workspace_floats >= s.floats), "iq_dense_decode: workspace too small");
+    const int64_t chunks = accumulate ? (max_tokens + JW - 1) / JW : 0;
+    const int64_t joins = n_seq * Hq + n_seq * pool.H * chunks;
+    IQ_CHECK_ARG(s.parts <= 65535 && joins <= 0xffffff, "iq_dense_decode: too many rows");
+    float *part = workspace + n_seq * Hq * s.logits;
+    const DecodeArgs a{pool, (const uint16_t *)q, q_ss, q_sh, lengths, (int32_t)max_tokens, (int32_t)s.span,
+                       (int32_t)s.parts, (int32_t)(Hq / pool.H), (int32_t)Hq, scale * LOG2E,
+                       Partials{part, (f32x2 *)(part + n_seq * Hq * s.parts * D)},
+                       accumulate ? workspace : nullptr, s.logits, out, o_ss, o_sh, out_dtype};
+    if (s.parts > 0) {
+        const dim3 grid((unsigned)pool.H, (unsigned)s.parts, (unsigned)n_seq);
+        if (dtype == IQ_F16) hipLaunchKernelGGL(dense_partials<true>, grid, dim3(NT), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL(dense_partials<false>, grid, dim3(NT), 0, (hipStream_t)stream, a);
+    }
+    hipLaunchKernelGGL(dense_join, dim3((unsigned)joins), dim3(NT), 0, (hipStream_t)stream, a, (int)n_seq);
+    IQ_CHECK_LAUNCH("dense_decode");
+    return IQ_OK;
+}

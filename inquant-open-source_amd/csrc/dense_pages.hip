@@ -1,0 +1,372 @@
+// Exact pages (gfx950): rows into pages, the rows a budget keeps of a prompt,
+// and eviction in place.
+//
+// A pool holds key and value [pages, H, B, 128] of 16-bit rows and, beside
+// every row, its accumulated attention weight (f32) and its position in the
+// sequence (i32), [pages, H, B] each.  Cache row r of a sequence is row r % B
+// of the page that its block table names at r / B; the heads of a sequence
+// hold the same number of rows but, once rows were evicted, not the same
+// positions.
+#include "dense_common.h"
+
+namespace {
+
+// ---------------------------------------------------------------- rows into pages
+
+struct WriteArgs {
+    const uint16_t *k, *v;
+    int64_t k_st, k_sh, v_st, v_sh;          // element strides (token, head)
+    const int32_t *cu, *start, *positions;   // start / positions may be null
+    const float *weights;                    // [H, w_stride] or null
+    int64_t w_stride;
+    const int32_t *keep;                     // [n, H, kept] or null
+    int64_t kept;
+    DensePool pool;
+};
+
+// Bound by memory: 512 bytes of keys and values are read and written per row
+// and head.  Sixteen lanes move a row (16 bytes of its key and of its value
+// each); a workgroup takes WR_ITEMS (row, head) pairs, heads innermost, so that
+// it reads one contiguous range of token-major rows (with `keep` rows
+// innermost: it then writes one contiguous range of a head's pages).
+constexpr int WR_ITEMS = 64;
+
+__global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
+{
+    const int seq = blockIdx.y, lane = threadIdx.x & 15, H = a.pool.H;
+    const int64_t t0 = a.cu[seq], len = a.cu[seq + 1] - t0;
+    const int64_t rows = a.keep ? a.kept : len;
+    const int64_t start = a.start ? a.start[seq] : 0;
+    const int32_t pos0 = a.positions ? a.positions[seq] : (int32_t)start;
+    const int64_t first = (int64_t)blockIdx.x * WR_ITEMS + (threadIdx.x >> 4);
+#pragma unroll
+    for (int i = 0; i < WR_ITEMS / 16; ++i) {
+        const int64_t item = first + 16 * i;
+        if (item >= rows * H) break;
+        int64_t h, j, source;
+        if (a.keep) {
+            h = item / a.kept;
+            j = item - h * a.kept;
+            source = a.keep[((int64_t)seq * H + h) * a.kept + j];
+            if (source < 0 || source >= len) continue;
+        } else {
+            j = source = item / H;
+            h = item - j * H;
+        }
+        const int64_t row = start + j;
+        const int64_t page = dense_page(a.pool, seq, row);
+        if (page < 0) continue;
+        const int64_t at = row & (a.pool.B - 1), token = t0 + source;
+        const u32x4 kv = ld16(a.k + token * a.k_st + h * a.k_sh + 8 * lane);
+        const u32x4 vv = ld16(a.v + token * a.v_st + h * a.v_sh + 8 * lane);
+        *(u32x4 *)(a.pool.key + page * a.pool.k_sp + h * a.pool.k_sh + at * a.pool.k_st + 8 * lane) = kv;
+        *(u32x4 *)(a.pool.value + page * a.pool.v_sp + h * a.pool.v_sh + at * a.pool.v_st + 8 * lane) = vv;
+        if (lane == 0 && a.pool.weights) {
+            const int64_t o = (page * H + h) * a.pool.B + at;
+            a.pool.weights[o] = a.weights ? a.weights[h * a.w_stride + token] : 0.0f;
+            a.pool.positions[o] = pos0 + (int32_t)source;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- selection
+
+// The `budget` largest of a row of sort keys, ties to the lowest index, by one
+// workgroup: the key of rank `budget` from three radix passes (11, 11 and 10
+// bits, histograms in LDS), then ranks in index order from ballots.  The keys
+// of SEL_CHUNK indices stay in LDS; longer rows are read again in every pass.
+constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_PER = 32, SEL_CHUNK = SEL_NT * SEL_PER;
+
+// Greater is better: NaN, then -inf .. +inf (both zeros alike), then the rows
+// that are always kept.
+__device__ __forceinline__ uint32_t sort_key(float w, bool always)
+{
+    if (always) return 0xffffffffu;
+    if (w != w) return 0;
+    const uint32_t u = __float_as_uint(w + 0.0f);   // -0 + 0 = +0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct SelectSmem {
+    uint32_t key[SEL_CHUNK];
+    uint32_t hist[2048];
+    uint32_t counts[SEL_PER * SEL_WAVES];     // kept-for-sure | ties << 16 per (j, wave), then their exclusive sums
+    uint32_t wave_sum[SEL_WAVES];
+    uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
+};
+
+// Exclusive sum over the workgroup of one value per thread, and the total.
+__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t *wave_sum, uint32_t &total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = (uint32_t)__shfl_up((int)x, d);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) wave_sum[wave] = x;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < SEL_WAVES; ++w) {
+        const uint32_t s = wave_sum[w];
+        all += s;
+        before += w < wave ? s : 0;
+    }
+    total = all;
+    return before + x - v;
+}
+
+// load(index) -> sort key, for index < len; emit(index, kept, rank): rank is
+// the number of kept indices below.
+template <class Load, class Emit>
+__device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int64_t budget, Load load, Emit emit)
+{
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const bool one = len <= SEL_CHUNK;
+    // a thread reads only the keys it wrote: indices base + 1024 j + t
+    auto fill = [&](int64_t base, int n) {
+#pragma unroll 8
+        for (int i = t; i < n; i += SEL_NT) sm.key[i] = load(base + i);
+    };
+    auto chunk_of = [&](int64_t base) { return (int)(len - base < SEL_CHUNK ? len - base : SEL_CHUNK); };
+    if (one) fill(0, (int)len);
+    uint32_t prefix = 0, need = 0xffffffffu;     // len <= budget: every key is at least 0
+    if (len > budget) {
+        need = (uint32_t)budget;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t mask = pass == 2 ? 1023 : 2047;
+            const uint32_t above = pass == 0 ? 0 : pass == 1 ? 0xffe00000u : 0xfffffc00u;
+            sm.hist[t] = 0;
+            sm.hist[t + SEL_NT] = 0;
+            __syncthreads();
+            for (int64_t base = 0; base < len; base += SEL_CHUNK) {
+                const int n = chunk_of(base);
+                if (!one) fill(base, n);
+#pragma unroll 4
+                for (int i = t; i < n; i += SEL_NT) {
+                    const uint32_t key = sm.key[i];
+                    if ((key & above) == prefix) atomicAdd(&sm.hist[(key >> shift) & mask], 1u);
+                }
+            }
+            __syncthreads();
+            // thread t takes the bins 2047 - 2 t and 2046 - 2 t: sums from the largest down
+            const uint32_t hi = sm.hist[2047 - 2 * t], lo = sm.hist[2046 - 2 * t];
+            uint32_t total;
+            const uint32_t before = block_exclusive(hi + lo, sm.wave_sum, total);
+            if (before < need && need <= before + hi + lo) {
+                const bool first = need <= before + hi;
+                sm.prefix = prefix | ((uint32_t)(first ? 2047 - 2 * t : 2046 - 2 * t) << shift);
+                sm.need = need - before - (first ? 0 : hi);
+            }
+            __syncthreads();
+            prefix = sm.prefix;
+            need = sm.need;
+        }
+    }
+    uint32_t sure0 = 0, ties0 = 0;               // kept for sure, and ties, in the chunks before
+    for (int64_t base = 0; base < len; base += SEL_CHUNK) {
+        const int n = chunk_of(base), steps = (n + SEL_NT - 1) / SEL_NT;
+        if (!one) fill(base, n);
+        // counts per (step, wavefront): index order
+        for (int j = 0; j < steps; ++j) {
+            const int i = j * SEL_NT + t;
+            const uint32_t key = i < n ? sm.key[i] : 0;
+            const uint64_t sure = __builtin_amdgcn_ballot_w64(i < n && key > prefix);
+            const uint64_t ties = __builtin_amdgcn_ballot_w64(i < n && key == prefix);
+            if (lane == 0)
+                sm.counts[j * SEL_WAVES + wave] = (uint32_t)__popcll(sure) | (uint32_t)__popcll(ties) << 16;
+        }
+        __syncthreads();
+        uint32_t total;
+        const uint32_t mine = t < steps * SEL_WAVES ? sm.counts[t] : 0;
+        const uint32_t before = block_exclusive(mine, sm.wave_sum, total);
+        if (t < steps * SEL_WAVES) sm.counts[t] = before;
+        __syncthreads();
+        for (int j = 0; j < steps; ++j) {
+            const int i = j * SEL_NT + t;
+            const uint32_t key = i < n ? sm.key[i] : 0;
+            const bool is_sure = i < n && key > prefix, is_tie = i < n && key == prefix;
+            const uint64_t sure = __builtin_amdgcn_ballot_w64(is_sure), ties = __builtin_amdgcn_ballot_w64(is_tie);
+            const uint64_t below = (1ull << lane) - 1;
+            const uint32_t c = sm.counts[j * SEL_WAVES + wave];
+            const uint32_t ns = sure0 + (c & 0xffffu) + (uint32_t)__popcll(sure & below);
+            const uint32_t nt = ties0 + (c >> 16) + (uint32_t)__popcll(ties & below);
+            if (i < n) emit(base + i, is_sure || (is_tie && nt < need), (int64_t)ns + (nt < need ? nt : need));
+        }
+        sure0 += total & 0xffffu;
+        ties0 += total >> 16;
+        __syncthreads();
+    }
+}
+
+struct SelectArgs {
+    const float *weights;
+    int64_t w_stride;
+    const int32_t *cu;
+    int64_t budget, sink, recent;
+    int32_t *keep;
+};
+
+__global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
+{
+    __shared__ SelectSmem sm;
+    const int h = blockIdx.x, seq = blockIdx.y;
+    const int64_t t0 = a.cu[seq], len = a.cu[seq + 1] - t0;
+    const float *w = a.weights + h * a.w_stride + t0;
+    int32_t *keep = a.keep + ((int64_t)seq * gridDim.x + h) * a.budget;
+    const int64_t newest = len - a.recent;
+    select_largest(
+        sm, len, a.budget, [&](int64_t i) { return sort_key(w[i], i < a.sink || i >= newest); },
+        [&](int64_t i, bool kept, int64_t rank) {
+            if (kept) keep[rank] = (int32_t)i;
+        });
+    for (int64_t i = (len > 0 ? len : 0) + threadIdx.x; i < a.budget; i += SEL_NT) keep[i] = -1;
+}
+
+// ---------------------------------------------------------------- eviction
+
+struct EvictArgs {
+    DensePool pool;
+    const int32_t *lengths, *seen;
+    int64_t max_tokens, budget, sink, recent, most;   // most: moves of a head at most
+    int32_t *new_lengths;
+    int32_t *moves;                                   // [n * H, 1 + 2 most]: count, evicted places, rows from behind
+};
+
+// Chooses the rows of one (head, sequence) and lists the moves: the evicted
+// places below the budget in order, and the kept rows behind it from the last.
+__global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
+{
+    __shared__ SelectSmem sm;
+    const int h = blockIdx.x, seq = blockIdx.y, H = a.pool.H, B = a.pool.B;
+    const int64_t have = a.lengths[seq];
+    const int64_t len = have < a.max_tokens ? have : a.max_tokens;
+    int32_t *list = a.moves + ((int64_t)seq * H + h) * (1 + 2 * a.most);
+    if (len <= a.budget) {
+        if (threadIdx.x == 0) list[0] = 0;
+        return;
+    }
+    const int64_t newest = (int64_t)a.seen[seq] - a.recent;
+    int32_t *holes = list + 1, *behind = holes + a.most;
+    select_largest(
+        sm, len, a.budget,
+        [&](int64_t i) {
+            const int64_t page = dense_page(a.pool, seq, i);
+            if (page < 0) return 0u;
+            const int64_t o = (page * H + h) * B + (i & (B - 1));
+            const int32_t p = a.pool.positions[o];
+            return sort_key(a.pool.weights[o], p < a.sink || p >= newest);
+        },
+        [&](int64_t i, bool kept, int64_t rank) {
+            if (i < a.budget) {
+                if (!kept) holes[i - rank] = (int32_t)i;
+                if (i == a.budget - 1) list[0] = (int32_t)(i + 1 - rank - (kept ? 1 : 0));
+            } else if (kept) {
+                behind[a.budget - 1 - rank] = (int32_t)i;
+            }
+        });
+}
+
+// Moves the kept rows into the evicted places; sixteen lanes a row.  The new
+// lengths are written here and not by the launch before, whose workgroups all
+// read the lengths: both may be one tensor.
+constexpr int MV_ROWS = 64;
+
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a)
+{
+    const int h = blockIdx.y % a.pool.H, seq = blockIdx.y / a.pool.H, lane = threadIdx.x & 15;
+    const int32_t *list = a.moves + (int64_t)blockIdx.y * (1 + 2 * a.most);
+    const int n = list[0];
+    const int32_t *holes = list + 1, *behind = holes + a.most;
+    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
+        const int32_t have = a.lengths[seq];
+        a.new_lengths[seq] = have < a.budget ? have : (int32_t)a.budget;
+    }
+#pragma unroll
+    for (int i = 0; i < MV_ROWS / 16; ++i) {
+        const int64_t m = (int64_t)blockIdx.x * MV_ROWS + 16 * i + (threadIdx.x >> 4);
+        if (m >= n) break;
+        dense_move(a.pool, seq, h, behind[n - 1 - m], holes[m], lane);
+    }
+}
+
+}  // namespace
+
+extern "C" int iq_dense_write(const void *k, const void *v, int dtype, int64_t k_st, int64_t k_sh, int64_t v_st,
+                              int64_t v_sh, const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen,
+                              const int32_t *start, const int32_t *positions, const float *weights, int64_t w_stride,
+                              const int32_t *keep, int64_t kept, const iq_dense_pages *pages, const int32_t *tables,
+                              int64_t bt_stride, int64_t bt_cols, void *stream)
+{
+    DensePool pool;
+    if (const int e = dense_pool("iq_dense_write", pages, dtype, tables, bt_stride, bt_cols, n_seq, pool)) return e;
+    IQ_CHECK_ARG(k && v && cu_seqlens, "iq_dense_write: null pointer");
+    IQ_CHECK_ARG(((uintptr_t)k | (uintptr_t)v) % 16 == 0 && (k_st | k_sh | v_st | v_sh) % 8 == 0,
+                 "iq_dense_write: key/value rows must be 16-byte aligned");
+    IQ_CHECK_ARG(max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL && kept >= 0 && kept <= 0x7fffffffLL,
+                 "iq_dense_write: bad row count");
+    const int64_t rows = keep ? kept : max_seqlen;
+    if (n_seq == 0 || rows == 0) return IQ_OK;
+    const int64_t groups = (rows * pool.H + WR_ITEMS - 1) / WR_ITEMS;
+    IQ_CHECK_ARG(groups <= 0xffffff, "iq_dense_write: too many rows");
+    const WriteArgs a{(const uint16_t *)k, (const uint16_t *)v, k_st, k_sh, v_st, v_sh, cu_seqlens, start, positions,
+                      weights, w_stride, keep, kept, pool};
+    hipLaunchKernelGGL(write_rows_kernel, dim3((unsigned)groups, (unsigned)n_seq), dim3(256), 0, (hipStream_t)stream,
+                       a);
+    IQ_CHECK_LAUNCH("dense_write");
+    return IQ_OK;
+}
+
+extern "C" int iq_select_rows(const float *weights, int64_t w_stride, int64_t H, const int32_t *cu_seqlens,
+                              int64_t n_seq, int64_t max_seqlen, int64_t budget, int64_t sink, int64_t recent,
+                              int32_t *keep, void *stream)
+{
+    IQ_CHECK_ARG(weights && cu_seqlens && keep, "iq_select_rows: null pointer");
+    IQ_CHECK_ARG(H >= 1 && H <= 65535 && n_seq >= 0 && n_seq <= 65535 && max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL,
+                 "iq_select_rows: bad head or sequence count or length");
+    IQ_CHECK_ARG(sink >= 0 && recent >= 0 && budget >= 1 && budget <= 0x7fffffffLL && sink + recent <= budget,
+                 "iq_select_rows: sink and recent rows must fit the budget");
+    if (n_seq == 0) return IQ_OK;
+    const SelectArgs a{weights, w_stride, cu_seqlens, budget, sink, recent, keep};
+    hipLaunchKernelGGL(select_rows_kernel, dim3((unsigned)H, (unsigned)n_seq), dim3(SEL_NT), 0, (hipStream_t)stream,
+                       a);
+    IQ_CHECK_LAUNCH("select_rows");
+    return IQ_OK;
+}
+
+extern "C" int64_t iq_dense_evict_ints(int64_t H, int64_t n_seq, int64_t max_tokens, int64_t budget)
+{
+    const int64_t over = max_tokens > budget ? max_tokens - budget : 0;
+    return n_seq * H * (1 + 2 * (over < budget ? over : budget));
+}
+
+extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int32_t *tables, int64_t bt_stride,
+                              int64_t bt_cols, const int32_t *lengths, const int32_t *seen, int64_t n_seq,
+                              int64_t max_tokens, int64_t budget, int64_t sink, int64_t recent, int32_t *new_lengths,
+                              int32_t *workspace, int64_t workspace_ints, void *stream)
+{
+    DensePool pool;
+    if (const int e = dense_pool("iq_dense_evict", pages, dtype, tables, bt_stride, bt_cols, n_seq, pool)) return e;
+    IQ_CHECK_ARG(pool.weights && pool.positions, "iq_dense_evict: pages without weights and positions");
+    IQ_CHECK_ARG(lengths && seen && new_lengths && workspace, "iq_dense_evict: null pointer");
+    IQ_CHECK_ARG(max_tokens >= 0 && max_tokens <= bt_cols * pool.B, "iq_dense_evict: max_tokens past the block tables");
+    IQ_CHECK_ARG(sink >= 0 && recent >= 0 && budget >= 1 && budget <= 0x7fffffffLL && sink + recent <= budget,
+                 "iq_dense_evict: sink and recent rows must fit the budget");
+    IQ_CHECK_ARG(workspace_ints >= iq_dense_evict_ints(pool.H, n_seq, max_tokens, budget),
+                 "iq_dense_evict: workspace too small");
+    IQ_CHECK_ARG(n_seq * pool.H <= 65535, "iq_dense_evict: too many sequences");
+    if (n_seq == 0) return IQ_OK;
+    const int64_t over = max_tokens > budget ? max_tokens - budget : 0, most = over < budget ? over : budget;
+    const EvictArgs a{pool, lengths, seen, max_tokens, budget, sink, recent, most, new_lengths, workspace};
+    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)pool.H, (unsigned)n_seq), dim3(SEL_NT), 0,
+                       (hipStream_t)stream, a);
+    const int64_t groups = most > 0 ? (most + MV_ROWS - 1) / MV_ROWS : 1;
+    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)groups, (unsigned)(n_seq * pool.H)), dim3(256), 0,
+                       (hipStream_t)stream, a);
+    IQ_CHECK_LAUNCH("dense_evict");
+    return IQ_OK;
+}

@@ -51,6 +51,8 @@ struct PrefillArgs {
     float c_log2;                                             // softmax scale * log2(e)
     int odt;
     int vec_out;                                              // output rows aligned for 4-channel stores
+    float *lse;                                               // [Hq, lse_sh]: log of each query's softmax sum (LSE kernels)
+    int64_t lse_sh;
 };
 
 // two stages: one is computed while the next tile lands in the other.  Rows
@@ -101,7 +103,7 @@ __device__ __forceinline__ float pair_sum(float v)
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
 }
 
-template <bool F16>
+template <bool F16, bool LSE>
 __global__ __launch_bounds__(NT, 2) void prefill_attn(PrefillArgs a)
 {
     __shared__ PrefillSmem sm;
@@ -277,6 +279,9 @@ __global__ __launch_bounds__(NT, 2) void prefill_attn(PrefillArgs a)
     }
     l_run = pair_sum(l_run);
     if (my_q < len) {
+        if constexpr (LSE)
+            if (h32 == 0)
+                a.lse[hq * a.lse_sh + start + my_q] = (m_run + __builtin_amdgcn_logf(l_run)) * 0.693147180559945309f;
         const float inv = 1.0f / l_run;
         const int64_t o = (int64_t)(start + my_q) * a.o_st + (int64_t)hq * a.o_sh + 4 * h32;
         // four consecutive channels per register group: one 16- or 8-byte store
@@ -313,11 +318,11 @@ __global__ __launch_bounds__(NT, 2) void prefill_attn(PrefillArgs a)
 
 }  // namespace
 
-extern "C" int iq_prefill_attention_tokens(const void *q, const void *k, const void *v, int dtype, int64_t q_st,
+extern "C" int iq_prefill_attention_lse(const void *q, const void *k, const void *v, int dtype, int64_t q_st,
                                     int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
                                     const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t Hq,
                                     int64_t H, int64_t head_dim, float scale, void *out, int64_t o_st,
-                                    int64_t o_sh, int out_dtype, void *stream)
+                                    int64_t o_sh, int out_dtype, float *lse, int64_t lse_sh, void *stream)
 {
     IQ_CHECK_ARG(q && k && v && out && cu_seqlens, "iq_prefill_attention: null pointer");
     IQ_CHECK_ARG(dtype == IQ_BF16 || dtype == IQ_F16, "iq_prefill_attention: q/k/v must be bf16 or f16");
@@ -328,6 +333,7 @@ extern "C" int iq_prefill_attention_tokens(const void *q, const void *k, const v
     IQ_CHECK_ARG(n_seq >= 1 && n_seq <= 65535 && max_seqlen >= 1 && max_seqlen <= 0x7fffffffLL - QT,
                  "iq_prefill_attention: bad sequence count or length");
     IQ_CHECK_ARG(tokens >= 0 && tokens <= (int64_t(1) << 60), "iq_prefill_attention: bad token count");
+    IQ_CHECK_ARG(!lse || scale > 0.0f, "iq_prefill_attention: the scale must be positive for the lse");
     // a key tile's rows are addressed by 32-bit byte offsets from its first row
     IQ_CHECK_ARG(k_st >= 0 && v_st >= 0 && k_st < (1LL << 25) && v_st < (1LL << 25),
                  "iq_prefill_attention: token stride too large");
@@ -375,13 +381,25 @@ extern "C" int iq_prefill_attention_tokens(const void *q, const void *k, const v
         const int64_t n = n_seq - s0 < most ? n_seq - s0 : most;
         PrefillArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, out, q_st, q_sh, k_st, k_sh,
                       v_st, v_sh, o_st, o_sh, cu_seqlens + s0, (int)tiles, (int)span, (int)share, (int)n, (int)Hq, (int)(Hq / H),
-                      scale * 1.44269504088896341f, out_dtype, vec_out};
+                      scale * 1.44269504088896341f, out_dtype, vec_out, lse, lse_sh};
         const dim3 grid((unsigned)(groups ? per_seq * n : per_seq), groups ? 1u : (unsigned)n), block(NT);
-        if (dtype == IQ_F16) hipLaunchKernelGGL(prefill_attn<true>, grid, block, 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL(prefill_attn<false>, grid, block, 0, (hipStream_t)stream, a);
+        const bool f16 = dtype == IQ_F16;
+        const auto kernel = lse ? f16 ? prefill_attn<true, true> : prefill_attn<false, true>
+                                : f16 ? prefill_attn<true, false> : prefill_attn<false, false>;
+        hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, a);
     }
     IQ_CHECK_LAUNCH("prefill_attn");
     return IQ_OK;
+}
+
+extern "C" int iq_prefill_attention_tokens(const void *q, const void *k, const void *v, int dtype, int64_t q_st,
+                                    int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                                    const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t Hq,
+                                    int64_t H, int64_t head_dim, float scale, void *out, int64_t o_st,
+                                    int64_t o_sh, int out_dtype, void *stream)
+{
+    return iq_prefill_attention_lse(q, k, v, dtype, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu_seqlens, n_seq, max_seqlen,
+                                    tokens, Hq, H, head_dim, scale, out, o_st, o_sh, out_dtype, nullptr, 0, stream);
 }
 
 extern "C" int iq_prefill_attention(const void *q, const void *k, const void *v, int dtype, int64_t q_st, int64_t q_sh,

@@ -1,0 +1,312 @@
+// The weight each key of a prompt receives from the prompt's queries (gfx950):
+//   weights[h][j] = sum over the queries i >= j and the query heads g of KV
+//   head h of exp(scale q_gi . k_j - lse_gi),
+// over all queries, whose lse the attention left, or over the last `window`
+// of each sequence, whose lse is computed here first.
+//
+// Keys are the rows of S^T = K Q^T on v_mfma_f32_32x32x16 and stay in
+// registers (64 per wavefront, 256 per workgroup) while tiles of 64 queries
+// stream through LDS, so a key's sum over the queries is one fp32 add per
+// logit in the lane that holds it, and is added over the 32 lanes (queries of
+// a tile) once, at the end.
+#include "decode_common.h"
+
+namespace {
+
+constexpr int D = 128;
+constexpr int NW = 4, NT = 64 * NW;
+constexpr int KW = 64;                       // keys per wavefront
+constexpr int KG = KW * NW;                  // keys per workgroup
+constexpr int QT = 64;                       // queries per tile
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+struct WeightArgs {
+    const uint16_t *q, *k;
+    int64_t q_st, q_sh, k_st, k_sh;          // element strides (token, head)
+    const int32_t *cu;
+    int max_len, H, Hq, G;                   // a sequence's rows past max_len are left out
+    int heads;                               // query heads a workgroup sums: 1, or G
+    int64_t window;                          // queries of each sequence from its end (all: its length)
+    float c_log2;
+    const float *lse;                        // natural log; token i of head hq at hq * lse_sh + i, or with
+    int64_t lse_sh;                          // `windowed`, window row i at ((seq * Hq) + hq) * window + i
+    int windowed;
+    f32x2 *ml;                               // the lse pass: (max, sum) per [seq, 64-key tile, Hq, window]
+    int tiles64;
+    float *out;                              // [H or Hq, out_sh]
+    int64_t out_sh;
+};
+
+struct __attribute__((aligned(16))) WeightSmem {
+    uint16_t q[2][QT * D];                   // chunk c of row r at slot c ^ (r % 16)
+};
+
+template <bool F16>
+__device__ __forceinline__ f32x16 mma3232(u32x4 a, u32x4 b, f32x16 c)
+{
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
+                                                      0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                       c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int length_of(const WeightArgs &a, int seq)
+{
+    const int len = a.cu[seq + 1] - a.cu[seq];
+    return len < a.max_len ? len : a.max_len;
+}
+
+__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+
+__device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32); }
+
+// LSEPASS: (max, sum) of every window query over this workgroup's keys, per
+// wavefront; else the keys' sums of exp(logit - lse).
+template <bool F16, bool LSEPASS>
+__global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
+{
+    __shared__ WeightSmem sm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c32 = lane & 31, h32 = lane >> 5;
+    const int seq = blockIdx.z, first_head = blockIdx.y * a.heads, h = first_head / a.G;
+    const int start = a.cu[seq], len = length_of(a, seq);
+    const int g0 = blockIdx.x * KG;
+    if (g0 >= len) return;                   // uniform
+    const int lo = (int64_t)len > a.window ? len - (int)a.window : 0;
+    const int q0 = lo > g0 ? lo : g0;        // the first query that sees one of these keys
+    const int k0 = g0 + KW * wave;           // this wavefront's first key
+    u32x4 kf[2][8];                          // A operand: key k0 + 32 kb + c32, channels 16 d + 8 h32 .. + 7
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const int key = k0 + 32 * kb + c32, kk = key < len ? key : len - 1;
+        const uint16_t *kp = a.k + (int64_t)(start + kk) * a.k_st + (int64_t)h * a.k_sh + 8 * h32;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) kf[kb][d] = ld16(kp + 16 * d);
+    }
+    f32x16 sum[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[kb][i] = 0.0f;
+    const int per = (len - q0 + QT - 1) / QT;               // query tiles of a head
+    const int total = per * a.heads;
+    const uint32_t lds_q = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&sm.q[0][0];
+    // sixteen of a tile's rows per wavefront, four (1 KB) per direct load; rows
+    // past the end repeat the last one
+    auto dma_tile = [&](int it, int st) {
+        const int head = first_head + it / per, qa = q0 + it % per * QT;
+        const uint16_t *qt = a.q + (int64_t)(start + qa) * a.q_st + (int64_t)head * a.q_sh;
+        const int last = len - 1 - qa;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r0 = 16 * wave + 4 * i, r = r0 + (lane >> 4), p = lane & 15;
+            const int rr = r < last ? r : last;
+            lds_load16(qt, (uint32_t)((rr * a.q_st + 8 * (p ^ (r & 15))) * 2),
+                       lds_q + (uint32_t)((st * QT + r0) * D * 2));
+        }
+    };
+    dma_tile(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    int s = 0;
+    for (int it = 0; it < total; ++it, s ^= 1) {
+        const int head = first_head + it / per, qa = q0 + it % per * QT;
+        float lse2[2];
+        if constexpr (!LSEPASS) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int i = qa + 32 * b + c32;
+                const int64_t at = a.windowed ? ((int64_t)seq * a.Hq + head) * a.window + (i - lo)
+                                              : (int64_t)head * a.lse_sh + start + i;
+                lse2[b] = i < len ? a.lse[at] * LOG2E : __builtin_inff();
+            }
+        }
+        if (it + 1 < total) dma_tile(it + 1, s ^ 1);
+        if (k0 < len && k0 <= qa + QT - 1) {                // some query of this tile sees a key of this wavefront
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const uint16_t *sq = sm.q[s] + (32 * b + c32) * D;
+                f32x16 sc[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const u32x4 qv = *(const u32x4 *)(sq + 8 * ((2 * d + h32) ^ (c32 & 15)));
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv, sc[kb]);
+                }
+                const int query = qa + 32 * b + c32;
+                if (qa + 32 * b < k0 + KW || k0 + KW > len) {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h32 + (i & 3);
+                            if (key > query || key >= len) sc[kb][i] = NEG_INF;   // the scale is positive
+                        }
+                }
+                if constexpr (LSEPASS) {
+                    float m = NEG_INF, l = 0.0f;
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i] * a.c_log2);
+                    m = pair_max(m);
+                    const float use = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -use));
+                    l = pair_sum(l);
+                    if (h32 == 0 && query < len)
+                        a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] =
+                            f32x2{m, l};
+                } else {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -lse2[b]));
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    if constexpr (!LSEPASS) {
+        float *out = a.out + (int64_t)(a.heads == 1 ? first_head : h) * a.out_sh + start;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float v = sum[kb][i];
+#pragma unroll
+                for (int d = 16; d; d >>= 1) v += __shfl_xor(v, d);
+                const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h32 + (i & 3);
+                if (c32 == 0 && key < len) out[key] = v;
+            }
+    }
+}
+
+// lse of the window's queries from the (max, sum) of their key tiles: 64 rows
+// (query heads and window queries of a sequence) per workgroup, the key tiles
+// over its wavefronts.
+__global__ __launch_bounds__(1024) void window_lse(WeightArgs a, float *lse)
+{
+    __shared__ float sm_m[16][64], sm_l[16][64];
+    const int seq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int len = length_of(a, seq);
+    const int lo = (int64_t)len > a.window ? len - (int)a.window : 0;
+    const int64_t rows = (int64_t)a.Hq * a.window, row = (int64_t)blockIdx.x * 64 + lane;
+    const int i = row < rows ? (int)(row % a.window) : 0, query = lo + i;
+    float M = NEG_INF, L = 0.0f;
+    if (row < rows && query < len) {
+        // tiles with a key at or before the query; the workgroup of a tile wrote every query from its first key on
+        for (int t = wave; t <= query / KW; t += 16) {
+            const f32x2 ml = a.ml[((int64_t)seq * a.tiles64 + t) * rows + row];
+            const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
+            L = L * __builtin_amdgcn_exp2f(M - use) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - use);
+            M = m;
+        }
+    }
+    sm_m[wave][lane] = M;
+    sm_l[wave][lane] = L;
+    __syncthreads();
+    if (wave || row >= rows || query >= len) return;
+    float m = NEG_INF, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) m = fmaxf(m, sm_m[w][lane]);
+    const float use = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) l = fmaf(__builtin_amdgcn_exp2f(sm_m[w][lane] - use), sm_l[w][lane], l);
+    lse[(int64_t)seq * rows + row] = (use + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// The query heads' sums of each KV head.
+__global__ __launch_bounds__(256) void add_heads(WeightArgs a, const float *part, int64_t tokens, float *out,
+                                                 int64_t out_sh)
+{
+    const int h = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= length_of(a, blockIdx.z)) return;
+    const int64_t at = a.cu[blockIdx.z] + i;
+    float v = 0.0f;
+    for (int g = 0; g < a.G; ++g) v += part[(int64_t)(h * a.G + g) * tokens + at];
+    out[h * out_sh + at] = v;
+}
+
+struct Scratch {
+    int64_t lse, ml, part;                   // floats of each
+};
+
+Scratch scratch_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t window, bool lse)
+{
+    Scratch s{0, 0, 0};
+    if (window > 0 && !lse) {
+        s.lse = n_seq * Hq * window;
+        s.ml = 2 * n_seq * ((max_seqlen + KW - 1) / KW) * Hq * window;
+    }
+    if (window == 0) s.part = Hq * tokens;
+    return s;
+}
+
+}  // namespace
+
+extern "C" int64_t iq_prefill_weights_floats(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens,
+                                             int64_t window, int have_lse)
+{
+    const Scratch s = scratch_of(Hq, n_seq, max_seqlen, tokens, window, have_lse != 0);
+    return s.lse + s.ml + s.part;
+}
+
+extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64_t q_st, int64_t q_sh, int64_t k_st,
+                                  int64_t k_sh, const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen,
+                                  int64_t tokens, int64_t Hq, int64_t H, int64_t window, float scale, const float *lse,
+                                  int64_t lse_sh, float *workspace, int64_t workspace_floats, float *out,
+                                  int64_t out_sh, void *stream)
+{
+    IQ_CHECK_ARG(q && k && cu_seqlens && out, "iq_prefill_weights: null pointer");
+    IQ_CHECK_ARG(dtype == IQ_BF16 || dtype == IQ_F16, "iq_prefill_weights: q/k must be bf16 or f16");
+    IQ_CHECK_ARG(H >= 1 && Hq >= 1 && Hq % H == 0 && Hq <= 65535, "iq_prefill_weights: heads %lld / %lld",
+                 (long long)Hq, (long long)H);
+    IQ_CHECK_ARG(n_seq >= 1 && n_seq <= 65535 && max_seqlen >= 1 && max_seqlen <= 0x3fffffff && tokens >= 0 &&
+                     tokens <= 0x7fffffffLL,
+                 "iq_prefill_weights: bad sequence count or length");
+    IQ_CHECK_ARG(((uintptr_t)q | (uintptr_t)k) % 16 == 0 && (q_st | q_sh | k_st | k_sh) % 8 == 0,
+                 "iq_prefill_weights: q/k rows must be 16-byte aligned");
+    // a query tile's rows are addressed by 32-bit byte offsets from its first row
+    IQ_CHECK_ARG(q_st >= 0 && q_st < (1LL << 25), "iq_prefill_weights: token stride too large");
+    IQ_CHECK_ARG(scale > 0.0f, "iq_prefill_weights: the scale must be positive");
+    IQ_CHECK_ARG(window >= 0 && window <= 65536 && (window > 0 || lse), "iq_prefill_weights: no window and no lse");
+    const Scratch s = scratch_of(Hq, n_seq, max_seqlen, tokens, window, lse != nullptr);
+    IQ_CHECK_ARG(s.lse + s.ml + s.part == 0 || (workspace && workspace_floats >= s.lse + s.ml + s.part),
+                 "iq_prefill_weights: workspace too small");
+    const int64_t tiles = (max_seqlen + KG - 1) / KG, G = Hq / H;
+    WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)max_seqlen, (int)H,
+                 (int)Hq, (int)G, (int)(window ? G : 1), window ? window : max_seqlen, scale * LOG2E, lse, lse_sh, 0,
+                 (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
+    const hipStream_t st = (hipStream_t)stream;
+    const bool f16 = dtype == IQ_F16;
+    const dim3 grid((unsigned)tiles, (unsigned)(Hq / a.heads), (unsigned)n_seq), block(NT);
+    if (window > 0 && !lse) {
+        float *own = workspace + s.ml;
+        hipLaunchKernelGGL((f16 ? prefill_weights<true, true> : prefill_weights<false, true>), grid, block, 0, st, a);
+        hipLaunchKernelGGL(window_lse, dim3((unsigned)((Hq * window + 63) / 64), (unsigned)n_seq), dim3(1024), 0, st, a,
+                           own);
+        a.lse = own;
+        a.windowed = 1;
+    }
+    if (window == 0) {
+        a.out = workspace;
+        a.out_sh = tokens;
+    }
+    hipLaunchKernelGGL((f16 ? prefill_weights<true, false> : prefill_weights<false, false>), grid, block, 0, st, a);
+    if (window == 0 && tokens > 0)
+        hipLaunchKernelGGL(add_heads, dim3((unsigned)((max_seqlen + 255) / 256), (unsigned)H, (unsigned)n_seq),
+                           dim3(256), 0, st, a, workspace, tokens, out, out_sh);
+    IQ_CHECK_LAUNCH("prefill_weights");
+    return IQ_OK;
+}

@@ -51,6 +51,14 @@ class CopySegment(ctypes.Structure):
                 ("dst_h", _i64), ("dst_t", _i64), ("tokens", _i64)]
 
 
+class DensePagesDesc(ctypes.Structure):
+    """Mirror of iq_dense_pages in include/inquant_hip.h: a pool of exact
+    pages (addresses, element strides of page, head and row, sizes)."""
+    _fields_ = [(name, ctypes.c_uint64) for name in ("key", "value", "weights", "positions")] + \
+               [(name, _i64) for name in ("k_sp", "k_sh", "k_st", "v_sp", "v_sh", "v_st", "pages", "heads",
+                                          "block_tokens")]
+
+
 _SIGNATURES = {
     "iq_abi_version": (_int, []),
     "iq_last_error": (ctypes.c_char_p, []),
@@ -89,6 +97,19 @@ _SIGNATURES = {
                                     _i64, _i64, _f32, _p, _i64, _i64, _int, _p]),
     "iq_prefill_attention_tokens": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                            _i64, _i64, _i64, _f32, _p, _i64, _i64, _int, _p]),
+    "iq_prefill_attention_lse": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64,
+                                        _i64, _i64, _i64, _f32, _p, _i64, _i64, _int, _p, _i64, _p]),
+    "iq_prefill_weights_floats": (_i64, [_i64, _i64, _i64, _i64, _i64, _int]),
+    "iq_prefill_weights": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32,
+                                  _p, _i64, _p, _i64, _p, _i64, _p]),
+    "iq_dense_write": (_int, [_p, _p, _int, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p,
+                              _p, _i64, _i64, _p]),
+    "iq_select_rows": (_int, [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _p, _p]),
+    "iq_dense_evict_ints": (_i64, [_i64, _i64, _i64, _i64]),
+    "iq_dense_evict": (_int, [_p, _int, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p]),
+    "iq_dense_workspace_floats": (_i64, [_i64, _i64, _i64, _i64, _int]),
+    "iq_dense_decode": (_int, [_p, _int, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _f32, _int, _p, _i64,
+                               _p, _i64, _i64, _int, _p]),
     "iq_page_bytes": (_i64, [_i64, _i64]),
     "iq_encode_pages": (_int, [_p, _p, _int, ctypes.POINTER(_i64), ctypes.POINTER(_i64), _i64, _i64, _i64, _p, _i64,
                                _p, _int, _p, _p, _p]),

@@ -1,0 +1,333 @@
+"""Exact pages: a paged cache of rows as they are, cut back by accumulated attention weight.
+
+The packed pages of ``layout`` code every row; these hold bf16 or f16 rows
+[pages, kv_heads, block_size, 128] (the shape ``pack_pages_into`` seals), and
+beside every row the attention weight it has accumulated and its position.
+
+* ``write_rows``       a prompt's rows, or the ones a selection kept, or the
+                       new rows of running sequences, into the pages;
+* ``dense_decode``     one token's attention per sequence over the pages, which
+                       on request adds each row's weight;
+* ``prefill_weights``  the weight each key of a prompt receives from its
+                       queries, or from the last few of them;
+* ``select_rows``      the rows a budget keeps of each prompt and KV head;
+* ``evict_rows``       the pages of running sequences cut back to the budget,
+                       in place.
+
+Everything is enqueued on the current stream of the tensors' GPU; nothing is
+read back.  Lengths, positions, block tables and kept rows live on the device
+and are trusted as the other entry points trust them: page ids outside the pool
+and rows outside a block table are skipped, not reported.  The reference has no
+counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from inquant import _native as nat
+from .layout import BLOCK_SIZES
+
+_ROWS = (torch.bfloat16, torch.float16)
+
+
+def _strides(pages):
+    """Strides of page, head and row; any will do for a dimension of one."""
+    return [s if n > 1 else 8 for n, s in zip(pages.shape[:3], pages.stride())]
+
+
+@dataclass(frozen=True, eq=False)
+class DensePages:
+    """The exact pages of one layer: ``key`` and ``value`` [pages, kv_heads,
+    block_size, 128] of bf16 or f16 (any page, head and row strides that are
+    multiples of 8 elements, 16-byte aligned; two views of one pool will do) and,
+    where rows are to be evicted, ``weights`` f32 and ``positions`` int32
+    [pages, kv_heads, block_size]."""
+    key: torch.Tensor
+    value: torch.Tensor
+    weights: torch.Tensor | None = None
+    positions: torch.Tensor | None = None
+
+    def __post_init__(self):
+        key, value = self.key, self.value
+        if key.ndim != 4 or key.shape != value.shape or key.shape[-1] != 128 or key.shape[2] not in BLOCK_SIZES \
+                or key.shape[0] < 1 or key.shape[1] < 1:
+            raise ValueError("Expected key and value pages [pages, kv_heads, 16/32/64/128/256, 128]")
+        if key.dtype not in _ROWS or value.dtype != key.dtype:
+            raise ValueError("Exact pages hold BF16 or FP16 rows")
+        for t in (key, value):
+            if t.stride(3) != 1 or any(s % 8 or s <= 0 for s in _strides(t)) or t.data_ptr() % 16:
+                raise ValueError("page rows must be contiguous, 16-byte aligned and not expanded")
+        if (self.weights is None) != (self.positions is None):
+            raise ValueError("Weights and positions go together")
+        if self.weights is not None:
+            for t, dtype in ((self.weights, torch.float32), (self.positions, torch.int32)):
+                if t.shape != key.shape[:3] or t.dtype != dtype or not t.is_contiguous():
+                    raise ValueError("Expected contiguous float32 weights and int32 positions "
+                                     "[pages, kv_heads, block_size]")
+        side = (self.weights, self.positions)
+        if len({t.device for t in (key, value, *side) if t is not None}) != 1:
+            raise ValueError("all tensors must share one GPU")
+        p = nat.DensePagesDesc(key.data_ptr(), value.data_ptr(), *(0 if t is None else t.data_ptr() for t in side),
+                               *_strides(key), *_strides(value), *key.shape[:3])
+        object.__setattr__(self, "_desc", ctypes.byref(p))
+
+    @classmethod
+    def allocate(cls, pages, block_size, heads, dtype=torch.bfloat16, device="cuda", *, evictable=True):
+        """A pool of its own; the rows' weights and positions start at zero."""
+        shape = (pages, heads, block_size)
+        side = [torch.zeros(shape, dtype=t, device=device) if evictable else None
+                for t in (torch.float32, torch.int32)]
+        return cls(torch.empty((*shape, 128), dtype=dtype, device=device),
+                   torch.empty((*shape, 128), dtype=dtype, device=device), *side)
+
+    @property
+    def block_size(self):
+        return self.key.shape[2]
+
+    @property
+    def heads(self):
+        return self.key.shape[1]
+
+    @property
+    def nbytes(self):
+        """Bytes of the rows and of what stands beside them."""
+        return sum(t.numel() * t.element_size() for t in (self.key, self.value, self.weights, self.positions)
+                   if t is not None)
+
+
+def _call(device, entry, *args):
+    """entry(*args, stream) on the tensors' GPU."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        nat.check(entry(*args, nat.stream_handle(device)))
+    else:
+        with torch.cuda.device(device):
+            nat.check(entry(*args, nat.stream_handle(device)))
+
+
+def _ints(t, shape, what):
+    if tuple(t.shape) != shape or t.dtype != torch.int32:
+        raise ValueError(f"Expected int32 {what}")
+    return t.contiguous()
+
+
+def _cu(cu_seqlens):
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2:
+        raise ValueError("cu_seqlens must be an int32 [sequences + 1] tensor")
+    return cu_seqlens.contiguous()
+
+
+def _tables(block_tables, n):
+    if block_tables.ndim != 2 or block_tables.shape[0] != n or block_tables.dtype != torch.int32 \
+            or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("Expected int32 block tables [sequences, pages per sequence]")
+    return block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1]
+
+
+def _token_rows(t, what, heads=None):
+    if t.ndim != 3 or t.shape[-1] != 128 or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"Expected {what} [tokens, heads, 128]")
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{what} rows must be contiguous and 16-byte aligned")
+
+
+def _budget(budget, sink, recent):
+    if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
+        raise ValueError("sink and recent rows must fit a budget of at least one row")
+
+
+def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=None, *, positions=None, weights=None,
+               keep=None):
+    """Rows of token-major key/value [tokens, kv_heads, 128] into the pages.
+
+    Row t of sequence i (cu_seqlens int32 [sequences + 1], none longer than
+    max_seqlen) goes to cache row start[i] + t of every head (``start`` int32
+    [sequences], None: 0); with ``keep`` int32 [sequences, kv_heads, kept]
+    (``select_rows``) head h takes only the rows keep[i, h, j], to cache row
+    start[i] + j, and entries outside the sequence are skipped.  Where the pages
+    have weights, the row's is weights[h, cu_seqlens[i] + t] (``weights`` f32
+    [kv_heads, tokens], None: 0) and its position positions[i] + t
+    (``positions`` int32 [sequences], None: ``start``).  Rows that a block table
+    [sequences, pages per sequence] does not reach are left out."""
+    _token_rows(key, "key", pages.heads)
+    _token_rows(value, "value", pages.heads)
+    if key.shape != value.shape or key.dtype != pages.key.dtype or value.dtype != key.dtype:
+        raise ValueError("key and value must have one shape and the pages' dtype")
+    cu = _cu(cu_seqlens)
+    n = cu.numel() - 1
+    table = _tables(block_tables, n)
+    if start is not None:
+        start = _ints(start, (n,), "start rows [sequences]")
+    if positions is not None:
+        positions = _ints(positions, (n,), "positions [sequences]")
+    if weights is not None and (tuple(weights.shape) != (pages.heads, key.shape[0]) or weights.dtype != torch.float32
+                                or weights.stride(1) != 1 and weights.shape[1] > 1):
+        raise ValueError("Expected float32 weights [kv_heads, tokens]")
+    if keep is not None:
+        if keep.ndim != 3 or keep.shape[:2] != (n, pages.heads):
+            raise ValueError("Expected int32 kept rows [sequences, kv_heads, kept]")
+        keep = _ints(keep, tuple(keep.shape), "kept rows [sequences, kv_heads, kept]")
+    device = nat.require_gpu(key, value, cu, pages.key, block_tables, start, positions, weights, keep,
+                             what="write_rows")
+    if key.shape[0] == 0 or block_tables.shape[1] == 0:
+        return
+    _call(device, nat.lib().iq_dense_write, key.data_ptr(), value.data_ptr(), nat.dtype_code(key.dtype),
+          key.stride(0), key.stride(1), value.stride(0), value.stride(1), cu.data_ptr(), n, int(max_seqlen),
+          nat.ptr(start), nat.ptr(positions), nat.ptr(weights), 0 if weights is None else weights.stride(0),
+          nat.ptr(keep), 0 if keep is None else keep.shape[2], pages._desc, *table)
+
+
+def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, output=None):
+    """The rows that a budget keeps of each sequence and KV head: the first
+    ``sink`` and the last ``recent`` rows, then by weight (``weights`` f32
+    [kv_heads, tokens], as ``prefill_weights`` gives them), ties to the lowest
+    row, NaN last.  Returns int32 [sequences, kv_heads, budget]: ascending rows
+    within the sequence, -1 behind the last.  max_seqlen >= every sequence
+    length."""
+    budget, sink, recent = int(budget), int(sink), int(recent)
+    _budget(budget, sink, recent)
+    if weights.ndim != 2 or weights.dtype != torch.float32 or weights.shape[0] < 1 \
+            or weights.stride(1) != 1 and weights.shape[1] > 1:
+        raise ValueError("Expected float32 weights [kv_heads, tokens]")
+    cu = _cu(cu_seqlens)
+    shape = (cu.numel() - 1, weights.shape[0], budget)
+    device = nat.require_gpu(weights, cu, output, what="select_rows")
+    if output is None:
+        output = torch.empty(shape, dtype=torch.int32, device=device)
+    elif tuple(output.shape) != shape or output.dtype != torch.int32 or not output.is_contiguous():
+        raise ValueError("output must be a contiguous int32 [sequences, kv_heads, budget] tensor")
+    if weights.shape[1] == 0:
+        return output.fill_(-1)
+    _call(device, nat.lib().iq_select_rows, weights.data_ptr(), weights.stride(0), weights.shape[0], cu.data_ptr(),
+          shape[0], int(max_seqlen), budget, sink, recent, output.data_ptr())
+    return output
+
+
+def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0, recent=0, output=None):
+    """Cuts every sequence of more than ``budget`` rows back to ``budget``, each
+    KV head by its own weights, in place.
+
+    lengths int32 [sequences]: the rows that each holds (max_tokens >= all of
+    them); seen int32 [sequences]: the tokens that it has seen.  Kept are the
+    rows at positions below ``sink`` or from seen - recent on, then by weight,
+    ties to the lowest cache row, NaN last.  The evicted cache rows below the
+    budget take, in order, the kept rows from the budget on, so only those
+    move; every other row stays as it is.  Returns the new lengths
+    min(lengths, budget), int32 [sequences] (``output`` may be ``lengths``).
+    No page may belong to two of the sequences."""
+    budget, sink, recent, max_tokens = int(budget), int(sink), int(recent), int(max_tokens)
+    _budget(budget, sink, recent)
+    if pages.weights is None:
+        raise ValueError("Eviction needs pages with weights and positions")
+    if lengths.ndim != 1:
+        raise ValueError("Expected int32 lengths [sequences]")
+    n = lengths.shape[0]
+    lengths, seen = _ints(lengths, (n,), "lengths [sequences]"), _ints(seen, (n,), "tokens seen [sequences]")
+    table = _tables(block_tables, n)
+    if not 0 <= max_tokens <= table[2] * pages.block_size:
+        raise ValueError("max_tokens must fit the block tables")
+    device = nat.require_gpu(lengths, seen, block_tables, pages.key, output, what="evict_rows")
+    if output is None:
+        output = torch.empty_like(lengths)
+    elif tuple(output.shape) != (n,) or output.dtype != torch.int32 or not output.is_contiguous():
+        raise ValueError("output must be a contiguous int32 [sequences] tensor")
+    if n == 0:
+        return output
+    need = nat.lib().iq_dense_evict_ints(pages.heads, n, max_tokens, budget)
+    scratch = torch.empty(need, dtype=torch.int32, device=device)
+    _call(device, nat.lib().iq_dense_evict, pages._desc, nat.dtype_code(pages.key.dtype), *table, lengths.data_ptr(),
+          seen.data_ptr(), n, max_tokens, budget, sink, recent, output.data_ptr(), scratch.data_ptr(), need)
+    return output
+
+
+def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspace, output=None, *,
+                 accumulate=False):
+    """One token's attention per sequence over its exact pages.
+
+    query [sequences, Hq, 128] of the pages' dtype, at most 16 query heads per
+    KV head; block_tables int32 [sequences, pages per sequence]; lengths int32
+    [sequences], the rows each sequence holds, the newest token's among them
+    (max_tokens >= all of them; a sequence without rows gives zeros).  Returns
+    (or fills) output [sequences, Hq, 128] of the query dtype or float32.
+    ``accumulate=True`` adds to each row's weight the softmax weights that the
+    query heads of its KV head gave it (for a page that two sequences share,
+    in an order that is not fixed)."""
+    hkv, n = pages.heads, query.shape[0]
+    if query.ndim != 3 or query.shape[-1] != 128 or query.dtype != pages.key.dtype:
+        raise ValueError("Expected a query [sequences, heads, 128] of the pages' dtype")
+    hq, max_tokens = query.shape[1], int(max_tokens)
+    if hq < 1 or hq % hkv or hq // hkv > 16:
+        raise ValueError("Expected 1..16 query heads per KV head")
+    if accumulate and pages.weights is None:
+        raise ValueError("Accumulation needs pages with weights and positions")
+    lengths = _ints(lengths, (n,), "lengths [sequences]")
+    table = _tables(block_tables, n)
+    if not 0 <= max_tokens <= table[2] * pages.block_size:
+        raise ValueError("max_tokens must fit the block tables")
+    if not math.isfinite(scale):
+        raise ValueError("the scale must be finite")
+    device = nat.require_gpu(query, pages.key, block_tables, lengths, output, what="dense_decode")
+    if query.stride(2) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.data_ptr() % 16:
+        query = query.contiguous()
+    if output is None:
+        output = torch.empty(query.shape, dtype=query.dtype, device=device)
+    elif output.shape != query.shape or output.stride(2) != 1 or output.dtype not in (query.dtype, torch.float32):
+        raise ValueError("output must be [sequences, heads, 128] of the query dtype or float32")
+    if n == 0:
+        return output
+    need = nat.lib().iq_dense_workspace_floats(hq, hkv, n, max_tokens, bool(accumulate))
+    scratch = workspace.acquire((need,), device)
+    _call(device, nat.lib().iq_dense_decode, query.data_ptr(), nat.dtype_code(query.dtype), query.stride(0),
+          query.stride(1), hq, n, pages._desc, *table, lengths.data_ptr(), max_tokens, float(scale),
+          bool(accumulate), scratch.data_ptr(), need, output.data_ptr(), output.stride(0), output.stride(1),
+          nat.dtype_code(output.dtype))
+    return output
+
+
+def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, window=None, output=None):
+    """The softmax weight that each key of a prompt receives, summed over the
+    queries that see it and over the query heads of its KV head: float32
+    [kv_heads, tokens].
+
+    query [tokens, Hq, 128], key [tokens, kv_heads, 128] (bf16 or f16),
+    sequences as ``prefill_attention`` takes them.  Over all queries, whose
+    ``lse`` [Hq, tokens] ``prefill_attention(..., lse=...)`` wrote, or with
+    ``window=w`` over the last w queries of each sequence (lse optional).
+    Tokens of no sequence are not written."""
+    _token_rows(query, "query")
+    _token_rows(key, "key")
+    if query.shape[0] != key.shape[0] or query.dtype not in _ROWS or key.dtype != query.dtype:
+        raise ValueError("Expected BF16 or FP16 query and key of the same tokens")
+    tokens, hq, h = query.shape[0], query.shape[1], key.shape[1]
+    if h < 1 or hq < 1 or hq % h:
+        raise ValueError("query heads must be a multiple of KV heads")
+    cu, max_seqlen = _cu(cu_seqlens), int(max_seqlen)
+    if max_seqlen < 1 or not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("max_seqlen and the scale must be positive")
+    if window is not None and int(window) < 1:
+        raise ValueError("the window must hold at least one query")
+    if window is None and lse is None:
+        raise ValueError("Weights of all queries need the lse of prefill_attention")
+    if lse is not None and (tuple(lse.shape) != (hq, tokens) or lse.dtype != torch.float32
+                            or lse.stride(1) != 1 and tokens > 1):
+        raise ValueError("Expected a float32 lse [query heads, tokens]")
+    device = nat.require_gpu(query, key, cu, lse, output, what="prefill_weights")
+    if output is None:
+        output = torch.empty((h, tokens), dtype=torch.float32, device=device)
+    elif tuple(output.shape) != (h, tokens) or output.dtype != torch.float32 \
+            or output.stride(1) != 1 and tokens > 1:
+        raise ValueError("output must be float32 [kv_heads, tokens]")
+    if tokens == 0:
+        return output
+    window = 0 if window is None else min(int(window), max_seqlen)
+    n = cu.numel() - 1
+    need = nat.lib().iq_prefill_weights_floats(hq, n, max_seqlen, tokens, window, lse is not None)
+    scratch = torch.empty(need, dtype=torch.float32, device=device)
+    _call(device, nat.lib().iq_prefill_weights, query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype),
+          query.stride(0), query.stride(1), key.stride(0), key.stride(1), cu.data_ptr(), n, max_seqlen, tokens, hq, h,
+          window, float(scale), nat.ptr(lse), 0 if lse is None else lse.stride(0), scratch.data_ptr(), need,
+          output.data_ptr(), output.stride(0))
+    return output

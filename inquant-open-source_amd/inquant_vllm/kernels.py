@@ -111,7 +111,7 @@ def paged_decode_batch(query, cache, block_tables, seq_info, dense, max_pages, l
     return output
 
 
-def prefill_attention(query, key, value, cu_seqlens, max_seqlen, scale, output=None, *, check_lengths=False):
+def prefill_attention(query, key, value, cu_seqlens, max_seqlen, scale, output=None, *, check_lengths=False, lse=None):
     """Causal self-attention of a prefill over its exact K/V (replaces the
     plugin's flash_attn_varlen_func(..., causal=True) call, backend.py:139-144).
 
@@ -124,7 +124,10 @@ def prefill_attention(query, key, value, cu_seqlens, max_seqlen, scale, output=N
     max_seqlen query rows per sequence, so the query rows of a sequence
     longer than max_seqlen past that count are not written.  cu_seqlens lives
     on the device and is not read back; with ``check_lengths=True`` the
-    lengths are read (one synchronization) and a longer sequence raises."""
+    lengths are read (one synchronization) and a longer sequence raises.
+
+    ``lse`` float32 [Hq, tokens]: filled with the log of each query's softmax
+    sum (scale > 0), which ``prefill_weights`` takes."""
     if query.ndim != 3 or key.ndim != 3 or key.shape != value.shape or query.shape[-1] != 128 \
             or key.shape[-1] != 128 or query.shape[0] != key.shape[0]:
         raise ValueError("Expected query [tokens, Hq, 128] and key/value [tokens, H, 128]")
@@ -145,10 +148,16 @@ def prefill_attention(query, key, value, cu_seqlens, max_seqlen, scale, output=N
     elif tuple(output.shape) != tuple(query.shape) or output.stride(-1) != 1 \
             or output.dtype not in (query.dtype, torch.float32):
         raise ValueError("output must be [tokens, Hq, 128] of the query dtype or float32")
+    if lse is not None:
+        if tuple(lse.shape) != (hq, query.shape[0]) or lse.dtype != torch.float32 \
+                or lse.stride(1) != 1 and lse.shape[1] > 1 or not scale > 0:
+            raise ValueError("lse must be float32 [query heads, tokens], and the scale positive")
+        nat.require_gpu(query, lse, what="prefill_attention")
     cu = cu_seqlens.contiguous()
-    nat.check(nat.lib().iq_prefill_attention_tokens(
+    nat.check(nat.lib().iq_prefill_attention_lse(
         query.data_ptr(), key.data_ptr(), value.data_ptr(), nat.dtype_code(query.dtype),
         query.stride(0), query.stride(1), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
         cu.data_ptr(), cu.numel() - 1, int(max_seqlen), query.shape[0], hq, h, 128, float(scale), output.data_ptr(),
-        output.stride(0), output.stride(1), nat.dtype_code(output.dtype), nat.stream_handle(query.device)))
+        output.stride(0), output.stride(1), nat.dtype_code(output.dtype), nat.ptr(lse),
+        0 if lse is None else lse.stride(0), nat.stream_handle(query.device)))
     return output
