@@ -26,7 +26,7 @@ struct WeightArgs {
     const uint16_t *q, *k;
     int64_t q_st, q_sh, k_st, k_sh;          // element strides (token, head)
     const int32_t *cu;
-    int max_len, H, Hq, G;                   // a sequence's rows past max_len are left out
+    int n_seq, max_len, H, Hq, G;              // a sequence's rows past max_len are left out
     int heads;                               // query heads a workgroup sums: 1, or G
     int64_t window;                          // queries of each sequence from its end (all: its length)
     float c_log2;
@@ -39,9 +39,26 @@ struct WeightArgs {
     int64_t out_sh;
 };
 
+// Three stages: a tile is computed while the next two land in the others.
+constexpr int ST = 3;
+
 struct __attribute__((aligned(16))) WeightSmem {
-    uint16_t q[2][QT * D];                   // chunk c of row r at slot c ^ (r % 16)
+    uint16_t q[ST][QT * D];                  // chunk c of row r at slot c ^ (r % 16)
+    float lse[ST][NW][QT];                   // a copy per wavefront
 };
+static_assert(2 * sizeof(WeightSmem) <= 160 * 1024, "two workgroups per compute unit");
+
+// lds_load16 with four bytes per lane
+__device__ __forceinline__ void lds_load4(const void *base, uint32_t voff, uint32_t lds_base)
+{
+    const uint64_t b = (uint64_t)(uintptr_t)base;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+    const uint64_t sb = (uint64_t)lo | ((uint64_t)hi << 32);
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sb),
+                 "s"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+}
 
 template <bool F16>
 __device__ __forceinline__ f32x16 mma3232(u32x4 a, u32x4 b, f32x16 c)
@@ -72,9 +89,13 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     __shared__ WeightSmem sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c32 = lane & 31, h32 = lane >> 5;
-    const int seq = blockIdx.z, first_head = blockIdx.y * a.heads, h = first_head / a.G;
+    // Key tiles from the first on: the first see the most queries, so the
+    // longest workgroups start first, over all sequences and heads.
+    const int lists = a.Hq / a.heads, per_tile = lists * a.n_seq;
+    const int tile = blockIdx.x / per_tile, rest = blockIdx.x - tile * per_tile;
+    const int seq = rest / lists, first_head = (rest - seq * lists) * a.heads, h = first_head / a.G;
     const int start = a.cu[seq], len = length_of(a, seq);
-    const int g0 = blockIdx.x * KG;
+    const int g0 = tile * KG;
     if (g0 >= len) return;                   // uniform
     const int lo = (int64_t)len > a.window ? len - (int)a.window : 0;
     const int q0 = lo > g0 ? lo : g0;        // the first query that sees one of these keys
@@ -92,39 +113,55 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[kb][i] = 0.0f;
-    const int per = (len - q0 + QT - 1) / QT;               // query tiles of a head
-    const int total = per * a.heads;
+    const int last_tile = q0 + (len - q0 - 1) / QT * QT;    // a head's tiles go from its last query back, so that
+    const int total = ((len - q0 - 1) / QT + 1) * a.heads;  // workgroups that start together read the same queries
     const uint32_t lds_q = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&sm.q[0][0];
-    // sixteen of a tile's rows per wavefront, four (1 KB) per direct load; rows
-    // past the end repeat the last one
-    auto dma_tile = [&](int it, int st) {
-        const int head = first_head + it / per, qa = q0 + it % per * QT;
-        const uint16_t *qt = a.q + (int64_t)(start + qa) * a.q_st + (int64_t)head * a.q_sh;
-        const int last = len - 1 - qa;
+    const uint32_t lds_l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float *)&sm.lse[0][wave][0];
+    // Direct loads of the next tile, and its place: sixteen of its rows per
+    // wavefront, four (1 KB) per load, and its lse; rows past the end repeat
+    // the last one.
+    int next_head = first_head, next_qa = last_tile, next_st = 0;
+    auto load_tile = [&]() {
+        const uint16_t *qt = a.q + (int64_t)(start + next_qa) * a.q_st + (int64_t)next_head * a.q_sh;
+        const int last = len - 1 - next_qa;
+        if constexpr (!LSEPASS) {
+            const float *lt = a.lse + (a.windowed ? ((int64_t)seq * a.Hq + next_head) * a.window + (next_qa - lo)
+                                                  : (int64_t)next_head * a.lse_sh + start + next_qa);
+            lds_load4(lt, (uint32_t)(lane < last ? lane : last) * 4, lds_l + (uint32_t)(next_st * NW * QT * 4));
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r0 = 16 * wave + 4 * i, r = r0 + (lane >> 4), p = lane & 15;
             const int rr = r < last ? r : last;
             lds_load16(qt, (uint32_t)((rr * a.q_st + 8 * (p ^ (r & 15))) * 2),
-                       lds_q + (uint32_t)((st * QT + r0) * D * 2));
+                       lds_q + (uint32_t)((next_st * QT + r0) * D * 2));
+        }
+        next_st = next_st == ST - 1 ? 0 : next_st + 1;
+        next_qa -= QT;
+        if (next_qa < q0) {
+            next_qa = last_tile;
+            ++next_head;
         }
     };
-    dma_tile(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    int s = 0;
-    for (int it = 0; it < total; ++it, s ^= 1) {
-        const int head = first_head + it / per, qa = q0 + it % per * QT;
-        float lse2[2];
-        if constexpr (!LSEPASS) {
+    load_tile();
+    if (total > 1) load_tile();
+    // the keys are waited for here, not in the loop
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int i = qa + 32 * b + c32;
-                const int64_t at = a.windowed ? ((int64_t)seq * a.Hq + head) * a.window + (i - lo)
-                                              : (int64_t)head * a.lse_sh + start + i;
-                lse2[b] = i < len ? a.lse[at] * LOG2E : __builtin_inff();
-            }
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) asm volatile("" : "+v"(kf[kb][d]));
+    int s = 0, head = first_head, qa = last_tile;
+    for (int it = 0; it < total; ++it) {
+        // this tile's loads have landed (the next tile's may be under way), and
+        // after the barrier that holds for every wavefront, as does that the
+        // tile before has been read
+        if (it + 1 < total) {
+            if constexpr (LSEPASS) asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(5)\n\ts_barrier" ::: "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        if (it + 1 < total) dma_tile(it + 1, s ^ 1);
+        if (it + 2 < total) load_tile();
         if (k0 < len && k0 <= qa + QT - 1) {                // some query of this tile sees a key of this wavefront
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -155,8 +192,8 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i] * a.c_log2);
-                    m = pair_max(m);
+                        for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i]);
+                    m = pair_max(m * a.c_log2);
                     const float use = m == NEG_INF ? 0.0f : m;
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
@@ -167,15 +204,22 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
                         a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] =
                             f32x2{m, l};
                 } else {
+                    // a query past the end weighs nothing
+                    const float lse2 = query < len ? sm.lse[s][wave][32 * b + c32] * LOG2E : __builtin_inff();
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -lse2[b]));
+                            sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -lse2));
                 }
             }
         }
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        s = s == ST - 1 ? 0 : s + 1;
+        qa -= QT;
+        if (qa < q0) {
+            qa = last_tile;
+            ++head;
+        }
     }
     if constexpr (!LSEPASS) {
         float *out = a.out + (int64_t)(a.heads == 1 ? first_head : h) * a.out_sh + start;
@@ -285,12 +329,14 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     IQ_CHECK_ARG(s.lse + s.ml + s.part == 0 || (workspace && workspace_floats >= s.lse + s.ml + s.part),
                  "iq_prefill_weights: workspace too small");
     const int64_t tiles = (max_seqlen + KG - 1) / KG, G = Hq / H;
-    WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)max_seqlen, (int)H,
+    WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq, (int)max_seqlen, (int)H,
                  (int)Hq, (int)G, (int)(window ? G : 1), window ? window : max_seqlen, scale * LOG2E, lse, lse_sh, 0,
                  (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
-    const dim3 grid((unsigned)tiles, (unsigned)(Hq / a.heads), (unsigned)n_seq), block(NT);
+    const int64_t items = tiles * (Hq / a.heads) * n_seq;
+    IQ_CHECK_ARG(items <= 0xffffff, "iq_prefill_weights: too many key tiles");
+    const dim3 grid((unsigned)items), block(NT);
     if (window > 0 && !lse) {
         float *own = workspace + s.ml;
         hipLaunchKernelGGL((f16 ? prefill_weights<true, true> : prefill_weights<false, true>), grid, block, 0, st, a);
