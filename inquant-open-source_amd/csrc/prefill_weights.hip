@@ -121,6 +121,14 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     // wavefront, four (1 KB) per load, and its lse; rows past the end repeat
     // the last one.
     int next_head = first_head, next_qa = last_tile, next_st = 0;
+    const uint32_t row_bytes = (uint32_t)a.q_st * 2;
+    uint32_t slot[4], whole[4];              // a load's chunk in its row, and its offset where no row is past the end
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 16 * wave + 4 * i + (lane >> 4);
+        slot[i] = 16 * ((lane & 15) ^ (r & 15));
+        whole[i] = r * row_bytes + slot[i];
+    }
     auto load_tile = [&]() {
         const uint16_t *qt = a.q + (int64_t)(start + next_qa) * a.q_st + (int64_t)next_head * a.q_sh;
         const int last = len - 1 - next_qa;
@@ -131,10 +139,12 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r0 = 16 * wave + 4 * i, r = r0 + (lane >> 4), p = lane & 15;
-            const int rr = r < last ? r : last;
-            lds_load16(qt, (uint32_t)((rr * a.q_st + 8 * (p ^ (r & 15))) * 2),
-                       lds_q + (uint32_t)((next_st * QT + r0) * D * 2));
+            uint32_t off = whole[i];
+            if (last < QT - 1) {
+                const int r = 16 * wave + 4 * i + (lane >> 4);
+                off = (uint32_t)(r < last ? r : last) * row_bytes + slot[i];
+            }
+            lds_load16(qt, off, lds_q + (uint32_t)((next_st * QT + 16 * wave + 4 * i) * D * 2));
         }
         next_st = next_st == ST - 1 ? 0 : next_st + 1;
         next_qa -= QT;
@@ -171,12 +181,15 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
+                u32x4 qv[8];
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const u32x4 qv = *(const u32x4 *)(sq + 8 * ((2 * d + h32) ^ (c32 & 15)));
+                for (int d = 0; d < 8; ++d) qv[d] = *(const u32x4 *)(sq + 8 * ((2 * d + h32) ^ (c32 & 15)));
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv, sc[kb]);
-                }
+                for (int d = 0; d < 8; ++d)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv[d], sc[kb]);
+                __builtin_amdgcn_sched_barrier(0);
                 const int query = qa + 32 * b + c32;
                 if (qa + 32 * b < k0 + KW || k0 + KW > len) {
 #pragma unroll
