@@ -122,12 +122,11 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     // the last one.
     int next_head = first_head, next_qa = last_tile, next_st = 0;
     const uint32_t row_bytes = (uint32_t)a.q_st * 2;
-    uint32_t slot[4], whole[4];              // a load's chunk in its row, and its offset where no row is past the end
+    uint32_t whole[4];                       // a load's offset where no row is past the end
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = 16 * wave + 4 * i + (lane >> 4);
-        slot[i] = 16 * ((lane & 15) ^ (r & 15));
-        whole[i] = r * row_bytes + slot[i];
+        whole[i] = r * row_bytes + 16 * ((lane & 15) ^ (r & 15));
     }
     auto load_tile = [&]() {
         const uint16_t *qt = a.q + (int64_t)(start + next_qa) * a.q_st + (int64_t)next_head * a.q_sh;
@@ -142,7 +141,7 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
             uint32_t off = whole[i];
             if (last < QT - 1) {
                 const int r = 16 * wave + 4 * i + (lane >> 4);
-                off = (uint32_t)(r < last ? r : last) * row_bytes + slot[i];
+                off -= (uint32_t)(r > last ? r - last : 0) * row_bytes;
             }
             lds_load16(qt, off, lds_q + (uint32_t)((next_st * QT + 16 * wave + 4 * i) * D * 2));
         }
@@ -160,74 +159,100 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int d = 0; d < 8; ++d) asm volatile("" : "+v"(kf[kb][d]));
-    int s = 0, head = first_head, qa = last_tile;
-    for (int it = 0; it < total; ++it) {
-        // this tile's loads have landed (the next tile's may be under way), and
-        // after the barrier that holds for every wavefront, as does that the
-        // tile before has been read
-        if (it + 1 < total) {
-            if constexpr (LSEPASS) asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
-            else asm volatile("s_waitcnt vmcnt(5)\n\ts_barrier" ::: "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        }
-        if (it + 2 < total) load_tile();
-        if (k0 < len && k0 <= qa + QT - 1) {                // some query of this tile sees a key of this wavefront
+    // Operands of 32 queries (column 32 b + c32, channels 16 d + 8 h32 .. + 7)
+    // and their logits S^T (keys k0 + 32 kb + 8 (i / 4) + 4 h32 + i % 4).  Each
+    // operand is replaced by the next half tile's as soon as it was used.
+    u32x4 qv[8];
+    auto operand = [&](int st, int b, int d) {
+        return *(const u32x4 *)(sm.q[st] + (32 * b + c32) * D + 8 * ((2 * d + h32) ^ (c32 & 15)));
+    };
+    auto mask = [&](int query, f32x16 *sc) {
+        const int lim = (query < len ? query : len - 1) - k0 - 4 * h32;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const uint16_t *sq = sm.q[s] + (32 * b + c32) * D;
-                f32x16 sc[2];
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 32 * kb + 8 * (i >> 2) + (i & 3);
+                if (key > lim) sc[kb][i] = NEG_INF;          // the scale is positive
+            }
+    };
+    // logits whose weights are still to be added, and their query's lse
+    f32x16 late[2];
+    float late_lse2 = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) late[kb][i] = NEG_INF;
+    auto add_weight = [&](int kb, int i) {
+        sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(late[kb][i], a.c_log2, -late_lse2));
+    };
+    // The products of a half tile, in the lse pass alone, else beside the
+    // weights of the half before: the matrix cores and the VALU have about the
+    // same work here (16 products of 32 cycles; 32 exponentials of 8 and 64
+    // other instructions of 4), and the barriers hold the compiler to it.
+    auto products = [&](int st, int b, f32x16 *sc) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv[d], sc[kb]);
+            qv[d] = operand(st, b, d);
+            if constexpr (!LSEPASS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) add_weight(d >> 2, 4 * (d & 3) + e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if constexpr (!LSEPASS) asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));   // added here, not at the loop's end
+    };
+    int s = 0, head = first_head, qa = last_tile;
+    if (total > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LSEPASS ? 4 : 5) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < 8; ++d) qv[d] = operand(0, 0, d);
+    for (int it = 0; it < total; ++it) {
+        const int after = s == ST - 1 ? 0 : s + 1;
+        const bool live = k0 < len && k0 <= qa + QT - 1;    // some query of this tile sees a key of this wavefront
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            if (b == 1) {
+                // The second half's operands are in registers, so this tile has
+                // been read.  The next tile's loads have landed, and after the
+                // barrier both hold for every wavefront.
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (it + 2 < total) load_tile();
+            }
+            const int query = qa + 32 * b + c32;
+            f32x16 sc[2];
+            products(b ? after : s, 1 - b, sc);
+            if constexpr (!LSEPASS) {
+                // a query past the end weighs nothing
+                late_lse2 = query < len ? sm.lse[s][wave][32 * b + c32] * LOG2E : __builtin_inff();
+                if (qa + 32 * b < k0 + KW || k0 + KW > len) mask(query, sc);
+                late[0] = sc[0];
+                late[1] = sc[1];
+            } else if (live) {
+                if (qa + 32 * b < k0 + KW || k0 + KW > len) mask(query, sc);
+                float m = NEG_INF, l = 0.0f;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
-                u32x4 qv[8];
+                    for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i]);
+                m = pair_max(m * a.c_log2);
+                const float use = m == NEG_INF ? 0.0f : m;
 #pragma unroll
-                for (int d = 0; d < 8; ++d) qv[d] = *(const u32x4 *)(sq + 8 * ((2 * d + h32) ^ (c32 & 15)));
-                __builtin_amdgcn_sched_barrier(0);
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int d = 0; d < 8; ++d)
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv[d], sc[kb]);
-                __builtin_amdgcn_sched_barrier(0);
-                const int query = qa + 32 * b + c32;
-                if (qa + 32 * b < k0 + KW || k0 + KW > len) {
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h32 + (i & 3);
-                            if (key > query || key >= len) sc[kb][i] = NEG_INF;   // the scale is positive
-                        }
-                }
-                if constexpr (LSEPASS) {
-                    float m = NEG_INF, l = 0.0f;
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i]);
-                    m = pair_max(m * a.c_log2);
-                    const float use = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -use));
-                    l = pair_sum(l);
-                    if (h32 == 0 && query < len)
-                        a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] =
-                            f32x2{m, l};
-                } else {
-                    // a query past the end weighs nothing
-                    const float lse2 = query < len ? sm.lse[s][wave][32 * b + c32] * LOG2E : __builtin_inff();
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -lse2));
-                }
+                    for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -use));
+                l = pair_sum(l);
+                if (h32 == 0 && query < len)
+                    a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] = f32x2{m, l};
             }
         }
-        s = s == ST - 1 ? 0 : s + 1;
+        s = after;
         qa -= QT;
         if (qa < q0) {
             qa = last_tile;
@@ -235,6 +260,8 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         }
     }
     if constexpr (!LSEPASS) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) add_weight(i >> 4, i & 15);
         float *out = a.out + (int64_t)(a.heads == 1 ? first_head : h) * a.out_sh + start;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
