@@ -9,6 +9,8 @@
 // stream through LDS, so a key's sum over the queries is one fp32 add per
 // logit in the lane that holds it, and is added over the 32 lanes (queries of
 // a tile) once, at the end.
+#include <type_traits>
+
 #include "decode_common.h"
 
 namespace {
@@ -29,6 +31,7 @@ struct WeightArgs {
     int n_seq, max_len, H, Hq, G;              // a sequence's rows past max_len are left out
     int heads;                               // query heads a workgroup sums: 1, or G
     int64_t window;                          // queries of each sequence from its end (all: its length)
+    int chunk, chunks, tiles;                // a workgroup's queries at most, their ranges, and key tiles
     float c_log2;
     const float *lse;                        // natural log; token i of head hq at hq * lse_sh + i, or with
     int64_t lse_sh;                          // `windowed`, window row i at ((seq * Hq) + hq) * window + i
@@ -39,7 +42,7 @@ struct WeightArgs {
     int64_t out_sh;
 };
 
-// Three stages: a tile is computed while the next two land in the others.
+// Three stages: a tile is computed while the next two are on their way.
 constexpr int ST = 3;
 
 struct __attribute__((aligned(16))) WeightSmem {
@@ -89,16 +92,24 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     __shared__ WeightSmem sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c32 = lane & 31, h32 = lane >> 5;
-    // Key tiles from the first on: the first see the most queries, so the
-    // longest workgroups start first, over all sequences and heads.
-    const int lists = a.Hq / a.heads, per_tile = lists * a.n_seq;
-    const int tile = blockIdx.x / per_tile, rest = blockIdx.x - tile * per_tile;
-    const int seq = rest / lists, first_head = (rest - seq * lists) * a.heads, h = first_head / a.G;
+    // An item is a (query range, key tile, sequence, head); the ranges go from
+    // the last back and the key tiles from the first on, so the workgroups that
+    // start together read the same queries and the ranges' short last items
+    // (on the diagonal) come after their long ones.
+    const int lists = a.Hq / a.heads;
+    int rest = blockIdx.x / lists;
+    const int first_head = (blockIdx.x - rest * lists) * a.heads, h = first_head / a.G;
+    const int seq = rest % a.n_seq;
+    rest /= a.n_seq;
+    const int tile = rest % a.tiles, range = a.chunks - 1 - rest / a.tiles;
     const int start = a.cu[seq], len = length_of(a, seq);
-    const int g0 = tile * KG;
-    if (g0 >= len) return;                   // uniform
-    const int lo = (int64_t)len > a.window ? len - (int)a.window : 0;
-    const int q0 = lo > g0 ? lo : g0;        // the first query that sees one of these keys
+    const int g0 = tile * KG, from = range * a.chunk;
+    const int end = len - from < a.chunk ? len : from + a.chunk;             // queries before it
+    if (g0 >= end || from >= len) return;    // uniform
+    int q0 = (int64_t)len > a.window ? len - (int)a.window : 0;              // the window's first query
+    const int lo = q0;
+    q0 = q0 > g0 ? q0 : g0;                  // the first that sees one of these keys
+    q0 = q0 > from ? q0 : from;
     const int k0 = g0 + KW * wave;           // this wavefront's first key
     u32x4 kf[2][8];                          // A operand: key k0 + 32 kb + c32, channels 16 d + 8 h32 .. + 7
 #pragma unroll
@@ -113,14 +124,14 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[kb][i] = 0.0f;
-    const int last_tile = q0 + (len - q0 - 1) / QT * QT;    // a head's tiles go from its last query back, so that
-    const int total = ((len - q0 - 1) / QT + 1) * a.heads;  // workgroups that start together read the same queries
+    const int last_tile = q0 + (end - q0 - 1) / QT * QT;    // a head's tiles go from its last query back
+    const int total = ((end - q0 - 1) / QT + 1) * a.heads;
     const uint32_t lds_q = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&sm.q[0][0];
     const uint32_t lds_l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float *)&sm.lse[0][wave][0];
     // Direct loads of the next tile, and its place: sixteen of its rows per
     // wavefront, four (1 KB) per load, and its lse; rows past the end repeat
     // the last one.
-    int next_head = first_head, next_qa = last_tile, next_st = 0;
+    int next_head = first_head, next_qa = last_tile;
     const uint32_t row_bytes = (uint32_t)a.q_st * 2;
     uint32_t whole[4];                       // a load's offset where no row is past the end
 #pragma unroll
@@ -128,13 +139,13 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         const int r = 16 * wave + 4 * i + (lane >> 4);
         whole[i] = r * row_bytes + 16 * ((lane & 15) ^ (r & 15));
     }
-    auto load_tile = [&]() {
+    auto load_tile = [&](int st) {
         const uint16_t *qt = a.q + (int64_t)(start + next_qa) * a.q_st + (int64_t)next_head * a.q_sh;
-        const int last = len - 1 - next_qa;
+        const int last = end - 1 - next_qa;
         if constexpr (!LSEPASS) {
             const float *lt = a.lse + (a.windowed ? ((int64_t)seq * a.Hq + next_head) * a.window + (next_qa - lo)
                                                   : (int64_t)next_head * a.lse_sh + start + next_qa);
-            lds_load4(lt, (uint32_t)(lane < last ? lane : last) * 4, lds_l + (uint32_t)(next_st * NW * QT * 4));
+            lds_load4(lt, (uint32_t)(lane < last ? lane : last) * 4, lds_l + (uint32_t)(st * NW * QT * 4));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -143,17 +154,17 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
                 const int r = 16 * wave + 4 * i + (lane >> 4);
                 off -= (uint32_t)(r > last ? r - last : 0) * row_bytes;
             }
-            lds_load16(qt, off, lds_q + (uint32_t)((next_st * QT + 16 * wave + 4 * i) * D * 2));
+            lds_load16(qt, off, lds_q + (uint32_t)((st * QT + 16 * wave + 4 * i) * D * 2));
         }
-        next_st = next_st == ST - 1 ? 0 : next_st + 1;
         next_qa -= QT;
         if (next_qa < q0) {
             next_qa = last_tile;
             ++next_head;
         }
     };
-    load_tile();
-    if (total > 1) load_tile();
+    load_tile(0);
+    if (total > 1) load_tile(1);
+    if (total > 2) load_tile(2);
     // the keys are waited for here, not in the loop
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -165,16 +176,6 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     u32x4 qv[8];
     auto operand = [&](int st, int b, int d) {
         return *(const u32x4 *)(sm.q[st] + (32 * b + c32) * D + 8 * ((2 * d + h32) ^ (c32 & 15)));
-    };
-    auto mask = [&](int query, f32x16 *sc) {
-        const int lim = (query < len ? query : len - 1) - k0 - 4 * h32;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = 32 * kb + 8 * (i >> 2) + (i & 3);
-                if (key > lim) sc[kb][i] = NEG_INF;          // the scale is positive
-            }
     };
     // logits whose weights are still to be added, and their query's lse
     f32x16 late[2];
@@ -208,71 +209,111 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         }
         if constexpr (!LSEPASS) asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));   // added here, not at the loop's end
     };
-    int s = 0, head = first_head, qa = last_tile;
-    if (total > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LSEPASS ? 4 : 5) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-#pragma unroll
-    for (int d = 0; d < 8; ++d) qv[d] = operand(0, 0, d);
-    for (int it = 0; it < total; ++it) {
-        const int after = s == ST - 1 ? 0 : s + 1;
-        const bool live = k0 < len && k0 <= qa + QT - 1;    // some query of this tile sees a key of this wavefront
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            if (b == 1) {
-                // The second half's operands are in registers, so this tile has
-                // been read.  The next tile's loads have landed, and after the
-                // barrier both hold for every wavefront.
+    constexpr int LOADS = LSEPASS ? 4 : 5;   // of a tile, per wavefront
+    int head = first_head, qa = last_tile, it = 0;
+    // Half b of the tile in stage st, leaving the operands of the next half.
+    auto half = [&](auto st_, auto b_) {
+        constexpr int st = decltype(st_)::value, b = decltype(b_)::value;
+        const int query = qa + 32 * b + c32;
+        // a query past the end weighs nothing
+        float lse2 = 0.0f;
+        if constexpr (!LSEPASS) lse2 = query < end ? sm.lse[st][wave][32 * b + c32] * LOG2E : __builtin_inff();
+        if constexpr (b == 1) {
+            // This half's operands are in registers, so the tile has been read;
+            // the next tile's loads have landed; after the barrier both hold for
+            // every wavefront.
+            if (it + 2 < total)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
+            else
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (it + 2 < total) load_tile();
-            }
-            const int query = qa + 32 * b + c32;
-            f32x16 sc[2];
-            products(b ? after : s, 1 - b, sc);
-            if constexpr (!LSEPASS) {
-                // a query past the end weighs nothing
-                late_lse2 = query < len ? sm.lse[s][wave][32 * b + c32] * LOG2E : __builtin_inff();
-                if (qa + 32 * b < k0 + KW || k0 + KW > len) mask(query, sc);
-                late[0] = sc[0];
-                late[1] = sc[1];
-            } else if (live) {
-                if (qa + 32 * b < k0 + KW || k0 + KW > len) mask(query, sc);
-                float m = NEG_INF, l = 0.0f;
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i]);
-                m = pair_max(m * a.c_log2);
-                const float use = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -use));
-                l = pair_sum(l);
-                if (h32 == 0 && query < len)
-                    a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] = f32x2{m, l};
-            }
+            if (it + 3 < total) load_tile(st);
         }
-        s = after;
+        f32x16 sc[2];
+        products(b ? (st + 1) % ST : st, 1 - b, sc);
+        const bool masked = qa + 32 * b < k0 + KW || k0 + KW > len;          // uniform
+        const int lim = (query < len ? query : len - 1) - k0 - 4 * h32;      // the last key that the query sees
+        auto seen = [&](int kb, int i) { return 32 * kb + 8 * (i >> 2) + (i & 3) <= lim; };
+        if constexpr (!LSEPASS) {
+            late[0] = sc[0];
+            late[1] = sc[1];
+            late_lse2 = lse2;
+            if (masked) {
+                // added at once, the unseen left out (whatever their logit and lse), so that nothing is pending
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -lse2));
+                        sum[kb][i] += seen(kb, i) ? w : 0.0f;
+                        late[kb][i] = NEG_INF;
+                    }
+                late_lse2 = 0.0f;
+            }
+        } else if (k0 < len && k0 <= qa + QT - 1) {          // some query of this tile sees a key of this wavefront
+            if (masked) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[kb][i] = seen(kb, i) ? sc[kb][i] : NEG_INF;   // the scale is positive
+            }
+            float m = NEG_INF, l = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i]);
+            m = pair_max(m * a.c_log2);
+            const float use = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -use));
+            l = pair_sum(l);
+            if (h32 == 0 && query < end)
+                a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] = f32x2{m, l};
+        }
+    };
+    auto next = [&]() {
         qa -= QT;
         if (qa < q0) {
             qa = last_tile;
             ++head;
         }
+        return ++it < total;
+    };
+    if (total > 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < 8; ++d) qv[d] = operand(0, 0, d);
+    const std::integral_constant<int, 0> zero{};
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, 2> two{};
+    while (true) {
+        half(zero, zero);
+        half(zero, one);
+        if (!next()) break;
+        half(one, zero);
+        half(one, one);
+        if (!next()) break;
+        half(two, zero);
+        half(two, one);
+        if (!next()) break;
     }
     if constexpr (!LSEPASS) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) add_weight(i >> 4, i & 15);
-        float *out = a.out + (int64_t)(a.heads == 1 ? first_head : h) * a.out_sh + start;
+        float *out = a.out + ((int64_t)range * a.Hq + (a.heads == 1 ? first_head : h)) * a.out_sh + start;
+        // Sums over the 32 queries: a swap of the odd 16-lane rows of one key's
+        // lanes with the even ones of another's leaves both keys in one register
+        // (the first block's in the even rows, the second's in the odd).
+        const int kb = (lane >> 4) & 1;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float v = sum[kb][i];
-#pragma unroll
-                for (int d = 16; d; d >>= 1) v += __shfl_xor(v, d);
-                const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h32 + (i & 3);
-                if (c32 == 0 && key < len) out[key] = v;
-            }
+        for (int i = 0; i < 16; ++i) {
+            const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0][i]), __float_as_uint(sum[1][i]),
+                                                            false, false);
+            const float v = row_sum16(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+            const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h32 + (i & 3);
+            if ((lane & 15) == 0 && key < len) out[key] = v;
+        }
     }
 }
 
@@ -310,21 +351,33 @@ __global__ __launch_bounds__(1024) void window_lse(WeightArgs a, float *lse)
     lse[(int64_t)seq * rows + row] = (use + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// The query heads' sums of each KV head.
+// The sums of each KV head's query heads and of the query ranges that see a key.
 __global__ __launch_bounds__(256) void add_heads(WeightArgs a, const float *part, int64_t tokens, float *out,
                                                  int64_t out_sh)
 {
-    const int h = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= length_of(a, blockIdx.z)) return;
+    const int h = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x, len = length_of(a, blockIdx.z);
+    if (i >= len) return;
     const int64_t at = a.cu[blockIdx.z] + i;
     float v = 0.0f;
-    for (int g = 0; g < a.G; ++g) v += part[(int64_t)(h * a.G + g) * tokens + at];
+    for (int range = i / a.chunk; range <= (len - 1) / a.chunk; ++range)
+        for (int g = 0; g < a.G; ++g) v += part[((int64_t)range * a.Hq + h * a.G + g) * tokens + at];
     out[h * out_sh + at] = v;
 }
 
 struct Scratch {
     int64_t lse, ml, part;                   // floats of each
 };
+
+// Queries of a workgroup: 4096, or fewer while that leaves the 512 that run at
+// once without a second one (a multiple of the key tile, so that a range either
+// sees a whole key tile or ends before it).
+int64_t chunk_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen)
+{
+    int64_t chunk = 4096;
+    const int64_t tiles = (max_seqlen + KG - 1) / KG;
+    while (chunk > 512 && tiles * Hq * n_seq * ((max_seqlen + chunk - 1) / chunk) < 2048) chunk /= 2;
+    return chunk;
+}
 
 Scratch scratch_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t window, bool lse)
 {
@@ -333,7 +386,10 @@ Scratch scratch_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens
         s.lse = n_seq * Hq * window;
         s.ml = 2 * n_seq * ((max_seqlen + KW - 1) / KW) * Hq * window;
     }
-    if (window == 0) s.part = Hq * tokens;
+    if (window == 0) {
+        const int64_t chunk = chunk_of(Hq, n_seq, max_seqlen);
+        s.part = (max_seqlen + chunk - 1) / chunk * Hq * tokens;
+    }
     return s;
 }
 
@@ -369,12 +425,13 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     IQ_CHECK_ARG(s.lse + s.ml + s.part == 0 || (workspace && workspace_floats >= s.lse + s.ml + s.part),
                  "iq_prefill_weights: workspace too small");
     const int64_t tiles = (max_seqlen + KG - 1) / KG, G = Hq / H;
+    const int64_t chunk = window ? 1 << 30 : chunk_of(Hq, n_seq, max_seqlen), chunks = (max_seqlen + chunk - 1) / chunk;
     WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq, (int)max_seqlen, (int)H,
-                 (int)Hq, (int)G, (int)(window ? G : 1), window ? window : max_seqlen, scale * LOG2E, lse, lse_sh, 0,
+                 (int)Hq, (int)G, (int)(window ? G : 1), window ? window : max_seqlen, (int)chunk, (int)chunks, (int)tiles, scale * LOG2E, lse, lse_sh, 0,
                  (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
-    const int64_t items = tiles * (Hq / a.heads) * n_seq;
+    const int64_t items = chunks * tiles * (Hq / a.heads) * n_seq;
     IQ_CHECK_ARG(items <= 0xffffff, "iq_prefill_weights: too many key tiles");
     const dim3 grid((unsigned)items), block(NT);
     if (window > 0 && !lse) {

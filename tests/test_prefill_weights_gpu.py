@@ -107,6 +107,33 @@ def test_poisoned_neighbours_and_untouched_tokens():
             _close(out[:, a:b], total, slack, 350 * hq // h)
 
 
+@pytest.mark.parametrize("window", [None, 200])
+def test_a_nan_query_weighs_only_what_it_sees(window):
+    from inquant_vllm import prefill_attention, prefill_weights
+    hq, h, n, bad = 4, 2, 600, 500
+    q, k, v, cu = _case(9, [n], hq, h, torch.bfloat16)
+    q[bad, 1] = math.nan                                     # of KV head 0
+    lse = torch.empty((hq, n), device="cuda")
+    prefill_attention(q, k, v, cu, n, SCALE, lse=lse)
+    got = prefill_weights(q, k, cu, n, SCALE, lse=None if window else lse, window=window)
+    assert got[0, :bad + 1].isnan().all()
+    q[bad, 1] = 0
+    total, _, slack = _expected(q, k, [n], SCALE, window or 0)
+    _close(got[0, bad + 1:], total[0, bad + 1:], slack, 2 * n)
+    _close(got[1], total[1], slack, 2 * n)
+
+
+def test_weights_of_a_long_prompt():
+    # more queries than one workgroup takes, keys past the first range, over one KV head
+    from inquant_vllm import prefill_attention, prefill_weights
+    lengths, hq, h = [9001, 4096, 70], 2, 1
+    q, k, v, cu = _case(10, lengths, hq, h, torch.float16)
+    lse = torch.empty((hq, sum(lengths)), device="cuda")
+    prefill_attention(q, k, v, cu, 9001, SCALE, lse=lse)
+    total, _, slack = _expected(q, k, lengths, SCALE, 0)
+    _close(prefill_weights(q, k, cu, 9001, SCALE, lse=lse), total, slack, 9001 * 2)
+
+
 def test_weights_in_a_graph():
     from inquant_vllm import prefill_attention, prefill_weights
     q, k, v, cu = _case(8, [300, 70], 28, 4, torch.bfloat16)
