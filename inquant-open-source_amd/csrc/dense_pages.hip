@@ -74,8 +74,9 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 // The `budget` largest of a row of sort keys, ties to the lowest index, by one
 // workgroup: the key of rank `budget` from three radix passes (11, 11 and 10
 // bits, histograms in LDS), then ranks in index order from ballots.  The keys
-// of SEL_CHUNK indices stay in LDS; longer rows are read again in every pass.
-constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_PER = 32, SEL_CHUNK = SEL_NT * SEL_PER;
+// of SEL_CHUNK indices stay in LDS, each wavefront its own range of them;
+// longer rows are read again in every pass.
+constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_CHUNK = 32768;
 
 // Greater is better: NaN, then -inf .. +inf (both zeros alike), then the rows
 // that are always kept.
@@ -90,33 +91,26 @@ __device__ __forceinline__ uint32_t sort_key(float w, bool always)
 struct SelectSmem {
     uint32_t key[SEL_CHUNK];
     uint32_t hist[2048];
-    uint32_t counts[SEL_PER * SEL_WAVES];     // kept-for-sure | ties << 16 per (j, wave), then their exclusive sums
     uint32_t wave_sum[SEL_WAVES];
     uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
 };
 
-// Exclusive sum over the workgroup of one value per thread, and the total.
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t *wave_sum, uint32_t &total)
+// Inclusive sum over the wavefront: sums of 1, 2, 4, .. 16 lanes of a row by
+// row shifts, then a row's last lane broadcast to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t y = (uint32_t)__shfl_up((int)x, d);
-        if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) wave_sum[wave] = x;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < SEL_WAVES; ++w) {
-        const uint32_t s = wave_sum[w];
-        all += s;
-        before += w < wave ? s : 0;
-    }
-    total = all;
-    return before + x - v;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+
+__device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
+{
+    v += dpp_u<0x111, 0xf>(v);               // row_shr:1
+    v += dpp_u<0x112, 0xf>(v);
+    v += dpp_u<0x114, 0xf>(v);
+    v += dpp_u<0x118, 0xf>(v);
+    v += dpp_u<0x142, 0xa>(v);               // row_bcast:15 into rows 1 and 3
+    return v + dpp_u<0x143, 0xc>(v);         // row_bcast:31 into rows 2 and 3
 }
 
 // load(index) -> sort key, for index < len; emit(index, kept, rank): rank is
@@ -124,15 +118,22 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t *wave_s
 template <class Load, class Emit>
 __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int64_t budget, Load load, Emit emit)
 {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const bool one = len <= SEL_CHUNK;
-    // a thread reads only the keys it wrote: indices base + 1024 j + t
-    auto fill = [&](int64_t base, int n) {
-#pragma unroll 8
-        for (int i = t; i < n; i += SEL_NT) sm.key[i] = load(base + i);
+    // of a chunk of n keys this wavefront holds first .. stop - 1; a lane reads only the keys it wrote
+    int first = 0, stop = 0;
+    auto range_of = [&](int64_t base) {
+        const int n = (int)(len - base < SEL_CHUNK ? len - base : SEL_CHUNK);
+        // the same places in every chunk of a longer row: no wavefront overwrites what another still reads
+        const int per = one ? ((n + SEL_NT - 1) / SEL_NT) * 64 : SEL_CHUNK / SEL_WAVES;
+        first = wave * per < n ? wave * per : n;
+        stop = first + per < n ? first + per : n;
     };
-    auto chunk_of = [&](int64_t base) { return (int)(len - base < SEL_CHUNK ? len - base : SEL_CHUNK); };
-    if (one) fill(0, (int)len);
+    auto fill = [&](int64_t base) {
+        range_of(base);
+#pragma unroll 8
+        for (int i = first + lane; i < stop; i += 64) sm.key[i] = load(base + i);
+    };
     uint32_t prefix = 0, need = 0xffffffffu;     // len <= budget: every key is at least 0
     if (len > budget) {
         need = (uint32_t)budget;
@@ -144,10 +145,9 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
             sm.hist[t + SEL_NT] = 0;
             __syncthreads();
             for (int64_t base = 0; base < len; base += SEL_CHUNK) {
-                const int n = chunk_of(base);
-                if (!one) fill(base, n);
+                if (!one || pass == 0) fill(base);
 #pragma unroll 4
-                for (int i = t; i < n; i += SEL_NT) {
+                for (int i = first + lane; i < stop; i += 64) {
                     const uint32_t key = sm.key[i];
                     if ((key & above) == prefix) atomicAdd(&sm.hist[(key >> shift) & mask], 1u);
                 }
@@ -155,51 +155,59 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
             __syncthreads();
             // thread t takes the bins 2047 - 2 t and 2046 - 2 t: sums from the largest down
             const uint32_t hi = sm.hist[2047 - 2 * t], lo = sm.hist[2046 - 2 * t];
-            uint32_t total;
-            const uint32_t before = block_exclusive(hi + lo, sm.wave_sum, total);
+            const uint32_t upto = wave_inclusive(hi + lo);
+            if (lane == 63) sm.wave_sum[wave] = upto;
+            __syncthreads();
+            uint32_t before = upto - hi - lo;
+#pragma unroll
+            for (int w = 0; w < SEL_WAVES; ++w) before += w < wave ? sm.wave_sum[w] : 0;
             if (before < need && need <= before + hi + lo) {
-                const bool first = need <= before + hi;
-                sm.prefix = prefix | ((uint32_t)(first ? 2047 - 2 * t : 2046 - 2 * t) << shift);
-                sm.need = need - before - (first ? 0 : hi);
+                const bool top = need <= before + hi;
+                sm.prefix = prefix | ((uint32_t)(top ? 2047 - 2 * t : 2046 - 2 * t) << shift);
+                sm.need = need - before - (top ? 0 : hi);
             }
             __syncthreads();
             prefix = sm.prefix;
             need = sm.need;
         }
+    } else if (one) {
+        fill(0);
     }
     uint32_t sure0 = 0, ties0 = 0;               // kept for sure, and ties, in the chunks before
     for (int64_t base = 0; base < len; base += SEL_CHUNK) {
-        const int n = chunk_of(base), steps = (n + SEL_NT - 1) / SEL_NT;
-        if (!one) fill(base, n);
-        // counts per (step, wavefront): index order
-        for (int j = 0; j < steps; ++j) {
-            const int i = j * SEL_NT + t;
-            const uint32_t key = i < n ? sm.key[i] : 0;
-            const uint64_t sure = __builtin_amdgcn_ballot_w64(i < n && key > prefix);
-            const uint64_t ties = __builtin_amdgcn_ballot_w64(i < n && key == prefix);
-            if (lane == 0)
-                sm.counts[j * SEL_WAVES + wave] = (uint32_t)__popcll(sure) | (uint32_t)__popcll(ties) << 16;
+        if (!one) fill(base);
+        uint32_t ns = 0, nt = 0;                 // of this wavefront
+#pragma unroll 4
+        for (int i = first; i < stop; i += 64) {
+            const uint32_t key = i + lane < stop ? sm.key[i + lane] : 0;
+            ns += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < stop && key > prefix));
+            nt += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < stop && key == prefix));
+        }
+        if (lane == 0) sm.wave_sum[wave] = ns | nt << 16;    // at most 2048 each
+        __syncthreads();
+        ns = sure0;
+        nt = ties0;
+#pragma unroll
+        for (int w = 0; w < SEL_WAVES; ++w) {
+            const uint32_t c = sm.wave_sum[w];
+            sure0 += c & 0xffffu;
+            ties0 += c >> 16;
+            ns += w < wave ? c & 0xffffu : 0;
+            nt += w < wave ? c >> 16 : 0;
         }
         __syncthreads();
-        uint32_t total;
-        const uint32_t mine = t < steps * SEL_WAVES ? sm.counts[t] : 0;
-        const uint32_t before = block_exclusive(mine, sm.wave_sum, total);
-        if (t < steps * SEL_WAVES) sm.counts[t] = before;
-        __syncthreads();
-        for (int j = 0; j < steps; ++j) {
-            const int i = j * SEL_NT + t;
-            const uint32_t key = i < n ? sm.key[i] : 0;
-            const bool is_sure = i < n && key > prefix, is_tie = i < n && key == prefix;
+#pragma unroll 2
+        for (int i = first; i < stop; i += 64) {
+            const bool live = i + lane < stop;
+            const uint32_t key = live ? sm.key[i + lane] : 0;
+            const bool is_sure = live && key > prefix, is_tie = live && key == prefix;
             const uint64_t sure = __builtin_amdgcn_ballot_w64(is_sure), ties = __builtin_amdgcn_ballot_w64(is_tie);
             const uint64_t below = (1ull << lane) - 1;
-            const uint32_t c = sm.counts[j * SEL_WAVES + wave];
-            const uint32_t ns = sure0 + (c & 0xffffu) + (uint32_t)__popcll(sure & below);
-            const uint32_t nt = ties0 + (c >> 16) + (uint32_t)__popcll(ties & below);
-            if (i < n) emit(base + i, is_sure || (is_tie && nt < need), (int64_t)ns + (nt < need ? nt : need));
+            const uint32_t s = ns + (uint32_t)__popcll(sure & below), e = nt + (uint32_t)__popcll(ties & below);
+            if (live) emit(base + i + lane, is_sure || (is_tie && e < need), (int64_t)s + (e < need ? e : need));
+            ns += (uint32_t)__popcll(sure);
+            nt += (uint32_t)__popcll(ties);
         }
-        sure0 += total & 0xffffu;
-        ties0 += total >> 16;
-        __syncthreads();
     }
 }
 

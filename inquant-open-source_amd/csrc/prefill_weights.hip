@@ -375,7 +375,7 @@ int64_t chunk_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen)
 {
     int64_t chunk = 4096;
     const int64_t tiles = (max_seqlen + KG - 1) / KG;
-    while (chunk > 512 && tiles * Hq * n_seq * ((max_seqlen + chunk - 1) / chunk) < 2048) chunk /= 2;
+    while (chunk > 512 && tiles * Hq * n_seq * ((max_seqlen + chunk - 1) / chunk) < 1024) chunk /= 2;
     return chunk;
 }
 
