@@ -73,10 +73,11 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 
 // The `budget` largest of a row of sort keys, ties to the lowest index, by one
 // workgroup: the key of rank `budget` from three radix passes (11, 11 and 10
-// bits, histograms in LDS), then ranks in index order from ballots.  The keys
-// of SEL_CHUNK indices stay in LDS, each wavefront its own range of them;
-// longer rows are read again in every pass.
-constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_CHUNK = 32768;
+// bits, histograms in LDS), then ranks in index order from one sum over the
+// threads.  Keys are loaded in index order, pass through LDS once and stay in
+// registers: a thread holds up to SEL_PER consecutive ones of a chunk of
+// 32768.  Longer rows are read again in every pass.
+constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_PER = 32, SEL_CHUNK = SEL_NT * SEL_PER;
 
 // Greater is better: NaN, then -inf .. +inf (both zeros alike), then the rows
 // that are always kept.
@@ -89,9 +90,9 @@ __device__ __forceinline__ uint32_t sort_key(float w, bool always)
 }
 
 struct SelectSmem {
-    uint32_t key[SEL_CHUNK];
-    uint32_t hist[2048];
-    uint32_t wave_sum[SEL_WAVES];
+    uint32_t key[SEL_NT * (SEL_PER + 1)];     // a thread's keys, one word apart from the next thread's
+    uint32_t hist[2][2048];                   // odd lanes count apart from even ones: fewer meet at a bin
+    uint32_t wave_sum[SEL_WAVES], wave_ties[SEL_WAVES];
     uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
 };
 
@@ -120,20 +121,33 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
 {
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const bool one = len <= SEL_CHUNK;
-    // of a chunk of n keys this wavefront holds first .. stop - 1; a lane reads only the keys it wrote
-    int first = 0, stop = 0;
-    auto range_of = [&](int64_t base) {
-        const int n = (int)(len - base < SEL_CHUNK ? len - base : SEL_CHUNK);
-        // the same places in every chunk of a longer row: no wavefront overwrites what another still reads
-        const int per = one ? ((n + SEL_NT - 1) / SEL_NT) * 64 : SEL_CHUNK / SEL_WAVES;
-        first = wave * per < n ? wave * per : n;
-        stop = first + per < n ? first + per : n;
-    };
+    int log2k = 2;                               // a thread holds 4, 8, 16 or 32 keys of a chunk
+    while (log2k < 5 && len > (int64_t)SEL_NT << log2k) ++log2k;
+    const int K = 1 << log2k;
+    uint32_t key[SEL_PER];
+    int mine = 0;                                // of them, real ones
     auto fill = [&](int64_t base) {
-        range_of(base);
+        const int n = (int)(len - base < SEL_CHUNK ? len - base : SEL_CHUNK);
+        __syncthreads();                         // the keys before were read
 #pragma unroll 8
-        for (int i = first + lane; i < stop; i += 64) sm.key[i] = load(base + i);
+        for (int i = t; i < n; i += SEL_NT) sm.key[i + (i >> log2k)] = load(base + i);
+        __syncthreads();
+        mine = n - (t << log2k) < K ? n - (t << log2k) : K;
+#pragma unroll
+        for (int j = 0; j < SEL_PER; ++j)
+            if (j < K) key[j] = sm.key[t * (K + 1) + j];
     };
+    // f(j, key) for this thread's real keys, in groups of four
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < SEL_PER; j += 4)
+            if (j < K) {
+#pragma unroll
+                for (int e = j; e < j + 4; ++e)
+                    if (e < mine) f(e, key[e]);
+            }
+    };
+    if (one) fill(0);
     uint32_t prefix = 0, need = 0xffffffffu;     // len <= budget: every key is at least 0
     if (len > budget) {
         need = (uint32_t)budget;
@@ -141,20 +155,18 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t mask = pass == 2 ? 1023 : 2047;
             const uint32_t above = pass == 0 ? 0 : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-            sm.hist[t] = 0;
-            sm.hist[t + SEL_NT] = 0;
+            for (int i = t; i < 2 * 2048; i += SEL_NT) sm.hist[0][i] = 0;
             __syncthreads();
             for (int64_t base = 0; base < len; base += SEL_CHUNK) {
-                if (!one || pass == 0) fill(base);
-#pragma unroll 4
-                for (int i = first + lane; i < stop; i += 64) {
-                    const uint32_t key = sm.key[i];
-                    if ((key & above) == prefix) atomicAdd(&sm.hist[(key >> shift) & mask], 1u);
-                }
+                if (!one) fill(base);
+                each([&](int, uint32_t k) {
+                    if ((k & above) == prefix) atomicAdd(&sm.hist[lane & 1][(k >> shift) & mask], 1u);
+                });
             }
             __syncthreads();
             // thread t takes the bins 2047 - 2 t and 2046 - 2 t: sums from the largest down
-            const uint32_t hi = sm.hist[2047 - 2 * t], lo = sm.hist[2046 - 2 * t];
+            const uint32_t hi = sm.hist[0][2047 - 2 * t] + sm.hist[1][2047 - 2 * t];
+            const uint32_t lo = sm.hist[0][2046 - 2 * t] + sm.hist[1][2046 - 2 * t];
             const uint32_t upto = wave_inclusive(hi + lo);
             if (lane == 63) sm.wave_sum[wave] = upto;
             __syncthreads();
@@ -170,44 +182,38 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
             prefix = sm.prefix;
             need = sm.need;
         }
-    } else if (one) {
-        fill(0);
     }
     uint32_t sure0 = 0, ties0 = 0;               // kept for sure, and ties, in the chunks before
     for (int64_t base = 0; base < len; base += SEL_CHUNK) {
         if (!one) fill(base);
-        uint32_t ns = 0, nt = 0;                 // of this wavefront
-#pragma unroll 4
-        for (int i = first; i < stop; i += 64) {
-            const uint32_t key = i + lane < stop ? sm.key[i + lane] : 0;
-            ns += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < stop && key > prefix));
-            nt += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i + lane < stop && key == prefix));
+        uint32_t ns = 0, nt = 0;
+        each([&](int, uint32_t k) {
+            ns += k > prefix;
+            nt += k == prefix;
+        });
+        const uint32_t us = wave_inclusive(ns), ut = wave_inclusive(nt);
+        if (lane == 63) {
+            sm.wave_sum[wave] = us;
+            sm.wave_ties[wave] = ut;
         }
-        if (lane == 0) sm.wave_sum[wave] = ns | nt << 16;    // at most 2048 each
         __syncthreads();
-        ns = sure0;
-        nt = ties0;
+        uint32_t s = sure0 + us - ns, e = ties0 + ut - nt;
 #pragma unroll
         for (int w = 0; w < SEL_WAVES; ++w) {
-            const uint32_t c = sm.wave_sum[w];
-            sure0 += c & 0xffffu;
-            ties0 += c >> 16;
-            ns += w < wave ? c & 0xffffu : 0;
-            nt += w < wave ? c >> 16 : 0;
+            const uint32_t ws = sm.wave_sum[w], wt = sm.wave_ties[w];
+            sure0 += ws;
+            ties0 += wt;
+            s += w < wave ? ws : 0;
+            e += w < wave ? wt : 0;
         }
         __syncthreads();
-#pragma unroll 2
-        for (int i = first; i < stop; i += 64) {
-            const bool live = i + lane < stop;
-            const uint32_t key = live ? sm.key[i + lane] : 0;
-            const bool is_sure = live && key > prefix, is_tie = live && key == prefix;
-            const uint64_t sure = __builtin_amdgcn_ballot_w64(is_sure), ties = __builtin_amdgcn_ballot_w64(is_tie);
-            const uint64_t below = (1ull << lane) - 1;
-            const uint32_t s = ns + (uint32_t)__popcll(sure & below), e = nt + (uint32_t)__popcll(ties & below);
-            if (live) emit(base + i + lane, is_sure || (is_tie && e < need), (int64_t)s + (e < need ? e : need));
-            ns += (uint32_t)__popcll(sure);
-            nt += (uint32_t)__popcll(ties);
-        }
+        const int64_t at = base + ((int64_t)t << log2k);
+        each([&](int j, uint32_t k) {
+            const bool is_sure = k > prefix, is_tie = k == prefix;
+            emit(at + j, is_sure || (is_tie && e < need), (int64_t)s + (e < need ? e : need));
+            s += is_sure;
+            e += is_tie;
+        });
     }
 }
 
