@@ -80,20 +80,25 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_PER = 32, SEL_CHUNK = SEL_NT * SEL_PER;
 
 // Greater is better: NaN, then -inf .. +inf (both zeros alike), then the rows
-// that are always kept.
+// that are always kept.  0 is no row.
 __device__ __forceinline__ uint32_t sort_key(float w, bool always)
 {
-    if (always) return 0xffffffffu;
-    if (w != w) return 0;
     const uint32_t u = __float_as_uint(w + 0.0f);   // -0 + 0 = +0
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t key = w != w ? 1u : u & 0x80000000u ? ~u : u | 0x80000000u;
+    return always ? 0xffffffffu : key;
 }
 
+// Copies of the histogram, by lane, so that fewer lanes meet at a bin.
+constexpr int SEL_COPIES = 4;
+
 struct SelectSmem {
-    uint32_t key[SEL_NT * (SEL_PER + 1)];     // a thread's keys, one word apart from the next thread's
-    uint32_t hist[2][2048];                   // odd lanes count apart from even ones: fewer meet at a bin
+    union {
+        uint32_t key[SEL_NT * (SEL_PER + 1)];     // a thread's keys, one word apart from the next thread's
+        uint32_t wide[SEL_COPIES][2048];          // the histograms of a row whose keys are all in registers
+    };
+    uint32_t hist[2048];                          // the histogram of a longer row
     uint32_t wave_sum[SEL_WAVES], wave_ties[SEL_WAVES];
-    uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
+    uint32_t prefix, need;                        // threshold bits so far, entries still to take of those that match
 };
 
 // Inclusive sum over the wavefront: sums of 1, 2, 4, .. 16 lanes of a row by
@@ -117,65 +122,74 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
 // load(index) -> sort key, for index < len; emit(index, kept, rank): rank is
 // the number of kept indices below.
 template <class Load, class Emit>
-__device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int64_t budget, Load load, Emit emit)
+__device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uint32_t budget, Load load, Emit emit)
 {
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const bool one = len <= SEL_CHUNK;
-    int log2k = 2;                               // a thread holds 4, 8, 16 or 32 keys of a chunk
-    while (log2k < 5 && len > (int64_t)SEL_NT << log2k) ++log2k;
-    const int K = 1 << log2k;
+    uint32_t log2k = 2;                          // a thread holds 4, 8, 16 or 32 keys of a chunk
+    while (log2k < 5 && len > (uint32_t)SEL_NT << log2k) ++log2k;
+    const uint32_t K = 1u << log2k;
     uint32_t key[SEL_PER];
-    int mine = 0;                                // of them, real ones
-    auto fill = [&](int64_t base) {
-        const int n = (int)(len - base < SEL_CHUNK ? len - base : SEL_CHUNK);
+    auto fill = [&](uint32_t base) {
+        const uint32_t n = len - base < SEL_CHUNK ? len - base : SEL_CHUNK;
         __syncthreads();                         // the keys before were read
-#pragma unroll 8
-        for (int i = t; i < n; i += SEL_NT) sm.key[i + (i >> log2k)] = load(base + i);
+#pragma unroll 16
+        for (uint32_t i = t; i < n; i += SEL_NT) sm.key[i + (i >> log2k)] = load(base + i);
         __syncthreads();
-        mine = n - (t << log2k) < K ? n - (t << log2k) : K;
+        const uint32_t first = t << log2k;
 #pragma unroll
-        for (int j = 0; j < SEL_PER; ++j)
-            if (j < K) key[j] = sm.key[t * (K + 1) + j];
+        for (uint32_t j = 0; j < SEL_PER; ++j)
+            if (j < K) key[j] = first + j < n ? sm.key[t * (K + 1) + j] : 0;
     };
-    // f(j, key) for this thread's real keys, in groups of four
-    auto each = [&](auto f) {
+    auto each = [&](auto f) {                    // in groups of four
 #pragma unroll
-        for (int j = 0; j < SEL_PER; j += 4)
+        for (uint32_t j = 0; j < SEL_PER; j += 4)
             if (j < K) {
 #pragma unroll
-                for (int e = j; e < j + 4; ++e)
-                    if (e < mine) f(e, key[e]);
+                for (uint32_t e = j; e < j + 4; ++e) f(e, key[e]);
             }
     };
     if (one) fill(0);
-    uint32_t prefix = 0, need = 0xffffffffu;     // len <= budget: every key is at least 0
+    uint32_t prefix = 0, need = 0;               // len <= budget: every row's key is above 0
     if (len > budget) {
-        need = (uint32_t)budget;
+        need = budget;
+        uint32_t *hist = one ? sm.wide[0] : sm.hist;
+        const uint32_t copies = one ? SEL_COPIES : 1, copy = (lane & (copies - 1)) * 2048;
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t mask = pass == 2 ? 1023 : 2047;
             const uint32_t above = pass == 0 ? 0 : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-            for (int i = t; i < 2 * 2048; i += SEL_NT) sm.hist[0][i] = 0;
+            __syncthreads();                     // keys or counts before were read
+            for (uint32_t i = t; i < copies * 2048; i += SEL_NT) hist[i] = 0;
             __syncthreads();
-            for (int64_t base = 0; base < len; base += SEL_CHUNK) {
+            for (uint32_t base = 0; base < len; base += SEL_CHUNK) {
                 if (!one) fill(base);
-                each([&](int, uint32_t k) {
-                    if ((k & above) == prefix) atomicAdd(&sm.hist[lane & 1][(k >> shift) & mask], 1u);
-                });
+                // at least `budget` rows: what is no row only adds to the count below all of them
+                if (pass == 0)
+                    each([&](uint32_t, uint32_t k) {
+                        if (k) atomicAdd(&hist[copy + (k >> 21)], 1u);
+                    });
+                else
+                    each([&](uint32_t, uint32_t k) {
+                        if ((k & above) == prefix) atomicAdd(&hist[copy + ((k >> shift) & mask)], 1u);
+                    });
             }
             __syncthreads();
             // thread t takes the bins 2047 - 2 t and 2046 - 2 t: sums from the largest down
-            const uint32_t hi = sm.hist[0][2047 - 2 * t] + sm.hist[1][2047 - 2 * t];
-            const uint32_t lo = sm.hist[0][2046 - 2 * t] + sm.hist[1][2046 - 2 * t];
+            uint32_t hi = 0, lo = 0;
+            for (uint32_t c = 0; c < copies; ++c) {
+                hi += hist[c * 2048 + 2047 - 2 * t];
+                lo += hist[c * 2048 + 2046 - 2 * t];
+            }
             const uint32_t upto = wave_inclusive(hi + lo);
             if (lane == 63) sm.wave_sum[wave] = upto;
             __syncthreads();
             uint32_t before = upto - hi - lo;
 #pragma unroll
-            for (int w = 0; w < SEL_WAVES; ++w) before += w < wave ? sm.wave_sum[w] : 0;
+            for (uint32_t w = 0; w < SEL_WAVES; ++w) before += w < wave ? sm.wave_sum[w] : 0;
             if (before < need && need <= before + hi + lo) {
                 const bool top = need <= before + hi;
-                sm.prefix = prefix | ((uint32_t)(top ? 2047 - 2 * t : 2046 - 2 * t) << shift);
+                sm.prefix = prefix | ((top ? 2047 - 2 * t : 2046 - 2 * t) << shift);
                 sm.need = need - before - (top ? 0 : hi);
             }
             __syncthreads();
@@ -184,10 +198,10 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
         }
     }
     uint32_t sure0 = 0, ties0 = 0;               // kept for sure, and ties, in the chunks before
-    for (int64_t base = 0; base < len; base += SEL_CHUNK) {
+    for (uint32_t base = 0; base < len; base += SEL_CHUNK) {
         if (!one) fill(base);
         uint32_t ns = 0, nt = 0;
-        each([&](int, uint32_t k) {
+        each([&](uint32_t, uint32_t k) {
             ns += k > prefix;
             nt += k == prefix;
         });
@@ -199,7 +213,7 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
         __syncthreads();
         uint32_t s = sure0 + us - ns, e = ties0 + ut - nt;
 #pragma unroll
-        for (int w = 0; w < SEL_WAVES; ++w) {
+        for (uint32_t w = 0; w < SEL_WAVES; ++w) {
             const uint32_t ws = sm.wave_sum[w], wt = sm.wave_ties[w];
             sure0 += ws;
             ties0 += wt;
@@ -207,10 +221,10 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, int64_t len, int6
             e += w < wave ? wt : 0;
         }
         __syncthreads();
-        const int64_t at = base + ((int64_t)t << log2k);
-        each([&](int j, uint32_t k) {
+        const uint32_t at = base + (t << log2k);
+        each([&](uint32_t j, uint32_t k) {
             const bool is_sure = k > prefix, is_tie = k == prefix;
-            emit(at + j, is_sure || (is_tie && e < need), (int64_t)s + (e < need ? e : need));
+            if (k) emit(at + j, is_sure || (is_tie && e < need), s + (e < need ? e : need));
             s += is_sure;
             e += is_tie;
         });
@@ -232,13 +246,13 @@ __global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
     const int64_t t0 = a.cu[seq], len = a.cu[seq + 1] - t0;
     const float *w = a.weights + h * a.w_stride + t0;
     int32_t *keep = a.keep + ((int64_t)seq * gridDim.x + h) * a.budget;
-    const int64_t newest = len - a.recent;
+    const uint32_t rows = len > 0 ? (uint32_t)len : 0, sink = (uint32_t)a.sink, recent = (uint32_t)a.recent;
     select_largest(
-        sm, len, a.budget, [&](int64_t i) { return sort_key(w[i], i < a.sink || i >= newest); },
-        [&](int64_t i, bool kept, int64_t rank) {
+        sm, rows, (uint32_t)a.budget, [&](uint32_t i) { return sort_key(w[i], i < sink || i + recent >= rows); },
+        [&](uint32_t i, bool kept, uint32_t rank) {
             if (kept) keep[rank] = (int32_t)i;
         });
-    for (int64_t i = (len > 0 ? len : 0) + threadIdx.x; i < a.budget; i += SEL_NT) keep[i] = -1;
+    for (int64_t i = (int64_t)rows + threadIdx.x; i < a.budget; i += SEL_NT) keep[i] = -1;
 }
 
 // ---------------------------------------------------------------- eviction
@@ -266,21 +280,25 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     }
     const int64_t newest = (int64_t)a.seen[seq] - a.recent;
     int32_t *holes = list + 1, *behind = holes + a.most;
+    const int32_t *table = a.pool.tables + seq * a.pool.bt_stride;
+    const uint32_t budget = (uint32_t)a.budget;
     select_largest(
-        sm, len, a.budget,
-        [&](int64_t i) {
-            const int64_t page = dense_page(a.pool, seq, i);
-            if (page < 0) return 0u;
-            const int64_t o = (page * H + h) * B + (i & (B - 1));
+        sm, (uint32_t)len, budget,
+        [&](uint32_t i) {
+            // a row of an id outside the pool counts as NaN
+            const int32_t id = table[i >> a.pool.shift];
+            const bool ok = id >= 0 && id < a.pool.pages;
+            const int64_t o = ((int64_t)(ok ? id : 0) * H + h) * B + (i & (B - 1));
+            const float w = a.pool.weights[o];
             const int32_t p = a.pool.positions[o];
-            return sort_key(a.pool.weights[o], p < a.sink || p >= newest);
+            return ok ? sort_key(w, p < a.sink || p >= newest) : 1u;
         },
-        [&](int64_t i, bool kept, int64_t rank) {
-            if (i < a.budget) {
+        [&](uint32_t i, bool kept, uint32_t rank) {
+            if (i < budget) {
                 if (!kept) holes[i - rank] = (int32_t)i;
-                if (i == a.budget - 1) list[0] = (int32_t)(i + 1 - rank - (kept ? 1 : 0));
+                if (i == budget - 1) list[0] = (int32_t)(budget - rank - (kept ? 1 : 0));
             } else if (kept) {
-                behind[a.budget - 1 - rank] = (int32_t)i;
+                behind[budget - 1 - rank] = (int32_t)i;
             }
         });
 }
