@@ -74,10 +74,12 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 // The `budget` largest of a row of sort keys, ties to the lowest index, by one
 // workgroup: the key of rank `budget` from three radix passes (11, 11 and 10
 // bits, histograms in LDS), then ranks in index order from one sum over the
-// threads.  Keys are loaded in index order, pass through LDS once and stay in
-// registers: a thread holds up to SEL_PER consecutive ones of a chunk of
-// 32768.  Longer rows are read again in every pass.
-constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_PER = 32, SEL_CHUNK = SEL_NT * SEL_PER;
+// threads.  Keys are loaded in index order and pass through LDS; a thread then
+// holds up to 32 consecutive ones of a chunk of 32768 in registers, and what
+// it finds of them (in the threshold's bin, kept, tied) as masks of 32 bits,
+// so that only the first pass spends more than a compare and an add on a key.
+// Longer rows are read again in every pass.
+constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_CHUNK = SEL_NT * 32;
 
 // Greater is better: NaN, then -inf .. +inf (both zeros alike), then the rows
 // that are always kept.  0 is no row.
@@ -88,17 +90,11 @@ __device__ __forceinline__ uint32_t sort_key(float w, bool always)
     return always ? 0xffffffffu : key;
 }
 
-// Copies of the histogram, by lane, so that fewer lanes meet at a bin.
-constexpr int SEL_COPIES = 4;
-
 struct SelectSmem {
-    union {
-        uint32_t key[SEL_NT * (SEL_PER + 1)];     // a thread's keys, one word apart from the next thread's
-        uint32_t wide[SEL_COPIES][2048];          // the histograms of a row whose keys are all in registers
-    };
-    uint32_t hist[2048];                          // the histogram of a longer row
+    uint32_t key[SEL_NT * 33];                // a thread's keys, one word apart from the next thread's
+    uint32_t hist[2][2048];                   // odd lanes count apart from even ones: fewer meet at a bin
     uint32_t wave_sum[SEL_WAVES], wave_ties[SEL_WAVES];
-    uint32_t prefix, need;                        // threshold bits so far, entries still to take of those that match
+    uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
 };
 
 // Inclusive sum over the wavefront: sums of 1, 2, 4, .. 16 lanes of a row by
@@ -119,68 +115,75 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
     return v + dpp_u<0x143, 0xc>(v);         // row_bcast:31 into rows 2 and 3
 }
 
-// load(index) -> sort key, for index < len; emit(index, kept, rank): rank is
-// the number of kept indices below.
-template <class Load, class Emit>
+// load(index) -> sort key, for index < len; emit(index, rows, kept, rank): of
+// the 32 indices from `index` on, the mask of those that are rows and of those
+// that are kept, and the number of kept ones before.  K keys per thread and
+// chunk.
+template <int K, class Load, class Emit>
 __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uint32_t budget, Load load, Emit emit)
 {
+    constexpr uint32_t CHUNK = SEL_NT * K;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const bool one = len <= SEL_CHUNK;
-    uint32_t log2k = 2;                          // a thread holds 4, 8, 16 or 32 keys of a chunk
-    while (log2k < 5 && len > (uint32_t)SEL_NT << log2k) ++log2k;
-    const uint32_t K = 1u << log2k;
-    uint32_t key[SEL_PER];
+    const bool one = K < 32 || len <= CHUNK;   // only the longest form takes rows of several chunks
+    uint32_t *const mine = sm.key + t * (K + 1);
+    uint32_t key[K];
     auto fill = [&](uint32_t base) {
-        const uint32_t n = len - base < SEL_CHUNK ? len - base : SEL_CHUNK;
+        const uint32_t n = len - base < CHUNK ? len - base : CHUNK;
         __syncthreads();                         // the keys before were read
-#pragma unroll 16
-        for (uint32_t i = t; i < n; i += SEL_NT) sm.key[i + (i >> log2k)] = load(base + i);
-        __syncthreads();
-        const uint32_t first = t << log2k;
+#pragma unroll 1
+        for (int j0 = 0; j0 < K; j0 += 16) {
+            uint32_t v[K < 16 ? K : 16];
 #pragma unroll
-        for (uint32_t j = 0; j < SEL_PER; ++j)
-            if (j < K) key[j] = first + j < n ? sm.key[t * (K + 1) + j] : 0;
-    };
-    auto each = [&](auto f) {                    // in groups of four
-#pragma unroll
-        for (uint32_t j = 0; j < SEL_PER; j += 4)
-            if (j < K) {
-#pragma unroll
-                for (uint32_t e = j; e < j + 4; ++e) f(e, key[e]);
+            for (int j = j0; j < j0 + 16 && j < K; ++j) {
+                const uint32_t i = t + j * SEL_NT;
+                v[j - j0] = load(base + (i < n ? i : n - 1));
             }
+#pragma unroll
+            for (int j = j0; j < j0 + 16 && j < K; ++j) {
+                const uint32_t i = t + j * SEL_NT;
+                sm.key[i + i / K] = i < n ? v[j - j0] : 0;
+            }
+            __builtin_amdgcn_sched_barrier(0);   // sixteen in flight; more would spill
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < K; ++j) key[j] = mine[j];
     };
-    if (one) fill(0);
+    // mask of this thread's keys for which f holds: a compare and an add with its carry each
+    auto where = [&](auto f) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = K - 1; j >= 0; --j) m = m + m + (f(key[j]) ? 1u : 0u);
+        return m;
+    };
+    if (one && len) fill(0);
     uint32_t prefix = 0, need = 0;               // len <= budget: every row's key is above 0
     if (len > budget) {
         need = budget;
-        uint32_t *hist = one ? sm.wide[0] : sm.hist;
-        const uint32_t copies = one ? SEL_COPIES : 1, copy = (lane & (copies - 1)) * 2048;
+        uint32_t match = 0;
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t mask = pass == 2 ? 1023 : 2047;
             const uint32_t above = pass == 0 ? 0 : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-            __syncthreads();                     // keys or counts before were read
-            for (uint32_t i = t; i < copies * 2048; i += SEL_NT) hist[i] = 0;
+            sm.hist[0][t] = sm.hist[0][t + SEL_NT] = sm.hist[1][t] = sm.hist[1][t + SEL_NT] = 0;
             __syncthreads();
-            for (uint32_t base = 0; base < len; base += SEL_CHUNK) {
+            uint32_t *const hist = sm.hist[lane & 1];
+            for (uint32_t base = 0; base < len; base += CHUNK) {
                 if (!one) fill(base);
-                // at least `budget` rows: what is no row only adds to the count below all of them
-                if (pass == 0)
-                    each([&](uint32_t, uint32_t k) {
-                        if (k) atomicAdd(&hist[copy + (k >> 21)], 1u);
-                    });
-                else
-                    each([&](uint32_t, uint32_t k) {
-                        if ((k & above) == prefix) atomicAdd(&hist[copy + ((k >> shift) & mask)], 1u);
-                    });
+                if (pass == 0) {
+#pragma unroll
+                    for (int j = 0; j < K; ++j)
+                        if (key[j]) atomicAdd(&hist[key[j] >> 21], 1u);
+                } else {
+                    for (match = where([&](uint32_t k) { return k && (k & above) == prefix; }); match;
+                         match &= match - 1)
+                        atomicAdd(&hist[(mine[__builtin_ctz(match)] >> shift) & mask], 1u);
+                }
             }
             __syncthreads();
             // thread t takes the bins 2047 - 2 t and 2046 - 2 t: sums from the largest down
-            uint32_t hi = 0, lo = 0;
-            for (uint32_t c = 0; c < copies; ++c) {
-                hi += hist[c * 2048 + 2047 - 2 * t];
-                lo += hist[c * 2048 + 2046 - 2 * t];
-            }
+            const uint32_t hi = sm.hist[0][2047 - 2 * t] + sm.hist[1][2047 - 2 * t];
+            const uint32_t lo = sm.hist[0][2046 - 2 * t] + sm.hist[1][2046 - 2 * t];
             const uint32_t upto = wave_inclusive(hi + lo);
             if (lane == 63) sm.wave_sum[wave] = upto;
             __syncthreads();
@@ -198,13 +201,12 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
         }
     }
     uint32_t sure0 = 0, ties0 = 0;               // kept for sure, and ties, in the chunks before
-    for (uint32_t base = 0; base < len; base += SEL_CHUNK) {
+    for (uint32_t base = 0; base < len; base += CHUNK) {
         if (!one) fill(base);
-        uint32_t ns = 0, nt = 0;
-        each([&](uint32_t, uint32_t k) {
-            ns += k > prefix;
-            nt += k == prefix;
-        });
+        uint32_t kept = where([&](uint32_t k) { return k > prefix; });
+        uint32_t ties = where([&](uint32_t k) { return k == prefix; });
+        const uint32_t rows = where([](uint32_t k) { return k != 0; });
+        const uint32_t ns = (uint32_t)__popc(kept), nt = (uint32_t)__popc(ties);
         const uint32_t us = wave_inclusive(ns), ut = wave_inclusive(nt);
         if (lane == 63) {
             sm.wave_sum[wave] = us;
@@ -221,14 +223,25 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
             e += w < wave ? wt : 0;
         }
         __syncthreads();
-        const uint32_t at = base + (t << log2k);
-        each([&](uint32_t j, uint32_t k) {
-            const bool is_sure = k > prefix, is_tie = k == prefix;
-            if (k) emit(at + j, is_sure || (is_tie && e < need), s + (e < need ? e : need));
-            s += is_sure;
-            e += is_tie;
-        });
+        // of the ties the first `need` of the row are kept
+        uint32_t take = e < need ? need - e : 0;
+        if (take < nt) {
+            uint32_t rest = ties;
+            for (; take; --take) rest &= rest - 1;
+            ties &= ~rest;
+        }
+        emit(base + t * K, rows, kept | ties, s + (e < need ? e : need));
     }
+}
+
+// The same with as few keys per thread as the row needs.
+template <class Load, class Emit>
+__device__ __forceinline__ void select_rows_of(SelectSmem &sm, uint32_t len, uint32_t budget, Load load, Emit emit)
+{
+    if (len <= SEL_NT * 4) select_largest<4>(sm, len, budget, load, emit);
+    else if (len <= SEL_NT * 8) select_largest<8>(sm, len, budget, load, emit);
+    else if (len <= SEL_NT * 16) select_largest<16>(sm, len, budget, load, emit);
+    else select_largest<32>(sm, len, budget, load, emit);
 }
 
 struct SelectArgs {
@@ -247,10 +260,10 @@ __global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
     const float *w = a.weights + h * a.w_stride + t0;
     int32_t *keep = a.keep + ((int64_t)seq * gridDim.x + h) * a.budget;
     const uint32_t rows = len > 0 ? (uint32_t)len : 0, sink = (uint32_t)a.sink, recent = (uint32_t)a.recent;
-    select_largest(
-        sm, rows, (uint32_t)a.budget, [&](uint32_t i) { return sort_key(w[i], i < sink || i + recent >= rows); },
-        [&](uint32_t i, bool kept, uint32_t rank) {
-            if (kept) keep[rank] = (int32_t)i;
+    select_rows_of(
+        sm, rows, (uint32_t)a.budget, [&](uint32_t i) { return sort_key(ldg_at<float>(w, 4 * i), i < sink || i + recent >= rows); },
+        [&](uint32_t i, uint32_t, uint32_t kept, uint32_t rank) {
+            for (; kept; kept &= kept - 1) keep[rank++] = (int32_t)(i + __builtin_ctz(kept));
         });
     for (int64_t i = (int64_t)rows + threadIdx.x; i < a.budget; i += SEL_NT) keep[i] = -1;
 }
@@ -282,7 +295,7 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     int32_t *holes = list + 1, *behind = holes + a.most;
     const int32_t *table = a.pool.tables + seq * a.pool.bt_stride;
     const uint32_t budget = (uint32_t)a.budget;
-    select_largest(
+    select_rows_of(
         sm, (uint32_t)len, budget,
         [&](uint32_t i) {
             // a row of an id outside the pool counts as NaN
@@ -293,13 +306,15 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
             const int32_t p = a.pool.positions[o];
             return ok ? sort_key(w, p < a.sink || p >= newest) : 1u;
         },
-        [&](uint32_t i, bool kept, uint32_t rank) {
-            if (i < budget) {
-                if (!kept) holes[i - rank] = (int32_t)i;
-                if (i == budget - 1) list[0] = (int32_t)(budget - rank - (kept ? 1 : 0));
-            } else if (kept) {
-                behind[budget - 1 - rank] = (int32_t)i;
-            }
+        [&](uint32_t i, uint32_t rows, uint32_t kept, uint32_t rank) {
+            const uint32_t below = i >= budget ? 0 : budget - i >= 32 ? ~0u : (1u << (budget - i)) - 1;
+            // evicted places below the budget: as many before one as indices less kept ones
+            uint32_t hole = i - rank;
+            for (uint32_t m = rows & ~kept & below; m; m &= m - 1) holes[hole++] = (int32_t)(i + __builtin_ctz(m));
+            rank += (uint32_t)__popc(kept & below);
+            if (i < budget && budget - i <= 32 && (below & rows) >> (budget - 1 - i)) list[0] = (int32_t)(budget - rank);
+            for (uint32_t m = kept & ~below; m; m &= m - 1)
+                behind[budget - 1 - rank++] = (int32_t)(i + __builtin_ctz(m));
         });
 }
 
