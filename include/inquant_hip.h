@@ -441,7 +441,7 @@ int iq_prefill_weights(const void *q, const void *k, int dtype, int64_t q_st, in
  * 128] of bf16 or f16 (element strides of page, head and row, multiples of 8;
  * 16-byte aligned; row strides below 2^24), block_tokens in {16, 32, 64, 128,
  * 256}, and optionally (both or neither) weights f32 and positions i32
- * [pages, heads, block_tokens], contiguous: the attention weight each row has
+ * [pages, heads, block_tokens], contiguous and 16-byte aligned: the attention weight each row has
  * accumulated and its position in the sequence.  Cache row r of sequence s is
  * row r % block_tokens of pool page tables[s * bt_stride + r / block_tokens]
  * (i32; bt_cols entries).  Rows of an id outside the pool are neither read nor

@@ -60,7 +60,8 @@ inline int dense_pool(const char *who, const iq_dense_pages *pages, int dtype, c
     // the rows of a 64-token tile are addressed by 32-bit byte offsets
     IQ_CHECK_ARG(pages->k_st >= 0 && pages->v_st >= 0 && pages->k_st < (1LL << 24) && pages->v_st < (1LL << 24),
                  "%s: row stride too large", who);
-    IQ_CHECK_ARG((pages->weights == 0) == (pages->positions == 0), "%s: weights and positions go together", who);
+    IQ_CHECK_ARG((pages->weights == 0) == (pages->positions == 0) && (pages->weights | pages->positions) % 16 == 0,
+                 "%s: weights and positions go together, 16-byte aligned", who);
     IQ_CHECK_ARG(n_seq >= 0 && n_seq <= 65535, "%s: bad sequence count", who);
     IQ_CHECK_ARG(bt_cols >= 0 && bt_cols * B <= 0x7fffffffLL && (tables || n_seq == 0 || bt_cols == 0),
                  "%s: bad block tables", who);

@@ -74,9 +74,8 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 // The `budget` largest of a row of sort keys, ties to the lowest index, by one
 // workgroup: the key of rank `budget` from three radix passes (11, 11 and 10
 // bits, histograms in LDS), then ranks in index order from one sum over the
-// threads.  Keys are loaded in index order and pass through LDS; a thread then
-// holds up to 32 consecutive ones of a chunk of 32768 in registers, and what
-// it finds of them (in the threshold's bin, kept, tied) as masks of 32 bits,
+// threads.  A thread holds up to 32 consecutive keys of a chunk of 32768 in
+// registers (and in LDS, by number), and what it finds of them (in the threshold's bin, kept, tied) as masks of 32 bits,
 // so that only the first pass spends more than a compare and an add on a key.
 // Longer rows are read again in every pass.
 constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_CHUNK = SEL_NT * 32;
@@ -92,7 +91,7 @@ __device__ __forceinline__ uint32_t sort_key(float w, bool always)
 
 struct SelectSmem {
     uint32_t key[SEL_NT * 33];                // a thread's keys, one word apart from the next thread's
-    uint32_t hist[2][2048];                   // odd lanes count apart from even ones: fewer meet at a bin
+    uint32_t hist[2][2048 + 32];              // odd lanes count apart from even ones, on other banks
     uint32_t wave_sum[SEL_WAVES], wave_ties[SEL_WAVES];
     uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
 };
@@ -115,8 +114,8 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
     return v + dpp_u<0x143, 0xc>(v);         // row_bcast:31 into rows 2 and 3
 }
 
-// load(index) -> sort key, for index < len; emit(index, rows, kept, rank): of
-// the 32 indices from `index` on, the mask of those that are rows and of those
+// load(index, end) -> the sort keys of four indices, of which only those below
+// `end` count; emit(index, rows, kept, rank): of the 32 indices from `index` on, the mask of those that are rows and of those
 // that are kept, and the number of kept ones before.  K keys per thread and
 // chunk.
 template <int K, class Load, class Emit>
@@ -127,27 +126,18 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
     const bool one = K < 32 || len <= CHUNK;   // only the longest form takes rows of several chunks
     uint32_t *const mine = sm.key + t * (K + 1);
     uint32_t key[K];
+    uint32_t rows = 0;                           // mask of those that are rows
     auto fill = [&](uint32_t base) {
-        const uint32_t n = len - base < CHUNK ? len - base : CHUNK;
-        __syncthreads();                         // the keys before were read
-#pragma unroll 1
-        for (int j0 = 0; j0 < K; j0 += 16) {
-            uint32_t v[K < 16 ? K : 16];
+        const uint32_t n = len - base < CHUNK ? len - base : CHUNK, at = t * K;
+        rows = at >= n ? 0 : n - at >= K ? (uint32_t)((1ull << K) - 1) : (1u << (n - at)) - 1;
 #pragma unroll
-            for (int j = j0; j < j0 + 16 && j < K; ++j) {
-                const uint32_t i = t + j * SEL_NT;
-                v[j - j0] = load(base + (i < n ? i : n - 1));
-            }
+        for (int j = 0; j < K; j += 4) {
+            const u32x4 v = load(base + at + j, base + n);
 #pragma unroll
-            for (int j = j0; j < j0 + 16 && j < K; ++j) {
-                const uint32_t i = t + j * SEL_NT;
-                sm.key[i + i / K] = i < n ? v[j - j0] : 0;
-            }
-            __builtin_amdgcn_sched_barrier(0);   // sixteen in flight; more would spill
+            for (int e = 0; e < 4; ++e) key[j + e] = rows >> (j + e) & 1 ? v[e] : 0;
         }
-        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < K; ++j) key[j] = mine[j];
+        for (int j = 0; j < K; ++j) mine[j] = key[j];
     };
     // mask of this thread's keys for which f holds: a compare and an add with its carry each
     auto where = [&](auto f) {
@@ -205,7 +195,6 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
         if (!one) fill(base);
         uint32_t kept = where([&](uint32_t k) { return k > prefix; });
         uint32_t ties = where([&](uint32_t k) { return k == prefix; });
-        const uint32_t rows = where([](uint32_t k) { return k != 0; });
         const uint32_t ns = (uint32_t)__popc(kept), nt = (uint32_t)__popc(ties);
         const uint32_t us = wave_inclusive(ns), ut = wave_inclusive(nt);
         if (lane == 63) {
@@ -252,6 +241,19 @@ struct SelectArgs {
     int32_t *keep;
 };
 
+// Four floats from index i on, at a 4-byte alignment; those from `end` on are
+// not read.
+typedef float f32x4_unaligned __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ f32x4 load_four(const float *p, uint32_t i, uint32_t end)
+{
+    if (i + 4 <= end) return (f32x4)ldg_at<f32x4_unaligned>(p, 4 * i);
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e)
+        if (i + e < end) x[e] = ldg_at<float>(p, 4 * (i + e));
+    return x;
+}
+
 __global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
 {
     __shared__ SelectSmem sm;
@@ -261,7 +263,13 @@ __global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
     int32_t *keep = a.keep + ((int64_t)seq * gridDim.x + h) * a.budget;
     const uint32_t rows = len > 0 ? (uint32_t)len : 0, sink = (uint32_t)a.sink, recent = (uint32_t)a.recent;
     select_rows_of(
-        sm, rows, (uint32_t)a.budget, [&](uint32_t i) { return sort_key(ldg_at<float>(w, 4 * i), i < sink || i + recent >= rows); },
+        sm, rows, (uint32_t)a.budget, [&](uint32_t i, uint32_t end) {
+            u32x4 keys;
+            const f32x4 x = load_four(w, i, end);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) keys[e] = sort_key(x[e], i + e < sink || i + e + recent >= rows);
+            return keys;
+        },
         [&](uint32_t i, uint32_t, uint32_t kept, uint32_t rank) {
             for (; kept; kept &= kept - 1) keep[rank++] = (int32_t)(i + __builtin_ctz(kept));
         });
@@ -297,14 +305,17 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     const uint32_t budget = (uint32_t)a.budget;
     select_rows_of(
         sm, (uint32_t)len, budget,
-        [&](uint32_t i) {
-            // a row of an id outside the pool counts as NaN
-            const int32_t id = table[i >> a.pool.shift];
+        [&](uint32_t i, uint32_t end) {
+            // four rows of one page; a row of an id outside the pool counts as NaN
+            const int32_t id = table[i < end ? i >> a.pool.shift : 0];
             const bool ok = id >= 0 && id < a.pool.pages;
             const int64_t o = ((int64_t)(ok ? id : 0) * H + h) * B + (i & (B - 1));
-            const float w = a.pool.weights[o];
-            const int32_t p = a.pool.positions[o];
-            return ok ? sort_key(w, p < a.sink || p >= newest) : 1u;
+            const f32x4 w = ldg<f32x4>(a.pool.weights + o);
+            const i32x4 p = ldg<i32x4>(a.pool.positions + o);
+            u32x4 keys;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) keys[e] = ok ? sort_key(w[e], p[e] < a.sink || p[e] >= newest) : 1u;
+            return keys;
         },
         [&](uint32_t i, uint32_t rows, uint32_t kept, uint32_t rank) {
             const uint32_t below = i >= budget ? 0 : budget - i >= 32 ? ~0u : (1u << (budget - i)) - 1;

@@ -65,8 +65,8 @@ class DensePages:
             raise ValueError("Weights and positions go together")
         if self.weights is not None:
             for t, dtype in ((self.weights, torch.float32), (self.positions, torch.int32)):
-                if t.shape != key.shape[:3] or t.dtype != dtype or not t.is_contiguous():
-                    raise ValueError("Expected contiguous float32 weights and int32 positions "
+                if t.shape != key.shape[:3] or t.dtype != dtype or not t.is_contiguous() or t.data_ptr() % 16:
+                    raise ValueError("Expected contiguous, 16-byte aligned float32 weights and int32 positions "
                                      "[pages, kv_heads, block_size]")
         side = (self.weights, self.positions)
         if len({t.device for t in (key, value, *side) if t is not None}) != 1:

@@ -26,6 +26,7 @@ def test_pages_are_checked():
         (key, key[:1].expand(4, -1, -1, -1)),                                  # pages that are one page
         (torch.zeros((4, 2, 16, 129), dtype=torch.bfloat16)[..., 1:], key),     # rows off 16 bytes
         (key, key, w, None), (key, key, None, p), (key, key, w.double(), p), (key, key, w, p.long()),
+        (key, key, torch.zeros(4 * 2 * 16 + 1)[1:].view(4, 2, 16), p),         # weights off 16 bytes
         (key, key, w[:3], p), (key, key, w.transpose(0, 1).contiguous().transpose(0, 1), p),
     ]
     for args in bad:
