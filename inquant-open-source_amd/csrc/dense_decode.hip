@@ -43,6 +43,7 @@ struct __attribute__((aligned(16))) DecodeSmem {
         float o[NW][16][D + 4];
     };
     float m[NW][16], l[NW][16];
+    float lse[16];
 };
 
 // ds_read_b64_tr_b16: when lane s of 16 reads row K0 + s / 4, channels
@@ -55,7 +56,63 @@ __device__ __forceinline__ u32x2 tr_read(const uint16_t *p)
     return __builtin_bit_cast(u32x2, v);
 }
 
-template <bool F16>
+__device__ __forceinline__ float row_max16(float v)
+{
+    v = fmaxf(v, dpp_f<0xb1>(v));            // as row_sum16
+    v = fmaxf(v, dpp_f<0x4e>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    return fmaxf(v, dpp_f<0x140>(v));
+}
+
+// Adds the weights of cache rows r, r + NT, r + 2 NT and r + 3 NT (those below
+// `end`) of a KV head, from their logits and the heads' lse; neighbouring lanes
+// take neighbouring rows, which meet in one line.  load() asks for the logits of
+// the first four heads.
+struct FirstRows {
+    float s[4][4];
+
+    __device__ __forceinline__ static const float *logits(const DecodeArgs &a, int64_t q0, int g, int r)
+    {
+        return a.logits + (q0 + g) * a.l_stride + r;
+    }
+    __device__ __forceinline__ void load(const DecodeArgs &a, int64_t q0, int r, int end)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = r + i * NT < end ? r + i * NT : end - 1;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) s[g][i] = *logits(a, q0, g < a.G ? g : a.G - 1, at);
+        }
+    }
+    __device__ __forceinline__ void add(const DecodeArgs &a, const float *lse, int h, int seq, int64_t q0, int r, int end)
+    {
+        float w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (g < a.G) {
+                const float x = lse[g];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] += __builtin_amdgcn_exp2f(s[g][i] - x);
+            }
+        for (int g = 4; g < a.G; ++g) {
+            const float x = lse[g];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r + i * NT < end) w[i] += __builtin_amdgcn_exp2f(*logits(a, q0, g, r + i * NT) - x);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (r + i * NT >= end) break;
+            const int64_t page = dense_page(a.pool, seq, r + i * NT);
+            // added in memory, so that sequences that share a page lose no weight
+            if (page >= 0)
+                unsafeAtomicAdd(a.pool.weights + (page * a.pool.H + h) * a.pool.B + ((r + i * NT) & (a.pool.B - 1)), w[i]);
+        }
+    }
+};
+
+// DIRECT: the rows are one partition; the outputs and weights are final.
+template <bool F16, bool DIRECT>
 __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
 {
     __shared__ DecodeSmem sm;
@@ -64,7 +121,12 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
     const int h = blockIdx.x, part = blockIdx.y, seq = blockIdx.z;
     const int have = a.lengths[seq], len = have < a.max_tokens ? have : a.max_tokens;
     const int t0 = part * a.span;
-    if (t0 >= len) return;                   // uniform; the join does not read this partition
+    if (t0 >= len) {                         // uniform; the join does not read this partition
+        if constexpr (DIRECT)                // no row: nothing to attend to
+            for (int i = tid; i < D * a.G; i += NT)
+                iq_store_as(a.out, seq * a.o_ss + (h * a.G + (i >> 7)) * a.o_sh + (i & 127), 0.0f, a.odt);
+        return;
+    }
     const int end = t0 + a.span < len ? t0 + a.span : len;
     const DensePool &p = a.pool;
     u32x4 qb[4];                             // B operand: column c16 = query head, channels 32 d + 8 g4 .. + 7
@@ -193,9 +255,27 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
         }
-        const int64_t row = ((int64_t)seq * a.Hq + h * a.G + g) * a.parts + part;
-        *(f32x4 *)(a.part.o + row * D + c) = o;
-        if (c == 0) a.part.ml[row] = f32x2{M, L};
+        if constexpr (DIRECT) {
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            const int64_t at = seq * a.o_ss + (h * a.G + g) * a.o_sh + c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) iq_store_as(a.out, at + e, L == 0.0f ? 0.0f : o[e] * inv, a.odt);
+            if (c == 0) sm.lse[g] = L == 0.0f ? __builtin_inff() : use + __builtin_amdgcn_logf(L);
+        } else {
+            const int64_t row = ((int64_t)seq * a.Hq + h * a.G + g) * a.parts + part;
+            *(f32x4 *)(a.part.o + row * D + c) = o;
+            if (c == 0) a.part.ml[row] = f32x2{M, L};
+        }
+    }
+    if constexpr (DIRECT) {
+        if (!a.logits) return;
+        const int64_t q0 = (int64_t)seq * a.Hq + h * a.G;
+        __syncthreads();                     // the logits and lse of every wavefront
+        for (int r = tid; r < len; r += 4 * NT) {
+            FirstRows rows;
+            rows.load(a, q0, r, len);
+            rows.add(a, sm.lse, h, seq, q0, r, len);
+        }
     }
 }
 
@@ -221,6 +301,7 @@ __global__ __launch_bounds__(NT) void dense_join(DecodeArgs a, int n)
         const int grp = tid >> 5, c = 4 * (tid & 31);
         float M = NEG_INF, L = 0.0f;
         f32x4 o = {0, 0, 0, 0};
+#pragma unroll 2
         for (int p = grp; p < live; p += 8) {
             const f32x2 ml = a.part.ml[base + p];
             const f32x4 x = *(const f32x4 *)(a.part.o + (base + p) * D + c);
@@ -257,39 +338,27 @@ __global__ __launch_bounds__(NT) void dense_join(DecodeArgs a, int n)
     const int item = (int)blockIdx.x - rows, H = a.pool.H;
     const int chunk = item % chunks, h = item / chunks % H, seq = item / chunks / H;
     const int have = a.lengths[seq], len = have < a.max_tokens ? have : a.max_tokens;
-    if (chunk * JW >= len) return;
-    const int live = (len + a.span - 1) / a.span;
+    const int r0 = chunk * JW, r1 = r0 + JW < len ? r0 + JW : len;
+    if (r0 >= len) return;
+    const int live = (len + a.span - 1) / a.span, lane = tid & 63;
     const int64_t q0 = (int64_t)seq * a.Hq + h * a.G;
+    // the first rows' logits travel while the lse is made
+    FirstRows first;
+    first.load(a, q0, r0 + tid, r1);
     for (int g = tid >> 6; g < a.G; g += NW) {
         float M = NEG_INF, L = 0.0f;
-        for (int p = tid & 63; p < live; p += 64) M = fmaxf(M, a.part.ml[(q0 + g) * a.parts + p][0]);
-#pragma unroll
-        for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
-        const float use = M == NEG_INF ? 0.0f : M;
-        for (int p = tid & 63; p < live; p += 64) {
+        for (int p = lane; p < live; p += 64) {
             const f32x2 ml = a.part.ml[(q0 + g) * a.parts + p];
-            L = fmaf(__builtin_amdgcn_exp2f(ml[0] - use), ml[1], L);
+            const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
+            L = L * __builtin_amdgcn_exp2f(M - use) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - use);
+            M = m;
         }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) L += __shfl_xor(L, d);
-        if ((tid & 63) == 0) sm.lse[g] = L == 0.0f ? __builtin_inff() : use + __builtin_amdgcn_logf(L);
+        const float m = xmax16(row_max16(M)), use = m == NEG_INF ? 0.0f : m;
+        L = xsum16(row_sum16(L * __builtin_amdgcn_exp2f(M - use)));
+        if (lane == 0) sm.lse[g] = L == 0.0f ? __builtin_inff() : use + __builtin_amdgcn_logf(L);
     }
     __syncthreads();
-    const int r0 = chunk * JW + 4 * tid;
-    if (r0 >= len) return;
-    f32x4 w = {0, 0, 0, 0};
-    for (int g = 0; g < a.G; ++g) {
-        const f32x4 s = *(const f32x4 *)(a.logits + (q0 + g) * a.l_stride + r0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(s[e] - sm.lse[g]);
-    }
-    const int64_t page = dense_page(a.pool, seq, r0);
-    if (page < 0) return;
-    // added in memory, so that sequences that share a page lose no weight
-    float *at = a.pool.weights + (page * H + h) * a.pool.B + (r0 & (a.pool.B - 1));
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (r0 + e < len) unsafeAtomicAdd(at + e, w[e]);
+    first.add(a, sm.lse, h, seq, q0, r0 + tid, r1);
 }
 
 struct Split {
@@ -298,13 +367,19 @@ struct Split {
 
 Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t max_tokens, bool accumulate)
 {
-    const int64_t steps = (max_tokens + PT - 1) / PT;
-    const int64_t per = (n * H * steps + 2047) / 2048;
+    // Workgroups: a few rounds of the 512 that run at once.  Batches take more,
+    // shorter ones, as their lengths differ (16 sequences of 2K-32K tokens, 28
+    // heads over 4: 144 us with 1024 places, 121 with 2048, 114 with 4096, 120
+    // with 8192; two of 128K, 32 over 8: 244, 251, 257, 269 with the join).
+    // Rows that two workgroups would share are left to one, which saves the
+    // join (one sequence of 300 rows: 15 us in two launches).
+    const int64_t steps = max_tokens <= 2 * PT ? 1 : (max_tokens + PT - 1) / PT;
+    const int64_t target = n < 4 ? 1024 : 4096, per = (n * H * steps + target - 1) / target;
     Split s;
-    s.span = PT * (per > 0 ? per : 1);
-    s.parts = (max_tokens + s.span - 1) / s.span;
+    s.span = PT * (max_tokens <= 2 * PT ? 2 : per);
+    s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
     s.logits = accumulate ? (max_tokens + 63) / 64 * 64 : 0;
-    s.floats = n * Hq * (s.parts * (D + 2) + s.logits);
+    s.floats = n * Hq * ((s.parts > 1 ? s.parts * (D + 2) : 0) + s.logits);
     return s;
 }
 
@@ -342,12 +417,12 @@ extern "C" int iq_dense_decode(const void *q, int dtype, int64_t q_ss, int64_t q
                        (int32_t)s.parts, (int32_t)(Hq / pool.H), (int32_t)Hq, scale * LOG2E,
                        Partials{part, (f32x2 *)(part + n_seq * Hq * s.parts * D)},
                        accumulate ? workspace : nullptr, s.logits, out, o_ss, o_sh, out_dtype};
-    if (s.parts > 0) {
-        const dim3 grid((unsigned)pool.H, (unsigned)s.parts, (unsigned)n_seq);
-        if (dtype == IQ_F16) hipLaunchKernelGGL(dense_partials<true>, grid, dim3(NT), 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL(dense_partials<false>, grid, dim3(NT), 0, (hipStream_t)stream, a);
-    }
-    hipLaunchKernelGGL(dense_join, dim3((unsigned)joins), dim3(NT), 0, (hipStream_t)stream, a, (int)n_seq);
+    const bool f16 = dtype == IQ_F16, direct = s.parts == 1;
+    const dim3 grid((unsigned)pool.H, (unsigned)s.parts, (unsigned)n_seq);
+    const auto kernel = direct ? f16 ? dense_partials<true, true> : dense_partials<false, true>
+                               : f16 ? dense_partials<true, false> : dense_partials<false, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, (hipStream_t)stream, a);
+    if (!direct) hipLaunchKernelGGL(dense_join, dim3((unsigned)joins), dim3(NT), 0, (hipStream_t)stream, a, (int)n_seq);
     IQ_CHECK_LAUNCH("dense_decode");
     return IQ_OK;
 }
