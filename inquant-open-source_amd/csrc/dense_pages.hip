@@ -288,6 +288,10 @@ struct EvictArgs {
 
 // Chooses the rows of one (head, sequence) and lists the moves: the evicted
 // places below the budget in order, and the kept rows behind it from the last.
+// MOVE: and makes them, where they are few (16 sequences of 2049 rows, one to
+// move: 8 us, and 11 with a launch of its own for the move); then the new
+// lengths are another tensor than the lengths, which other heads still read.
+template <bool MOVE>
 __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
 {
     __shared__ SelectSmem sm;
@@ -295,6 +299,7 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     const int64_t have = a.lengths[seq];
     const int64_t len = have < a.max_tokens ? have : a.max_tokens;
     int32_t *list = a.moves + ((int64_t)seq * H + h) * (1 + 2 * a.most);
+    if (MOVE && h == 0 && threadIdx.x == 0) a.new_lengths[seq] = have < a.budget ? (int32_t)have : (int32_t)a.budget;
     if (len <= a.budget) {
         if (threadIdx.x == 0) list[0] = 0;
         return;
@@ -327,6 +332,12 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
             for (uint32_t m = kept & ~below; m; m &= m - 1)
                 behind[budget - 1 - rank++] = (int32_t)(i + __builtin_ctz(m));
         });
+    if constexpr (MOVE) {
+        __syncthreads();
+        const int n = list[0];
+        for (int m = threadIdx.x >> 4; m < n; m += SEL_NT / 16)
+            dense_move(a.pool, seq, h, behind[n - 1 - m], holes[m], threadIdx.x & 15);
+    }
 }
 
 // Moves the kept rows into the evicted places; sixteen lanes a row.  The new
@@ -420,11 +431,15 @@ extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int3
     if (n_seq == 0) return IQ_OK;
     const int64_t over = max_tokens > budget ? max_tokens - budget : 0, most = over < budget ? over : budget;
     const EvictArgs a{pool, lengths, seen, max_tokens, budget, sink, recent, most, new_lengths, workspace};
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)pool.H, (unsigned)n_seq), dim3(SEL_NT), 0,
-                       (hipStream_t)stream, a);
-    const int64_t groups = most > 0 ? (most + MV_ROWS - 1) / MV_ROWS : 1;
-    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)groups, (unsigned)(n_seq * pool.H)), dim3(256), 0,
-                       (hipStream_t)stream, a);
+    const dim3 rows((unsigned)pool.H, (unsigned)n_seq), block(SEL_NT);
+    if (most <= 2 * SEL_NT / 16 && (new_lengths + n_seq <= lengths || lengths + n_seq <= new_lengths)) {
+        hipLaunchKernelGGL(evict_select_kernel<true>, rows, block, 0, (hipStream_t)stream, a);
+    } else {
+        hipLaunchKernelGGL(evict_select_kernel<false>, rows, block, 0, (hipStream_t)stream, a);
+        const int64_t groups = most > 0 ? (most + MV_ROWS - 1) / MV_ROWS : 1;
+        hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)groups, (unsigned)(n_seq * pool.H)), dim3(256), 0,
+                           (hipStream_t)stream, a);
+    }
     IQ_CHECK_LAUNCH("dense_evict");
     return IQ_OK;
 }

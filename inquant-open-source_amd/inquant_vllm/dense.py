@@ -32,6 +32,7 @@ from inquant import _native as nat
 from .layout import BLOCK_SIZES
 
 _ROWS = (torch.bfloat16, torch.float16)
+_I32, _F32 = torch.int32, torch.float32
 
 
 def _strides(pages):
@@ -73,7 +74,11 @@ class DensePages:
             raise ValueError("all tensors must share one GPU")
         p = nat.DensePagesDesc(key.data_ptr(), value.data_ptr(), *(0 if t is None else t.data_ptr() for t in side),
                                *_strides(key), *_strides(value), *key.shape[:3])
-        object.__setattr__(self, "_desc", ctypes.byref(p))
+        # what every call asks for: the descriptor, its dtype code, the GPU, and the sizes
+        for name, value in (("_desc", ctypes.byref(p)), ("_dtype", key.dtype), ("_gpu", key.get_device()),
+                            ("_code", nat.dtype_code(key.dtype)), ("block_size", key.shape[2]),
+                            ("heads", key.shape[1])):
+            object.__setattr__(self, name, value)
 
     @classmethod
     def allocate(cls, pages, block_size, heads, dtype=torch.bfloat16, device="cuda", *, evictable=True):
@@ -85,53 +90,73 @@ class DensePages:
                    torch.empty((*shape, 128), dtype=dtype, device=device), *side)
 
     @property
-    def block_size(self):
-        return self.key.shape[2]
-
-    @property
-    def heads(self):
-        return self.key.shape[1]
-
-    @property
     def nbytes(self):
         """Bytes of the rows and of what stands beside them."""
         return sum(t.numel() * t.element_size() for t in (self.key, self.value, self.weights, self.positions)
                    if t is not None)
 
 
-def _call(device, entry, *args):
-    """entry(*args, stream) on the tensors' GPU."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        nat.check(entry(*args, nat.stream_handle(device)))
+def _on_gpu(gpu, what, *tensors):
+    """All tensors on one GPU: the index that the first (or ``gpu``) says.  The
+    common case costs one integer per tensor, any other takes require_gpu's errors."""
+    for t in tensors:
+        if t is not None and t.get_device() != gpu or gpu < 0:
+            nat.require_gpu(*tensors, what=what)
+            raise ValueError("all tensors must share one GPU")
+    return gpu
+
+
+_entries: dict = {}
+
+
+def _entry(name):
+    """A library function, looked up once."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(nat.lib(), name)
+    return fn
+
+
+def _call(gpu, name, *args):
+    """Calls the entry point on the current stream of a GPU, with that GPU current."""
+    stream = torch._C._cuda_getCurrentRawStream(gpu)
+    if gpu == torch._C._cuda_getDevice():
+        status = _entry(name)(*args, stream)
     else:
-        with torch.cuda.device(device):
-            nat.check(entry(*args, nat.stream_handle(device)))
+        with torch.cuda.device(gpu):
+            status = _entry(name)(*args, stream)
+    if status:
+        nat.check(status)
 
 
 def _ints(t, shape, what):
-    if tuple(t.shape) != shape or t.dtype != torch.int32:
+    if t.shape != shape or t.dtype is not _I32:
         raise ValueError(f"Expected int32 {what}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _cu(cu_seqlens):
-    if cu_seqlens.dtype != torch.int32 or cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2:
+    if cu_seqlens.dtype is not _I32 or cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2:
         raise ValueError("cu_seqlens must be an int32 [sequences + 1] tensor")
-    return cu_seqlens.contiguous()
+    return cu_seqlens if cu_seqlens.is_contiguous() else cu_seqlens.contiguous()
 
 
 def _tables(block_tables, n):
-    if block_tables.ndim != 2 or block_tables.shape[0] != n or block_tables.dtype != torch.int32 \
-            or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] != n or block_tables.dtype is not _I32 \
+            or (shape[1] > 1 and block_tables.stride(1) != 1):
         raise ValueError("Expected int32 block tables [sequences, pages per sequence]")
-    return block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1]
+    return block_tables.data_ptr(), block_tables.stride(0), shape[1]
 
 
 def _token_rows(t, what, heads=None):
-    if t.ndim != 3 or t.shape[-1] != 128 or (heads is not None and t.shape[1] != heads):
+    """Shape and strides of token-major rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != 128 or (heads is not None and shape[1] != heads):
         raise ValueError(f"Expected {what} [tokens, heads, 128]")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or t.data_ptr() % 16:
         raise ValueError(f"{what} rows must be contiguous and 16-byte aligned")
+    return shape, stride
 
 
 def _budget(budget, sink, recent):
@@ -152,32 +177,33 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
     [kv_heads, tokens], None: 0) and its position positions[i] + t
     (``positions`` int32 [sequences], None: ``start``).  Rows that a block table
     [sequences, pages per sequence] does not reach are left out."""
-    _token_rows(key, "key", pages.heads)
-    _token_rows(value, "value", pages.heads)
-    if key.shape != value.shape or key.dtype != pages.key.dtype or value.dtype != key.dtype:
+    heads = pages.heads
+    shape, ks = _token_rows(key, "key", heads)
+    vshape, vs = _token_rows(value, "value", heads)
+    if shape != vshape or key.dtype is not pages._dtype or value.dtype is not pages._dtype:
         raise ValueError("key and value must have one shape and the pages' dtype")
     cu = _cu(cu_seqlens)
-    n = cu.numel() - 1
+    n, tokens = cu.shape[0] - 1, shape[0]
     table = _tables(block_tables, n)
     if start is not None:
         start = _ints(start, (n,), "start rows [sequences]")
     if positions is not None:
         positions = _ints(positions, (n,), "positions [sequences]")
-    if weights is not None and (tuple(weights.shape) != (pages.heads, key.shape[0]) or weights.dtype != torch.float32
-                                or weights.stride(1) != 1 and weights.shape[1] > 1):
+    if weights is not None and (weights.shape != (heads, tokens) or weights.dtype is not _F32
+                                or weights.stride(1) != 1 and tokens > 1):
         raise ValueError("Expected float32 weights [kv_heads, tokens]")
     if keep is not None:
-        if keep.ndim != 3 or keep.shape[:2] != (n, pages.heads):
+        if keep.ndim != 3 or keep.shape[:2] != (n, heads):
             raise ValueError("Expected int32 kept rows [sequences, kv_heads, kept]")
-        keep = _ints(keep, tuple(keep.shape), "kept rows [sequences, kv_heads, kept]")
-    device = nat.require_gpu(key, value, cu, pages.key, block_tables, start, positions, weights, keep,
-                             what="write_rows")
-    if key.shape[0] == 0 or block_tables.shape[1] == 0:
+        keep = _ints(keep, keep.shape, "kept rows [sequences, kv_heads, kept]")
+    gpu = _on_gpu(pages._gpu, "write_rows", key, value, cu, block_tables, start, positions, weights, keep)
+    if tokens == 0 or table[2] == 0:
         return
-    _call(device, nat.lib().iq_dense_write, key.data_ptr(), value.data_ptr(), nat.dtype_code(key.dtype),
-          key.stride(0), key.stride(1), value.stride(0), value.stride(1), cu.data_ptr(), n, int(max_seqlen),
-          nat.ptr(start), nat.ptr(positions), nat.ptr(weights), 0 if weights is None else weights.stride(0),
-          nat.ptr(keep), 0 if keep is None else keep.shape[2], pages._desc, *table)
+    _call(gpu, "iq_dense_write", key.data_ptr(), value.data_ptr(), pages._code, ks[0], ks[1], vs[0], vs[1],
+          cu.data_ptr(), n, int(max_seqlen), None if start is None else start.data_ptr(),
+          None if positions is None else positions.data_ptr(), None if weights is None else weights.data_ptr(),
+          0 if weights is None else weights.stride(0), None if keep is None else keep.data_ptr(),
+          0 if keep is None else keep.shape[2], pages._desc, *table)
 
 
 def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, output=None):
@@ -189,20 +215,20 @@ def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, ou
     length."""
     budget, sink, recent = int(budget), int(sink), int(recent)
     _budget(budget, sink, recent)
-    if weights.ndim != 2 or weights.dtype != torch.float32 or weights.shape[0] < 1 \
+    if weights.ndim != 2 or weights.dtype is not _F32 or weights.shape[0] < 1 \
             or weights.stride(1) != 1 and weights.shape[1] > 1:
         raise ValueError("Expected float32 weights [kv_heads, tokens]")
     cu = _cu(cu_seqlens)
-    shape = (cu.numel() - 1, weights.shape[0], budget)
-    device = nat.require_gpu(weights, cu, output, what="select_rows")
+    n, (h, tokens) = cu.shape[0] - 1, weights.shape
+    gpu = _on_gpu(weights.get_device(), "select_rows", weights, cu, output)
     if output is None:
-        output = torch.empty(shape, dtype=torch.int32, device=device)
-    elif tuple(output.shape) != shape or output.dtype != torch.int32 or not output.is_contiguous():
+        output = torch.empty((n, h, budget), dtype=_I32, device=weights.device)
+    elif output.shape != (n, h, budget) or output.dtype is not _I32 or not output.is_contiguous():
         raise ValueError("output must be a contiguous int32 [sequences, kv_heads, budget] tensor")
-    if weights.shape[1] == 0:
+    if tokens == 0:
         return output.fill_(-1)
-    _call(device, nat.lib().iq_select_rows, weights.data_ptr(), weights.stride(0), weights.shape[0], cu.data_ptr(),
-          shape[0], int(max_seqlen), budget, sink, recent, output.data_ptr())
+    _call(gpu, "iq_select_rows", weights.data_ptr(), weights.stride(0), h, cu.data_ptr(), n, int(max_seqlen), budget,
+          sink, recent, output.data_ptr())
     return output
 
 
@@ -229,17 +255,18 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
     table = _tables(block_tables, n)
     if not 0 <= max_tokens <= table[2] * pages.block_size:
         raise ValueError("max_tokens must fit the block tables")
-    device = nat.require_gpu(lengths, seen, block_tables, pages.key, output, what="evict_rows")
+    gpu = _on_gpu(pages._gpu, "evict_rows", lengths, seen, block_tables, output)
     if output is None:
         output = torch.empty_like(lengths)
-    elif tuple(output.shape) != (n,) or output.dtype != torch.int32 or not output.is_contiguous():
+    elif output.shape != (n,) or output.dtype is not _I32 or not output.is_contiguous():
         raise ValueError("output must be a contiguous int32 [sequences] tensor")
     if n == 0:
         return output
-    need = nat.lib().iq_dense_evict_ints(pages.heads, n, max_tokens, budget)
-    scratch = torch.empty(need, dtype=torch.int32, device=device)
-    _call(device, nat.lib().iq_dense_evict, pages._desc, nat.dtype_code(pages.key.dtype), *table, lengths.data_ptr(),
-          seen.data_ptr(), n, max_tokens, budget, sink, recent, output.data_ptr(), scratch.data_ptr(), need)
+    # a count and two lists of the most moves that a head can need
+    need = n * pages.heads * (1 + 2 * max(0, min(budget, max_tokens - budget)))
+    scratch = torch.empty(need, dtype=_I32, device=lengths.device)
+    _call(gpu, "iq_dense_evict", pages._desc, pages._code, *table, lengths.data_ptr(), seen.data_ptr(), n, max_tokens,
+          budget, sink, recent, output.data_ptr(), scratch.data_ptr(), need)
     return output
 
 
@@ -255,10 +282,10 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     ``accumulate=True`` adds to each row's weight the softmax weights that the
     query heads of its KV head gave it (for a page that two sequences share,
     in an order that is not fixed)."""
-    hkv, n = pages.heads, query.shape[0]
-    if query.ndim != 3 or query.shape[-1] != 128 or query.dtype != pages.key.dtype:
+    shape, hkv, max_tokens = query.shape, pages.heads, int(max_tokens)
+    if len(shape) != 3 or shape[2] != 128 or query.dtype is not pages._dtype:
         raise ValueError("Expected a query [sequences, heads, 128] of the pages' dtype")
-    hq, max_tokens = query.shape[1], int(max_tokens)
+    n, hq = shape[0], shape[1]
     if hq < 1 or hq % hkv or hq // hkv > 16:
         raise ValueError("Expected 1..16 query heads per KV head")
     if accumulate and pages.weights is None:
@@ -269,21 +296,26 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
         raise ValueError("max_tokens must fit the block tables")
     if not math.isfinite(scale):
         raise ValueError("the scale must be finite")
-    device = nat.require_gpu(query, pages.key, block_tables, lengths, output, what="dense_decode")
-    if query.stride(2) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.data_ptr() % 16:
+    gpu = _on_gpu(pages._gpu, "dense_decode", query, block_tables, lengths, output)
+    qs = query.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
         query = query.contiguous()
+        qs = query.stride()
     if output is None:
-        output = torch.empty(query.shape, dtype=query.dtype, device=device)
-    elif output.shape != query.shape or output.stride(2) != 1 or output.dtype not in (query.dtype, torch.float32):
+        output = torch.empty(shape, dtype=query.dtype, device=query.device)
+        code = pages._code
+    elif output.shape != shape or output.stride(2) != 1 or output.dtype is not query.dtype and output.dtype is not _F32:
         raise ValueError("output must be [sequences, heads, 128] of the query dtype or float32")
+    else:
+        code = nat.IQ_F32 if output.dtype is _F32 else pages._code
     if n == 0:
         return output
-    need = nat.lib().iq_dense_workspace_floats(hq, hkv, n, max_tokens, bool(accumulate))
-    scratch = workspace.acquire((need,), device)
-    _call(device, nat.lib().iq_dense_decode, query.data_ptr(), nat.dtype_code(query.dtype), query.stride(0),
-          query.stride(1), hq, n, pages._desc, *table, lengths.data_ptr(), max_tokens, float(scale),
-          bool(accumulate), scratch.data_ptr(), need, output.data_ptr(), output.stride(0), output.stride(1),
-          nat.dtype_code(output.dtype))
+    accumulate = 1 if accumulate else 0
+    need = _entry("iq_dense_workspace_floats")(hq, hkv, n, max_tokens, accumulate)
+    scratch = workspace.acquire((need,), query.device)
+    _call(gpu, "iq_dense_decode", query.data_ptr(), pages._code, qs[0], qs[1], hq, n, pages._desc, *table,
+          lengths.data_ptr(), max_tokens, scale, accumulate, scratch.data_ptr(), need, output.data_ptr(),
+          output.stride(0), output.stride(1), code)
     return output
 
 
@@ -297,11 +329,10 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
     ``lse`` [Hq, tokens] ``prefill_attention(..., lse=...)`` wrote, or with
     ``window=w`` over the last w queries of each sequence (lse optional).
     Tokens of no sequence are not written."""
-    _token_rows(query, "query")
-    _token_rows(key, "key")
-    if query.shape[0] != key.shape[0] or query.dtype not in _ROWS or key.dtype != query.dtype:
+    (tokens, hq, _), qs = _token_rows(query, "query")
+    (rows, h, _), ks = _token_rows(key, "key")
+    if tokens != rows or query.dtype not in _ROWS or key.dtype is not query.dtype:
         raise ValueError("Expected BF16 or FP16 query and key of the same tokens")
-    tokens, hq, h = query.shape[0], query.shape[1], key.shape[1]
     if h < 1 or hq < 1 or hq % h:
         raise ValueError("query heads must be a multiple of KV heads")
     cu, max_seqlen = _cu(cu_seqlens), int(max_seqlen)
@@ -311,23 +342,20 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         raise ValueError("the window must hold at least one query")
     if window is None and lse is None:
         raise ValueError("Weights of all queries need the lse of prefill_attention")
-    if lse is not None and (tuple(lse.shape) != (hq, tokens) or lse.dtype != torch.float32
-                            or lse.stride(1) != 1 and tokens > 1):
+    if lse is not None and (lse.shape != (hq, tokens) or lse.dtype is not _F32 or lse.stride(1) != 1 and tokens > 1):
         raise ValueError("Expected a float32 lse [query heads, tokens]")
-    device = nat.require_gpu(query, key, cu, lse, output, what="prefill_weights")
+    gpu = _on_gpu(query.get_device(), "prefill_weights", query, key, cu, lse, output)
     if output is None:
-        output = torch.empty((h, tokens), dtype=torch.float32, device=device)
-    elif tuple(output.shape) != (h, tokens) or output.dtype != torch.float32 \
-            or output.stride(1) != 1 and tokens > 1:
+        output = torch.empty((h, tokens), dtype=_F32, device=query.device)
+    elif output.shape != (h, tokens) or output.dtype is not _F32 or output.stride(1) != 1 and tokens > 1:
         raise ValueError("output must be float32 [kv_heads, tokens]")
     if tokens == 0:
         return output
     window = 0 if window is None else min(int(window), max_seqlen)
-    n = cu.numel() - 1
-    need = nat.lib().iq_prefill_weights_floats(hq, n, max_seqlen, tokens, window, lse is not None)
-    scratch = torch.empty(need, dtype=torch.float32, device=device)
-    _call(device, nat.lib().iq_prefill_weights, query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype),
-          query.stride(0), query.stride(1), key.stride(0), key.stride(1), cu.data_ptr(), n, max_seqlen, tokens, hq, h,
-          window, float(scale), nat.ptr(lse), 0 if lse is None else lse.stride(0), scratch.data_ptr(), need,
-          output.data_ptr(), output.stride(0))
+    n = cu.shape[0] - 1
+    need = _entry("iq_prefill_weights_floats")(hq, n, max_seqlen, tokens, window, lse is not None)
+    scratch = torch.empty(need, dtype=_F32, device=query.device)
+    _call(gpu, "iq_prefill_weights", query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype), qs[0], qs[1], ks[0],
+          ks[1], cu.data_ptr(), n, max_seqlen, tokens, hq, h, window, scale, nat.ptr(lse),
+          0 if lse is None else lse.stride(0), scratch.data_ptr(), need, output.data_ptr(), output.stride(0))
     return output

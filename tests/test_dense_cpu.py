@@ -125,7 +125,7 @@ def test_refusals_of_the_library():
     for change in bad:
         assert decode(pages(**change)) == -1, change
     assert decode(pages(), hq=5) == -1 and decode(pages(), hq=34) == -1 and decode(pages(), most=33) == -1
-    assert decode(pages(), floats=10) == -1 and b"workspace" in lib.iq_last_error()
+    assert decode(pages(), floats=10, accumulate=1) == -1 and b"workspace" in lib.iq_last_error()
     assert decode(pages(), dtype=nat.IQ_F32) == -1
     assert decode(pages(weights=0, positions=0), accumulate=1) == -1
     evict = lambda p, budget=8, sink=0, ints=1 << 20: lib.iq_dense_evict(

@@ -370,8 +370,16 @@ def test_evict_rows_is_exact(case, kind):
             pages.positions[table[i, at // B].long(), h, at % B] = order
     exp = _copy(pages)
     _plain_evict(exp, table.cpu(), lengths, seen, budget, sink, recent)
+    first = [t.clone() for t in _fields(pages)]
     new = evict_rows(pages, table, i32(lengths), i32(seen), max(lengths), budget, sink=sink, recent=recent)
     assert new.tolist() == [min(n, budget) for n in lengths]
+    _same(pages, exp)
+    # the same with the new lengths in the place of the old ones
+    for t, start in zip(_fields(pages), first):
+        t.copy_(start)
+    held = i32(lengths)
+    assert evict_rows(pages, table, held, i32(seen), max(lengths), budget, sink=sink, recent=recent, output=held) is held
+    assert held.tolist() == new.tolist()
     _same(pages, exp)
 
 
