@@ -29,18 +29,28 @@ struct WeightArgs {
     int64_t q_st, q_sh, k_st, k_sh;          // element strides (token, head)
     const int32_t *cu;
     int n_seq, max_len, H, Hq, G;              // a sequence's rows past max_len are left out
-    int heads;                               // query heads a workgroup sums: 1, or G
-    int64_t window;                          // queries of each sequence from its end (all: its length)
+    int window;                              // WINDOW: queries of each sequence from its end
     int chunk, chunks, tiles;                // a workgroup's queries at most, their ranges, and key tiles
     float c_log2;
-    const float *lse;                        // natural log; token i of head hq at hq * lse_sh + i, or with
-    int64_t lse_sh;                          // `windowed`, window row i at ((seq * Hq) + hq) * window + i
-    int windowed;
-    f32x2 *ml;                               // the lse pass: (max, sum) per [seq, 64-key tile, Hq, window]
+    const float *lse;                        // natural log, token i of head hq at hq * lse_sh + i; with lse_sh 0
+    int64_t lse_sh;                          // window row r of (seq, h) at (seq * H + h) * G * window + r
+    f32x2 *ml;                               // the lse pass: (max, sum) per [seq, 64-key tile, H, window row]
     int tiles64;
-    float *out;                              // [H or Hq, out_sh]
+    float *out;                              // [H, out_sh]; all queries: [ranges, Hq, out_sh]
     int64_t out_sh;
 };
+
+// The last queries of a sequence, and the window's rows of a KV head: row
+// g n + i is query `lo` + i of its query head g.
+struct Window {
+    int lo, n, rows;
+};
+
+__device__ __forceinline__ Window window_of(const WeightArgs &a, int len)
+{
+    const int n = len < a.window ? len : a.window;
+    return {len - n, n, n * a.G};
+}
 
 // Three stages: a tile is computed while the next two are on their way.
 constexpr int ST = 3;
@@ -50,6 +60,21 @@ struct __attribute__((aligned(16))) WeightSmem {
     float lse[ST][NW][QT];                   // a copy per wavefront
 };
 static_assert(2 * sizeof(WeightSmem) <= 160 * 1024, "two workgroups per compute unit");
+
+// lds_load16 from an address of each lane's own
+__device__ __forceinline__ void lds_gather16(const void *p, uint32_t lds_base)
+{
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"((uint64_t)(uintptr_t)p),
+                 "s"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+}
+
+__device__ __forceinline__ void lds_gather4(const void *p, uint32_t lds_base)
+{
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"((uint64_t)(uintptr_t)p),
+                 "s"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+}
 
 // lds_load16 with four bytes per lane
 __device__ __forceinline__ void lds_load4(const void *base, uint32_t voff, uint32_t lds_base)
@@ -80,15 +105,29 @@ __device__ __forceinline__ int length_of(const WeightArgs &a, int seq)
     return len < a.max_len ? len : a.max_len;
 }
 
-__device__ __forceinline__ float pair_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+// over the lane pair l, l ^ 32 (one query's two halves)
+__device__ __forceinline__ float pair_max(float v)
+{
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+}
 
-__device__ __forceinline__ float pair_sum(float v) { return v + __shfl_xor(v, 32); }
+__device__ __forceinline__ float pair_sum(float v)
+{
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
 
-// LSEPASS: (max, sum) of every window query over this workgroup's keys, per
-// wavefront; else the keys' sums of exp(logit - lse).
-template <bool F16, bool LSEPASS>
+enum Pass { ALL, WINDOW, WINDOW_LSE };
+
+// ALL: the keys' sums over the queries of one query head and range; WINDOW:
+// over the rows of the window (packed: the query heads of a KV head follow each
+// other, so that small windows fill the tiles); WINDOW_LSE: (max, sum) of every
+// window row over this workgroup's keys, per wavefront.
+template <bool F16, Pass PASS>
 __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
 {
+    constexpr bool LSEPASS = PASS == WINDOW_LSE, ROWS = PASS != ALL;
     __shared__ WeightSmem sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c32 = lane & 31, h32 = lane >> 5;
@@ -96,20 +135,19 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     // the last back and the key tiles from the first on, so the workgroups that
     // start together read the same queries and the ranges' short last items
     // (on the diagonal) come after their long ones.
-    const int lists = a.Hq / a.heads;
+    const int lists = ROWS ? a.H : a.Hq;
     int rest = blockIdx.x / lists;
-    const int first_head = (blockIdx.x - rest * lists) * a.heads, h = first_head / a.G;
+    const int list = blockIdx.x - rest * lists, h = ROWS ? list : list / a.G;
     const int seq = rest % a.n_seq;
     rest /= a.n_seq;
-    const int tile = rest % a.tiles, range = a.chunks - 1 - rest / a.tiles;
+    const int tile = rest % a.tiles, range = ROWS ? 0 : a.chunks - 1 - rest / a.tiles;
     const int start = a.cu[seq], len = length_of(a, seq);
     const int g0 = tile * KG, from = range * a.chunk;
-    const int end = len - from < a.chunk ? len : from + a.chunk;             // queries before it
-    if (g0 >= end || from >= len) return;    // uniform
-    int q0 = (int64_t)len > a.window ? len - (int)a.window : 0;              // the window's first query
-    const int lo = q0;
-    q0 = q0 > g0 ? q0 : g0;                  // the first that sees one of these keys
-    q0 = q0 > from ? q0 : from;
+    // "queries" are query positions, or with ROWS rows of the window
+    const Window win = window_of(a, len);
+    const int end = ROWS ? win.rows : len - from < a.chunk ? len : from + a.chunk;
+    if (g0 >= (ROWS ? len : end) || from >= len) return;     // uniform
+    const int q0 = ROWS ? 0 : g0 > from ? g0 : from;         // the first that sees one of these keys
     const int k0 = g0 + KW * wave;           // this wavefront's first key
     u32x4 kf[2][8];                          // A operand: key k0 + 32 kb + c32, channels 16 d + 8 h32 .. + 7
 #pragma unroll
@@ -124,14 +162,14 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum[kb][i] = 0.0f;
-    const int last_tile = q0 + (end - q0 - 1) / QT * QT;    // a head's tiles go from its last query back
-    const int total = ((end - q0 - 1) / QT + 1) * a.heads;
+    const int total = (end - q0 - 1) / QT + 1;
+    const int last_tile = q0 + (total - 1) * QT;            // the tiles go from the last back
     const uint32_t lds_q = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&sm.q[0][0];
     const uint32_t lds_l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) float *)&sm.lse[0][wave][0];
     // Direct loads of the next tile, and its place: sixteen of its rows per
     // wavefront, four (1 KB) per load, and its lse; rows past the end repeat
     // the last one.
-    int next_head = first_head, next_qa = last_tile;
+    int next_qa = last_tile;
     const uint32_t row_bytes = (uint32_t)a.q_st * 2;
     uint32_t whole[4];                       // a load's offset where no row is past the end
 #pragma unroll
@@ -139,28 +177,45 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         const int r = 16 * wave + 4 * i + (lane >> 4);
         whole[i] = r * row_bytes + 16 * ((lane & 15) ^ (r & 15));
     }
+    const float *own_lse = a.lse + (int64_t)(seq * a.H + h) * a.G * a.window;
     auto load_tile = [&](int st) {
-        const uint16_t *qt = a.q + (int64_t)(start + next_qa) * a.q_st + (int64_t)next_head * a.q_sh;
         const int last = end - 1 - next_qa;
-        if constexpr (!LSEPASS) {
-            const float *lt = a.lse + (a.windowed ? ((int64_t)seq * a.Hq + next_head) * a.window + (next_qa - lo)
-                                                  : (int64_t)next_head * a.lse_sh + start + next_qa);
-            lds_load4(lt, (uint32_t)(lane < last ? lane : last) * 4, lds_l + (uint32_t)(st * NW * QT * 4));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t off = whole[i];
-            if (last < QT - 1) {
-                const int r = 16 * wave + 4 * i + (lane >> 4);
-                off -= (uint32_t)(r > last ? r - last : 0) * row_bytes;
+        const uint32_t to_l = lds_l + (uint32_t)(st * NW * QT * 4);
+        if constexpr (ROWS) {
+            // head and query of the tile's row r
+            auto place = [&](int r, int &head, int &i) {
+                const int row = next_qa + (r < last ? r : last), g = row / win.n;
+                i = row - g * win.n;
+                head = h * a.G + g;
+                return row;
+            };
+            int head, i;
+            if constexpr (!LSEPASS) {
+                const int row = place(lane, head, i);
+                lds_gather4(a.lse_sh ? a.lse + head * a.lse_sh + start + win.lo + i : own_lse + row, to_l);
             }
-            lds_load16(qt, off, lds_q + (uint32_t)((st * QT + 16 * wave + 4 * i) * D * 2));
+#pragma unroll
+            for (int l = 0; l < 4; ++l) {
+                const int r = 16 * wave + 4 * l + (lane >> 4);
+                place(r, head, i);
+                const uint16_t *qp = a.q + (int64_t)(start + win.lo + i) * a.q_st + (int64_t)head * a.q_sh;
+                lds_gather16(qp + 8 * ((lane & 15) ^ (r & 15)),
+                             lds_q + (uint32_t)((st * QT + 16 * wave + 4 * l) * D * 2));
+            }
+        } else {
+            const uint16_t *qt = a.q + (int64_t)(start + next_qa) * a.q_st + (int64_t)list * a.q_sh;
+            lds_load4(a.lse + (int64_t)list * a.lse_sh + start + next_qa, (uint32_t)(lane < last ? lane : last) * 4, to_l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t off = whole[i];
+                if (last < QT - 1) {
+                    const int r = 16 * wave + 4 * i + (lane >> 4);
+                    off -= (uint32_t)(r > last ? r - last : 0) * row_bytes;
+                }
+                lds_load16(qt, off, lds_q + (uint32_t)((st * QT + 16 * wave + 4 * i) * D * 2));
+            }
         }
         next_qa -= QT;
-        if (next_qa < q0) {
-            next_qa = last_tile;
-            ++next_head;
-        }
     };
     load_tile(0);
     if (total > 1) load_tile(1);
@@ -177,20 +232,49 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     auto operand = [&](int st, int b, int d) {
         return *(const u32x4 *)(sm.q[st] + (32 * b + c32) * D + 8 * ((2 * d + h32) ^ (c32 & 15)));
     };
-    // logits whose weights are still to be added, and their query's lse
+    // Logits that are still to be worked off, of the half tile before: their
+    // query's lse, or the row whose (max, sum) they give.
     f32x16 late[2];
     float late_lse2 = 0.0f;
+    int late_row = -1;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) late[kb][i] = NEG_INF;
-    auto add_weight = [&](int kb, int i) {
-        sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(late[kb][i], a.c_log2, -late_lse2));
+    float m = 0.0f, use = 0.0f, l = 0.0f;
+    // Four of a lane's 32 logits, in step d of 8.
+    auto work_off = [&](int d) {
+        if constexpr (LSEPASS) {
+            if (d == 0) {
+                m = NEG_INF;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) m = fmaxf(m, late[kb][i]);
+                m = pair_max(m * a.c_log2);
+                use = m == NEG_INF ? 0.0f : m;
+                l = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                l += __builtin_amdgcn_exp2f(fmaf(late[d >> 2][4 * (d & 3) + e], a.c_log2, -use));
+            if (d == 7) {
+                l = pair_sum(l);
+                if (h32 == 0 && late_row >= 0)
+                    a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.H + h) * a.G * a.window + late_row] = f32x2{m, l};
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int kb = d >> 2, i = 4 * (d & 3) + e;
+                sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(late[kb][i], a.c_log2, -late_lse2));
+            }
+        }
     };
-    // The products of a half tile, in the lse pass alone, else beside the
-    // weights of the half before: the matrix cores and the VALU have about the
-    // same work here (16 products of 32 cycles; 32 exponentials of 8 and 64
-    // other instructions of 4), and the barriers hold the compiler to it.
+    // The products of a half tile beside what the half before leaves to do: the
+    // matrix cores and the VALU have about the same work here (16 products of 32
+    // cycles; 32 exponentials of 8 and 64 other instructions of 4), and the
+    // barriers hold the compiler to it.
     auto products = [&](int st, int b, f32x16 *sc) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -201,16 +285,13 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv[d], sc[kb]);
             qv[d] = operand(st, b, d);
-            if constexpr (!LSEPASS) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) add_weight(d >> 2, 4 * (d & 3) + e);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            work_off(d);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (!LSEPASS) asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));   // added here, not at the loop's end
     };
     constexpr int LOADS = LSEPASS ? 4 : 5;   // of a tile, per wavefront
-    int head = first_head, qa = last_tile, it = 0;
+    int qa = last_tile, it = 0;
     // Half b of the tile in stage st, leaving the operands of the next half.
     auto half = [&](auto st_, auto b_) {
         constexpr int st = decltype(st_)::value, b = decltype(b_)::value;
@@ -230,14 +311,24 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         }
         f32x16 sc[2];
         products(b ? (st + 1) % ST : st, 1 - b, sc);
-        const bool masked = qa + 32 * b < k0 + KW || k0 + KW > len;          // uniform
-        const int lim = (query < len ? query : len - 1) - k0 - 4 * h32;      // the last key that the query sees
+        const bool masked = (ROWS ? win.lo : qa + 32 * b) < k0 + KW || k0 + KW > len;    // uniform
+        int lim = KW;                                        // the last key that the query sees, from k0 + 4 h32
+        if (masked) {
+            const int row = query < end ? query : end - 1, at = ROWS ? win.lo + row % win.n : row;
+            lim = at - k0 - 4 * h32;
+        }
         auto seen = [&](int kb, int i) { return 32 * kb + 8 * (i >> 2) + (i & 3) <= lim; };
-        if constexpr (!LSEPASS) {
-            late[0] = sc[0];
-            late[1] = sc[1];
-            late_lse2 = lse2;
-            if (masked) {
+        late[0] = sc[0];
+        late[1] = sc[1];
+        late_lse2 = lse2;
+        late_row = query < end && k0 < len ? query : -1;
+        if (masked) {
+            if constexpr (LSEPASS) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) late[kb][i] = seen(kb, i) ? sc[kb][i] : NEG_INF;   // the scale is positive
+            } else {
                 // added at once, the unseen left out (whatever their logit and lse), so that nothing is pending
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -249,35 +340,10 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
                     }
                 late_lse2 = 0.0f;
             }
-        } else if (k0 < len && k0 <= qa + QT - 1) {          // some query of this tile sees a key of this wavefront
-            if (masked) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[kb][i] = seen(kb, i) ? sc[kb][i] : NEG_INF;   // the scale is positive
-            }
-            float m = NEG_INF, l = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) m = fmaxf(m, sc[kb][i]);
-            m = pair_max(m * a.c_log2);
-            const float use = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -use));
-            l = pair_sum(l);
-            if (h32 == 0 && query < end)
-                a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.Hq + head) * a.window + (query - lo)] = f32x2{m, l};
         }
     };
     auto next = [&]() {
         qa -= QT;
-        if (qa < q0) {
-            qa = last_tile;
-            ++head;
-        }
         return ++it < total;
     };
     if (total > 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
@@ -298,10 +364,10 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         half(two, one);
         if (!next()) break;
     }
-    if constexpr (!LSEPASS) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) add_weight(i >> 4, i & 15);
-        float *out = a.out + ((int64_t)range * a.Hq + (a.heads == 1 ? first_head : h)) * a.out_sh + start;
+    for (int d = 0; d < 8; ++d) work_off(d);
+    if constexpr (!LSEPASS) {
+        float *out = a.out + ((int64_t)range * a.Hq + list) * a.out_sh + start;
         // Sums over the 32 queries: a swap of the odd 16-lane rows of one key's
         // lanes with the even ones of another's leaves both keys in one register
         // (the first block's in the even rows, the second's in the odd).
@@ -317,38 +383,37 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     }
 }
 
-// lse of the window's queries from the (max, sum) of their key tiles: 64 rows
-// (query heads and window queries of a sequence) per workgroup, the key tiles
-// over its wavefronts.
-__global__ __launch_bounds__(1024) void window_lse(WeightArgs a, float *lse)
+// lse of the window's rows from the (max, sum) of their key tiles: sixteen rows
+// of a (sequence, KV head) per workgroup, the key tiles over 64 groups of lanes.
+constexpr int LR = 16, LG = 64;
+
+__global__ __launch_bounds__(LR * LG) void window_lse(WeightArgs a, float *lse)
 {
-    __shared__ float sm_m[16][64], sm_l[16][64];
-    const int seq = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int len = length_of(a, seq);
-    const int lo = (int64_t)len > a.window ? len - (int)a.window : 0;
-    const int64_t rows = (int64_t)a.Hq * a.window, row = (int64_t)blockIdx.x * 64 + lane;
-    const int i = row < rows ? (int)(row % a.window) : 0, query = lo + i;
-    float M = NEG_INF, L = 0.0f;
-    if (row < rows && query < len) {
-        // tiles with a key at or before the query; the workgroup of a tile wrote every query from its first key on
-        for (int t = wave; t <= query / KW; t += 16) {
-            const f32x2 ml = a.ml[((int64_t)seq * a.tiles64 + t) * rows + row];
-            const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
-            L = L * __builtin_amdgcn_exp2f(M - use) + ml[1] * __builtin_amdgcn_exp2f(ml[0] - use);
-            M = m;
-        }
+    __shared__ f32x2 sm[LG][LR];
+    const int seq = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % LR, group = threadIdx.x / LR;
+    const int len = length_of(a, seq), row = blockIdx.x * LR + lane;
+    const Window win = window_of(a, len);
+    const int64_t all = (int64_t)a.G * a.window;
+    f32x2 mine = {NEG_INF, 0.0f};
+    auto join = [](f32x2 x, f32x2 y) {
+        const float m = fmaxf(x[0], y[0]), use = m == NEG_INF ? 0.0f : m;
+        return f32x2{m, x[1] * __builtin_amdgcn_exp2f(x[0] - use) + y[1] * __builtin_amdgcn_exp2f(y[0] - use)};
+    };
+    if (row < win.rows) {
+        // the tiles that hold a key at or before the last query (the others' keys are unseen: (-inf, 0))
+        const f32x2 *ml = a.ml + ((int64_t)seq * a.tiles64 * a.H + h) * all + row;
+#pragma unroll 4
+        for (int t = group; t <= (len - 1) / KW; t += LG) mine = join(mine, ml[t * a.H * all]);
     }
-    sm_m[wave][lane] = M;
-    sm_l[wave][lane] = L;
+    sm[group][lane] = mine;
     __syncthreads();
-    if (wave || row >= rows || query >= len) return;
-    float m = NEG_INF, l = 0.0f;
+    if (group >= 4) return;                  // the first wavefront
 #pragma unroll
-    for (int w = 0; w < 16; ++w) m = fmaxf(m, sm_m[w][lane]);
-    const float use = m == NEG_INF ? 0.0f : m;
+    for (int g = group + 4; g < LG; g += 4) mine = join(mine, sm[g][lane]);
 #pragma unroll
-    for (int w = 0; w < 16; ++w) l = fmaf(__builtin_amdgcn_exp2f(sm_m[w][lane] - use), sm_l[w][lane], l);
-    lse[(int64_t)seq * rows + row] = (use + __builtin_amdgcn_logf(l)) * LN2;
+    for (int d = 16; d < 64; d *= 2) mine = join(mine, f32x2{__shfl_xor(mine[0], d), __shfl_xor(mine[1], d)});
+    if (group == 0 && row < win.rows)
+        lse[((int64_t)seq * a.H + h) * all + row] = (mine[0] == NEG_INF ? 0.0f : mine[0] + __builtin_amdgcn_logf(mine[1])) * LN2;
 }
 
 // The sums of each KV head's query heads and of the query ranges that see a key.
@@ -421,35 +486,39 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     IQ_CHECK_ARG(q_st >= 0 && q_st < (1LL << 25), "iq_prefill_weights: token stride too large");
     IQ_CHECK_ARG(scale > 0.0f, "iq_prefill_weights: the scale must be positive");
     IQ_CHECK_ARG(window >= 0 && window <= 65536 && (window > 0 || lse), "iq_prefill_weights: no window and no lse");
+    IQ_CHECK_ARG(!lse || lse_sh > 0, "iq_prefill_weights: bad lse stride");
     const Scratch s = scratch_of(Hq, n_seq, max_seqlen, tokens, window, lse != nullptr);
     IQ_CHECK_ARG(s.lse + s.ml + s.part == 0 || (workspace && workspace_floats >= s.lse + s.ml + s.part),
                  "iq_prefill_weights: workspace too small");
     const int64_t tiles = (max_seqlen + KG - 1) / KG, G = Hq / H;
     const int64_t chunk = window ? 1 << 30 : chunk_of(Hq, n_seq, max_seqlen), chunks = (max_seqlen + chunk - 1) / chunk;
-    WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq, (int)max_seqlen, (int)H,
-                 (int)Hq, (int)G, (int)(window ? G : 1), window ? window : max_seqlen, (int)chunk, (int)chunks, (int)tiles, scale * LOG2E, lse, lse_sh, 0,
-                 (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
+    WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq,
+                 (int)max_seqlen, (int)H, (int)Hq, (int)G, (int)window, (int)chunk, (int)chunks, (int)tiles,
+                 scale * LOG2E, lse, lse_sh, (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
-    const int64_t items = chunks * tiles * (Hq / a.heads) * n_seq;
+    const int64_t items = chunks * tiles * (window ? H : Hq) * n_seq;
     IQ_CHECK_ARG(items <= 0xffffff, "iq_prefill_weights: too many key tiles");
     const dim3 grid((unsigned)items), block(NT);
-    if (window > 0 && !lse) {
-        float *own = workspace + s.ml;
-        hipLaunchKernelGGL((f16 ? prefill_weights<true, true> : prefill_weights<false, true>), grid, block, 0, st, a);
-        hipLaunchKernelGGL(window_lse, dim3((unsigned)((Hq * window + 63) / 64), (unsigned)n_seq), dim3(1024), 0, st, a,
-                           own);
-        a.lse = own;
-        a.windowed = 1;
-    }
-    if (window == 0) {
+    if (window > 0) {
+        if (!lse) {
+            float *own = workspace + s.ml;
+            hipLaunchKernelGGL((f16 ? prefill_weights<true, WINDOW_LSE> : prefill_weights<false, WINDOW_LSE>), grid,
+                               block, 0, st, a);
+            hipLaunchKernelGGL(window_lse, dim3((unsigned)((G * window + LR - 1) / LR), (unsigned)H, (unsigned)n_seq),
+                               dim3(LR * LG), 0, st, a, own);
+            a.lse = own;
+            a.lse_sh = 0;
+        }
+        hipLaunchKernelGGL((f16 ? prefill_weights<true, WINDOW> : prefill_weights<false, WINDOW>), grid, block, 0, st,
+                           a);
+    } else {
         a.out = workspace;
         a.out_sh = tokens;
-    }
-    hipLaunchKernelGGL((f16 ? prefill_weights<true, false> : prefill_weights<false, false>), grid, block, 0, st, a);
-    if (window == 0 && tokens > 0)
+        hipLaunchKernelGGL((f16 ? prefill_weights<true, ALL> : prefill_weights<false, ALL>), grid, block, 0, st, a);
         hipLaunchKernelGGL(add_heads, dim3((unsigned)((max_seqlen + 255) / 256), (unsigned)H, (unsigned)n_seq),
                            dim3(256), 0, st, a, workspace, tokens, out, out_sh);
+    }
     IQ_CHECK_LAUNCH("prefill_weights");
     return IQ_OK;
 }

@@ -327,7 +327,8 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
     query [tokens, Hq, 128], key [tokens, kv_heads, 128] (bf16 or f16),
     sequences as ``prefill_attention`` takes them.  Over all queries, whose
     ``lse`` [Hq, tokens] ``prefill_attention(..., lse=...)`` wrote, or with
-    ``window=w`` over the last w queries of each sequence (lse optional).
+    ``window=w`` over the last w queries of each sequence (lse optional; w at
+    most 4096, or all with the lse).
     Tokens of no sequence are not written."""
     (tokens, hq, _), qs = _token_rows(query, "query")
     (rows, h, _), ks = _token_rows(key, "key")
@@ -352,10 +353,14 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
     if tokens == 0:
         return output
     window = 0 if window is None else min(int(window), max_seqlen)
+    if lse is not None and window == max_seqlen:
+        window = 0                           # every query
+    if window > 4096:
+        raise ValueError("Windows of more than 4096 queries and less than all are not supported")
     n = cu.shape[0] - 1
     need = _entry("iq_prefill_weights_floats")(hq, n, max_seqlen, tokens, window, lse is not None)
     scratch = torch.empty(need, dtype=_F32, device=query.device)
     _call(gpu, "iq_prefill_weights", query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype), qs[0], qs[1], ks[0],
           ks[1], cu.data_ptr(), n, max_seqlen, tokens, hq, h, window, scale, nat.ptr(lse),
-          0 if lse is None else lse.stride(0), scratch.data_ptr(), need, output.data_ptr(), output.stride(0))
+          0 if lse is None else max(1, lse.stride(0)), scratch.data_ptr(), need, output.data_ptr(), output.stride(0))
     return output
