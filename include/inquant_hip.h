@@ -486,9 +486,13 @@ int iq_select_rows(const float *weights, int64_t w_stride, int64_t H, const int3
  * The evicted cache rows below `budget` take, in order, the kept rows from
  * `budget` on (key, value, weight and position); all other rows stay as they
  * are.  lengths i32: rows each sequence holds (at most max_tokens are
- * considered); new_lengths i32: min(lengths, budget).  workspace: i32,
- * iq_dense_evict_ints elements.  No page may belong to two sequences.
+ * considered); new_lengths i32: min(lengths, budget), which may take the place
+ * of lengths.  workspace: i32, iq_dense_evict_ints elements (none while a head
+ * moves at most IQ_DENSE_FEW_MOVES rows: min(budget, max_tokens - budget)).
+ * No page may belong to two sequences.
  */
+#define IQ_DENSE_FEW_MOVES 128
+
 int64_t iq_dense_evict_ints(int64_t H, int64_t n_seq, int64_t max_tokens, int64_t budget);
 
 int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,

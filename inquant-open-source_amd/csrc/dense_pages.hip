@@ -282,26 +282,34 @@ struct EvictArgs {
     DensePool pool;
     const int32_t *lengths, *seen;
     int64_t max_tokens, budget, sink, recent, most;   // most: moves of a head at most
-    int32_t *new_lengths;
+    int32_t *new_lengths;                             // null where another launch writes them
     int32_t *moves;                                   // [n * H, 1 + 2 most]: count, evicted places, rows from behind
 };
 
+__device__ __forceinline__ void evict_length(const EvictArgs &a, int seq)
+{
+    const int32_t have = a.lengths[seq];
+    a.new_lengths[seq] = have < a.budget ? have : (int32_t)a.budget;
+}
+
 // Chooses the rows of one (head, sequence) and lists the moves: the evicted
 // places below the budget in order, and the kept rows behind it from the last.
-// MOVE: and makes them, where they are few (16 sequences of 2049 rows, one to
-// move: 8 us, and 11 with a launch of its own for the move); then the new
-// lengths are another tensor than the lengths, which other heads still read.
+// MOVE: at most FEW of them, listed in LDS and made here (16 sequences of 2049
+// rows, one to move: 8 us, and 11 with a launch of its own for the move).
+constexpr int FEW = IQ_DENSE_FEW_MOVES;
+
 template <bool MOVE>
 __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
 {
     __shared__ SelectSmem sm;
+    __shared__ int32_t few[1 + 2 * FEW];
     const int h = blockIdx.x, seq = blockIdx.y, H = a.pool.H, B = a.pool.B;
     const int64_t have = a.lengths[seq];
     const int64_t len = have < a.max_tokens ? have : a.max_tokens;
-    int32_t *list = a.moves + ((int64_t)seq * H + h) * (1 + 2 * a.most);
-    if (MOVE && h == 0 && threadIdx.x == 0) a.new_lengths[seq] = have < a.budget ? (int32_t)have : (int32_t)a.budget;
+    int32_t *list = MOVE ? few : a.moves + ((int64_t)seq * H + h) * (1 + 2 * a.most);
+    if (MOVE && a.new_lengths && h == 0 && threadIdx.x == 0) evict_length(a, seq);
     if (len <= a.budget) {
-        if (threadIdx.x == 0) list[0] = 0;
+        if (!MOVE && threadIdx.x == 0) list[0] = 0;
         return;
     }
     const int64_t newest = (int64_t)a.seen[seq] - a.recent;
@@ -340,9 +348,15 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     }
 }
 
-// Moves the kept rows into the evicted places; sixteen lanes a row.  The new
-// lengths are written here and not by the launch before, whose workgroups all
-// read the lengths: both may be one tensor.
+// New lengths in the place of the old ones, which every head's workgroup reads:
+// by the launch after them.
+__global__ void evict_lengths_kernel(EvictArgs a, int n)
+{
+    const int seq = blockIdx.x * 256 + threadIdx.x;
+    if (seq < n) evict_length(a, seq);
+}
+
+// Moves the kept rows into the evicted places; sixteen lanes a row.
 constexpr int MV_ROWS = 64;
 
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a)
@@ -351,10 +365,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a)
     const int32_t *list = a.moves + (int64_t)blockIdx.y * (1 + 2 * a.most);
     const int n = list[0];
     const int32_t *holes = list + 1, *behind = holes + a.most;
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
-        const int32_t have = a.lengths[seq];
-        a.new_lengths[seq] = have < a.budget ? have : (int32_t)a.budget;
-    }
+    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) evict_length(a, seq);
 #pragma unroll
     for (int i = 0; i < MV_ROWS / 16; ++i) {
         const int64_t m = (int64_t)blockIdx.x * MV_ROWS + 16 * i + (threadIdx.x >> 4);
@@ -409,8 +420,8 @@ extern "C" int iq_select_rows(const float *weights, int64_t w_stride, int64_t H,
 
 extern "C" int64_t iq_dense_evict_ints(int64_t H, int64_t n_seq, int64_t max_tokens, int64_t budget)
 {
-    const int64_t over = max_tokens > budget ? max_tokens - budget : 0;
-    return n_seq * H * (1 + 2 * (over < budget ? over : budget));
+    const int64_t over = max_tokens > budget ? max_tokens - budget : 0, most = over < budget ? over : budget;
+    return most <= FEW ? 0 : n_seq * H * (1 + 2 * most);
 }
 
 extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int32_t *tables, int64_t bt_stride,
@@ -421,24 +432,30 @@ extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int3
     DensePool pool;
     if (const int e = dense_pool("iq_dense_evict", pages, dtype, tables, bt_stride, bt_cols, n_seq, pool)) return e;
     IQ_CHECK_ARG(pool.weights && pool.positions, "iq_dense_evict: pages without weights and positions");
-    IQ_CHECK_ARG(lengths && seen && new_lengths && workspace, "iq_dense_evict: null pointer");
+    IQ_CHECK_ARG(lengths && seen && new_lengths, "iq_dense_evict: null pointer");
     IQ_CHECK_ARG(max_tokens >= 0 && max_tokens <= bt_cols * pool.B, "iq_dense_evict: max_tokens past the block tables");
     IQ_CHECK_ARG(sink >= 0 && recent >= 0 && budget >= 1 && budget <= 0x7fffffffLL && sink + recent <= budget,
                  "iq_dense_evict: sink and recent rows must fit the budget");
-    IQ_CHECK_ARG(workspace_ints >= iq_dense_evict_ints(pool.H, n_seq, max_tokens, budget),
-                 "iq_dense_evict: workspace too small");
+    const int64_t ints = iq_dense_evict_ints(pool.H, n_seq, max_tokens, budget);
+    IQ_CHECK_ARG(ints == 0 || (workspace && workspace_ints >= ints), "iq_dense_evict: workspace too small");
     IQ_CHECK_ARG(n_seq * pool.H <= 65535, "iq_dense_evict: too many sequences");
     if (n_seq == 0) return IQ_OK;
     const int64_t over = max_tokens > budget ? max_tokens - budget : 0, most = over < budget ? over : budget;
-    const EvictArgs a{pool, lengths, seen, max_tokens, budget, sink, recent, most, new_lengths, workspace};
+    EvictArgs a{pool, lengths, seen, max_tokens, budget, sink, recent, most, new_lengths, workspace};
     const dim3 rows((unsigned)pool.H, (unsigned)n_seq), block(SEL_NT);
-    if (most <= 2 * SEL_NT / 16 && (new_lengths + n_seq <= lengths || lengths + n_seq <= new_lengths)) {
-        hipLaunchKernelGGL(evict_select_kernel<true>, rows, block, 0, (hipStream_t)stream, a);
+    const hipStream_t st = (hipStream_t)stream;
+    if (most <= FEW) {
+        const bool apart = new_lengths + n_seq <= lengths || lengths + n_seq <= new_lengths;
+        if (!apart) a.new_lengths = nullptr;
+        hipLaunchKernelGGL(evict_select_kernel<true>, rows, block, 0, st, a);
+        a.new_lengths = new_lengths;
+        if (!apart)
+            hipLaunchKernelGGL(evict_lengths_kernel, dim3((unsigned)((n_seq + 255) / 256)), dim3(256), 0, st, a,
+                               (int)n_seq);
     } else {
-        hipLaunchKernelGGL(evict_select_kernel<false>, rows, block, 0, (hipStream_t)stream, a);
-        const int64_t groups = most > 0 ? (most + MV_ROWS - 1) / MV_ROWS : 1;
-        hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)groups, (unsigned)(n_seq * pool.H)), dim3(256), 0,
-                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL(evict_select_kernel<false>, rows, block, 0, st, a);
+        hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)((most + MV_ROWS - 1) / MV_ROWS),
+                                                   (unsigned)(n_seq * pool.H)), dim3(256), 0, st, a);
     }
     IQ_CHECK_LAUNCH("dense_evict");
     return IQ_OK;

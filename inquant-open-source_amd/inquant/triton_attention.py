@@ -87,6 +87,15 @@ class SharedDecodeWorkspace:
             have = self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
         return have[:needed].view(shape)
 
+    def floats(self, needed, device):
+        """Address and size of at least ``needed`` floats, and the handle of the
+        stream they belong to (``acquire`` without a tensor to show for it)."""
+        handle = self._pin.check(device)
+        have = self.tensor
+        if have is None or have.numel() < needed:
+            have = self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
+        return have.data_ptr(), have.numel(), handle
+
 
 class _BlockFormat:
     """Layout shared by all blocks of a decode state."""

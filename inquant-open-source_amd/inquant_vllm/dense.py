@@ -33,6 +33,7 @@ from .layout import BLOCK_SIZES
 
 _ROWS = (torch.bfloat16, torch.float16)
 _I32, _F32 = torch.int32, torch.float32
+_FEW_MOVES = 128        # iq_dense_evict takes no workspace up to here (IQ_DENSE_FEW_MOVES)
 
 
 def _strides(pages):
@@ -117,14 +118,17 @@ def _entry(name):
     return fn
 
 
-def _call(gpu, name, *args):
-    """Calls the entry point on the current stream of a GPU, with that GPU current."""
-    stream = torch._C._cuda_getCurrentRawStream(gpu)
+def _status(gpu, name, *args):
+    """Calls the entry point with its GPU current."""
     if gpu == torch._C._cuda_getDevice():
-        status = _entry(name)(*args, stream)
-    else:
-        with torch.cuda.device(gpu):
-            status = _entry(name)(*args, stream)
+        return _entry(name)(*args)
+    with torch.cuda.device(gpu):
+        return _entry(name)(*args)
+
+
+def _call(gpu, name, *args):
+    """The same on the GPU's current stream; a failure raises."""
+    status = _status(gpu, name, *args, torch._C._cuda_getCurrentRawStream(gpu))
     if status:
         nat.check(status)
 
@@ -262,11 +266,13 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
         raise ValueError("output must be a contiguous int32 [sequences] tensor")
     if n == 0:
         return output
-    # a count and two lists of the most moves that a head can need
-    need = n * pages.heads * (1 + 2 * max(0, min(budget, max_tokens - budget)))
-    scratch = torch.empty(need, dtype=_I32, device=lengths.device)
+    # few moves are listed on the chip
+    need, scratch = 0, None
+    if max_tokens - budget > _FEW_MOVES:
+        need = _entry("iq_dense_evict_ints")(pages.heads, n, max_tokens, budget)
+        scratch = torch.empty(need, dtype=_I32, device=lengths.device)
     _call(gpu, "iq_dense_evict", pages._desc, pages._code, *table, lengths.data_ptr(), seen.data_ptr(), n, max_tokens,
-          budget, sink, recent, output.data_ptr(), scratch.data_ptr(), need)
+          budget, sink, recent, output.data_ptr(), None if scratch is None else scratch.data_ptr(), need)
     return output
 
 
@@ -311,11 +317,20 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     if n == 0:
         return output
     accumulate = 1 if accumulate else 0
-    need = _entry("iq_dense_workspace_floats")(hq, hkv, n, max_tokens, accumulate)
-    scratch = workspace.acquire((need,), query.device)
-    _call(gpu, "iq_dense_decode", query.data_ptr(), pages._code, qs[0], qs[1], hq, n, pages._desc, *table,
-          lengths.data_ptr(), max_tokens, scale, accumulate, scratch.data_ptr(), need, output.data_ptr(),
-          output.stride(0), output.stride(1), code)
+    device, os = query.device, output.stride()
+
+    def call(floats):
+        return _status(gpu, "iq_dense_decode", query.data_ptr(), pages._code, qs[0], qs[1], hq, n, pages._desc, *table,
+                       lengths.data_ptr(), max_tokens, scale, accumulate, *floats[:2], output.data_ptr(), os[0], os[1],
+                       code, floats[2])
+    # the scratch that is there serves most calls; the library says when it does not
+    floats = workspace.floats(0, device)
+    status = call(floats)
+    if status:
+        need = _entry("iq_dense_workspace_floats")(hq, hkv, n, max_tokens, accumulate)
+        if need > floats[1]:
+            status = call(workspace.floats(need, device))
+        nat.check(status)
     return output
 
 

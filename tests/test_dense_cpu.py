@@ -129,9 +129,10 @@ def test_refusals_of_the_library():
     assert decode(pages(), dtype=nat.IQ_F32) == -1
     assert decode(pages(weights=0, positions=0), accumulate=1) == -1
     evict = lambda p, budget=8, sink=0, ints=1 << 20: lib.iq_dense_evict(
-        p, nat.IQ_BF16, fake, 2, 2, fake, fake, 1, 32, budget, sink, 0, fake, fake, ints, None)
+        p, nat.IQ_BF16, fake, 40, 40, fake, fake, 1, 640, budget, sink, 0, fake, fake, ints, None)
     assert evict(pages(weights=0, positions=0)) == -1 and evict(pages(), budget=0) == -1
-    assert evict(pages(), sink=9) == -1 and evict(pages(), ints=3) == -1
+    assert evict(pages(), sink=9) == -1 and evict(pages(), budget=300, ints=3) == -1
+    assert lib.iq_dense_evict_ints(2, 1, 640, 300) == 2 * 601 and lib.iq_dense_evict_ints(2, 1, 640, 600) == 0
     assert lib.iq_select_rows(fake, 8, 2, fake, 1, 8, 4, 3, 2, fake, None) == -1
     assert lib.iq_dense_write(fake, fake + 2, nat.IQ_BF16, 256, 128, 256, 128, fake, 1, 3, None, None, None, 0, None, 0,
                               pages(), fake, 2, 2, None) == -1
