@@ -14,9 +14,10 @@
 namespace {
 
 constexpr int D = 128;
-constexpr int NW = 4, NT = 64 * NW;
+constexpr int NT = 256;                      // threads of the join, and of a partition's workgroup
 constexpr int WT = 64;                       // rows per wavefront and step
-constexpr int PT = WT * NW;                  // rows per workgroup and step
+constexpr int PT = WT * NT / 64;             // rows per workgroup of a partition and step
+constexpr int ONE_MOST = 512;                // rows that a workgroup takes in one step
 constexpr float LOG2E = 1.44269504088896341f;
 
 struct DecodeArgs {
@@ -31,12 +32,13 @@ struct DecodeArgs {
     int64_t l_stride;
     void *out;
     int64_t o_ss, o_sh;
-    int odt;
+    int odt, accumulate;
 };
 
 // V rows of a step in LDS: 256 bytes each, the 16-byte chunk c of row r at
 // slot c ^ 4 (r % 4) ^ 2 (r / 4 % 2), so that the transposed reads of 32 lanes
 // (two groups of four rows, 32 bytes each) hit 64 distinct banks.
+template <int NW>
 struct __attribute__((aligned(16))) DecodeSmem {
     union {
         uint16_t v[NW][WT * D];
@@ -111,11 +113,17 @@ struct FirstRows {
     }
 };
 
-// DIRECT: the rows are one partition; the outputs and weights are final.
-template <bool F16, bool DIRECT>
-__global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
+// PARTS: one of several partitions.  DIRECT: the only one; the outputs and
+// weights are final.  ONE: the only one, and each wavefront's rows are one step,
+// whose logits stay in registers until the lse is known.
+enum Mode { PARTS, DIRECT_LOOP, ONE };
+
+template <bool F16, Mode MODE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void dense_partials(DecodeArgs a)
 {
-    __shared__ DecodeSmem sm;
+    constexpr bool DIRECT = MODE != PARTS;
+    constexpr int THREADS = 64 * NW;
+    __shared__ DecodeSmem<NW> sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     const int h = blockIdx.x, part = blockIdx.y, seq = blockIdx.z;
@@ -123,7 +131,7 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
     const int t0 = part * a.span;
     if (t0 >= len) {                         // uniform; the join does not read this partition
         if constexpr (DIRECT)                // no row: nothing to attend to
-            for (int i = tid; i < D * a.G; i += NT)
+            for (int i = tid; i < D * a.G; i += THREADS)
                 iq_store_as(a.out, seq * a.o_ss + (h * a.G + (i >> 7)) * a.o_sh + (i & 127), 0.0f, a.odt);
         return;
     }
@@ -142,9 +150,11 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
     for (int cb = 0; cb < 8; ++cb) acc[cb] = f32x4{0, 0, 0, 0};
     const uint32_t lds_v = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)&sm.v[wave][0];
     const int32_t *table = p.tables + seq * p.bt_stride;
-    for (int c0 = t0 + WT * wave; c0 < end; c0 += PT) {
+    f32x4 sc[4];                             // S^T rows 16 t + 4 g4 + i (cache rows), column c16
+    int64_t at[4];                           // ONE: the tiles' first weights
+    int last[4];                             // a tile's last live row; -1: none, or its page is not in the pool
+    for (int c0 = t0 + WT * wave; c0 < end; c0 += WT * NW) {
         const uint16_t *kt[4], *vt[4];       // first row of each 16-row tile
-        int last[4];                         // its last live row; -1: none, its page is not in the pool
         u32x4 kf[4][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -156,6 +166,7 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
             const int row = tb & (p.B - 1);
             kt[t] = p.key + page * p.k_sp + h * p.k_sh + row * p.k_st;
             vt[t] = p.value + page * p.v_sp + h * p.v_sh + row * p.v_st;
+            at[t] = (page * p.H + h) * p.B + row;
             const int rest = len - 1 - tb;
             last[t] = rest < 15 ? rest : 15;
             const int r = c16 < last[t] ? c16 : last[t];
@@ -174,7 +185,6 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
             const int chunk = c16 ^ (4 * (rl & 3)) ^ (2 * ((rl >> 2) & 1));
             lds_load16(vt[t], (uint32_t)(r * (int)p.v_st + 8 * chunk) * 2, lds_v + (uint32_t)(4 * i * D * 2));
         }
-        f32x4 sc[4];                         // S^T rows 16 t + 4 g4 + i (cache rows), column c16
 #pragma unroll
         for (int t = 0; t < 4; ++t) sc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -189,7 +199,7 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
                 sc[t][i] = 4 * g4 + i <= last[t] ? sc[t][i] * a.c_log2 : NEG_INF;
                 cmax = fmaxf(cmax, sc[t][i]);
             }
-        if (a.logits && c16 < a.G) {
+        if (MODE != ONE && a.logits && c16 < a.G) {
             float *lp = a.logits + (int64_t)(seq * a.Hq + h * a.G + c16) * a.l_stride + c0 + 4 * g4;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
         sm.l[wave][c16] = l_run;
     }
     __syncthreads();
-    for (int i = tid; i < 32 * a.G; i += NT) {
+    for (int i = tid; i < 32 * a.G; i += THREADS) {
         const int g = i >> 5, c = 4 * (i & 31);
         float M = NEG_INF;
 #pragma unroll
@@ -267,7 +277,31 @@ __global__ __launch_bounds__(NT, 2) void dense_partials(DecodeArgs a)
             if (c == 0) a.part.ml[row] = f32x2{M, L};
         }
     }
-    if constexpr (DIRECT) {
+    if constexpr (MODE == ONE) {
+        if (!a.accumulate) return;
+        __syncthreads();                     // the lse of every head
+        if (t0 + WT * wave >= end) return;   // a wavefront without rows has no logits either
+        const float lse = c16 < a.G ? sm.lse[c16] : __builtin_inff();
+        // lane (4 t + i, g4) takes row 16 t + 4 g4 + i
+        float mine = 0.0f;
+        int64_t base = at[0];
+        int most = last[0];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if (c16 >> 2 == t) {
+                base = at[t];
+                most = last[t];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float w = row_sum16(__builtin_amdgcn_exp2f(sc[t][i] - lse));
+                if (c16 == 4 * t + i) mine = w;
+            }
+        }
+        const int r = 4 * g4 + (c16 & 3);
+        if (r <= most) unsafeAtomicAdd(p.weights + base + r, mine);
+    }
+    if constexpr (MODE == DIRECT_LOOP) {
         if (!a.logits) return;
         const int64_t q0 = (int64_t)seq * a.Hq + h * a.G;
         __syncthreads();                     // the logits and lse of every wavefront
@@ -345,7 +379,7 @@ __global__ __launch_bounds__(NT) void dense_join(DecodeArgs a, int n)
     // the first rows' logits travel while the lse is made
     FirstRows first;
     first.load(a, q0, r0 + tid, r1);
-    for (int g = tid >> 6; g < a.G; g += NW) {
+    for (int g = tid >> 6; g < a.G; g += NT / 64) {
         float M = NEG_INF, L = 0.0f;
         for (int p = lane; p < live; p += 64) {
             const f32x2 ml = a.part.ml[(q0 + g) * a.parts + p];
@@ -371,14 +405,16 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t max_tokens, bool accumu
     // shorter ones, as their lengths differ (16 sequences of 2K-32K tokens, 28
     // heads over 4: 144 us with 1024 places, 121 with 2048, 114 with 4096, 120
     // with 8192; two of 128K, 32 over 8: 244, 251, 257, 269 with the join).
-    // Rows that two workgroups would share are left to one, which saves the
-    // join (one sequence of 300 rows: 15 us in two launches).
-    const int64_t steps = max_tokens <= 2 * PT ? 1 : (max_tokens + PT - 1) / PT;
+    // Up to ONE_MOST rows are left to one workgroup, which saves the join and the
+    // logits' way through memory (one sequence of 300 rows, 28 heads over 4: 14.3
+    // us in two launches, 10.9 in one of four wavefronts that loops).
+    const int64_t steps = (max_tokens + PT - 1) / PT;
     const int64_t target = n < 4 ? 1024 : 4096, per = (n * H * steps + target - 1) / target;
     Split s;
-    s.span = PT * (max_tokens <= 2 * PT ? 2 : per);
+    const bool one = max_tokens <= ONE_MOST;
+    s.span = one ? ONE_MOST : PT * per;
     s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
-    s.logits = accumulate ? (max_tokens + 63) / 64 * 64 : 0;
+    s.logits = accumulate && !one ? (max_tokens + 63) / 64 * 64 : 0;
     s.floats = n * Hq * ((s.parts > 1 ? s.parts * (D + 2) : 0) + s.logits);
     return s;
 }
@@ -416,12 +452,18 @@ extern "C" int iq_dense_decode(const void *q, int dtype, int64_t q_ss, int64_t q
     const DecodeArgs a{pool, (const uint16_t *)q, q_ss, q_sh, lengths, (int32_t)max_tokens, (int32_t)s.span,
                        (int32_t)s.parts, (int32_t)(Hq / pool.H), (int32_t)Hq, scale * LOG2E,
                        Partials{part, (f32x2 *)(part + n_seq * Hq * s.parts * D)},
-                       accumulate ? workspace : nullptr, s.logits, out, o_ss, o_sh, out_dtype};
+                       s.logits ? workspace : nullptr, s.logits, out, o_ss, o_sh, out_dtype, accumulate};
     const bool f16 = dtype == IQ_F16, direct = s.parts == 1;
     const dim3 grid((unsigned)pool.H, (unsigned)s.parts, (unsigned)n_seq);
-    const auto kernel = direct ? f16 ? dense_partials<true, true> : dense_partials<false, true>
-                               : f16 ? dense_partials<true, false> : dense_partials<false, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, (hipStream_t)stream, a);
+    if (max_tokens <= ONE_MOST && max_tokens > PT) {
+        const auto kernel = f16 ? dense_partials<true, ONE, 8> : dense_partials<false, ONE, 8>;
+        hipLaunchKernelGGL(kernel, grid, dim3(2 * NT), 0, (hipStream_t)stream, a);
+    } else {
+        const auto kernel = max_tokens <= PT ? f16 ? dense_partials<true, ONE, 4> : dense_partials<false, ONE, 4>
+                            : direct ? f16 ? dense_partials<true, DIRECT_LOOP, 4> : dense_partials<false, DIRECT_LOOP, 4>
+                                     : f16 ? dense_partials<true, PARTS, 4> : dense_partials<false, PARTS, 4>;
+        hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, (hipStream_t)stream, a);
+    }
     if (!direct) hipLaunchKernelGGL(dense_join, dim3((unsigned)joins), dim3(NT), 0, (hipStream_t)stream, a, (int)n_seq);
     IQ_CHECK_LAUNCH("dense_decode");
     return IQ_OK;

@@ -73,6 +73,7 @@ class SharedDecodeWorkspace:
 
     def __init__(self):
         self.tensor = None
+        self._lent = None           # allocations that ``floats`` gave out and a captured graph may still use
         self._pin = _StreamPin("Shared decode workspace requires one CUDA stream per cache")
 
     @property
@@ -84,15 +85,23 @@ class SharedDecodeWorkspace:
         needed = math.prod(shape)
         have = self.tensor
         if have is None or have.numel() < needed:
+            if self._lent is not None:
+                self._lent.append(have)
             have = self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
         return have[:needed].view(shape)
 
     def floats(self, needed, device):
         """Address and size of at least ``needed`` floats, and the handle of the
-        stream they belong to (``acquire`` without a tensor to show for it)."""
+        stream they belong to.  Grows by doubling, and keeps what it outgrew: the
+        address may stand in a captured graph."""
         handle = self._pin.check(device)
         have = self.tensor
+        if self._lent is None:
+            self._lent = []
         if have is None or have.numel() < needed:
+            if have is not None:
+                self._lent.append(have)
+                needed = max(needed, 2 * have.numel())
             have = self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
         return have.data_ptr(), have.numel(), handle
 

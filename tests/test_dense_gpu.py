@@ -66,6 +66,9 @@ DECODE = [
     (12, 1, 256, [5000, 256, 255]),
     (2, 2, 16, [0]),
     (28, 4, 16, [40000, 9, 33333]),
+    (14, 2, 32, [512, 511, 449, 1, 0]),
+    (28, 4, 64, [513, 600]),
+    (8, 8, 16, [700] * 140),
 ]
 
 
@@ -195,6 +198,31 @@ def test_decode_in_a_graph_replays_with_new_lengths_on_another_stream():
         torch.cuda.synchronize()
         assert torch.equal(got, eager) and torch.equal(weights, pages.weights)
         _check_decode(q, pages, table, now, SCALE, got, start, True)
+
+
+def test_decode_captured_before_its_workspace_grew():
+    """A graph replays on the scratch it was captured with, whatever outgrew it since."""
+    from inquant_vllm import dense_decode
+    gen = generator(7)
+    h, hq, B, dtype = 2, 16, 32, torch.float16
+    pages = pool(gen, 700, h, B, dtype)
+    table = tables(gen, [3000, 17000], B, 700)
+    q, workspace = rows(gen, 2, hq, 128, dtype=dtype), _workspace()
+    small, big = i32([3000]), i32([3000, 17000])
+    out, start = torch.empty((1, hq, 128), dtype=dtype, device="cuda"), pages.weights.clone()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        dense_decode(q[:1], pages, table[:1], small, 3000, SCALE, workspace, out, accumulate=True)
+    stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(stream):
+            dense_decode(q, pages, table, big, 17000, SCALE, workspace, accumulate=True)
+            others = [torch.full((1 << 18,), float(i), device="cuda") for i in range(8)]
+            pages.weights.copy_(start)
+            graph.replay()
+        torch.cuda.synchronize()
+        _check_decode(q[:1], pages, table, [3000], SCALE, out, start, True)
+        assert all((x == float(i)).all() for i, x in enumerate(others))
 
 
 # ---------------------------------------------------------------- writing
