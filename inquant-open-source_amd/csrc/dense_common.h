@@ -25,23 +25,42 @@ __device__ __forceinline__ int64_t dense_page(const DensePool &p, int64_t seq, i
     return id >= 0 && id < p.pages ? id : -1;
 }
 
-// Copies cache row `from` of a head to cache row `to` (16 lanes: a row each of
-// key and value, and by the first lane its weight and position).
-__device__ __forceinline__ void dense_move(const DensePool &p, int64_t seq, int64_t h, int64_t from, int64_t to,
-                                           int lane)
+// Copies cache rows from[i] of a head to cache rows to[i] (16 lanes: a row each
+// of key and value, and by the first lane its weight and position; rows below 0
+// are none).  All loads go before all stores: no row is both read and written.
+template <int N>
+__device__ __forceinline__ void dense_move(const DensePool &p, int64_t seq, int64_t h, const int32_t *from,
+                                           const int32_t *to, int lane)
 {
-    const int64_t pf = dense_page(p, seq, from), pt = dense_page(p, seq, to);
-    if (pf < 0 || pt < 0) return;
-    const int64_t rf = from & (p.B - 1), rt = to & (p.B - 1);
-    const u32x4 k = ld16(p.key + pf * p.k_sp + h * p.k_sh + rf * p.k_st + 8 * lane);
-    const u32x4 v = ld16(p.value + pf * p.v_sp + h * p.v_sh + rf * p.v_st + 8 * lane);
-    *(u32x4 *)(p.key + pt * p.k_sp + h * p.k_sh + rt * p.k_st + 8 * lane) = k;
-    *(u32x4 *)(p.value + pt * p.v_sp + h * p.v_sh + rt * p.v_st + 8 * lane) = v;
-    if (lane == 0) {
-        const int64_t of = (pf * p.H + h) * p.B + rf, ot = (pt * p.H + h) * p.B + rt;
-        p.weights[ot] = p.weights[of];
-        p.positions[ot] = p.positions[of];
+    int64_t pf[N], pt[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        pf[i] = dense_page(p, seq, from[i]);
+        pt[i] = dense_page(p, seq, to[i]);
     }
+    u32x4 k[N], v[N];
+    float w[N];
+    int32_t pos[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (pf[i] >= 0 && pt[i] >= 0) {
+            const int64_t r = from[i] & (p.B - 1), o = (pf[i] * p.H + h) * p.B + r;
+            k[i] = ld16(p.key + pf[i] * p.k_sp + h * p.k_sh + r * p.k_st + 8 * lane);
+            v[i] = ld16(p.value + pf[i] * p.v_sp + h * p.v_sh + r * p.v_st + 8 * lane);
+            w[i] = p.weights[o];
+            pos[i] = p.positions[o];
+        }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (pf[i] >= 0 && pt[i] >= 0) {
+            const int64_t r = to[i] & (p.B - 1), o = (pt[i] * p.H + h) * p.B + r;
+            *(u32x4 *)(p.key + pt[i] * p.k_sp + h * p.k_sh + r * p.k_st + 8 * lane) = k[i];
+            *(u32x4 *)(p.value + pt[i] * p.v_sp + h * p.v_sh + r * p.v_st + 8 * lane) = v[i];
+            if (lane == 0) {
+                p.weights[o] = w[i];
+                p.positions[o] = pos[i];
+            }
+        }
 }
 
 // Checks the pages and block tables of an entry point and fills `pool`.

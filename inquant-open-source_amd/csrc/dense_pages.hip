@@ -26,46 +26,43 @@ struct WriteArgs {
 
 // Bound by memory: 512 bytes of keys and values are read and written per row
 // and head.  Sixteen lanes move a row (16 bytes of its key and of its value
-// each); a workgroup takes WR_ITEMS (row, head) pairs, heads innermost, so that
-// it reads one contiguous range of token-major rows (with `keep` rows
-// innermost: it then writes one contiguous range of a head's pages).
-constexpr int WR_ITEMS = 64;
+// each), a workgroup sixteen (row, head) pairs, heads innermost: it reads one
+// contiguous range of token-major rows (with `keep` rows are innermost: it
+// writes one contiguous range of a head's pages).  The rows stream past the
+// caches, and one row per lane keeps eight wavefronts on a SIMD: 61994 rows of
+// seven prompts, 8 heads: 92 us (5.6 TB/s), 98 with ordinary stores, 106 with
+// four rows a lane one after the other, 111 with four at once.
+constexpr int WR_ITEMS = 16;
 
 __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 {
-    const int seq = blockIdx.y, lane = threadIdx.x & 15, H = a.pool.H;
-    const int64_t t0 = a.cu[seq], len = a.cu[seq + 1] - t0;
-    const int64_t rows = a.keep ? a.kept : len;
-    const int64_t start = a.start ? a.start[seq] : 0;
-    const int32_t pos0 = a.positions ? a.positions[seq] : (int32_t)start;
-    const int64_t first = (int64_t)blockIdx.x * WR_ITEMS + (threadIdx.x >> 4);
-#pragma unroll
-    for (int i = 0; i < WR_ITEMS / 16; ++i) {
-        const int64_t item = first + 16 * i;
-        if (item >= rows * H) break;
-        int64_t h, j, source;
-        if (a.keep) {
-            h = item / a.kept;
-            j = item - h * a.kept;
-            source = a.keep[((int64_t)seq * H + h) * a.kept + j];
-            if (source < 0 || source >= len) continue;
-        } else {
-            j = source = item / H;
-            h = item - j * H;
-        }
-        const int64_t row = start + j;
-        const int64_t page = dense_page(a.pool, seq, row);
-        if (page < 0) continue;
-        const int64_t at = row & (a.pool.B - 1), token = t0 + source;
-        const u32x4 kv = ld16(a.k + token * a.k_st + h * a.k_sh + 8 * lane);
-        const u32x4 vv = ld16(a.v + token * a.v_st + h * a.v_sh + 8 * lane);
-        *(u32x4 *)(a.pool.key + page * a.pool.k_sp + h * a.pool.k_sh + at * a.pool.k_st + 8 * lane) = kv;
-        *(u32x4 *)(a.pool.value + page * a.pool.v_sp + h * a.pool.v_sh + at * a.pool.v_st + 8 * lane) = vv;
-        if (lane == 0 && a.pool.weights) {
-            const int64_t o = (page * H + h) * a.pool.B + at;
-            a.pool.weights[o] = a.weights ? a.weights[h * a.w_stride + token] : 0.0f;
-            a.pool.positions[o] = pos0 + (int32_t)source;
-        }
+    const int seq = blockIdx.y, lane = threadIdx.x & 15;
+    const uint32_t H = (uint32_t)a.pool.H, kept = (uint32_t)a.kept;
+    const int64_t t0 = a.cu[seq], have = a.cu[seq + 1] - t0;
+    const uint32_t len = have > 0 ? (uint32_t)have : 0, item = blockIdx.x * WR_ITEMS + (threadIdx.x >> 4);
+    if (item >= (uint64_t)(a.keep ? kept : len) * H) return;
+    uint32_t h, j, source;
+    if (a.keep) {
+        h = item / kept;
+        j = item - h * kept;
+        source = (uint32_t)a.keep[((int64_t)seq * H + h) * kept + j];
+    } else {
+        j = source = item / H;
+        h = item - j * H;
+    }
+    const int64_t start = a.start ? a.start[seq] : 0, row = start + j;
+    const int64_t page = dense_page(a.pool, seq, row), at = row & (a.pool.B - 1), token = t0 + source;
+    if (source >= len || page < 0) return;               // an entry below 0 is past any length
+    const u32x4 kv = ld16(a.k + token * a.k_st + h * a.k_sh + 8 * lane);
+    const u32x4 vv = ld16(a.v + token * a.v_st + h * a.v_sh + 8 * lane);
+    __builtin_nontemporal_store(
+        kv, (u32x4 *)(a.pool.key + page * a.pool.k_sp + h * a.pool.k_sh + at * a.pool.k_st + 8 * lane));
+    __builtin_nontemporal_store(
+        vv, (u32x4 *)(a.pool.value + page * a.pool.v_sp + h * a.pool.v_sh + at * a.pool.v_st + 8 * lane));
+    if (lane == 0 && a.pool.weights) {
+        const int64_t o = (page * H + h) * a.pool.B + at;
+        a.pool.weights[o] = a.weights ? a.weights[h * a.w_stride + token] : 0.0f;
+        a.pool.positions[o] = (a.positions ? a.positions[seq] : (int32_t)start) + (int32_t)source;
     }
 }
 
@@ -343,8 +340,14 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     if constexpr (MOVE) {
         __syncthreads();
         const int n = list[0];
-        for (int m = threadIdx.x >> 4; m < n; m += SEL_NT / 16)
-            dense_move(a.pool, seq, h, behind[n - 1 - m], holes[m], threadIdx.x & 15);
+        int32_t from[FEW * 16 / SEL_NT], to[FEW * 16 / SEL_NT];
+#pragma unroll
+        for (int i = 0; i < FEW * 16 / SEL_NT; ++i) {
+            const int m = i * (SEL_NT / 16) + (threadIdx.x >> 4);
+            from[i] = m < n ? behind[n - 1 - m] : -1;
+            to[i] = m < n ? holes[m] : -1;
+        }
+        dense_move<FEW * 16 / SEL_NT>(a.pool, seq, h, from, to, threadIdx.x & 15);
     }
 }
 
@@ -357,7 +360,7 @@ __global__ void evict_lengths_kernel(EvictArgs a, int n)
 }
 
 // Moves the kept rows into the evicted places; sixteen lanes a row.
-constexpr int MV_ROWS = 64;
+constexpr int MV_ROWS = 16;
 
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a)
 {
@@ -366,12 +369,15 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a)
     const int n = list[0];
     const int32_t *holes = list + 1, *behind = holes + a.most;
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) evict_length(a, seq);
+    if ((int)blockIdx.x * MV_ROWS >= n) return;
+    int32_t from[MV_ROWS / 16], to[MV_ROWS / 16];
 #pragma unroll
     for (int i = 0; i < MV_ROWS / 16; ++i) {
-        const int64_t m = (int64_t)blockIdx.x * MV_ROWS + 16 * i + (threadIdx.x >> 4);
-        if (m >= n) break;
-        dense_move(a.pool, seq, h, behind[n - 1 - m], holes[m], lane);
+        const int m = blockIdx.x * MV_ROWS + 16 * i + (threadIdx.x >> 4);
+        from[i] = m < n ? behind[n - 1 - m] : -1;
+        to[i] = m < n ? holes[m] : -1;
     }
+    dense_move<MV_ROWS / 16>(a.pool, seq, h, from, to, lane);
 }
 
 }  // namespace
