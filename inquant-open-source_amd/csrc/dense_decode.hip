@@ -118,6 +118,20 @@ struct FirstRows {
 // whose logits stay in registers until the lse is known.
 enum Mode { PARTS, DIRECT_LOOP, ONE };
 
+// lds_load16 past the caches, as the keys are read: rows are read once per call
+// (16 sequences of 2K-32K tokens: 107 us, 110 with both through the caches, 114
+// with one each way).
+__device__ __forceinline__ void lds_load16_nt(const void *base, uint32_t voff, uint32_t lds_base)
+{
+    const uint64_t b = (uint64_t)(uintptr_t)base;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+    const uint64_t sb = (uint64_t)lo | ((uint64_t)hi << 32);
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sb),
+                 "s"(__builtin_amdgcn_readfirstlane(lds_base))
+                 : "memory");
+}
+
 template <bool F16, Mode MODE, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void dense_partials(DecodeArgs a)
 {
@@ -183,7 +197,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_partials(DecodeArgs a)
             const int lim = len - 1 - (c0 + 16 * t < len ? c0 + 16 * t : (len - 1) & ~15);
             const int r = rl < lim ? rl : lim;
             const int chunk = c16 ^ (4 * (rl & 3)) ^ (2 * ((rl >> 2) & 1));
-            lds_load16(vt[t], (uint32_t)(r * (int)p.v_st + 8 * chunk) * 2, lds_v + (uint32_t)(4 * i * D * 2));
+            lds_load16_nt(vt[t], (uint32_t)(r * (int)p.v_st + 8 * chunk) * 2, lds_v + (uint32_t)(4 * i * D * 2));
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) sc[t] = f32x4{0, 0, 0, 0};
