@@ -242,10 +242,10 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) late[kb][i] = NEG_INF;
     float m = 0.0f, use = 0.0f, l = 0.0f;
-    // Four of a lane's 32 logits, in step d of 8.
-    auto work_off = [&](int d) {
+    // Two of a lane's 32 logits, in half e of step d of 8.
+    auto work_off = [&](int d, int part) {
         if constexpr (LSEPASS) {
-            if (d == 0) {
+            if (d == 0 && part == 0) {
                 m = NEG_INF;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -256,16 +256,16 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
                 l = 0.0f;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 2 * part; e < 2 * part + 2; ++e)
                 l += __builtin_amdgcn_exp2f(fmaf(late[d >> 2][4 * (d & 3) + e], a.c_log2, -use));
-            if (d == 7) {
+            if (d == 7 && part == 1) {
                 l = pair_sum(l);
                 if (h32 == 0 && late_row >= 0)
                     a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.H + h) * a.G * a.window + late_row] = f32x2{m, l};
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 2 * part; e < 2 * part + 2; ++e) {
                 const int kb = d >> 2, i = 4 * (d & 3) + e;
                 sum[kb][i] += __builtin_amdgcn_exp2f(fmaf(late[kb][i], a.c_log2, -late_lse2));
             }
@@ -282,10 +282,12 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) sc[kb] = mma3232<F16>(kf[kb][d], qv[d], sc[kb]);
+            sc[0] = mma3232<F16>(kf[0][d], qv[d], sc[0]);
+            work_off(d, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            sc[1] = mma3232<F16>(kf[1][d], qv[d], sc[1]);
             qv[d] = operand(st, b, d);
-            work_off(d);
+            work_off(d, 1);
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (!LSEPASS) asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));   // added here, not at the loop's end
@@ -365,7 +367,7 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         if (!next()) break;
     }
 #pragma unroll
-    for (int d = 0; d < 8; ++d) work_off(d);
+    for (int d = 0; d < 16; ++d) work_off(d >> 1, d & 1);
     if constexpr (!LSEPASS) {
         float *out = a.out + ((int64_t)range * a.Hq + list) * a.out_sh + start;
         // Sums over the 32 queries: a swap of the odd 16-lane rows of one key's
