@@ -170,7 +170,8 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     // wavefront, four (1 KB) per load, and its lse; rows past the end repeat
     // the last one.
     int next_qa = last_tile;
-    const uint32_t row_bytes = (uint32_t)a.q_st * 2;
+    const uint32_t row_bytes = (uint32_t)a.q_st * 2, head_bytes = (uint32_t)a.q_sh * 2;
+    const float win_rcp = 1.0f / (float)win.n;
     uint32_t whole[4];                       // a load's offset where no row is past the end
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -182,24 +183,28 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         const int last = end - 1 - next_qa;
         const uint32_t to_l = lds_l + (uint32_t)(st * NW * QT * 4);
         if constexpr (ROWS) {
-            // head and query of the tile's row r
-            auto place = [&](int r, int &head, int &i) {
-                const int row = next_qa + (r < last ? r : last), g = row / win.n;
-                i = row - g * win.n;
-                head = h * a.G + g;
+            // query head (of this KV head) and query of the tile's row r.  The quotient
+            // by a reciprocal is exact: rows are below 2^21, and the half keeps its
+            // error (2^-22 of it) from the next whole number.
+            auto place = [&](int r, uint32_t &g, uint32_t &i) {
+                const int row = next_qa + (r < last ? r : last);
+                g = (uint32_t)(((float)row + 0.5f) * win_rcp);
+                i = (uint32_t)row - g * (uint32_t)win.n;
                 return row;
             };
-            int head, i;
+            uint32_t g, i;
             if constexpr (!LSEPASS) {
-                const int row = place(lane, head, i);
-                lds_gather4(a.lse_sh ? a.lse + head * a.lse_sh + start + win.lo + i : own_lse + row, to_l);
+                const int row = place(lane, g, i);
+                lds_gather4(a.lse_sh ? (const char *)(a.lse + (int64_t)h * a.G * a.lse_sh + start + win.lo) +
+                                           (int64_t)g * a.lse_sh * 4 + 4 * i
+                                     : (const char *)(own_lse + row), to_l);
             }
+            const char *first = (const char *)(a.q + (int64_t)(start + win.lo) * a.q_st + (int64_t)h * a.G * a.q_sh);
 #pragma unroll
             for (int l = 0; l < 4; ++l) {
                 const int r = 16 * wave + 4 * l + (lane >> 4);
-                place(r, head, i);
-                const uint16_t *qp = a.q + (int64_t)(start + win.lo + i) * a.q_st + (int64_t)head * a.q_sh;
-                lds_gather16(qp + 8 * ((lane & 15) ^ (r & 15)),
+                place(r, g, i);
+                lds_gather16(first + (uint64_t)i * row_bytes + (uint64_t)g * head_bytes + 16 * ((lane & 15) ^ (r & 15)),
                              lds_q + (uint32_t)((st * QT + 16 * wave + 4 * l) * D * 2));
             }
         } else {
@@ -485,7 +490,9 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     IQ_CHECK_ARG(((uintptr_t)q | (uintptr_t)k) % 16 == 0 && (q_st | q_sh | k_st | k_sh) % 8 == 0,
                  "iq_prefill_weights: q/k rows must be 16-byte aligned");
     // a query tile's rows are addressed by 32-bit byte offsets from its first row
-    IQ_CHECK_ARG(q_st >= 0 && q_st < (1LL << 25), "iq_prefill_weights: token stride too large");
+    IQ_CHECK_ARG(q_st >= 0 && q_st < (1LL << 25) && q_sh >= 0 && q_sh < (1LL << 31),
+                 "iq_prefill_weights: query strides too large");
+    IQ_CHECK_ARG(Hq / H * window < (1LL << 21), "iq_prefill_weights: window too large");
     IQ_CHECK_ARG(scale > 0.0f, "iq_prefill_weights: the scale must be positive");
     IQ_CHECK_ARG(window >= 0 && window <= 65536 && (window > 0 || lse), "iq_prefill_weights: no window and no lse");
     IQ_CHECK_ARG(!lse || lse_sh > 0, "iq_prefill_weights: bad lse stride");
