@@ -412,7 +412,7 @@ extern "C" int iq_select_rows(const float *weights, int64_t w_stride, int64_t H,
                               int32_t *keep, void *stream)
 {
     IQ_CHECK_ARG(weights && cu_seqlens && keep, "iq_select_rows: null pointer");
-    IQ_CHECK_ARG(H >= 1 && H <= 65535 && n_seq >= 0 && n_seq <= 65535 && max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL,
+    IQ_CHECK_ARG(H >= 1 && H <= 65535 && n_seq >= 0 && n_seq <= 65535 && max_seqlen >= 0 && max_seqlen <= 0x3fffffff,
                  "iq_select_rows: bad head or sequence count or length");
     IQ_CHECK_ARG(sink >= 0 && recent >= 0 && budget >= 1 && budget <= 0x7fffffffLL && sink + recent <= budget,
                  "iq_select_rows: sink and recent rows must fit the budget");

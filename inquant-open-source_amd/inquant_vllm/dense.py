@@ -154,13 +154,15 @@ def _tables(block_tables, n):
 
 
 def _token_rows(t, what, heads=None):
-    """Shape and strides of token-major rows."""
+    """Shape and (token, head) strides of token-major rows."""
     shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[2] != 128 or (heads is not None and shape[1] != heads):
         raise ValueError(f"Expected {what} [tokens, heads, 128]")
-    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or t.data_ptr() % 16:
+    # any stride will do for a dimension of one
+    st, sh = stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
+    if stride[2] != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
         raise ValueError(f"{what} rows must be contiguous and 16-byte aligned")
-    return shape, stride
+    return shape, (st, sh)
 
 
 def _budget(budget, sink, recent):

@@ -117,14 +117,14 @@ def test_refusals_of_the_library():
                  v_sh=2048, v_st=128, pages=4, heads=2, block_tokens=16)
         return ctypes.byref(nat.DensePagesDesc(**{**f, **more}))
 
-    def decode(p, hq=4, most=32, floats=1 << 30, dtype=nat.IQ_BF16, accumulate=0):
-        return lib.iq_dense_decode(fake, dtype, 512, 128, hq, 1, p, fake, 2, 2, fake, most, 0.1, accumulate, fake, floats,
+    def decode(p, hq=4, most=640, floats=1 << 30, dtype=nat.IQ_BF16, accumulate=0):
+        return lib.iq_dense_decode(fake, dtype, 512, 128, hq, 1, p, fake, 40, 40, fake, most, 0.1, accumulate, fake, floats,
                                    fake, 512, 128, nat.IQ_BF16, None)
     bad = [dict(key=0), dict(heads=0), dict(pages=0), dict(block_tokens=48), dict(key=fake + 8), dict(k_st=100),
            dict(k_st=1 << 24), dict(weights=0)]
     for change in bad:
         assert decode(pages(**change)) == -1, change
-    assert decode(pages(), hq=5) == -1 and decode(pages(), hq=34) == -1 and decode(pages(), most=33) == -1
+    assert decode(pages(), hq=5) == -1 and decode(pages(), hq=34) == -1 and decode(pages(), most=641) == -1
     assert decode(pages(), floats=10, accumulate=1) == -1 and b"workspace" in lib.iq_last_error()
     assert decode(pages(), dtype=nat.IQ_F32) == -1
     assert decode(pages(weights=0, positions=0), accumulate=1) == -1

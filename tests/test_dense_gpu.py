@@ -154,21 +154,30 @@ def test_decode_skips_ids_outside_the_pool_and_adds_shared_pages():
     assert ((pages.weights.double() - total).abs() <= bound).all()
 
 
-def test_decode_past_2_31_elements():
-    # pages whose rows start past 2^32 bytes of the pool
-    from inquant_vllm import DensePages, dense_decode
+def test_pages_past_2_31_elements():
+    """Rows past 2^32 bytes of the pool: decoded, written and evicted."""
+    from inquant_vllm import DensePages, dense_decode, evict_rows, write_rows
     gen = generator(5)
-    h, B, count = 8, 256, 9000
-    key = torch.empty((count, h, B, 128), dtype=torch.bfloat16, device="cuda")
-    value = torch.empty_like(key)
-    assert key.numel() > 1 << 31
-    ids = [8999, 0, 8500]
-    for p in ids:
-        key[p], value[p] = rows(gen, h, B, 128, dtype=torch.bfloat16), rows(gen, h, B, 128, dtype=torch.bfloat16)
-    pages = DensePages(key, value)
-    q = rows(gen, 1, 16, 128, dtype=torch.bfloat16)
-    out = dense_decode(q, pages, i32([ids]), i32([700]), 700, SCALE, _workspace())
-    _check_decode(q, pages, i32([ids]), [700], SCALE, out, None, False)
+    h, B, count, dtype = 8, 256, 9000, torch.bfloat16
+    pages = DensePages.allocate(count, B, h, dtype)
+    assert pages.key.numel() > 1 << 31
+    table = i32([[8999, 0, 8500]])
+    key, value = rows(gen, 700, h, 128, dtype=dtype), rows(gen, 700, h, 128, dtype=dtype)
+    weights = torch.rand((h, 700), generator=gen, device="cuda")
+    write_rows(key, value, offsets([700]), 700, pages, table, weights=weights)
+    for field, want in ((pages.key, key), (pages.value, value)):
+        assert torch.equal(cache_rows(field, table[0], 700), want.transpose(0, 1))
+    assert torch.equal(cache_rows(pages.weights, table[0], 700), weights)
+    q, before = rows(gen, 1, 16, 128, dtype=dtype), pages.weights.clone()
+    out = dense_decode(q, pages, table, i32([700]), 700, SCALE, _workspace(), accumulate=True)
+    _check_decode(q, pages, table, [700], SCALE, out, before, True)
+    evict_rows(pages, table, i32([700]), i32([700]), 700, 300, sink=4, recent=100)
+    kept = cache_rows(pages.positions, table[0], 300).long().sort(-1).values
+    for head in range(h):
+        assert set(range(4)) | set(range(600, 700)) <= set(kept[head].tolist())
+        where = cache_rows(pages.positions, table[0], 300)[head].long()
+        assert torch.equal(cache_rows(pages.key, table[0], 300)[head], key[where, head])
+        assert torch.equal(cache_rows(pages.value, table[0], 300)[head], value[where, head])
 
 
 def test_decode_in_a_graph_replays_with_new_lengths_on_another_stream():
@@ -292,6 +301,17 @@ def test_write_rows_is_exact(case, dtype):
     write_rows(key, value, offsets(lengths), max(lengths), pages, table, None if start is None else i32(start),
                positions=None if start is None else i32(positions), weights=weights, keep=keep)
     _same(pages, exp)
+
+
+def test_write_one_token_of_odd_strides():
+    from inquant_vllm import write_rows
+    gen = generator(30)
+    pages = pool(gen, 4, 1, 16, torch.float16)
+    # dimensions of one, whose strides say nothing
+    key = torch.as_strided(rows(gen, 4, 128, dtype=torch.float16), (1, 1, 128), (3, 5, 1))
+    write_rows(key, key, offsets([1]), 1, pages, i32([[2]]), i32([7]))
+    assert torch.equal(pages.key[2, 0, 7], key[0, 0]) and torch.equal(pages.value[2, 0, 7], key[0, 0])
+    assert pages.weights[2, 0, 7] == 0 and pages.positions[2, 0, 7] == 7
 
 
 # ---------------------------------------------------------------- selection
