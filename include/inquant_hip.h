@@ -42,6 +42,7 @@
  *   iq_prefill_attention extensions/vllm/src/inquant_vllm/backend.py:139-144
  *                       (flash_attn_varlen_func, causal prefill on exact K/V);
  *                       iq_prefill_attention_tokens, the same with the token count
+ *                       (iq_prefill_attention_lse: and each query's lse)
  *   iq_tail_append      src/inquant/cache.py:256-259,283-286 (the dense tail
  *                       concatenation of append_for_attention / _append)
  */

@@ -8,7 +8,11 @@
 // registers (64 per wavefront, 256 per workgroup) while tiles of 64 queries
 // stream through LDS, so a key's sum over the queries is one fp32 add per
 // logit in the lane that holds it, and is added over the 32 lanes (queries of
-// a tile) once, at the end.
+// a tile) once, at the end.  Bound by the matrix cores and the VALU together: a
+// 32 x 64 half tile has 16 products of 32 cycles and, per lane, 32 exponentials
+// of 8 and 64 fused multiply-adds and adds of 4, which overlap in part (311 ns a
+// half and SIMD in a loop of nothing else, the products alone 227).  8192 causal
+// queries, 28 heads over 4: 255 us, 0.94 PFLOP/s.
 #include <type_traits>
 
 #include "decode_common.h"
