@@ -34,7 +34,7 @@ struct WeightArgs {
     const int32_t *cu;
     int n_seq, max_len, H, Hq, G;              // a sequence's rows past max_len are left out
     int window;                              // WINDOW: queries of each sequence from its end
-    int chunk, chunks, tiles;                // a workgroup's queries at most, their ranges, and key tiles
+    int chunk, chunks;                       // a workgroup's queries at most, and their ranges
     float c_log2;
     const float *lse;                        // natural log, token i of head hq at hq * lse_sh + i; with lse_sh 0
     int64_t lse_sh;                          // window row r of (seq, h) at (seq * H + h) * G * window + r
@@ -135,16 +135,30 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     __shared__ WeightSmem sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c32 = lane & 31, h32 = lane >> 5;
-    // An item is a (query range, key tile, sequence, head); the ranges go from
-    // the last back and the key tiles from the first on, so the workgroups that
-    // start together read the same queries and the ranges' short last items
-    // (on the diagonal) come after their long ones.
+    // An item is a (query range, key tile, sequence, head), the longest first:
+    // ranges that see all of a key tile's queries (the last range, which may be
+    // short, after the others), then the ranges on the diagonal, whose j-th key
+    // tile sees all queries but 256 j.
     const int lists = ROWS ? a.H : a.Hq;
     int rest = blockIdx.x / lists;
     const int list = blockIdx.x - rest * lists, h = ROWS ? list : list / a.G;
     const int seq = rest % a.n_seq;
     rest /= a.n_seq;
-    const int tile = rest % a.tiles, range = ROWS ? 0 : a.chunks - 1 - rest / a.tiles;
+    int tile = rest, range = 0;
+    if constexpr (!ROWS) {
+        const int m = a.chunk / KG, full = m * a.chunks * (a.chunks - 1) / 2;    // key tiles per range; whole items
+        if (rest < full) {
+            range = a.chunks > 2 ? a.chunks - 2 : 1;
+            while (tile >= range * m) {
+                tile -= range * m;
+                range = range > 1 ? range - 1 : a.chunks - 1;
+            }
+        } else {
+            rest -= full;
+            range = a.chunks - 1 - rest % a.chunks;
+            tile = range * m + rest / a.chunks;
+        }
+    }
     const int start = a.cu[seq], len = length_of(a, seq);
     const int g0 = tile * KG, from = range * a.chunk;
     // "queries" are query positions, or with ROWS rows of the window
@@ -444,15 +458,36 @@ struct Scratch {
     int64_t lse, ml, part;                   // floats of each
 };
 
-// Queries of a workgroup: 4096, or fewer while that leaves the 512 that run at
-// once without a second one (a multiple of the key tile, so that a range either
-// sees a whole key tile or ends before it).
+// Queries of a workgroup at most, a power of two and of whole key tiles (so that a
+// range sees a whole key tile or ends before it): the one for which the longest
+// prompt ends first, by the 64-query tiles of all workgroups over the 512 places,
+// those of the longest workgroup, and some of its tail; a workgroup's start counts
+// as four tiles.  The starts weigh against short ranges, idle places against long
+// ones (28 heads over 4, 8192 queries: 4096 a workgroup; 4096 queries: 1024, 84 us
+// against 92 with the tiles in order and no estimate; 1000 queries: 512, 23 us, and
+// 26 with 256).
 int64_t chunk_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen)
 {
-    int64_t chunk = 4096;
-    const int64_t tiles = (max_seqlen + KG - 1) / KG;
-    while (chunk > 512 && tiles * Hq * n_seq * ((max_seqlen + chunk - 1) / chunk) < 1024) chunk /= 2;
-    return chunk;
+    int64_t best = 512;
+    double least = 1e30;
+    for (int64_t chunk = best; chunk <= 8192; chunk *= 2) {
+        const int64_t ranges = (max_seqlen + chunk - 1) / chunk;
+        double all = 0, longest = 0;
+        for (int64_t r = 0; r < ranges; ++r) {
+            const int64_t n = max_seqlen - r * chunk < chunk ? max_seqlen - r * chunk : chunk;   // its queries
+            const double whole = (double)((n + QT - 1) / QT), diagonal = (double)((n + KG - 1) / KG);
+            all += (double)(r * chunk / KG) * (whole + 4) + diagonal * (whole / 2 + 4);
+            longest = whole + 4 > longest ? whole + 4 : longest;
+        }
+        all *= (double)(Hq * n_seq) / 512;
+        const double cost = (all > longest ? all : longest) + longest / 8;
+        if (cost < least) {
+            least = cost;
+            best = chunk;
+        }
+        if (ranges == 1) break;
+    }
+    return best;
 }
 
 Scratch scratch_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t window, bool lse)
@@ -511,11 +546,12 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     const int64_t tiles = (max_seqlen + KG - 1) / KG, G = Hq / H;
     const int64_t chunk = window ? 1 << 30 : chunk_of(Hq, n_seq, max_seqlen), chunks = (max_seqlen + chunk - 1) / chunk;
     WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq,
-                 (int)max_seqlen, (int)H, (int)Hq, (int)G, (int)window, (int)chunk, (int)chunks, (int)tiles,
+                 (int)max_seqlen, (int)H, (int)Hq, (int)G, (int)window, (int)chunk, (int)chunks,
                  scale * LOG2E, lse, lse_sh, (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
-    const int64_t items = chunks * tiles * (window ? H : Hq) * n_seq;
+    const int64_t m = chunk / KG, units = window ? tiles : m * chunks * (chunks - 1) / 2 + m * chunks;
+    const int64_t items = units * (window ? H : Hq) * n_seq;
     IQ_CHECK_ARG(items <= 0xffffff, "iq_prefill_weights: too many key tiles");
     const dim3 grid((unsigned)items), block(NT);
     if (window > 0) {
