@@ -348,13 +348,14 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         late_lse2 = lse2;
         late_row = query < end && k0 < len ? query : -1;
         if (masked) {
-            if constexpr (LSEPASS) {
+            // an lse that is NaN or -inf would turn the unseen's -inf into NaN
+            if (LSEPASS || !__builtin_amdgcn_ballot_w64(!(lse2 > NEG_INF))) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) late[kb][i] = seen(kb, i) ? sc[kb][i] : NEG_INF;   // the scale is positive
             } else {
-                // added at once, the unseen left out (whatever their logit and lse), so that nothing is pending
+                // added at once, the unseen left out, so that nothing is pending
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
