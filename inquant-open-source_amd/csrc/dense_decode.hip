@@ -171,6 +171,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_partials(DecodeArgs a)
     for (int c0 = t0 + WT * wave; c0 < end; c0 += WT * NW) {
         const uint16_t *kt[4], *vt[4];       // first row of each 16-row tile
         u32x4 kf[4][4];
+        uint32_t outside = 0;                // tiles of ids outside the pool, which read page 0
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             // a tile past the end reads the tile of the last row again (masked)
@@ -178,6 +179,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_partials(DecodeArgs a)
             const int id = table[tb >> p.shift];
             const bool ok = id >= 0 && id < p.pages;
             const int64_t page = ok ? id : 0;
+            outside |= ok ? 0 : 1u << t;
             const int row = tb & (p.B - 1);
             kt[t] = p.key + page * p.k_sp + h * p.k_sh + row * p.k_st;
             vt[t] = p.value + page * p.v_sp + h * p.v_sh + row * p.v_st;
@@ -242,6 +244,12 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_partials(DecodeArgs a)
         for (int cb = 0; cb < 8; ++cb) acc[cb] *= alpha;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wavefront's V rows have landed
         const uint16_t *sv = sm.v[wave];
+        // a weight of 0 does not hide what page 0 may hold (NaN, infinities)
+        for (; outside; outside &= outside - 1) {
+            uint16_t *rows = sm.v[wave] + 16 * __builtin_ctz(outside) * D;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(u32x4 *)(rows + (4 * i + g4) * D + 8 * c16) = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll

@@ -154,6 +154,35 @@ def test_decode_skips_ids_outside_the_pool_and_adds_shared_pages():
     assert ((pages.weights.double() - total).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+@pytest.mark.parametrize("length,bound", [(60, 60), (200, 500), (1500, 1500), (700, 700)])
+def test_ids_outside_the_pool_let_nothing_of_page_0_through(poison, length, bound):
+    from inquant_vllm import dense_decode
+    print(f"dense decode outside {poison} {length} {bound}", flush=True)
+    gen = generator(length)
+    h, hq, B, n = 4, 8, 16, 800 if length == 700 else 2     # 800 sequences: one workgroup takes all rows of each
+    count = -(-length // B) + 1
+    pages = pool(gen, count, h, B, torch.bfloat16)
+    pages.key[0], pages.value[0] = poison, poison
+    table = (1 + torch.arange(-(-bound // B), device="cuda") % (count - 1)).to(torch.int32).expand(n, -1).clone()
+    outside = torch.arange(table.shape[1], device="cuda") % 3 == 1
+    table[:, outside] = i32([-1, count])[torch.arange(int(outside.sum()), device="cuda") % 2]
+    q = rows(gen, 1, hq, 128, dtype=torch.bfloat16).expand(n, -1, -1)
+    before = pages.weights.clone()
+    out = dense_decode(q, pages, table, i32([length] * n), bound, SCALE, _workspace(), accumulate=True)
+    at = torch.arange(length, device="cuda")
+    at = at[~outside[at // B]]
+    page = table[0, at // B].long()
+    k, v = (f[page, :, at % B].transpose(0, 1) for f in (pages.key, pages.value))
+    exp, _, w, slack = attend(q[0].unsqueeze(1), k, v, SCALE)
+    assert float((out.double() - exp[:, 0]).abs().max()) <= output_bound(v, torch.bfloat16, torch.bfloat16, slack)
+    total = before.double()
+    total[page, :, at % B] += n * w.t()
+    # every sequence's weight is added in turn: n roundings of the sum
+    bound = (total - before.double()).abs() * (4 * slack + 2.0 ** -18) + total.abs() * (n + 1) * 2.0 ** -24
+    assert ((pages.weights.double() - total).abs() <= bound).all()
+
+
 def test_pages_past_2_31_elements():
     """Rows past 2^32 bytes of the pool: decoded, written and evicted."""
     from inquant_vllm import DensePages, dense_decode, evict_rows, write_rows
