@@ -351,8 +351,8 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     }
 }
 
-// New lengths in the place of the old ones, which every head's workgroup reads:
-// by the launch after them.
+// New lengths in the place of the old ones or of the tokens seen, which every
+// head's workgroup reads: by the launch after them.
 __global__ void evict_lengths_kernel(EvictArgs a, int n)
 {
     const int seq = blockIdx.x * 256 + threadIdx.x;
@@ -451,7 +451,8 @@ extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int3
     const dim3 rows((unsigned)pool.H, (unsigned)n_seq), block(SEL_NT);
     const hipStream_t st = (hipStream_t)stream;
     if (most <= FEW) {
-        const bool apart = new_lengths + n_seq <= lengths || lengths + n_seq <= new_lengths;
+        const auto away = [&](const int32_t *p) { return new_lengths + n_seq <= p || p + n_seq <= new_lengths; };
+        const bool apart = away(lengths) && away(seen);
         if (!apart) a.new_lengths = nullptr;
         hipLaunchKernelGGL(evict_select_kernel<true>, rows, block, 0, st, a);
         a.new_lengths = new_lengths;

@@ -248,7 +248,7 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
     ties to the lowest cache row, NaN last.  The evicted cache rows below the
     budget take, in order, the kept rows from the budget on, so only those
     move; every other row stays as it is.  Returns the new lengths
-    min(lengths, budget), int32 [sequences] (``output`` may be ``lengths``).
+    min(lengths, budget), int32 [sequences] (``output`` may be ``lengths`` or ``seen``).
     No page may belong to two of the sequences."""
     budget, sink, recent, max_tokens = int(budget), int(sink), int(recent), int(max_tokens)
     _budget(budget, sink, recent)
@@ -307,13 +307,15 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     gpu = _on_gpu(pages._gpu, "dense_decode", query, block_tables, lengths, output)
     qs = query.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
-        query = query.contiguous()
+        query = query.clone(memory_format=torch.contiguous_format)
         qs = query.stride()
     if output is None:
         output = torch.empty(shape, dtype=query.dtype, device=query.device)
         code = pages._code
     elif output.shape != shape or output.stride(2) != 1 or output.dtype is not query.dtype and output.dtype is not _F32:
         raise ValueError("output must be [sequences, heads, 128] of the query dtype or float32")
+    elif n > 1 and output.stride(0) < 128 or hq > 1 and output.stride(1) < 128:
+        raise ValueError("the output's rows must not overlap")
     else:
         code = nat.IQ_F32 if output.dtype is _F32 else pages._code
     if n == 0:
@@ -367,8 +369,12 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         output = torch.empty((h, tokens), dtype=_F32, device=query.device)
     elif output.shape != (h, tokens) or output.dtype is not _F32 or output.stride(1) != 1 and tokens > 1:
         raise ValueError("output must be float32 [kv_heads, tokens]")
+    elif h > 1 and output.stride(0) < tokens:
+        raise ValueError("the output's heads must not overlap")
     if tokens == 0:
         return output
+    if lse is not None and lse.stride(0) < 1:
+        lse = lse.contiguous()               # one row for every head
     window = 0 if window is None else min(int(window), max_seqlen)
     if lse is not None and window == max_seqlen:
         window = 0                           # every query

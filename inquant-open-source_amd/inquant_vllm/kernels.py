@@ -150,8 +150,8 @@ def prefill_attention(query, key, value, cu_seqlens, max_seqlen, scale, output=N
         raise ValueError("output must be [tokens, Hq, 128] of the query dtype or float32")
     if lse is not None:
         if tuple(lse.shape) != (hq, query.shape[0]) or lse.dtype != torch.float32 \
-                or lse.stride(1) != 1 and lse.shape[1] > 1 or not scale > 0:
-            raise ValueError("lse must be float32 [query heads, tokens], and the scale positive")
+                or lse.stride(1) != 1 and lse.shape[1] > 1 or hq > 1 and lse.stride(0) < lse.shape[1] or not scale > 0:
+            raise ValueError("lse must be float32 [query heads, tokens], not expanded, and the scale positive")
         nat.require_gpu(query, lse, what="prefill_attention")
     cu = cu_seqlens.contiguous()
     nat.check(nat.lib().iq_prefill_attention_lse(

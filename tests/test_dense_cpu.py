@@ -144,6 +144,7 @@ def test_refusals_of_the_library():
 
 def test_prefill_attention_refuses_a_wrong_lse():
     q, k, cu = _rows(3, 4), _rows(), torch.tensor([0, 3], dtype=I32)
-    for lse in (torch.zeros((4, 2)), torch.zeros((4, 3)).double(), torch.zeros((3, 4)).t()):
+    for lse in (torch.zeros((4, 2)), torch.zeros((4, 3)).double(), torch.zeros((3, 4)).t(),
+                torch.zeros(3).expand(4, 3)):
         with pytest.raises((ValueError, RuntimeError)):
             prefill_attention(q, k, k, cu, 3, 0.1, lse=lse)

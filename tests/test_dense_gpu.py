@@ -154,6 +154,26 @@ def test_decode_skips_ids_outside_the_pool_and_adds_shared_pages():
     assert ((pages.weights.double() - total).abs() <= bound).all()
 
 
+def test_decode_one_query_of_odd_strides():
+    from inquant_vllm import dense_decode
+    gen = generator(6)
+    pages = pool(gen, 10, 1, 16, torch.bfloat16)
+    table, lengths = tables(gen, [77], 16, 10), i32([77])
+    wide = rows(gen, 2 * 128 + 1, dtype=torch.bfloat16)
+    want = dense_decode(wide[:128].clone().view(1, 1, 128), pages, table, lengths, 77, SCALE, _workspace())
+    # rows of one sequence and head may have any stride
+    out = torch.empty(300, dtype=torch.bfloat16, device="cuda").as_strided((1, 1, 128), (5, 3, 1))
+    assert dense_decode(wide.as_strided((1, 1, 128), (3, 5, 1)), pages, table, lengths, 77, SCALE, _workspace(),
+                        out).data_ptr() == out.data_ptr()
+    assert torch.equal(out, want)
+    with pytest.raises(ValueError, match="overlap"):
+        dense_decode(wide[:128].view(1, 1, 128).expand(1, 4, 128), pages, table, lengths, 77, SCALE, _workspace(),
+                     out.expand(1, 4, 128))
+    # and a row that is not aligned is copied
+    want = dense_decode(wide[1:129].clone().view(1, 1, 128), pages, table, lengths, 77, SCALE, _workspace())
+    assert torch.equal(dense_decode(wide[1:129].view(1, 1, 128), pages, table, lengths, 77, SCALE, _workspace()), want)
+
+
 @pytest.mark.parametrize("poison", [math.nan, math.inf])
 @pytest.mark.parametrize("length,bound", [(60, 60), (200, 500), (1500, 1500), (700, 700)])
 def test_ids_outside_the_pool_let_nothing_of_page_0_through(poison, length, bound):
@@ -482,6 +502,23 @@ def test_evict_in_a_graph_and_lengths_as_output():
         torch.cuda.synchronize()
         assert held.tolist() == [100, 100, 60]
         _same(pages, exp)
+
+
+@pytest.mark.parametrize("alias", ["lengths", "seen"])
+def test_evict_into_its_own_arguments(alias):
+    from inquant_vllm import evict_rows
+    gen = generator(81)
+    B, h, budget, lengths = 16, 8, 100, [130, 101, 60] * 20
+    pages = pool(gen, 600, h, B, torch.bfloat16)
+    table = tables(gen, lengths, B, 600)
+    args = {"lengths": i32(lengths), "seen": i32([1000 + i for i in range(60)])}
+    # positions that a wrong count of tokens seen would keep or not
+    pages.positions.copy_(torch.randint(0, 1100, pages.positions.shape, generator=gen, device="cuda"))
+    exp = _copy(pages)
+    _plain_evict(exp, table.cpu(), lengths, args["seen"].tolist(), budget, 4, 60)
+    got = evict_rows(pages, table, **args, max_tokens=130, budget=budget, sink=4, recent=60, output=args[alias])
+    assert got is args[alias] and got.tolist() == [100, 100, 60] * 20
+    _same(pages, exp)
 
 
 # ---------------------------------------------------------------- together

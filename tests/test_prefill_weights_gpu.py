@@ -123,6 +123,20 @@ def test_a_nan_query_weighs_only_what_it_sees(window):
     _close(got[1], total[1], slack, 2 * n)
 
 
+@pytest.mark.parametrize("window", [None, 16])
+@pytest.mark.parametrize("heads", [(4, 2), (1, 1)], ids=str)
+def test_one_lse_for_every_head(window, heads):
+    from inquant_vllm import prefill_weights
+    hq, h = heads
+    q, k, _, cu = _case(11, [150], hq, h, torch.bfloat16)
+    lse = torch.full((150,), 3.0, device="cuda").expand(hq, 150)
+    got = prefill_weights(q, k, cu, 150, SCALE, lse=lse, window=window)
+    assert torch.equal(got, prefill_weights(q, k, cu, 150, SCALE, lse=lse.clone(), window=window))
+    if h > 1:
+        with pytest.raises(ValueError, match="overlap"):
+            prefill_weights(q, k, cu, 150, SCALE, lse=lse, window=window, output=got[:1].expand(h, 150))
+
+
 def test_weights_of_a_long_prompt():
     # more queries than one workgroup takes, keys past the first range, over one KV head
     from inquant_vllm import prefill_attention, prefill_weights
