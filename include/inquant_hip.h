@@ -436,6 +436,23 @@ int iq_prefill_weights(const void *q, const void *k, int dtype, int64_t q_st, in
                        int64_t Hq, int64_t H, int64_t window, float scale, const float *lse, int64_t lse_sh,
                        float *workspace, int64_t workspace_floats, float *out, int64_t out_sh, void *stream);
 
+typedef struct iq_prefill_weights_args {
+    uint64_t q, k;
+    int64_t dtype, q_st, q_sh, k_st, k_sh;
+    uint64_t cu_seqlens;
+    int64_t n_seq, max_seqlen, tokens, Hq, H, window;
+    double scale;
+    uint64_t lse;
+    int64_t lse_sh;
+    uint64_t workspace;
+    int64_t workspace_floats;
+    uint64_t out;
+    int64_t out_sh;
+    uint64_t stream;
+} iq_prefill_weights_args;
+
+int iq_prefill_weights_from(const iq_prefill_weights_args *args);
+
 /*
  * ---------------------------------------------------------------- exact pages
  * A pool of exact (unpacked) rows: key and value [pages, heads, block_tokens,
@@ -447,6 +464,10 @@ int iq_prefill_weights(const void *q, const void *k, int dtype, int64_t q_st, in
  * row r % block_tokens of pool page tables[s * bt_stride + r / block_tokens]
  * (i32; bt_cols entries).  Rows of an id outside the pool are neither read nor
  * written.  No counterpart in the reference.
+ *
+ * Each entry point below and iq_prefill_weights also takes its arguments, in
+ * their order, as one struct of 8-byte fields (..._from): a binding packs them
+ * at once instead of converting each (from Python 0.4 us a call instead of 2).
  */
 typedef struct iq_dense_pages {
     uint64_t key, value, weights, positions;
@@ -470,6 +491,22 @@ int iq_dense_write(const void *k, const void *v, int dtype, int64_t k_st, int64_
                    int64_t kept, const iq_dense_pages *pages, const int32_t *tables, int64_t bt_stride,
                    int64_t bt_cols, void *stream);
 
+typedef struct iq_dense_write_args {
+    uint64_t k, v;
+    int64_t dtype, k_st, k_sh, v_st, v_sh;
+    uint64_t cu_seqlens;
+    int64_t n_seq, max_seqlen;
+    uint64_t start, positions, weights;
+    int64_t w_stride;
+    uint64_t keep;
+    int64_t kept;
+    uint64_t pages, tables;
+    int64_t bt_stride, bt_cols;
+    uint64_t stream;
+} iq_dense_write_args;
+
+int iq_dense_write_from(const iq_dense_write_args *args);
+
 /*
  * The rows a budget keeps of each sequence and head: the first `sink` and the
  * last `recent` rows, then by weight (weights f32, row t of sequence i and
@@ -480,6 +517,16 @@ int iq_dense_write(const void *k, const void *v, int dtype, int64_t k_st, int64_
 int iq_select_rows(const float *weights, int64_t w_stride, int64_t H, const int32_t *cu_seqlens, int64_t n_seq,
                    int64_t max_seqlen, int64_t budget, int64_t sink, int64_t recent, int32_t *keep, void *stream);
 
+typedef struct iq_select_rows_args {
+    uint64_t weights;
+    int64_t w_stride, H;
+    uint64_t cu_seqlens;
+    int64_t n_seq, max_seqlen, budget, sink, recent;
+    uint64_t keep, stream;
+} iq_select_rows_args;
+
+int iq_select_rows_from(const iq_select_rows_args *args);
+
 /*
  * Cuts every head of every sequence of more than `budget` rows back to
  * `budget`, in place: kept are the rows at positions below `sink` or from
@@ -488,7 +535,7 @@ int iq_select_rows(const float *weights, int64_t w_stride, int64_t H, const int3
  * `budget` on (key, value, weight and position); all other rows stay as they
  * are.  lengths i32: rows each sequence holds (at most max_tokens are
  * considered); new_lengths i32: min(lengths, budget), which may take the place
- * of lengths.  workspace: i32, iq_dense_evict_ints elements (none while a head
+ * of lengths or of seen.  workspace: i32, iq_dense_evict_ints elements (none while a head
  * moves at most IQ_DENSE_FEW_MOVES rows: min(budget, max_tokens - budget)).
  * No page may belong to two sequences.
  */
@@ -500,6 +547,20 @@ int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int32_t *tables
                    const int32_t *lengths, const int32_t *seen, int64_t n_seq, int64_t max_tokens, int64_t budget,
                    int64_t sink, int64_t recent, int32_t *new_lengths, int32_t *workspace, int64_t workspace_ints,
                    void *stream);
+
+typedef struct iq_dense_evict_args {
+    uint64_t pages;
+    int64_t dtype;
+    uint64_t tables;
+    int64_t bt_stride, bt_cols;
+    uint64_t lengths, seen;
+    int64_t n_seq, max_tokens, budget, sink, recent;
+    uint64_t new_lengths, workspace;
+    int64_t workspace_ints;
+    uint64_t stream;
+} iq_dense_evict_args;
+
+int iq_dense_evict_from(const iq_dense_evict_args *args);
 
 /*
  * One token's attention per sequence over its first lengths[i] cache rows (at
@@ -519,6 +580,24 @@ int iq_dense_decode(const void *q, int dtype, int64_t q_ss, int64_t q_sh, int64_
                     const iq_dense_pages *pages, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
                     const int32_t *lengths, int64_t max_tokens, float scale, int accumulate, float *workspace,
                     int64_t workspace_floats, void *out, int64_t o_ss, int64_t o_sh, int out_dtype, void *stream);
+
+typedef struct iq_dense_decode_args {
+    uint64_t q;
+    int64_t dtype, q_ss, q_sh, Hq, n_seq;
+    uint64_t pages, tables;
+    int64_t bt_stride, bt_cols;
+    uint64_t lengths;
+    int64_t max_tokens;
+    double scale;
+    int64_t accumulate;
+    uint64_t workspace;
+    int64_t workspace_floats;
+    uint64_t out;
+    int64_t o_ss, o_sh, out_dtype;
+    uint64_t stream;
+} iq_dense_decode_args;
+
+int iq_dense_decode_from(const iq_dense_decode_args *args);
 
 /*
  * Dense tail append of a cache layer.  buf holds [2 (keys, values), H,

@@ -491,3 +491,13 @@ extern "C" int iq_dense_decode(const void *q, int dtype, int64_t q_ss, int64_t q
     IQ_CHECK_LAUNCH("dense_decode");
     return IQ_OK;
 }
+
+extern "C" int iq_dense_decode_from(const iq_dense_decode_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_dense_decode: null arguments");
+    return iq_dense_decode((const void *)a->q, (int)a->dtype, a->q_ss, a->q_sh, a->Hq, a->n_seq,
+                           (const iq_dense_pages *)a->pages, (const int32_t *)a->tables, a->bt_stride, a->bt_cols,
+                           (const int32_t *)a->lengths, a->max_tokens, (float)a->scale, (int)a->accumulate,
+                           (float *)a->workspace, a->workspace_floats, (void *)a->out, a->o_ss, a->o_sh,
+                           (int)a->out_dtype, (void *)a->stream);
+}

@@ -467,3 +467,29 @@ extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int3
     IQ_CHECK_LAUNCH("dense_evict");
     return IQ_OK;
 }
+
+extern "C" int iq_dense_write_from(const iq_dense_write_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_dense_write: null arguments");
+    return iq_dense_write((const void *)a->k, (const void *)a->v, (int)a->dtype, a->k_st, a->k_sh, a->v_st, a->v_sh,
+                          (const int32_t *)a->cu_seqlens, a->n_seq, a->max_seqlen, (const int32_t *)a->start,
+                          (const int32_t *)a->positions, (const float *)a->weights, a->w_stride,
+                          (const int32_t *)a->keep, a->kept, (const iq_dense_pages *)a->pages,
+                          (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (void *)a->stream);
+}
+
+extern "C" int iq_select_rows_from(const iq_select_rows_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_select_rows: null arguments");
+    return iq_select_rows((const float *)a->weights, a->w_stride, a->H, (const int32_t *)a->cu_seqlens, a->n_seq,
+                          a->max_seqlen, a->budget, a->sink, a->recent, (int32_t *)a->keep, (void *)a->stream);
+}
+
+extern "C" int iq_dense_evict_from(const iq_dense_evict_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_dense_evict: null arguments");
+    return iq_dense_evict((const iq_dense_pages *)a->pages, (int)a->dtype, (const int32_t *)a->tables, a->bt_stride,
+                          a->bt_cols, (const int32_t *)a->lengths, (const int32_t *)a->seen, a->n_seq, a->max_tokens,
+                          a->budget, a->sink, a->recent, (int32_t *)a->new_lengths, (int32_t *)a->workspace,
+                          a->workspace_ints, (void *)a->stream);
+}

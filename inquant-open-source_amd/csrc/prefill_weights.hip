@@ -582,3 +582,13 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     IQ_CHECK_LAUNCH("prefill_weights");
     return IQ_OK;
 }
+
+extern "C" int iq_prefill_weights_from(const iq_prefill_weights_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_prefill_weights: null arguments");
+    return iq_prefill_weights((const void *)a->q, (const void *)a->k, (int)a->dtype, a->q_st, a->q_sh, a->k_st,
+                              a->k_sh, (const int32_t *)a->cu_seqlens, a->n_seq, a->max_seqlen, a->tokens, a->Hq,
+                              a->H, a->window, (float)a->scale, (const float *)a->lse, a->lse_sh,
+                              (float *)a->workspace, a->workspace_floats, (float *)a->out, a->out_sh,
+                              (void *)a->stream);
+}

@@ -110,6 +110,8 @@ _SIGNATURES = {
     "iq_dense_workspace_floats": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "iq_dense_decode": (_int, [_p, _int, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _f32, _int, _p, _i64,
                                _p, _i64, _i64, _int, _p]),
+    **{name + "_from": (_int, [ctypes.c_char_p]) for name in ("iq_prefill_weights", "iq_dense_write", "iq_select_rows",
+                                                              "iq_dense_evict", "iq_dense_decode")},
     "iq_page_bytes": (_i64, [_i64, _i64]),
     "iq_encode_pages": (_int, [_p, _p, _int, ctypes.POINTER(_i64), ctypes.POINTER(_i64), _i64, _i64, _i64, _p, _i64,
                                _p, _int, _p, _p, _p]),

@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -75,8 +76,8 @@ class DensePages:
             raise ValueError("all tensors must share one GPU")
         p = nat.DensePagesDesc(key.data_ptr(), value.data_ptr(), *(0 if t is None else t.data_ptr() for t in side),
                                *_strides(key), *_strides(value), *key.shape[:3])
-        # what every call asks for: the descriptor, its dtype code, the GPU, and the sizes
-        for name, value in (("_desc", ctypes.byref(p)), ("_dtype", key.dtype), ("_gpu", key.get_device()),
+        # what every call asks for: the descriptor and its address, the dtype and its code, the GPU, and the sizes
+        for name, value in (("_pages", p), ("_desc", ctypes.addressof(p)), ("_dtype", key.dtype), ("_gpu", key.get_device()),
                             ("_code", nat.dtype_code(key.dtype)), ("block_size", key.shape[2]),
                             ("heads", key.shape[1])):
             object.__setattr__(self, name, value)
@@ -98,15 +99,24 @@ class DensePages:
 
 
 def _on_gpu(gpu, what, *tensors):
-    """All tensors on one GPU: the index that the first (or ``gpu``) says.  The
-    common case costs one integer per tensor, any other takes require_gpu's errors."""
+    """All tensors on one GPU, whose index is ``gpu``.  The common case costs one
+    integer per tensor, any other takes require_gpu's errors."""
     for t in tensors:
-        if t is not None and t.get_device() != gpu or gpu < 0:
-            nat.require_gpu(*tensors, what=what)
-            raise ValueError("all tensors must share one GPU")
-    return gpu
+        if t is not None and t.get_device() != gpu:
+            break
+    else:
+        if gpu >= 0:
+            return
+    nat.require_gpu(*tensors, what=what)
+    raise ValueError("all tensors must share one GPU")
 
 
+# The arguments of the entry points that take them as a struct, 8 bytes each: Q an
+# address (0: none), q a number, d the scale.  ctypes takes 2 us to convert twenty
+# arguments one by one, 0.4 for a packed struct.
+_ARGUMENTS = {name: struct.Struct("=" + fields).pack for name, fields in {
+    "iq_dense_write": "2Q5qQ2q3QqQq2Q2qQ", "iq_select_rows": "Q2qQ5q2Q", "iq_dense_evict": "QqQ2q2Q5q2QqQ",
+    "iq_dense_decode": "Q5q2Q2qQqdqQqQ3qQ", "iq_prefill_weights": "2Q5qQ6qdQqQqQqQ"}.items()}
 _entries: dict = {}
 
 
@@ -120,10 +130,11 @@ def _entry(name):
 
 def _status(gpu, name, *args):
     """Calls the entry point with its GPU current."""
+    call, args = _entry(name + "_from"), _ARGUMENTS[name](*args)
     if gpu == torch._C._cuda_getDevice():
-        return _entry(name)(*args)
+        return call(args)
     with torch.cuda.device(gpu):
-        return _entry(name)(*args)
+        return call(args)
 
 
 def _call(gpu, name, *args):
@@ -133,6 +144,10 @@ def _call(gpu, name, *args):
         nat.check(status)
 
 
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _ints(t, shape, what):
     if t.shape != shape or t.dtype is not _I32:
         raise ValueError(f"Expected int32 {what}")
@@ -140,17 +155,18 @@ def _ints(t, shape, what):
 
 
 def _cu(cu_seqlens):
-    if cu_seqlens.dtype is not _I32 or cu_seqlens.ndim != 1 or cu_seqlens.numel() < 2:
+    """The offsets, contiguous, and the number of sequences."""
+    shape = cu_seqlens.shape
+    if cu_seqlens.dtype is not _I32 or len(shape) != 1 or shape[0] < 2:
         raise ValueError("cu_seqlens must be an int32 [sequences + 1] tensor")
-    return cu_seqlens if cu_seqlens.is_contiguous() else cu_seqlens.contiguous()
+    return cu_seqlens if cu_seqlens.is_contiguous() else cu_seqlens.contiguous(), shape[0] - 1
 
 
 def _tables(block_tables, n):
-    shape = block_tables.shape
-    if len(shape) != 2 or shape[0] != n or block_tables.dtype is not _I32 \
-            or (shape[1] > 1 and block_tables.stride(1) != 1):
+    shape, stride = block_tables.shape, block_tables.stride()
+    if len(shape) != 2 or shape[0] != n or block_tables.dtype is not _I32 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError("Expected int32 block tables [sequences, pages per sequence]")
-    return block_tables.data_ptr(), block_tables.stride(0), shape[1]
+    return block_tables.data_ptr(), stride[0], shape[1]
 
 
 def _token_rows(t, what, heads=None):
@@ -188,8 +204,7 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
     vshape, vs = _token_rows(value, "value", heads)
     if shape != vshape or key.dtype is not pages._dtype or value.dtype is not pages._dtype:
         raise ValueError("key and value must have one shape and the pages' dtype")
-    cu = _cu(cu_seqlens)
-    n, tokens = cu.shape[0] - 1, shape[0]
+    (cu, n), tokens = _cu(cu_seqlens), shape[0]
     table = _tables(block_tables, n)
     if start is not None:
         start = _ints(start, (n,), "start rows [sequences]")
@@ -202,14 +217,14 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
         if keep.ndim != 3 or keep.shape[:2] != (n, heads):
             raise ValueError("Expected int32 kept rows [sequences, kv_heads, kept]")
         keep = _ints(keep, keep.shape, "kept rows [sequences, kv_heads, kept]")
-    gpu = _on_gpu(pages._gpu, "write_rows", key, value, cu, block_tables, start, positions, weights, keep)
+    gpu = pages._gpu
+    _on_gpu(gpu, "write_rows", key, value, cu, block_tables, start, positions, weights, keep)
     if tokens == 0 or table[2] == 0:
         return
     _call(gpu, "iq_dense_write", key.data_ptr(), value.data_ptr(), pages._code, ks[0], ks[1], vs[0], vs[1],
-          cu.data_ptr(), n, int(max_seqlen), None if start is None else start.data_ptr(),
-          None if positions is None else positions.data_ptr(), None if weights is None else weights.data_ptr(),
-          0 if weights is None else weights.stride(0), None if keep is None else keep.data_ptr(),
-          0 if keep is None else keep.shape[2], pages._desc, *table)
+          cu.data_ptr(), n, int(max_seqlen), _ptr(start), _ptr(positions), _ptr(weights),
+          0 if weights is None else weights.stride(0), _ptr(keep), 0 if keep is None else keep.shape[2], pages._desc,
+          *table)
 
 
 def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, output=None):
@@ -224,9 +239,9 @@ def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, ou
     if weights.ndim != 2 or weights.dtype is not _F32 or weights.shape[0] < 1 \
             or weights.stride(1) != 1 and weights.shape[1] > 1:
         raise ValueError("Expected float32 weights [kv_heads, tokens]")
-    cu = _cu(cu_seqlens)
-    n, (h, tokens) = cu.shape[0] - 1, weights.shape
-    gpu = _on_gpu(weights.get_device(), "select_rows", weights, cu, output)
+    (cu, n), (h, tokens) = _cu(cu_seqlens), weights.shape
+    gpu = weights.get_device()
+    _on_gpu(gpu, "select_rows", weights, cu, output)
     if output is None:
         output = torch.empty((n, h, budget), dtype=_I32, device=weights.device)
     elif output.shape != (n, h, budget) or output.dtype is not _I32 or not output.is_contiguous():
@@ -261,7 +276,8 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
     table = _tables(block_tables, n)
     if not 0 <= max_tokens <= table[2] * pages.block_size:
         raise ValueError("max_tokens must fit the block tables")
-    gpu = _on_gpu(pages._gpu, "evict_rows", lengths, seen, block_tables, output)
+    gpu = pages._gpu
+    _on_gpu(gpu, "evict_rows", lengths, seen, block_tables, output)
     if output is None:
         output = torch.empty_like(lengths)
     elif output.shape != (n,) or output.dtype is not _I32 or not output.is_contiguous():
@@ -274,7 +290,7 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
         need = _entry("iq_dense_evict_ints")(pages.heads, n, max_tokens, budget)
         scratch = torch.empty(need, dtype=_I32, device=lengths.device)
     _call(gpu, "iq_dense_evict", pages._desc, pages._code, *table, lengths.data_ptr(), seen.data_ptr(), n, max_tokens,
-          budget, sink, recent, output.data_ptr(), None if scratch is None else scratch.data_ptr(), need)
+          budget, sink, recent, output.data_ptr(), _ptr(scratch), need)
     return output
 
 
@@ -293,7 +309,7 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     shape, hkv, max_tokens = query.shape, pages.heads, int(max_tokens)
     if len(shape) != 3 or shape[2] != 128 or query.dtype is not pages._dtype:
         raise ValueError("Expected a query [sequences, heads, 128] of the pages' dtype")
-    n, hq = shape[0], shape[1]
+    n, hq, _ = shape
     if hq < 1 or hq % hkv or hq // hkv > 16:
         raise ValueError("Expected 1..16 query heads per KV head")
     if accumulate and pages.weights is None:
@@ -304,36 +320,32 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
         raise ValueError("max_tokens must fit the block tables")
     if not math.isfinite(scale):
         raise ValueError("the scale must be finite")
-    gpu = _on_gpu(pages._gpu, "dense_decode", query, block_tables, lengths, output)
+    gpu = pages._gpu
+    _on_gpu(gpu, "dense_decode", query, block_tables, lengths, output)
     qs = query.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
         query = query.clone(memory_format=torch.contiguous_format)
         qs = query.stride()
     if output is None:
         output = torch.empty(shape, dtype=query.dtype, device=query.device)
-        code = pages._code
-    elif output.shape != shape or output.stride(2) != 1 or output.dtype is not query.dtype and output.dtype is not _F32:
+    dtype, os = output.dtype, output.stride()
+    if output.shape != shape or os[2] != 1 or dtype is not pages._dtype and dtype is not _F32:
         raise ValueError("output must be [sequences, heads, 128] of the query dtype or float32")
-    elif n > 1 and output.stride(0) < 128 or hq > 1 and output.stride(1) < 128:
+    if os[0] < 128 and n > 1 or os[1] < 128 and hq > 1:
         raise ValueError("the output's rows must not overlap")
-    else:
-        code = nat.IQ_F32 if output.dtype is _F32 else pages._code
     if n == 0:
         return output
-    accumulate = 1 if accumulate else 0
-    device, os = query.device, output.stride()
-
-    def call(floats):
-        return _status(gpu, "iq_dense_decode", query.data_ptr(), pages._code, qs[0], qs[1], hq, n, pages._desc, *table,
-                       lengths.data_ptr(), max_tokens, scale, accumulate, *floats[:2], output.data_ptr(), os[0], os[1],
-                       code, floats[2])
     # the scratch that is there serves most calls; the library says when it does not
-    floats = workspace.floats(0, device)
-    status = call(floats)
+    scratch, have, stream = workspace.floats(0, query.device)
+    args = [query.data_ptr(), pages._code, qs[0], qs[1], hq, n, pages._desc, *table, lengths.data_ptr(), max_tokens,
+            scale, bool(accumulate), scratch, have, output.data_ptr(), os[0], os[1],
+            nat.IQ_F32 if dtype is _F32 else pages._code, stream]
+    status = _status(gpu, "iq_dense_decode", *args)
     if status:
-        need = _entry("iq_dense_workspace_floats")(hq, hkv, n, max_tokens, accumulate)
-        if need > floats[1]:
-            status = call(workspace.floats(need, device))
+        need = _entry("iq_dense_workspace_floats")(hq, hkv, n, max_tokens, bool(accumulate))
+        if need > have:
+            args[14:16] = workspace.floats(need, query.device)[:2]
+            status = _status(gpu, "iq_dense_decode", *args)
         nat.check(status)
     return output
 
@@ -355,7 +367,7 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         raise ValueError("Expected BF16 or FP16 query and key of the same tokens")
     if h < 1 or hq < 1 or hq % h:
         raise ValueError("query heads must be a multiple of KV heads")
-    cu, max_seqlen = _cu(cu_seqlens), int(max_seqlen)
+    (cu, n), max_seqlen = _cu(cu_seqlens), int(max_seqlen)
     if max_seqlen < 1 or not (scale > 0 and math.isfinite(scale)):
         raise ValueError("max_seqlen and the scale must be positive")
     if window is not None and int(window) < 1:
@@ -364,7 +376,8 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         raise ValueError("Weights of all queries need the lse of prefill_attention")
     if lse is not None and (lse.shape != (hq, tokens) or lse.dtype is not _F32 or lse.stride(1) != 1 and tokens > 1):
         raise ValueError("Expected a float32 lse [query heads, tokens]")
-    gpu = _on_gpu(query.get_device(), "prefill_weights", query, key, cu, lse, output)
+    gpu = query.get_device()
+    _on_gpu(gpu, "prefill_weights", query, key, cu, lse, output)
     if output is None:
         output = torch.empty((h, tokens), dtype=_F32, device=query.device)
     elif output.shape != (h, tokens) or output.dtype is not _F32 or output.stride(1) != 1 and tokens > 1:
@@ -380,10 +393,9 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         window = 0                           # every query
     if window > 4096:
         raise ValueError("Windows of more than 4096 queries and less than all are not supported")
-    n = cu.shape[0] - 1
     need = _entry("iq_prefill_weights_floats")(hq, n, max_seqlen, tokens, window, lse is not None)
     scratch = torch.empty(need, dtype=_F32, device=query.device)
     _call(gpu, "iq_prefill_weights", query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype), qs[0], qs[1], ks[0],
-          ks[1], cu.data_ptr(), n, max_seqlen, tokens, hq, h, window, scale, nat.ptr(lse),
+          ks[1], cu.data_ptr(), n, max_seqlen, tokens, hq, h, window, scale, _ptr(lse),
           0 if lse is None else max(1, lse.stride(0)), scratch.data_ptr(), need, output.data_ptr(), output.stride(0))
     return output

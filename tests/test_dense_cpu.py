@@ -140,6 +140,15 @@ def test_refusals_of_the_library():
         fake, fake, nat.IQ_BF16, q_st, 128, 256, 128, fake, 1, 8, 8, 4, 2, window, scale, lse, 8, fake, 1 << 20, fake, 8,
         None)
     assert weights(scale=0.0) == -1 and weights(window=0) == -1 and weights(q_st=1 << 25) == -1
+    # the same with the arguments in a struct
+    from inquant_vllm import dense
+    pool = pages()
+    assert lib.iq_dense_decode_from(dense._ARGUMENTS["iq_dense_decode"](
+        fake, nat.IQ_BF16, 512, 128, 4, 1, ctypes.addressof(pool._obj), fake, 40, 40, fake, 641, 0.1, 0, fake, 1 << 30,
+        fake, 512, 128, nat.IQ_BF16, 0)) == -1
+    assert b"max_tokens" in lib.iq_last_error()
+    for name in dense._ARGUMENTS:
+        assert getattr(lib, name + "_from")(None) == -1 and b"null arguments" in lib.iq_last_error()
 
 
 def test_prefill_attention_refuses_a_wrong_lse():
