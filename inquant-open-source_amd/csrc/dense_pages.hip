@@ -7,6 +7,8 @@
 // of the page that its block table names at r / B; the heads of a sequence
 // hold the same number of rows but, once rows were evicted, not the same
 // positions.
+#include <type_traits>
+
 #include "dense_common.h"
 
 namespace {
@@ -111,8 +113,9 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
     return v + dpp_u<0x143, 0xc>(v);         // row_bcast:31 into rows 2 and 3
 }
 
-// load(index, end) -> the sort keys of four indices, of which only those below
-// `end` count; emit(index, rows, kept, rank): of the 32 indices from `index` on, the mask of those that are rows and of those
+// load(index, end, from, to, whole) -> the sort keys of four indices, of which only
+// those below `end` count (all, if whole), for a wavefront that takes [from, to);
+// emit(index, rows, kept, rank): of the 32 indices from `index` on, the mask of those that are rows and of those
 // that are kept, and the number of kept ones before.  K keys per thread and
 // chunk.
 template <int K, class Load, class Emit>
@@ -124,14 +127,26 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
     uint32_t *const mine = sm.key + t * (K + 1);
     uint32_t key[K];
     uint32_t rows = 0;                           // mask of those that are rows
+    bool whole = false;                          // uniform: all of the wavefront's are
     auto fill = [&](uint32_t base) {
         const uint32_t n = len - base < CHUNK ? len - base : CHUNK, at = t * K;
         rows = at >= n ? 0 : n - at >= K ? (uint32_t)((1ull << K) - 1) : (1u << (n - at)) - 1;
+        const uint32_t from = base + wave * 64 * K;
+        whole = (wave + 1) * 64 * K <= n;
+        if (whole) {
 #pragma unroll
-        for (int j = 0; j < K; j += 4) {
-            const u32x4 v = load(base + at + j, base + n);
+            for (int j = 0; j < K; j += 4) {
+                const u32x4 v = load(base + at + j, base + n, from, from + 64 * K, std::true_type{});
 #pragma unroll
-            for (int e = 0; e < 4; ++e) key[j + e] = rows >> (j + e) & 1 ? v[e] : 0;
+                for (int e = 0; e < 4; ++e) key[j + e] = v[e];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < K; j += 4) {
+                const u32x4 v = load(base + at + j, base + n, from, from + 64 * K, std::false_type{});
+#pragma unroll
+                for (int e = 0; e < 4; ++e) key[j + e] = rows >> (j + e) & 1 ? v[e] : 0;
+            }
         }
 #pragma unroll
         for (int j = 0; j < K; ++j) mine[j] = key[j];
@@ -157,12 +172,15 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
             uint32_t *const hist = sm.hist[lane & 1];
             for (uint32_t base = 0; base < len; base += CHUNK) {
                 if (!one) fill(base);
-                if (pass == 0) {
+                if (pass == 0 && whole) {
+#pragma unroll
+                    for (int j = 0; j < K; ++j) atomicAdd(&hist[key[j] >> 21], 1u);
+                } else if (pass == 0) {
 #pragma unroll
                     for (int j = 0; j < K; ++j)
                         if (key[j]) atomicAdd(&hist[key[j] >> 21], 1u);
                 } else {
-                    for (match = where([&](uint32_t k) { return k && (k & above) == prefix; }); match;
+                    for (match = where([&](uint32_t k) { return (k & above) == prefix; }) & rows; match;
                          match &= match - 1)
                         atomicAdd(&hist[(mine[__builtin_ctz(match)] >> shift) & mask], 1u);
                 }
@@ -260,11 +278,16 @@ __global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
     int32_t *keep = a.keep + ((int64_t)seq * gridDim.x + h) * a.budget;
     const uint32_t rows = len > 0 ? (uint32_t)len : 0, sink = (uint32_t)a.sink, recent = (uint32_t)a.recent;
     select_rows_of(
-        sm, rows, (uint32_t)a.budget, [&](uint32_t i, uint32_t end) {
+        sm, rows, (uint32_t)a.budget, [&](uint32_t i, uint32_t end, uint32_t from, uint32_t to, auto whole) {
             u32x4 keys;
-            const f32x4 x = load_four(w, i, end);
+            const f32x4 x = whole ? (f32x4)ldg_at<f32x4_unaligned>(w, 4 * i) : load_four(w, i, end);
+            if (whole && from >= sink && to + recent <= rows) {          // uniform: none is kept always
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) keys[e] = sort_key(x[e], i + e < sink || i + e + recent >= rows);
+                for (uint32_t e = 0; e < 4; ++e) keys[e] = sort_key(x[e], false);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) keys[e] = sort_key(x[e], i + e < sink || i + e + recent >= rows);
+            }
             return keys;
         },
         [&](uint32_t i, uint32_t, uint32_t kept, uint32_t rank) {
@@ -315,9 +338,9 @@ __global__ __launch_bounds__(SEL_NT) void evict_select_kernel(EvictArgs a)
     const uint32_t budget = (uint32_t)a.budget;
     select_rows_of(
         sm, (uint32_t)len, budget,
-        [&](uint32_t i, uint32_t end) {
+        [&](uint32_t i, uint32_t end, uint32_t, uint32_t, auto whole) {
             // four rows of one page; a row of an id outside the pool counts as NaN
-            const int32_t id = table[i < end ? i >> a.pool.shift : 0];
+            const int32_t id = table[whole || i < end ? i >> a.pool.shift : 0];
             const bool ok = id >= 0 && id < a.pool.pages;
             const int64_t o = ((int64_t)(ok ? id : 0) * H + h) * B + (i & (B - 1));
             const f32x4 w = ldg<f32x4>(a.pool.weights + o);

@@ -34,6 +34,8 @@ from .layout import BLOCK_SIZES
 
 _ROWS = (torch.bfloat16, torch.float16)
 _I32, _F32 = torch.int32, torch.float32
+_current = getattr(torch._C, "_cuda_getDevice", None)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _FEW_MOVES = 128        # iq_dense_evict takes no workspace up to here (IQ_DENSE_FEW_MOVES)
 
 
@@ -121,17 +123,21 @@ _entries: dict = {}
 
 
 def _entry(name):
-    """A library function, looked up once."""
-    fn = _entries.get(name)
-    if fn is None:
-        fn = _entries[name] = getattr(nat.lib(), name)
-    return fn
+    """A library function, looked up once; with ``_from`` beside what packs its arguments."""
+    found = _entries.get(name)
+    if found is None:
+        found = getattr(nat.lib(), name)
+        if name.endswith("_from"):
+            found = found, _ARGUMENTS[name[:-5]]
+        _entries[name] = found
+    return found
 
 
 def _status(gpu, name, *args):
     """Calls the entry point with its GPU current."""
-    call, args = _entry(name + "_from"), _ARGUMENTS[name](*args)
-    if gpu == torch._C._cuda_getDevice():
+    call, pack = _entries.get(name) or _entry(name)
+    args = pack(*args)
+    if gpu == _current():
         return call(args)
     with torch.cuda.device(gpu):
         return call(args)
@@ -139,7 +145,7 @@ def _status(gpu, name, *args):
 
 def _call(gpu, name, *args):
     """The same on the GPU's current stream; a failure raises."""
-    status = _status(gpu, name, *args, torch._C._cuda_getCurrentRawStream(gpu))
+    status = _status(gpu, name, *args, _stream(gpu))
     if status:
         nat.check(status)
 
@@ -210,8 +216,9 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
         start = _ints(start, (n,), "start rows [sequences]")
     if positions is not None:
         positions = _ints(positions, (n,), "positions [sequences]")
+    ws = (0, 1) if weights is None else weights.stride()
     if weights is not None and (weights.shape != (heads, tokens) or weights.dtype is not _F32
-                                or weights.stride(1) != 1 and tokens > 1):
+                                or ws[1] != 1 and tokens > 1):
         raise ValueError("Expected float32 weights [kv_heads, tokens]")
     if keep is not None:
         if keep.ndim != 3 or keep.shape[:2] != (n, heads):
@@ -221,10 +228,9 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
     _on_gpu(gpu, "write_rows", key, value, cu, block_tables, start, positions, weights, keep)
     if tokens == 0 or table[2] == 0:
         return
-    _call(gpu, "iq_dense_write", key.data_ptr(), value.data_ptr(), pages._code, ks[0], ks[1], vs[0], vs[1],
-          cu.data_ptr(), n, int(max_seqlen), _ptr(start), _ptr(positions), _ptr(weights),
-          0 if weights is None else weights.stride(0), _ptr(keep), 0 if keep is None else keep.shape[2], pages._desc,
-          *table)
+    _call(gpu, "iq_dense_write_from", key.data_ptr(), value.data_ptr(), pages._code, ks[0], ks[1], vs[0], vs[1],
+          cu.data_ptr(), n, int(max_seqlen), _ptr(start), _ptr(positions), _ptr(weights), ws[0], _ptr(keep),
+          0 if keep is None else keep.shape[2], pages._desc, *table)
 
 
 def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, output=None):
@@ -248,7 +254,7 @@ def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, ou
         raise ValueError("output must be a contiguous int32 [sequences, kv_heads, budget] tensor")
     if tokens == 0:
         return output.fill_(-1)
-    _call(gpu, "iq_select_rows", weights.data_ptr(), weights.stride(0), h, cu.data_ptr(), n, int(max_seqlen), budget,
+    _call(gpu, "iq_select_rows_from", weights.data_ptr(), weights.stride(0), h, cu.data_ptr(), n, int(max_seqlen), budget,
           sink, recent, output.data_ptr())
     return output
 
@@ -289,7 +295,7 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
     if max_tokens - budget > _FEW_MOVES:
         need = _entry("iq_dense_evict_ints")(pages.heads, n, max_tokens, budget)
         scratch = torch.empty(need, dtype=_I32, device=lengths.device)
-    _call(gpu, "iq_dense_evict", pages._desc, pages._code, *table, lengths.data_ptr(), seen.data_ptr(), n, max_tokens,
+    _call(gpu, "iq_dense_evict_from", pages._desc, pages._code, *table, lengths.data_ptr(), seen.data_ptr(), n, max_tokens,
           budget, sink, recent, output.data_ptr(), _ptr(scratch), need)
     return output
 
@@ -340,12 +346,12 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     args = [query.data_ptr(), pages._code, qs[0], qs[1], hq, n, pages._desc, *table, lengths.data_ptr(), max_tokens,
             scale, bool(accumulate), scratch, have, output.data_ptr(), os[0], os[1],
             nat.IQ_F32 if dtype is _F32 else pages._code, stream]
-    status = _status(gpu, "iq_dense_decode", *args)
+    status = _status(gpu, "iq_dense_decode_from", *args)
     if status:
         need = _entry("iq_dense_workspace_floats")(hq, hkv, n, max_tokens, bool(accumulate))
         if need > have:
             args[14:16] = workspace.floats(need, query.device)[:2]
-            status = _status(gpu, "iq_dense_decode", *args)
+            status = _status(gpu, "iq_dense_decode_from", *args)
         nat.check(status)
     return output
 
@@ -395,7 +401,7 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         raise ValueError("Windows of more than 4096 queries and less than all are not supported")
     need = _entry("iq_prefill_weights_floats")(hq, n, max_seqlen, tokens, window, lse is not None)
     scratch = torch.empty(need, dtype=_F32, device=query.device)
-    _call(gpu, "iq_prefill_weights", query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype), qs[0], qs[1], ks[0],
+    _call(gpu, "iq_prefill_weights_from", query.data_ptr(), key.data_ptr(), nat.dtype_code(query.dtype), qs[0], qs[1], ks[0],
           ks[1], cu.data_ptr(), n, max_seqlen, tokens, hq, h, window, scale, _ptr(lse),
           0 if lse is None else max(1, lse.stride(0)), scratch.data_ptr(), need, output.data_ptr(), output.stride(0))
     return output
