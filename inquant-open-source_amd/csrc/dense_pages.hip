@@ -74,9 +74,10 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 // workgroup: the key of rank `budget` from three radix passes (11, 11 and 10
 // bits, histograms in LDS), then ranks in index order from one sum over the
 // threads.  A thread holds up to 32 consecutive keys of a chunk of 32768 in
-// registers (and in LDS, by number), and what it finds of them (in the threshold's bin, kept, tied) as masks of 32 bits,
-// so that only the first pass spends more than a compare and an add on a key.
-// Longer rows are read again in every pass.
+// registers, and what it finds of them (kept, tied) as masks of 32 bits.  Its
+// wavefront reads them side by side and passes them on through LDS (a lane's own
+// keys are 128 bytes from the next lane's: 9500 cycles of 40000 for a row of
+// 32000, read so).  Longer rows are read again in every pass.
 constexpr int SEL_NT = 1024, SEL_WAVES = SEL_NT / 64, SEL_CHUNK = SEL_NT * 32;
 
 // Greater is better: NaN, then -inf .. +inf (both zeros alike), then the rows
@@ -88,11 +89,13 @@ __device__ __forceinline__ uint32_t sort_key(float w, bool always)
     return always ? 0xffffffffu : key;
 }
 
-struct SelectSmem {
-    uint32_t key[SEL_NT * 33];                // a thread's keys, one word apart from the next thread's
-    uint32_t hist[2][2048 + 32];              // odd lanes count apart from even ones, on other banks
+struct __attribute__((aligned(16))) SelectSmem {
+    union {
+        uint32_t stage[SEL_NT * 36];          // a thread's keys, 16 bytes apart from the next thread's
+        uint32_t hist[4][2048 + 8];           // neighbouring lanes count apart, on other banks
+    };
     uint32_t wave_sum[SEL_WAVES], wave_ties[SEL_WAVES];
-    uint32_t prefix, need;                    // threshold bits so far, entries still to take of those that match them
+    uint32_t prefix, need, match;             // threshold bits so far, entries still to take of those that match them, these
 };
 
 // Inclusive sum over the wavefront: sums of 1, 2, 4, .. 16 lanes of a row by
@@ -118,38 +121,50 @@ __device__ __forceinline__ uint32_t wave_inclusive(uint32_t v)
 // emit(index, rows, kept, rank): of the 32 indices from `index` on, the mask of those that are rows and of those
 // that are kept, and the number of kept ones before.  K keys per thread and
 // chunk.
-template <int K, class Load, class Emit>
+template <int K, bool ONE, class Load, class Emit>
 __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uint32_t budget, Load load, Emit emit)
 {
-    constexpr uint32_t CHUNK = SEL_NT * K;
+    constexpr uint32_t CHUNK = SEL_NT * K;     // ONE: at least the row
+    constexpr bool STAGED = ONE && K > 4;
+    // copies of the first pass's histogram, which counts every key (32000 rows: 33000
+    // cycles with 4, 34000 with 2 or 8; an atomic of 64 keys takes 17)
+    constexpr int COPIES = K > 16 ? 4 : 2;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const bool one = K < 32 || len <= CHUNK;   // only the longest form takes rows of several chunks
-    uint32_t *const mine = sm.key + t * (K + 1);
     uint32_t key[K];
     uint32_t rows = 0;                           // mask of those that are rows
     bool whole = false;                          // uniform: all of the wavefront's are
-    auto fill = [&](uint32_t base) {
-        const uint32_t n = len - base < CHUNK ? len - base : CHUNK, at = t * K;
-        rows = at >= n ? 0 : n - at >= K ? (uint32_t)((1ull << K) - 1) : (1u << (n - at)) - 1;
+    auto read = [&](uint32_t base, uint32_t n, auto all) {
         const uint32_t from = base + wave * 64 * K;
-        whole = (wave + 1) * 64 * K <= n;
-        if (whole) {
+#pragma unroll
+        for (int j = 0; j < K; j += 4) {
+            const uint32_t i = STAGED ? 64 * j + 4 * lane : lane * K + j;    // of the wavefront's keys
+            u32x4 v = load(from + i, base + n, from, from + 64 * K, all);
+            if (!all)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) v[e] = from + i + e < base + n ? v[e] : 0;
+            if constexpr (STAGED) *(u32x4 *)(sm.stage + (64 * wave + i / K) * (K + 4) + i % K) = v;
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) key[j + e] = v[e];
+        }
+        if constexpr (STAGED) {                  // within the wavefront
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
             for (int j = 0; j < K; j += 4) {
-                const u32x4 v = load(base + at + j, base + n, from, from + 64 * K, std::true_type{});
+                const u32x4 v = *(const u32x4 *)(sm.stage + t * (K + 4) + j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) key[j + e] = v[e];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < K; j += 4) {
-                const u32x4 v = load(base + at + j, base + n, from, from + 64 * K, std::false_type{});
-#pragma unroll
-                for (int e = 0; e < 4; ++e) key[j + e] = rows >> (j + e) & 1 ? v[e] : 0;
-            }
         }
-#pragma unroll
-        for (int j = 0; j < K; ++j) mine[j] = key[j];
+    };
+    auto fill = [&](uint32_t base) {
+        const uint32_t n = len - base < CHUNK ? len - base : CHUNK, at = t * K;
+        rows = at >= n ? 0 : n - at >= K ? (uint32_t)((1ull << K) - 1) : (1u << (n - at)) - 1;
+        whole = (wave + 1) * 64 * K <= n;
+        if (whole) read(base, n, std::true_type{});
+        else read(base, n, std::false_type{});
     };
     // mask of this thread's keys for which f holds: a compare and an add with its carry each
     auto where = [&](auto f) {
@@ -158,20 +173,26 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
         for (int j = K - 1; j >= 0; --j) m = m + m + (f(key[j]) ? 1u : 0u);
         return m;
     };
-    if (one && len) fill(0);
-    uint32_t prefix = 0, need = 0;               // len <= budget: every row's key is above 0
+    if (ONE && len) fill(0);
+    uint32_t prefix = 1, need = 0;               // len <= budget: every row's key is at least 1
+    bool all = true;                             // uniform: whose key is the threshold is kept
     if (len > budget) {
+        prefix = 0;
         need = budget;
-        uint32_t match = 0;
+        if (STAGED) __syncthreads();             // the histograms take the place of the staged keys
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const uint32_t mask = pass == 2 ? 1023 : 2047;
             const uint32_t above = pass == 0 ? 0 : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-            sm.hist[0][t] = sm.hist[0][t + SEL_NT] = sm.hist[1][t] = sm.hist[1][t + SEL_NT] = 0;
+            const int copies = pass == 0 ? COPIES : 2;
+#pragma unroll
+            for (int c = 0; c < COPIES; ++c)
+                if (c < copies) sm.hist[c][t] = sm.hist[c][t + SEL_NT] = 0;
             __syncthreads();
-            uint32_t *const hist = sm.hist[lane & 1];
+            uint32_t *const hist = sm.hist[lane & (copies - 1)];
             for (uint32_t base = 0; base < len; base += CHUNK) {
-                if (!one) fill(base);
+                if (!ONE) fill(base);
+                // what is no row counts as the lowest key, below every threshold
                 if (pass == 0 && whole) {
 #pragma unroll
                     for (int j = 0; j < K; ++j) atomicAdd(&hist[key[j] >> 21], 1u);
@@ -180,15 +201,20 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
                     for (int j = 0; j < K; ++j)
                         if (key[j]) atomicAdd(&hist[key[j] >> 21], 1u);
                 } else {
-                    for (match = where([&](uint32_t k) { return (k & above) == prefix; }) & rows; match;
-                         match &= match - 1)
-                        atomicAdd(&hist[(mine[__builtin_ctz(match)] >> shift) & mask], 1u);
+#pragma unroll
+                    for (int j = 0; j < K; ++j)
+                        if ((key[j] & above) == prefix) atomicAdd(&hist[(key[j] >> shift) & mask], 1u);
                 }
             }
             __syncthreads();
             // thread t takes the bins 2047 - 2 t and 2046 - 2 t: sums from the largest down
-            const uint32_t hi = sm.hist[0][2047 - 2 * t] + sm.hist[1][2047 - 2 * t];
-            const uint32_t lo = sm.hist[0][2046 - 2 * t] + sm.hist[1][2046 - 2 * t];
+            uint32_t hi = 0, lo = 0;
+#pragma unroll
+            for (int c = 0; c < COPIES; ++c)
+                if (c < copies) {
+                    hi += sm.hist[c][2047 - 2 * t];
+                    lo += sm.hist[c][2046 - 2 * t];
+                }
             const uint32_t upto = wave_inclusive(hi + lo);
             if (lane == 63) sm.wave_sum[wave] = upto;
             __syncthreads();
@@ -199,19 +225,26 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
                 const bool top = need <= before + hi;
                 sm.prefix = prefix | ((top ? 2047 - 2 * t : 2046 - 2 * t) << shift);
                 sm.need = need - before - (top ? 0 : hi);
+                sm.match = top ? hi : lo;
             }
             __syncthreads();
             prefix = sm.prefix;
             need = sm.need;
         }
+        all = __builtin_amdgcn_readfirstlane(sm.match == need);
     }
     uint32_t sure0 = 0, ties0 = 0;               // kept for sure, and ties, in the chunks before
     for (uint32_t base = 0; base < len; base += CHUNK) {
-        if (!one) fill(base);
-        uint32_t kept = where([&](uint32_t k) { return k > prefix; });
-        uint32_t ties = where([&](uint32_t k) { return k == prefix; });
-        const uint32_t ns = (uint32_t)__popc(kept), nt = (uint32_t)__popc(ties);
-        const uint32_t us = wave_inclusive(ns), ut = wave_inclusive(nt);
+        if (!ONE) fill(base);
+        const uint32_t floor = all ? prefix - 1 : prefix;    // the threshold is a row's key, at least 1
+        uint32_t kept = where([&](uint32_t k) { return k > floor; });
+        const uint32_t ns = (uint32_t)__popc(kept), us = wave_inclusive(ns);
+        uint32_t ties = 0, nt = 0, ut = 0;
+        if (!all) {
+            ties = where([&](uint32_t k) { return k == prefix; });
+            nt = (uint32_t)__popc(ties);
+            ut = wave_inclusive(nt);
+        }
         if (lane == 63) {
             sm.wave_sum[wave] = us;
             sm.wave_ties[wave] = ut;
@@ -242,10 +275,11 @@ __device__ __forceinline__ void select_largest(SelectSmem &sm, uint32_t len, uin
 template <class Load, class Emit>
 __device__ __forceinline__ void select_rows_of(SelectSmem &sm, uint32_t len, uint32_t budget, Load load, Emit emit)
 {
-    if (len <= SEL_NT * 4) select_largest<4>(sm, len, budget, load, emit);
-    else if (len <= SEL_NT * 8) select_largest<8>(sm, len, budget, load, emit);
-    else if (len <= SEL_NT * 16) select_largest<16>(sm, len, budget, load, emit);
-    else select_largest<32>(sm, len, budget, load, emit);
+    if (len <= SEL_NT * 4) select_largest<4, true>(sm, len, budget, load, emit);
+    else if (len <= SEL_NT * 8) select_largest<8, true>(sm, len, budget, load, emit);
+    else if (len <= SEL_NT * 16) select_largest<16, true>(sm, len, budget, load, emit);
+    else if (len <= SEL_CHUNK) select_largest<32, true>(sm, len, budget, load, emit);
+    else select_largest<32, false>(sm, len, budget, load, emit);
 }
 
 struct SelectArgs {
