@@ -9,7 +9,7 @@
 // with (max, sum); a second launch joins the partitions.  The weights need the
 // joined lse, so the first launch also leaves the logits (4 bytes per row and
 // query head against 512 read per row and KV head).  Bound by HBM: 16 sequences of
-// 2K-32K tokens, 28 heads over 4, 549 MB: 107 us (5.15 TB/s) and 5 for the join.
+// 2K-32K tokens, 28 heads over 4, 549 MB: 104 us (5.3 TB/s) and 5 for the join.
 #include "dense_common.h"
 
 namespace {

@@ -349,7 +349,7 @@ __device__ __forceinline__ void evict_length(const EvictArgs &a, int seq)
 // Chooses the rows of one (head, sequence) and lists the moves: the evicted
 // places below the budget in order, and the kept rows behind it from the last.
 // MOVE: at most FEW of them, listed in LDS and made here (16 sequences of 2049
-// rows, one to move: 8 us, and 11 with a launch of its own for the move).
+// rows, one to move: 8.7 us, and 12 with a launch of its own for the move).
 constexpr int FEW = IQ_DENSE_FEW_MOVES;
 
 template <bool MOVE>
