@@ -521,6 +521,37 @@ def test_evict_into_its_own_arguments(alias):
     _same(pages, exp)
 
 
+@pytest.mark.parametrize("kind", ["spread", "ties", "odd"])
+@pytest.mark.parametrize("lengths,budget", [([8192, 8193, 4097], 4096), ([12001, 16384], 12000), ([16385, 20003, 32767], 900)],
+                         ids=str)
+def test_select_rows_of_every_width(lengths, budget, kind):
+    from inquant_vllm import select_rows
+    gen, h = generator(60), 2
+    print(f"select {lengths} {budget} {kind}", flush=True)
+    w = _sel_weights(gen, h, sum(lengths), kind)
+    got, cpu, first = select_rows(w, offsets(lengths), max(lengths), budget, sink=3, recent=70).cpu(), w.cpu(), 0
+    for i, n in enumerate(lengths):
+        for head in range(h):
+            exp = keep_rows(cpu[head, first:first + n].tolist(), [j < 3 or j >= n - 70 for j in range(n)], budget)
+            assert got[i, head].tolist() == exp, (i, head)
+        first += n
+
+
+@pytest.mark.parametrize("lengths,budget", [([130, 101], 100), ([9000], 600)], ids=str)
+def test_evict_of_more_always_kept_rows_than_the_budget(lengths, budget):
+    from inquant_vllm import evict_rows
+    gen = generator(82)
+    B, h = 16, 2
+    pages = pool(gen, 600, h, B, torch.bfloat16)
+    table = tables(gen, lengths, B, 600)
+    pages.positions.copy_(torch.randint(0, 6, pages.positions.shape, generator=gen, device="cuda"))
+    for sink, recent in ((5, 0), (0, 1), (6, 1)):            # of positions 0..5 seen
+        exp = _copy(pages)
+        _plain_evict(exp, table.cpu(), lengths, [6] * len(lengths), budget, sink, recent)
+        evict_rows(pages, table, i32(lengths), i32([6] * len(lengths)), max(lengths), budget, sink=sink, recent=recent)
+        _same(pages, exp)
+
+
 # ---------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
