@@ -56,6 +56,14 @@ __device__ __forceinline__ Window window_of(const WeightArgs &a, int len)
     return {len - n, n, n * a.G};
 }
 
+// Row r = g n + i of a window is query i of head g.  The quotient by a reciprocal
+// is exact: rows are below 2^21, and the half keeps its error (2^-22 of it) from
+// the next whole number.
+__device__ __forceinline__ uint32_t head_of(int row, float rcp)
+{
+    return (uint32_t)(((float)row + 0.5f) * rcp);
+}
+
 // Three stages: a tile is computed while the next two are on their way.
 constexpr int ST = 3;
 
@@ -120,6 +128,19 @@ __device__ __forceinline__ float pair_sum(float v)
 {
     const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
+// Of 2 N values of each lane, lanes with bit N set keep the upper half, the others
+// the lower, with their partner's (CTRL; its bit N is the other) added.
+template <int N, int CTRL>
+__device__ __forceinline__ void halve(float *v, int lane)
+{
+    const bool upper = lane & N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float keep = upper ? v[i + N] : v[i], give = upper ? v[i] : v[i + N];
+        v[i] = keep + dpp_f<CTRL>(give);
+    }
 }
 
 enum Pass { ALL, WINDOW, WINDOW_LSE };
@@ -201,12 +222,10 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         const int last = end - 1 - next_qa;
         const uint32_t to_l = lds_l + (uint32_t)(st * NW * QT * 4);
         if constexpr (ROWS) {
-            // query head (of this KV head) and query of the tile's row r.  The quotient
-            // by a reciprocal is exact: rows are below 2^21, and the half keeps its
-            // error (2^-22 of it) from the next whole number.
+            // query head (of this KV head) and query of the tile's row r
             auto place = [&](int r, uint32_t &g, uint32_t &i) {
                 const int row = next_qa + (r < last ? r : last);
-                g = (uint32_t)(((float)row + 0.5f) * win_rcp);
+                g = head_of(row, win_rcp);
                 i = (uint32_t)row - g * (uint32_t)win.n;
                 return row;
             };
@@ -337,12 +356,24 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         f32x16 sc[2];
         products(b ? (st + 1) % ST : st, 1 - b, sc);
         const bool masked = (ROWS ? win.lo : qa + 32 * b) < k0 + KW || k0 + KW > len;    // uniform
-        int lim = KW;                                        // the last key that the query sees, from k0 + 4 h32
+        // A lane's keys, in the order of bit 16 kb + i, that its query does not see.  Taken
+        // apart as one mask: a compare and a selection per key wait for each other's
+        // condition (18 cycles a key, and 8).
+        uint32_t unseen = 0;
         if (masked) {
-            const int row = query < end ? query : end - 1, at = ROWS ? win.lo + row % win.n : row;
-            lim = at - k0 - 4 * h32;
+            const int row = query < end ? query : end - 1;
+            const int at = ROWS ? win.lo + row - (int)head_of(row, win_rcp) * win.n : row;
+            const int n = at - k0 - 4 * h32 + 1;             // keys up to the query's own, from k0 + 4 h32
+            const int bits = n <= 0 ? 0 : 4 * (n >> 3) + ((n & 7) < 4 ? n & 7 : 4);
+            unseen = bits < 32 ? ~0u << bits : 0;
         }
-        auto seen = [&](int kb, int i) { return 32 * kb + 8 * (i >> 2) + (i & 3) <= lim; };
+        auto instead = [&](int kb, int i, uint32_t other, float x) {    // `other` where the key is unseen
+            uint32_t y;
+            asm("v_bfi_b32 %0, %1, %2, %3"
+                : "=v"(y)
+                : "v"(__builtin_amdgcn_sbfe((int)unseen, 16 * kb + i, 1)), "s"(other), "v"(__float_as_uint(x)));
+            return __uint_as_float(y);
+        };
         late[0] = sc[0];
         late[1] = sc[1];
         late_lse2 = lse2;
@@ -353,7 +384,8 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) late[kb][i] = seen(kb, i) ? sc[kb][i] : NEG_INF;   // the scale is positive
+                    for (int i = 0; i < 16; ++i)             // the scale is positive
+                        late[kb][i] = instead(kb, i, __float_as_uint(NEG_INF), sc[kb][i]);
             } else {
                 // added at once, the unseen left out, so that nothing is pending
 #pragma unroll
@@ -361,7 +393,7 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const float w = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c_log2, -lse2));
-                        sum[kb][i] += seen(kb, i) ? w : 0.0f;
+                        sum[kb][i] += instead(kb, i, 0, w);
                         late[kb][i] = NEG_INF;
                     }
                 late_lse2 = 0.0f;
@@ -396,16 +428,22 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
         float *out = a.out + ((int64_t)range * a.Hq + list) * a.out_sh + start;
         // Sums over the 32 queries: a swap of the odd 16-lane rows of one key's
         // lanes with the even ones of another's leaves both keys in one register
-        // (the first block's in the even rows, the second's in the odd).
-        const int kb = (lane >> 4) & 1;
+        // (the first block's in the even rows, the second's in the odd); then the
+        // lanes of a row halve the 16 keys that they add for each other, until
+        // lane i holds key i.
+        float v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0][i]), __float_as_uint(sum[1][i]),
                                                             false, false);
-            const float v = row_sum16(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-            const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h32 + (i & 3);
-            if ((lane & 15) == 0 && key < len) out[key] = v;
+            v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
         }
+        halve<8, 0x140>(v, lane);                            // row_mirror
+        halve<4, 0x141>(v, lane);                            // row_half_mirror
+        halve<2, 0x4e>(v, lane);                             // quad_perm: xor 2
+        halve<1, 0xb1>(v, lane);                             // xor 1
+        const int i = lane & 15, key = k0 + 32 * ((lane >> 4) & 1) + 8 * (i >> 2) + 4 * h32 + (i & 3);
+        if (key < len) out[key] = v[0];
     }
 }
 
