@@ -226,7 +226,8 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
         keep = _ints(keep, keep.shape, "kept rows [sequences, kv_heads, kept]")
     gpu = pages._gpu
     _on_gpu(gpu, "write_rows", key, value, cu, block_tables, start, positions, weights, keep)
-    if tokens == 0 or table[2] == 0:
+    # a selection of no row is an address of 0, which stands for every row
+    if tokens == 0 or table[2] == 0 or keep is not None and keep.shape[2] == 0:
         return
     _call(gpu, "iq_dense_write_from", key.data_ptr(), value.data_ptr(), pages._code, ks[0], ks[1], vs[0], vs[1],
           cu.data_ptr(), n, int(max_seqlen), _ptr(start), _ptr(positions), _ptr(weights), ws[0], _ptr(keep),
