@@ -50,7 +50,8 @@ class DensePages:
     block_size, 128] of bf16 or f16 (any page, head and row strides that are
     multiples of 8 elements, 16-byte aligned; two views of one pool will do) and,
     where rows are to be evicted, ``weights`` f32 and ``positions`` int32
-    [pages, kv_heads, block_size]."""
+    [pages, kv_heads, block_size].  The tensors' addresses are taken here, once:
+    they must keep their memory.  A deep copy or a pickle holds memory of its own."""
     key: torch.Tensor
     value: torch.Tensor
     weights: torch.Tensor | None = None
@@ -83,6 +84,9 @@ class DensePages:
                             ("_code", nat.dtype_code(key.dtype)), ("block_size", key.shape[2]),
                             ("heads", key.shape[1])):
             object.__setattr__(self, name, value)
+
+    def __reduce__(self):       # copies and pickles describe the tensors that they hold
+        return type(self), (self.key, self.value, self.weights, self.positions)
 
     @classmethod
     def allocate(cls, pages, block_size, heads, dtype=torch.bfloat16, device="cuda", *, evictable=True):

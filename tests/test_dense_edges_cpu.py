@@ -27,3 +27,33 @@ def test_an_empty_selection_writes_nothing(calls):
     assert [name for name, _ in calls] == ["iq_dense_write_from"] * 2
     with pytest.raises(ValueError):
         write_rows(k, k, cu, 3, pages, table, keep=torch.zeros((1, 3, 0), dtype=I32))
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "copy"])
+@pytest.mark.parametrize("evictable", [True, False])
+@pytest.mark.parametrize("halves", [True, False])
+def test_copies_of_pages_describe_their_own_memory(how, evictable, halves):
+    import copy
+    import ctypes
+    import pickle
+    from inquant import _native as nat
+    if halves:
+        both = torch.randn((4, 2, 3, 16, 128)).bfloat16()
+        key, value = both[:, 0], both[:, 1]
+    else:
+        key, value = torch.randn((4, 16, 3, 128)).half().transpose(1, 2), torch.randn((4, 3, 16, 136)).half()[..., :128]
+    side = (torch.randn((4, 3, 16)), torch.arange(192, dtype=I32).view(4, 3, 16)) if evictable else ()
+    first = DensePages(key, value, *side)
+    made = {"deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x)), "copy": copy.copy}[how](first)
+    desc = ctypes.cast(made._desc, ctypes.POINTER(nat.DensePagesDesc)).contents
+    own = ctypes.addressof(made._pages)
+    assert made._desc == own and (how == "copy" or own != ctypes.addressof(first._pages))
+    for name in ("key", "value", "weights", "positions"):
+        mine, theirs = getattr(made, name), getattr(first, name)
+        assert getattr(desc, name) == (0 if mine is None else mine.data_ptr())
+        if mine is not None:
+            assert torch.equal(mine, theirs) and (mine.data_ptr() == theirs.data_ptr()) == (how == "copy")
+    assert (desc.k_sp, desc.k_sh, desc.k_st) == made.key.stride()[:3]
+    assert (desc.v_sp, desc.v_sh, desc.v_st) == made.value.stride()[:3]
+    assert (desc.pages, desc.heads, desc.block_tokens) == (4, 3, 16)
+    assert (made.block_size, made.heads, made._dtype, made._code) == (16, 3, first._dtype, first._code)
