@@ -424,7 +424,8 @@ int iq_prefill_attention_lse(const void *q, const void *k, const void *v, int dt
  * each sequence; window == 0: over all, with the lse of
  * iq_prefill_attention_lse (with a window the lse may be NULL: it is computed
  * from the workspace).  q [tokens, Hq, 128], k [tokens, H, 128], sequences and
- * strides as iq_prefill_attention (head size 128; q token stride below 2^25).
+ * strides as iq_prefill_attention (head size 128; q token stride below 2^25); a
+ * sequence longer than max_seqlen counts as its first max_seqlen tokens.
  * Tokens of no sequence are not written.  workspace: f32,
  * iq_prefill_weights_floats elements, 16-byte aligned.
  */
@@ -477,8 +478,8 @@ typedef struct iq_dense_pages {
 
 /*
  * Writes rows of token-major k / v [tokens, heads, 128] (element strides;
- * 16-byte aligned rows; sequences [cu_seqlens[i], cu_seqlens[i + 1]), none
- * longer than max_seqlen) into the pages: row t of sequence i to cache row
+ * 16-byte aligned rows; sequences [cu_seqlens[i], cu_seqlens[i + 1]), rows from
+ * max_seqlen on left out) into the pages: row t of sequence i to cache row
  * start[i] + t (start NULL: 0) of every head.  With keep i32 [n_seq, heads,
  * kept] head h takes only the rows keep[i][h][j], to cache row start[i] + j
  * (entries outside the sequence are skipped).  Beside row t go its weight
@@ -511,7 +512,8 @@ int iq_dense_write_from(const iq_dense_write_args *args);
  * The rows a budget keeps of each sequence and head: the first `sink` and the
  * last `recent` rows, then by weight (weights f32, row t of sequence i and
  * head h at h * w_stride + cu_seqlens[i] + t), ties to the lowest row, NaN
- * last.  keep i32 [n_seq, H, budget]: ascending rows within the sequence, -1
+ * last.  A sequence longer than max_seqlen counts as its first max_seqlen rows.
+ * keep i32 [n_seq, H, budget]: ascending rows within the sequence, -1
  * behind the last.
  */
 int iq_select_rows(const float *weights, int64_t w_stride, int64_t H, const int32_t *cu_seqlens, int64_t n_seq,

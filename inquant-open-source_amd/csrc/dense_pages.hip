@@ -15,6 +15,13 @@ namespace {
 
 // ---------------------------------------------------------------- rows into pages
 
+// Rows of sequence `seq` that an entry point considers.
+__device__ __forceinline__ uint32_t dense_length(const int32_t *cu, int seq, uint32_t max_len)
+{
+    const int64_t have = (int64_t)cu[seq + 1] - cu[seq];
+    return have <= 0 ? 0 : have < max_len ? (uint32_t)have : max_len;
+}
+
 struct WriteArgs {
     const uint16_t *k, *v;
     int64_t k_st, k_sh, v_st, v_sh;          // element strides (token, head)
@@ -23,6 +30,7 @@ struct WriteArgs {
     int64_t w_stride;
     const int32_t *keep;                     // [n, H, kept] or null
     int64_t kept;
+    uint32_t max_len;                        // a sequence's rows past it are left out
     DensePool pool;
 };
 
@@ -40,8 +48,8 @@ __global__ __launch_bounds__(256) void write_rows_kernel(WriteArgs a)
 {
     const int seq = blockIdx.y, lane = threadIdx.x & 15;
     const uint32_t H = (uint32_t)a.pool.H, kept = (uint32_t)a.kept;
-    const int64_t t0 = a.cu[seq], have = a.cu[seq + 1] - t0;
-    const uint32_t len = have > 0 ? (uint32_t)have : 0, item = blockIdx.x * WR_ITEMS + (threadIdx.x >> 4);
+    const int64_t t0 = a.cu[seq];
+    const uint32_t len = dense_length(a.cu, seq, a.max_len), item = blockIdx.x * WR_ITEMS + (threadIdx.x >> 4);
     if (item >= (uint64_t)(a.keep ? kept : len) * H) return;
     uint32_t h, j, source;
     if (a.keep) {
@@ -286,6 +294,7 @@ struct SelectArgs {
     const float *weights;
     int64_t w_stride;
     const int32_t *cu;
+    uint32_t max_len;                        // a sequence's rows past it are left out
     int64_t budget, sink, recent;
     int32_t *keep;
 };
@@ -307,10 +316,9 @@ __global__ __launch_bounds__(SEL_NT) void select_rows_kernel(SelectArgs a)
 {
     __shared__ SelectSmem sm;
     const int h = blockIdx.x, seq = blockIdx.y;
-    const int64_t t0 = a.cu[seq], len = a.cu[seq + 1] - t0;
-    const float *w = a.weights + h * a.w_stride + t0;
+    const float *w = a.weights + h * a.w_stride + a.cu[seq];
     int32_t *keep = a.keep + ((int64_t)seq * gridDim.x + h) * a.budget;
-    const uint32_t rows = len > 0 ? (uint32_t)len : 0, sink = (uint32_t)a.sink, recent = (uint32_t)a.recent;
+    const uint32_t rows = dense_length(a.cu, seq, a.max_len), sink = (uint32_t)a.sink, recent = (uint32_t)a.recent;
     select_rows_of(
         sm, rows, (uint32_t)a.budget, [&](uint32_t i, uint32_t end, uint32_t from, uint32_t to, auto whole) {
             u32x4 keys;
@@ -457,7 +465,7 @@ extern "C" int iq_dense_write(const void *k, const void *v, int dtype, int64_t k
     const int64_t groups = (rows * pool.H + WR_ITEMS - 1) / WR_ITEMS;
     IQ_CHECK_ARG(groups <= 0xffffff, "iq_dense_write: too many rows");
     const WriteArgs a{(const uint16_t *)k, (const uint16_t *)v, k_st, k_sh, v_st, v_sh, cu_seqlens, start, positions,
-                      weights, w_stride, keep, kept, pool};
+                      weights, w_stride, keep, kept, (uint32_t)max_seqlen, pool};
     hipLaunchKernelGGL(write_rows_kernel, dim3((unsigned)groups, (unsigned)n_seq), dim3(256), 0, (hipStream_t)stream,
                        a);
     IQ_CHECK_LAUNCH("dense_write");
@@ -474,7 +482,7 @@ extern "C" int iq_select_rows(const float *weights, int64_t w_stride, int64_t H,
     IQ_CHECK_ARG(sink >= 0 && recent >= 0 && budget >= 1 && budget <= 0x7fffffffLL && sink + recent <= budget,
                  "iq_select_rows: sink and recent rows must fit the budget");
     if (n_seq == 0) return IQ_OK;
-    const SelectArgs a{weights, w_stride, cu_seqlens, budget, sink, recent, keep};
+    const SelectArgs a{weights, w_stride, cu_seqlens, (uint32_t)max_seqlen, budget, sink, recent, keep};
     hipLaunchKernelGGL(select_rows_kernel, dim3((unsigned)H, (unsigned)n_seq), dim3(SEL_NT), 0, (hipStream_t)stream,
                        a);
     IQ_CHECK_LAUNCH("select_rows");

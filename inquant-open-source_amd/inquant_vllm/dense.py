@@ -200,8 +200,8 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
                keep=None):
     """Rows of token-major key/value [tokens, kv_heads, 128] into the pages.
 
-    Row t of sequence i (cu_seqlens int32 [sequences + 1], none longer than
-    max_seqlen) goes to cache row start[i] + t of every head (``start`` int32
+    Row t of sequence i (cu_seqlens int32 [sequences + 1]; rows from max_seqlen
+    on are left out) goes to cache row start[i] + t of every head (``start`` int32
     [sequences], None: 0); with ``keep`` int32 [sequences, kv_heads, kept]
     (``select_rows``) head h takes only the rows keep[i, h, j], to cache row
     start[i] + j, and entries outside the sequence are skipped.  Where the pages
@@ -243,8 +243,8 @@ def select_rows(weights, cu_seqlens, max_seqlen, budget, *, sink=0, recent=0, ou
     ``sink`` and the last ``recent`` rows, then by weight (``weights`` f32
     [kv_heads, tokens], as ``prefill_weights`` gives them), ties to the lowest
     row, NaN last.  Returns int32 [sequences, kv_heads, budget]: ascending rows
-    within the sequence, -1 behind the last.  max_seqlen >= every sequence
-    length."""
+    within the sequence, -1 behind the last.  A sequence longer than max_seqlen
+    counts as its first max_seqlen rows, as ``prefill_weights`` takes it."""
     budget, sink, recent = int(budget), int(sink), int(recent)
     _budget(budget, sink, recent)
     if weights.ndim != 2 or weights.dtype is not _F32 or weights.shape[0] < 1 \
@@ -371,7 +371,8 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
     ``lse`` [Hq, tokens] ``prefill_attention(..., lse=...)`` wrote, or with
     ``window=w`` over the last w queries of each sequence (lse optional; w at
     most 4096, or all with the lse).
-    Tokens of no sequence are not written."""
+    A sequence longer than max_seqlen counts as its first max_seqlen tokens.
+    Tokens of no sequence, and those past max_seqlen, are not written."""
     (tokens, hq, _), qs = _token_rows(query, "query")
     (rows, h, _), ks = _token_rows(key, "key")
     if tokens != rows or query.dtype not in _ROWS or key.dtype is not query.dtype:

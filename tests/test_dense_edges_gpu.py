@@ -45,3 +45,52 @@ def test_a_copy_of_pages_works_on_its_own_memory():
     assert _equal(pages, start) and not _equal(fork, start)
     changed = [t.clone() for t in _fields(fork)]
     assert torch.equal(use(pages), got) and _equal(pages, changed) and _equal(fork, changed)
+
+
+@pytest.mark.parametrize("h", [1, 3, 16])
+def test_rows_past_max_seqlen_are_left_out(h):
+    """Of sequences longer than the bound every operator takes the same first rows."""
+    from densecase import cache_rows, keep_rows
+    from inquant_vllm import prefill_weights, select_rows, write_rows
+    bound, lengths = 37, [10, 50, 38, 0, 37]
+    print(f"past max_seqlen {h}", flush=True)
+    gen, tokens, n = generator(10 + h), sum(lengths), len(lengths)
+    taken = [min(x, bound) for x in lengths]
+    key, value = (rows(gen, tokens, h, 128, dtype=torch.bfloat16) for _ in range(2))
+    cu, w = offsets(lengths), torch.rand((h, tokens), generator=gen, device="cuda")
+    table = torch.arange(4 * n, device="cuda").view(n, 4).to(torch.int32)
+    pages = pool(gen, 4 * n, h, 16, torch.bfloat16)
+    start = [t.clone() for t in _fields(pages)]
+    write_rows(key, value, cu, bound, pages, table, weights=w)
+    first = 0
+    for i, m in enumerate(taken):
+        for field, want in zip(_fields(pages)[:3], (key.transpose(0, 1), value.transpose(0, 1), w)):
+            assert torch.equal(cache_rows(field, table[i], m), want[:, first:first + m])
+        for field, was in zip(_fields(pages), start):
+            assert torch.equal(cache_rows(field, table[i], 64)[:, m:], cache_rows(was, table[i], 64)[:, m:])
+        first += lengths[i]
+    got, host, first = select_rows(w, cu, bound, 20, sink=2, recent=5).tolist(), w.cpu(), 0
+    for i, m in enumerate(taken):
+        always = [j < 2 or j >= m - 5 for j in range(m)]
+        for head in range(h):
+            exp = keep_rows(host[head, first:first + m].tolist(), always, 20)
+            assert got[i][head] == exp + [-1] * (20 - len(exp)), (i, head)
+        first += lengths[i]
+    # kept rows past the bound are skipped as those outside the sequence are
+    for t, was in zip(_fields(pages), start):
+        t.copy_(was)
+    keep = i32([[[36, 37, 9, 40]] * h] * n)
+    write_rows(key, value, cu, bound, pages, table, weights=w, keep=keep)
+    first = 0
+    for i, m in enumerate(taken):
+        for j, r in enumerate((36, 37, 9, 40)):
+            want = key[first + r] if r < m else cache_rows(start[0], table[i], 64)[:, j]
+            assert torch.equal(cache_rows(pages.key, table[i], 64)[:, j], want), (i, j)
+        first += lengths[i]
+    # the weights of a prompt are of the same rows: those of the sequences cut to the bound
+    part = torch.cat([torch.arange(f, f + m, device="cuda") for f, m in zip(cu.tolist(), taken)])
+    q = rows(gen, tokens, 2 * h, 128, dtype=torch.bfloat16)
+    out = torch.full((h, tokens), -5.0, device="cuda")
+    prefill_weights(q, key, cu, bound, SCALE, window=8, output=out)
+    cut = prefill_weights(q[part], key[part], offsets(taken), bound, SCALE, window=8)
+    assert torch.equal(out[:, part], cut) and int((out == -5.0).sum()) == h * (tokens - len(part))
