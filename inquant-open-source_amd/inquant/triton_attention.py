@@ -69,7 +69,7 @@ class SharedDecodeWorkspace:
     """fp32 scratch of one request, reused by all its layers on one stream.
 
     The cache counts it once; decode states do not.  The allocation only
-    grows (to the largest request seen)."""
+    grows: to the largest request seen, or after ``floats`` by doubling."""
 
     def __init__(self):
         self.tensor = None
@@ -78,31 +78,37 @@ class SharedDecodeWorkspace:
 
     @property
     def nbytes(self) -> int:
-        return self.tensor.untyped_storage().nbytes() if self.tensor is not None else 0
+        held = [*(self._lent or ()), *(() if self.tensor is None else (self.tensor,))]
+        return sum(t.untyped_storage().nbytes() for t in held)
+
+    def _grow(self, needed, device):
+        """An allocation of at least ``needed`` floats.  Once one was lent, what
+        is outgrown is kept, and sizes double: the past stays below the present."""
+        have = self.tensor
+        if have is not None and self._lent is not None:
+            self._lent.append(have)
+            needed = max(needed, 2 * have.numel())
+        self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
+        return self.tensor
 
     def acquire(self, shape, device):
         self._pin.check(device)
         needed = math.prod(shape)
         have = self.tensor
         if have is None or have.numel() < needed:
-            if self._lent is not None:
-                self._lent.append(have)
-            have = self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
+            have = self._grow(needed, device)
         return have[:needed].view(shape)
 
     def floats(self, needed, device):
         """Address and size of at least ``needed`` floats, and the handle of the
-        stream they belong to.  Grows by doubling, and keeps what it outgrew: the
-        address may stand in a captured graph."""
+        stream they belong to.  Whatever outgrows them, they are kept: the address
+        may stand in a captured graph."""
         handle = self._pin.check(device)
         have = self.tensor
         if self._lent is None:
             self._lent = []
         if have is None or have.numel() < needed:
-            if have is not None:
-                self._lent.append(have)
-                needed = max(needed, 2 * have.numel())
-            have = self.tensor = torch.empty(needed, dtype=torch.float32, device=device)
+            have = self._grow(needed, device)
         return have.data_ptr(), have.numel(), handle
 
 

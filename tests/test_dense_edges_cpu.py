@@ -57,3 +57,44 @@ def test_copies_of_pages_describe_their_own_memory(how, evictable, halves):
     assert (desc.v_sp, desc.v_sh, desc.v_st) == made.value.stride()[:3]
     assert (desc.pages, desc.heads, desc.block_tokens) == (4, 3, 16)
     assert (made.block_size, made.heads, made._dtype, made._code) == (16, 3, first._dtype, first._code)
+
+
+def test_a_lent_workspace_keeps_a_bounded_past():
+    """What a captured graph may still use is kept, counted, and never more than what is in use."""
+    from inquant.triton_attention import SharedDecodeWorkspace
+
+    class Pin:
+        def check(self, device):
+            return 0
+
+    def fresh():
+        ws = SharedDecodeWorkspace()
+        ws._pin = Pin()
+        return ws
+    ws = fresh()
+    ws.acquire((10, 10), "cpu")
+    ws.acquire((11, 10), "cpu")
+    assert ws.tensor.numel() == 110 and ws.nbytes == 440              # before a loan: what is asked for, nothing kept
+    address, have, _ = ws.floats(64, "cpu")
+    assert (address, have) == (ws.tensor.data_ptr(), 110)
+    lent = [ws.tensor]
+    for size in range(120, 4000, 37):                                 # a decode whose partitions grow with its context
+        assert ws.acquire((size,), "cpu").shape == (size,)
+        if ws.tensor is not lent[-1]:
+            lent.append(ws.tensor)
+        if size % 5 == 0:
+            address, have, _ = ws.floats(size + 3, "cpu")
+            assert have >= size + 3 and address == ws.tensor.data_ptr()
+            if ws.tensor is not lent[-1]:
+                lent.append(ws.tensor)
+    assert [t.data_ptr() for t in ws._lent] == [t.data_ptr() for t in lent[:-1]]
+    past = sum(t.numel() for t in ws._lent)
+    assert len(lent) > 3 and past <= ws.tensor.numel()
+    assert ws.nbytes == 4 * (past + ws.tensor.numel())
+    ws = fresh()
+    assert ws.floats(0, "cpu")[1] == 0 and ws.acquire((5,), "cpu").numel() == 5
+    assert fresh().nbytes == 0 and ws.nbytes == 20
+    ws = fresh()
+    ws._lent = []                                                     # lent, but nothing allocated yet
+    ws.acquire((3,), "cpu")
+    assert ws.nbytes == 12
