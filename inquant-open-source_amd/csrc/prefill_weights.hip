@@ -38,8 +38,9 @@ struct WeightArgs {
     float c_log2;
     const float *lse;                        // natural log, token i of head hq at hq * lse_sh + i; with lse_sh 0
     int64_t lse_sh;                          // window row r of (seq, h) at (seq * H + h) * G * window + r
-    f32x2 *ml;                               // the lse pass: (max, sum) per [seq, 64-key tile, H, window row]
-    int tiles64;
+    f32x2 *ml;                               // the lse pass: (max, sum) per [64-key tile, H, window row of the slice]
+    int tiles64;                             // a sequence's first of those tiles: see tile_base
+    int row0, ml_rows;                       // the slice: window rows row0 .. row0 + ml_rows - 1 of each KV head
     float *out;                              // [H, out_sh]; all queries: [ranges, Hq, out_sh]
     int64_t out_sh;
 };
@@ -117,6 +118,15 @@ __device__ __forceinline__ int length_of(const WeightArgs &a, int seq)
     return len < a.max_len ? len : a.max_len;
 }
 
+// The lse pass keeps its (max, sum) per 64 keys: sequence i's from tile i * tiles64
+// on, or with tiles64 0 from cu[i] / 64 + i on (no two overlap: of consecutive
+// sequences the base grows by cu[i + 1] / 64 - cu[i] / 64 + 1, at least the tiles
+// of sequence i), so that one long prompt of a batch does not size the others'.
+__device__ __forceinline__ int64_t tile_base(const WeightArgs &a, int seq)
+{
+    return a.tiles64 ? (int64_t)seq * a.tiles64 : (int64_t)(a.cu[seq] / KW) + seq;
+}
+
 // over the lane pair l, l ^ 32 (one query's two halves)
 __device__ __forceinline__ float pair_max(float v)
 {
@@ -184,10 +194,12 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
     const int g0 = tile * KG, from = range * a.chunk;
     // "queries" are query positions, or with ROWS rows of the window
     const Window win = window_of(a, len);
-    const int end = ROWS ? win.rows : len - from < a.chunk ? len : from + a.chunk;
-    if (g0 >= (ROWS ? len : end) || from >= len) return;     // uniform
-    const int q0 = ROWS ? 0 : g0 > from ? g0 : from;         // the first that sees one of these keys
+    const int slice = LSEPASS ? a.row0 + a.ml_rows : win.rows;
+    const int end = ROWS ? win.rows < slice ? win.rows : slice : len - from < a.chunk ? len : from + a.chunk;
+    const int q0 = LSEPASS ? a.row0 : ROWS ? 0 : g0 > from ? g0 : from;  // the first that sees one of these keys
+    if (g0 >= (ROWS ? len : end) || from >= len || LSEPASS && q0 >= end) return;     // uniform
     const int k0 = g0 + KW * wave;           // this wavefront's first key
+    f32x2 *const ml = LSEPASS ? a.ml + ((tile_base(a, seq) + k0 / KW) * a.H + h) * a.ml_rows - a.row0 : nullptr;
     u32x4 kf[2][8];                          // A operand: key k0 + 32 kb + c32, channels 16 d + 8 h32 .. + 7
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -302,8 +314,7 @@ __global__ __launch_bounds__(NT, 2) void prefill_weights(WeightArgs a)
                 l += __builtin_amdgcn_exp2f(fmaf(late[d >> 2][4 * (d & 3) + e], a.c_log2, -use));
             if (d == 7 && part == 1) {
                 l = pair_sum(l);
-                if (h32 == 0 && late_row >= 0)
-                    a.ml[(((int64_t)seq * a.tiles64 + k0 / KW) * a.H + h) * a.G * a.window + late_row] = f32x2{m, l};
+                if (h32 == 0 && late_row >= 0) ml[late_row] = f32x2{m, l};
             }
         } else {
 #pragma unroll
@@ -455,19 +466,19 @@ __global__ __launch_bounds__(LR * LG) void window_lse(WeightArgs a, float *lse)
 {
     __shared__ f32x2 sm[LG][LR];
     const int seq = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % LR, group = threadIdx.x / LR;
-    const int len = length_of(a, seq), row = blockIdx.x * LR + lane;
+    const int len = length_of(a, seq), row = a.row0 + blockIdx.x * LR + lane;
     const Window win = window_of(a, len);
-    const int64_t all = (int64_t)a.G * a.window;
+    const bool live = row < win.rows && row < a.row0 + a.ml_rows;
     f32x2 mine = {NEG_INF, 0.0f};
     auto join = [](f32x2 x, f32x2 y) {
         const float m = fmaxf(x[0], y[0]), use = m == NEG_INF ? 0.0f : m;
         return f32x2{m, x[1] * __builtin_amdgcn_exp2f(x[0] - use) + y[1] * __builtin_amdgcn_exp2f(y[0] - use)};
     };
-    if (row < win.rows) {
+    if (live) {
         // the tiles that hold a key at or before the last query (the others' keys are unseen: (-inf, 0))
-        const f32x2 *ml = a.ml + ((int64_t)seq * a.tiles64 * a.H + h) * all + row;
+        const f32x2 *ml = a.ml + (tile_base(a, seq) * a.H + h) * a.ml_rows + row - a.row0;
 #pragma unroll 4
-        for (int t = group; t <= (len - 1) / KW; t += LG) mine = join(mine, ml[t * a.H * all]);
+        for (int t = group; t <= (len - 1) / KW; t += LG) mine = join(mine, ml[(int64_t)t * a.H * a.ml_rows]);
     }
     sm[group][lane] = mine;
     __syncthreads();
@@ -476,8 +487,12 @@ __global__ __launch_bounds__(LR * LG) void window_lse(WeightArgs a, float *lse)
     for (int g = group + 4; g < LG; g += 4) mine = join(mine, sm[g][lane]);
 #pragma unroll
     for (int d = 16; d < 64; d *= 2) mine = join(mine, f32x2{__shfl_xor(mine[0], d), __shfl_xor(mine[1], d)});
-    if (group == 0 && row < win.rows)
-        lse[((int64_t)seq * a.H + h) * all + row] = (mine[0] == NEG_INF ? 0.0f : mine[0] + __builtin_amdgcn_logf(mine[1])) * LN2;
+    if (group == 0 && live) {
+        const int g = (int)head_of(row, 1.0f / (float)win.n);
+        float *to = a.lse_sh ? lse + (int64_t)(h * a.G + g) * a.lse_sh + a.cu[seq] + win.lo + row - g * win.n
+                             : lse + ((int64_t)seq * a.H + h) * a.G * a.window + row;
+        *to = (mine[0] == NEG_INF ? 0.0f : mine[0] + __builtin_amdgcn_logf(mine[1])) * LN2;
+    }
 }
 
 // The sums of each KV head's query heads and of the query ranges that see a key.
@@ -495,7 +510,15 @@ __global__ __launch_bounds__(256) void add_heads(WeightArgs a, const float *part
 
 struct Scratch {
     int64_t lse, ml, part;                   // floats of each
+    int64_t tiles;                           // 64-key tiles that ml holds of each head and row
+    bool by_seq;                             // a sequence's tiles: as many for each; else by its tokens
+    int64_t lse_sh;                          // the own lse: 0 by window rows, else [Hq, tokens]
 };
+
+// The lse pass goes over the window's rows in slices whose (max, sum) take 256 MiB
+// at most, or 64 rows: a 4096-query window over 32K tokens, 28 heads over 4, has
+// 470 MB of them, 64 queries over 32K 7 (one slice, as everything below the bound).
+constexpr int64_t ML_MOST = 1 << 26;         // floats
 
 // Queries of a workgroup at most, a power of two and of whole key tiles (so that a
 // range sees a whole key tile or ends before it): the one for which the longest
@@ -532,10 +555,16 @@ int64_t chunk_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen)
 
 Scratch scratch_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen, int64_t tokens, int64_t window, bool lse)
 {
-    Scratch s{0, 0, 0};
+    Scratch s{};
     if (window > 0 && !lse) {
-        s.lse = n_seq * Hq * window;
-        s.ml = 2 * n_seq * ((max_seqlen + KW - 1) / KW) * Hq * window;
+        const int64_t even = n_seq * ((max_seqlen + KW - 1) / KW), sum = tokens / KW + n_seq;
+        s.by_seq = even <= sum || 2 * even * Hq * window <= ML_MOST;
+        s.tiles = s.by_seq ? even : sum;
+        s.lse_sh = n_seq * window <= tokens ? 0 : tokens;
+        s.lse = Hq * (s.lse_sh ? tokens : n_seq * window);
+        const int64_t whole = 2 * s.tiles * Hq * window, least = 2 * s.tiles * Hq * QT;
+        const int64_t most = ML_MOST > least ? ML_MOST : least;
+        s.ml = whole < most ? whole : most;
     }
     if (window == 0) {
         const int64_t chunk = chunk_of(Hq, n_seq, max_seqlen);
@@ -587,7 +616,7 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     const int64_t chunk = window ? 1 << 30 : chunk_of(Hq, n_seq, max_seqlen), chunks = (max_seqlen + chunk - 1) / chunk;
     WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq,
                  (int)max_seqlen, (int)H, (int)Hq, (int)G, (int)window, (int)chunk, (int)chunks,
-                 scale * LOG2E, lse, lse_sh, (f32x2 *)workspace, (int)((max_seqlen + KW - 1) / KW), out, out_sh};
+                 scale * LOG2E, lse, lse_sh, (f32x2 *)workspace, s.by_seq ? (int)((max_seqlen + KW - 1) / KW) : 0, 0, 0, out, out_sh};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
     const int64_t m = chunk / KG, units = window ? tiles : m * chunks * (chunks - 1) / 2 + m * chunks;
@@ -597,12 +626,18 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     if (window > 0) {
         if (!lse) {
             float *own = workspace + s.ml;
-            hipLaunchKernelGGL((f16 ? prefill_weights<true, WINDOW_LSE> : prefill_weights<false, WINDOW_LSE>), grid,
-                               block, 0, st, a);
-            hipLaunchKernelGGL(window_lse, dim3((unsigned)((G * window + LR - 1) / LR), (unsigned)H, (unsigned)n_seq),
-                               dim3(LR * LG), 0, st, a, own);
+            const int64_t fit = s.ml / (2 * s.tiles * H);    // whole tiles of rows, as without slices
+            a.lse_sh = s.lse_sh;
+            a.ml_rows = (int)(fit < G * window ? fit / QT * QT : G * window);
+            for (int64_t row0 = 0; row0 < G * window; row0 += a.ml_rows) {
+                const int64_t rows = G * window - row0 < a.ml_rows ? G * window - row0 : a.ml_rows;
+                a.row0 = (int)row0;
+                hipLaunchKernelGGL((f16 ? prefill_weights<true, WINDOW_LSE> : prefill_weights<false, WINDOW_LSE>), grid,
+                                   block, 0, st, a);
+                hipLaunchKernelGGL(window_lse, dim3((unsigned)((rows + LR - 1) / LR), (unsigned)H, (unsigned)n_seq),
+                                   dim3(LR * LG), 0, st, a, own);
+            }
             a.lse = own;
-            a.lse_sh = 0;
         }
         hipLaunchKernelGGL((f16 ? prefill_weights<true, WINDOW> : prefill_weights<false, WINDOW>), grid, block, 0, st,
                            a);

@@ -371,6 +371,10 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
     ``lse`` [Hq, tokens] ``prefill_attention(..., lse=...)`` wrote, or with
     ``window=w`` over the last w queries of each sequence (lse optional; w at
     most 4096, or all with the lse).
+    Scratch of a call: with the lse and no window 4 bytes per token, query head
+    and range of queries (one up to 16384, more for a long prompt); for a window's
+    own lse up to 256 MiB (or 512 bytes per query head and 64 keys, if that is
+    more) and 4 bytes per query head and window row.
     A sequence longer than max_seqlen counts as its first max_seqlen tokens.
     Tokens of no sequence, and those past max_seqlen, are not written."""
     (tokens, hq, _), qs = _token_rows(query, "query")

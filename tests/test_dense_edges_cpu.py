@@ -98,3 +98,39 @@ def test_a_lent_workspace_keeps_a_bounded_past():
     ws._lent = []                                                     # lent, but nothing allocated yet
     ws.acquire((3,), "cpu")
     assert ws.nbytes == 12
+
+
+def _window_floats(hq, n, longest, tokens, window):
+    from inquant import _native as nat
+    return nat.lib().iq_prefill_weights_floats(hq, n, longest, tokens, window, 0)
+
+
+@pytest.mark.parametrize("hq,n,longest,tokens,window", [
+    (32, 16, 32768, 16 * 32768, 4096), (28, 8, 32768, 8 * 32768, 4096), (32, 1, 131072, 131072, 4096),
+    (32, 64, 131072, 131072 + 63 * 100, 256), (16, 1000, 4096, 4096 + 999 * 10, 4096), (64, 1, 1 << 20, 1 << 20, 4096),
+    (32, 60000, 32768, 92767, 64)])
+def test_scratch_of_a_window_is_bounded(hq, n, longest, tokens, window):
+    # (max, sum) of 256 MiB or of 64 rows, and the rows' lse, never more than one per token
+    tiles = min(n * -(-longest // 64), tokens // 64 + n)
+    most = max(1 << 26, 2 * tiles * hq * 64) + hq * min(n * window, tokens)
+    assert _window_floats(hq, n, longest, tokens, window) <= most
+
+
+def test_scratch_of_a_small_window_holds_every_tile_and_row():
+    for hq, n, longest, window in ((28, 1, 32768, 64), (32, 3, 9000, 100), (16, 1, 1, 1)):
+        assert _window_floats(hq, n, longest, n * longest, window) == \
+            2 * n * -(-longest // 64) * hq * window + n * hq * window
+
+
+def test_tiles_placed_by_their_tokens_do_not_overlap():
+    import random
+    rng = random.Random(1)
+    for _ in range(300):
+        at = start = rng.choice([0, 0, 63, 1000])
+        ends, n = [0], rng.randint(1, 30)                    # an end of the sequence before: none below its base
+        for i in range(n):
+            base, length = at // 64 + i, rng.choice([0, 1, 63, 64, 65, rng.randint(0, 3000)])
+            assert base >= ends[-1]
+            ends.append(base + -(-length // 64))
+            at += length
+        assert ends[-1] <= at // 64 + n, start

@@ -94,3 +94,28 @@ def test_rows_past_max_seqlen_are_left_out(h):
     prefill_weights(q, key, cu, bound, SCALE, window=8, output=out)
     cut = prefill_weights(q[part], key[part], offsets(taken), bound, SCALE, window=8)
     assert torch.equal(out[:, part], cut) and int((out == -5.0).sum()) == h * (tokens - len(part))
+
+
+@pytest.mark.parametrize("lengths,heads,window,dtype", [
+    # several slices of rows, the tiles placed by their tokens
+    ([5, 16500, 0, 64], (32, 2), 4096, torch.bfloat16),
+    # several slices, a sequence's tiles as many for each
+    ([17000], (32, 4), 4096, torch.float16),
+    # one long prompt of many: tiles placed by their tokens, the lse by tokens
+    ([0, 63, 64, 65, 129, 1, 5000] + [70, 3, 128] * 11, (16, 2), 1000, torch.float16),
+    ([1] * 30 + [4096] + [2] * 9, (16, 16), 2048, torch.bfloat16),
+], ids=["slices-tokens", "slices", "ragged", "ones"])
+def test_a_window_in_slices_of_bounded_scratch(lengths, heads, window, dtype):
+    from test_prefill_weights_gpu import _case, _close, _expected
+    from inquant_vllm import prefill_attention, prefill_weights
+    hq, h = heads
+    print(f"window {window} of {lengths} {heads} {dtype}", flush=True)
+    q, k, v, cu = _case(len(lengths) + hq, lengths, hq, h, dtype)
+    total, _, slack = _expected(q, k, lengths, SCALE, window)
+    longest, tokens = max(lengths), sum(lengths)
+    got = prefill_weights(q, k, cu, longest, SCALE, window=window)
+    _close(got, total, slack, window * hq // h)
+    lse = torch.full((hq, tokens), float("nan"), device="cuda")
+    prefill_attention(q, k, v, cu, longest, SCALE, lse=lse)
+    _close(prefill_weights(q, k, cu, longest, SCALE, window=window, lse=lse), total, slack, window * hq // h)
+    assert torch.equal(prefill_weights(q, k, cu, longest, SCALE, window=window), got)
