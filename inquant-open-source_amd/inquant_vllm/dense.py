@@ -191,6 +191,12 @@ def _token_rows(t, what, heads=None):
     return shape, (st, sh)
 
 
+def _apart(n, m, a, b):
+    """Whether rows of 128 elements at i a + j b, i < n and j < m, overlap nowhere."""
+    at = sorted(i * a + j * b for i in range(n) for j in range(m))
+    return all(y - x >= 128 for x, y in zip(at, at[1:]))
+
+
 def _budget(budget, sink, recent):
     if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
         raise ValueError("sink and recent rows must fit a budget of at least one row")
@@ -342,7 +348,7 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     dtype, os = output.dtype, output.stride()
     if output.shape != shape or os[2] != 1 or dtype is not pages._dtype and dtype is not _F32:
         raise ValueError("output must be [sequences, heads, 128] of the query dtype or float32")
-    if os[0] < 128 and n > 1 or os[1] < 128 and hq > 1:
+    if (os[1] < 128 or os[0] < 128 + os[1] * (hq - 1)) and not _apart(n, hq, *os[:2]):
         raise ValueError("the output's rows must not overlap")
     if n == 0:
         return output

@@ -134,3 +134,28 @@ def test_tiles_placed_by_their_tokens_do_not_overlap():
             ends.append(base + -(-length // 64))
             at += length
         assert ends[-1] <= at // 64 + n, start
+
+
+def test_decode_refuses_outputs_whose_rows_overlap(calls, monkeypatch):
+    from inquant_vllm import dense_decode
+    from inquant.triton_attention import SharedDecodeWorkspace
+    ran = []
+    monkeypatch.setattr(dense, "_status", lambda *a: ran.append(a) or 0)
+    monkeypatch.setattr(SharedDecodeWorkspace, "floats", lambda *a: (0, 0, 0))
+    n, hq = 3, 4
+    pages = DensePages.allocate(4, 16, 2, device="cpu")
+    q, table, lengths = torch.zeros((n, hq, 128), dtype=torch.bfloat16), torch.zeros((n, 1), dtype=I32), torch.ones(n, dtype=I32)
+
+    def call(*strides, n=n, hq=hq):
+        out = torch.zeros(10000).as_strided((n, hq, 128), strides)
+        return dense_decode(q[:n, :hq], pages, table[:n], lengths[:n], 16, 0.1, SharedDecodeWorkspace(), out)
+    for strides in ((128, 128, 1), (256, 128, 1), (511, 128, 1), (128, 383, 1), (256, 256, 1), (0, 128, 1), (512, 64, 1),
+                    (128, 256, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            call(*strides)
+    assert ran == []
+    for strides in ((512, 128, 1), (513, 128, 1), (128, 384, 1), (700, 130, 1), (128, 391, 1)):
+        call(*strides)
+    call(640, 256, 1)                                        # a sequence's rows between those of the next
+    call(5, 128, 1, n=1)
+    assert len(ran) == 7
