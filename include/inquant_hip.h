@@ -537,7 +537,7 @@ int iq_select_rows_from(const iq_select_rows_args *args);
  * `budget` on (key, value, weight and position); all other rows stay as they
  * are.  lengths i32: rows each sequence holds (at most max_tokens are
  * considered); new_lengths i32: min(lengths, budget), which may take the place
- * of lengths or of seen.  workspace: i32, iq_dense_evict_ints elements (none while a head
+ * of lengths (all of them, or none) or of seen.  workspace: i32, iq_dense_evict_ints elements (none while a head
  * moves at most IQ_DENSE_FEW_MOVES rows: min(budget, max_tokens - budget)).
  * No page may belong to two sequences.
  */

@@ -511,12 +511,14 @@ extern "C" int iq_dense_evict(const iq_dense_pages *pages, int dtype, const int3
     IQ_CHECK_ARG(ints == 0 || (workspace && workspace_ints >= ints), "iq_dense_evict: workspace too small");
     IQ_CHECK_ARG(n_seq * pool.H <= 65535, "iq_dense_evict: too many sequences");
     if (n_seq == 0) return IQ_OK;
+    const auto away = [&](const int32_t *p) { return new_lengths + n_seq <= p || p + n_seq <= new_lengths; };
+    // in the place of another sequence's length a new one would be read as its old one
+    IQ_CHECK_ARG(new_lengths == lengths || away(lengths), "iq_dense_evict: new and old lengths overlap in part");
     const int64_t over = max_tokens > budget ? max_tokens - budget : 0, most = over < budget ? over : budget;
     EvictArgs a{pool, lengths, seen, max_tokens, budget, sink, recent, most, new_lengths, workspace};
     const dim3 rows((unsigned)pool.H, (unsigned)n_seq), block(SEL_NT);
     const hipStream_t st = (hipStream_t)stream;
     if (most <= FEW) {
-        const auto away = [&](const int32_t *p) { return new_lengths + n_seq <= p || p + n_seq <= new_lengths; };
         const bool apart = away(lengths) && away(seen);
         if (!apart) a.new_lengths = nullptr;
         hipLaunchKernelGGL(evict_select_kernel<true>, rows, block, 0, st, a);

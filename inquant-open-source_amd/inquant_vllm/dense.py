@@ -299,6 +299,8 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
         output = torch.empty_like(lengths)
     elif output.shape != (n,) or output.dtype is not _I32 or not output.is_contiguous():
         raise ValueError("output must be a contiguous int32 [sequences] tensor")
+    elif 0 < abs(output.data_ptr() - lengths.data_ptr()) < 4 * n:
+        raise ValueError("output must be lengths itself or not overlap them")
     if n == 0:
         return output
     # few moves are listed on the chip

@@ -159,3 +159,30 @@ def test_decode_refuses_outputs_whose_rows_overlap(calls, monkeypatch):
     call(640, 256, 1)                                        # a sequence's rows between those of the next
     call(5, 128, 1, n=1)
     assert len(ran) == 7
+
+
+def test_eviction_refuses_lengths_that_overlap_the_new_ones(calls):
+    """In the place of the old ones or apart: a sequence's new length must not be another's old one."""
+    import ctypes
+    from inquant import _native as nat
+    from inquant_vllm import evict_rows
+    pages, table = DensePages.allocate(4, 16, 2, device="cpu"), torch.zeros((4, 2), dtype=I32)
+    held, seen = torch.full((9,), 20, dtype=I32), torch.full((9,), 30, dtype=I32)
+    for shift in (1, 3):
+        for a, b in ((held[:4], held[shift:shift + 4]), (held[shift:shift + 4], held[:4])):
+            with pytest.raises(ValueError, match="overlap"):
+                evict_rows(pages, table, a, seen[:4], 32, 8, output=b)
+    assert calls == []
+    for out in (held[:4], held[4:8], seen[:4], seen[1:5], None):
+        evict_rows(pages, table, held[:4], seen[:4], 32, 8, output=out)
+    strided = held[:8:2]                                     # copied before the call
+    evict_rows(pages, table, strided, seen[:4], 32, 8, output=held[1:5])
+    assert len(calls) == 6
+    # and the library
+    fake = 1 << 20
+    desc = nat.DensePagesDesc(fake, fake, fake, fake, 4096, 2048, 128, 4096, 2048, 128, 4, 2, 16)
+    for new in (fake + 4, fake - 12):
+        for most in (32, 640):
+            assert nat.lib().iq_dense_evict(ctypes.byref(desc), nat.IQ_BF16, fake, 40, 40, fake, fake, 4, most, 300, 0,
+                                            0, new, fake, 1 << 20, None) == -1
+            assert b"overlap" in nat.lib().iq_last_error()
