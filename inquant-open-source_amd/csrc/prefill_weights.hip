@@ -491,7 +491,8 @@ __global__ __launch_bounds__(LR * LG) void window_lse(WeightArgs a, float *lse)
         const int g = (int)head_of(row, 1.0f / (float)win.n);
         float *to = a.lse_sh ? lse + (int64_t)(h * a.G + g) * a.lse_sh + a.cu[seq] + win.lo + row - g * win.n
                              : lse + ((int64_t)seq * a.H + h) * a.G * a.window + row;
-        *to = (mine[0] == NEG_INF ? 0.0f : mine[0] + __builtin_amdgcn_logf(mine[1])) * LN2;
+        // as the attention's: a maximum of -inf leaves -inf, or NaN if one logit was
+        *to = (mine[0] + __builtin_amdgcn_logf(mine[1])) * LN2;
     }
 }
 

@@ -119,3 +119,30 @@ def test_a_window_in_slices_of_bounded_scratch(lengths, heads, window, dtype):
     prefill_attention(q, k, v, cu, longest, SCALE, lse=lse)
     _close(prefill_weights(q, k, cu, longest, SCALE, window=window, lse=lse), total, slack, window * hq // h)
     assert torch.equal(prefill_weights(q, k, cu, longest, SCALE, window=window), got)
+
+
+@pytest.mark.parametrize("nan_key", [None, 0, 40, 299])
+@pytest.mark.parametrize("window", [1, 20])
+def test_a_window_over_logits_of_minus_infinity(nan_key, window):
+    """A query whose logits are all -inf or NaN has no softmax: its own lse says so, as the attention's does."""
+    from inquant_vllm import prefill_attention, prefill_weights
+    n, scale = 300, 0.5
+    print(f"window of -inf {nan_key} {window}", flush=True)
+    gen = generator(20)
+    q, k = (rows(gen, n, 2, 128, dtype=torch.bfloat16) for _ in range(2))
+    q[:, 0] = 0
+    q[:, 0, 5] = 1.0                                         # head 0 reads channel 5 only
+    k[:, 0, 5] = float("-inf")
+    if nan_key is not None:
+        k[nan_key, 0, 5] = float("nan")
+    cu, lse = offsets([n]), torch.empty((2, n), device="cuda")
+    got = prefill_weights(q, k, cu, n, scale, window=window)
+    at = torch.arange(n, device="cuda")
+    logits = torch.where(at <= at[n - window:, None], k[:, 0, 5].double() * scale, float("-inf"))
+    p = (logits - logits.logsumexp(-1, keepdim=True)).exp()
+    p = torch.where(at <= at[n - window:, None], p, 0.0)     # an unseen key weighs nothing
+    assert torch.equal(got[0].isnan(), p.sum(0).isnan()) and got[0].isnan().all()
+    assert not got[1].isnan().any()
+    prefill_attention(q, k, k, cu, n, scale, lse=lse)
+    with_lse = prefill_weights(q, k, cu, n, scale, window=window, lse=lse)
+    assert torch.equal(with_lse.isnan(), got.isnan())
