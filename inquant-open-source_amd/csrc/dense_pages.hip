@@ -18,8 +18,9 @@ namespace {
 // Rows of sequence `seq` that an entry point considers.
 __device__ __forceinline__ uint32_t dense_length(const int32_t *cu, int seq, uint32_t max_len)
 {
-    const int64_t have = (int64_t)cu[seq + 1] - cu[seq];
-    return have <= 0 ? 0 : have < max_len ? (uint32_t)have : max_len;
+    const int32_t have = cu[seq + 1] - cu[seq];
+    const uint32_t len = have > 0 ? (uint32_t)have : 0;
+    return len < max_len ? len : max_len;
 }
 
 struct WriteArgs {
