@@ -197,6 +197,13 @@ def _apart(n, m, a, b):
     return all(y - x >= 128 for x, y in zip(at, at[1:]))
 
 
+def _meet(x, y):
+    """Whether two float32 tensors of rows of unit stride may share memory."""
+    x0, y0 = x.data_ptr(), y.data_ptr()
+    return x0 < y0 + 4 * ((y.shape[0] - 1) * y.stride(0) + y.shape[1]) \
+        and y0 < x0 + 4 * ((x.shape[0] - 1) * x.stride(0) + x.shape[1])
+
+
 def _budget(budget, sink, recent):
     if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
         raise ValueError("sink and recent rows must fit a budget of at least one row")
@@ -412,6 +419,8 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
         return output
     if lse is not None and lse.stride(0) < 1:
         lse = lse.contiguous()               # one row for every head
+    if lse is not None and _meet(lse, output):
+        lse = lse.clone()                    # read while weights are written
     window = 0 if window is None else min(int(window), max_seqlen)
     if lse is not None and window == max_seqlen:
         window = 0                           # every query

@@ -186,3 +186,20 @@ def test_eviction_refuses_lengths_that_overlap_the_new_ones(calls):
             assert nat.lib().iq_dense_evict(ctypes.byref(desc), nat.IQ_BF16, fake, 40, 40, fake, fake, 4, most, 300, 0,
                                             0, new, fake, 1 << 20, None) == -1
             assert b"overlap" in nat.lib().iq_last_error()
+
+
+def test_weights_in_the_place_of_the_lse_read_a_copy(calls):
+    """Workgroups write a key's weight while others still read the lse of its memory."""
+    from inquant_vllm import prefill_weights
+    q, k, cu = torch.zeros((20, 4, 128)).half(), torch.zeros((20, 4, 128)).half(), torch.tensor([0, 20], dtype=I32)
+    memory = torch.zeros(400)
+
+    def lse_address(lse, **more):
+        prefill_weights(q, k, cu, 20, 0.1, lse=lse, **more)
+        return calls[-1][1][15]
+    lse = memory[:80].view(4, 20)
+    for out in (lse, memory[40:120].view(4, 20), memory[60:260].view(4, 50)[:, :20], memory[79:159].view(4, 20)):
+        assert not memory.data_ptr() <= lse_address(lse, output=out) < memory.data_ptr() + 1600
+    apart = memory[80:160].view(4, 20)
+    assert lse_address(lse, output=apart) == lse.data_ptr() == lse_address(lse)
+    assert lse_address(apart, output=lse, window=3) == apart.data_ptr()

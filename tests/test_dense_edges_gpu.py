@@ -146,3 +146,18 @@ def test_a_window_over_logits_of_minus_infinity(nan_key, window):
     prefill_attention(q, k, k, cu, n, scale, lse=lse)
     with_lse = prefill_weights(q, k, cu, n, scale, window=window, lse=lse)
     assert torch.equal(with_lse.isnan(), got.isnan())
+
+
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 2)], ids=str)
+def test_weights_in_the_place_of_the_lse(heads, window):
+    from inquant_vllm import prefill_attention, prefill_weights
+    hq, h = heads
+    gen, n = generator(30), 700
+    q, k = rows(gen, n, hq, 128, dtype=torch.bfloat16), rows(gen, n, h, 128, dtype=torch.bfloat16)
+    lse, cu = torch.empty((hq, n), device="cuda"), offsets([n])
+    prefill_attention(q, k, k, cu, n, SCALE, lse=lse)
+    want = prefill_weights(q, k, cu, n, SCALE, lse=lse, window=window)
+    rest = lse[h:].clone()
+    got = prefill_weights(q, k, cu, n, SCALE, lse=lse, window=window, output=lse[:h])
+    assert got.data_ptr() == lse.data_ptr() and torch.equal(got, want) and torch.equal(lse[h:], rest)
