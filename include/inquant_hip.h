@@ -570,7 +570,8 @@ int iq_dense_evict_from(const iq_dense_evict_args *args);
  * 16-byte aligned rows), Hq a multiple of heads with at most 16 query heads
  * per KV head; out [n_seq, Hq, 128] of out_dtype (unit channel stride).  fp32
  * logits, softmax and accumulation; softmax weights rounded to the pages'
- * dtype before P.V.  A sequence without a row to read gives zeros.  With
+ * dtype before P.V.  A sequence without a row to read, or whose logits are all
+ * -inf, gives zeros.  With
  * accumulate != 0 each row's weights, summed over the query heads of its KV
  * head, are added to pages->weights (in an order that is only not fixed for a
  * page that two sequences share).  workspace: f32, iq_dense_workspace_floats

@@ -12,7 +12,8 @@
 // 32 x 64 half tile has 16 products of 32 cycles and, per lane, 32 exponentials
 // of 8 and 64 fused multiply-adds and adds of 4, which overlap in part (311 ns a
 // half and SIMD in a loop of nothing else, the products alone 227).  8192 causal
-// queries, 28 heads over 4: 238 us, 1.01 PFLOP/s (32768: 1.17).
+// queries, 28 heads over 4, with the heads' sums: 238-241 us, 1.0 PFLOP/s (32768:
+// 3.38 ms, 1.14).
 #include <type_traits>
 
 #include "decode_common.h"
@@ -526,10 +527,10 @@ constexpr int64_t ML_MOST = 1 << 26;         // floats
 // prompt ends first, by the 64-query tiles of all workgroups over the 512 places,
 // those of the longest workgroup, and some of its tail; a workgroup's start counts
 // as four tiles.  The starts weigh against short ranges, idle places against long
-// ones (28 heads over 4, 8192 queries: 4096 a workgroup; 4096 queries: 1024, 84 us
-// against 92 with the tiles in order and no estimate; 1000 queries: 512, 23 us, and
-// 26 with 256; 32768 queries: all of them, 3.29 ms at 1.17 PFLOP/s, and 3.35 with
-// 8192, which also leave four times the sums to add).
+// ones (28 heads over 4, 8192 queries: 4096 a workgroup, 241 us, and 255 with all of
+// them; 4096 queries: 1024, 84 us against 92 with the tiles in order and no
+// estimate; 1000 queries: 512, 23 us, and 26 with 256; 32768 queries: 16384, 3.38 ms,
+// 3.41 with 8192 and 3.43 with all of them.  From 64K on the sizes are within 2%).
 int64_t chunk_of(int64_t Hq, int64_t n_seq, int64_t max_seqlen)
 {
     int64_t best = 512;
@@ -617,7 +618,8 @@ extern "C" int iq_prefill_weights(const void *q, const void *k, int dtype, int64
     const int64_t chunk = window ? 1 << 30 : chunk_of(Hq, n_seq, max_seqlen), chunks = (max_seqlen + chunk - 1) / chunk;
     WeightArgs a{(const uint16_t *)q, (const uint16_t *)k, q_st, q_sh, k_st, k_sh, cu_seqlens, (int)n_seq,
                  (int)max_seqlen, (int)H, (int)Hq, (int)G, (int)window, (int)chunk, (int)chunks,
-                 scale * LOG2E, lse, lse_sh, (f32x2 *)workspace, s.by_seq ? (int)((max_seqlen + KW - 1) / KW) : 0, 0, 0, out, out_sh};
+                 scale * LOG2E, lse, lse_sh, (f32x2 *)workspace, s.by_seq ? (int)((max_seqlen + KW - 1) / KW) : 0, 0, 0,
+                 out, out_sh};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
     const int64_t m = chunk / KG, units = window ? tiles : m * chunks * (chunks - 1) / 2 + m * chunks;

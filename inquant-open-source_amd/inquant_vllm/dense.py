@@ -221,7 +221,8 @@ def write_rows(key, value, cu_seqlens, max_seqlen, pages, block_tables, start=No
     have weights, the row's is weights[h, cu_seqlens[i] + t] (``weights`` f32
     [kv_heads, tokens], None: 0) and its position positions[i] + t
     (``positions`` int32 [sequences], None: ``start``).  Rows that a block table
-    [sequences, pages per sequence] does not reach are left out."""
+    [sequences, pages per sequence] does not reach are left out.  key and value
+    must not lie in the rows that are written."""
     heads = pages.heads
     shape, ks = _token_rows(key, "key", heads)
     vshape, vs = _token_rows(value, "value", heads)
@@ -287,7 +288,8 @@ def evict_rows(pages, block_tables, lengths, seen, max_tokens, budget, *, sink=0
     ties to the lowest cache row, NaN last.  The evicted cache rows below the
     budget take, in order, the kept rows from the budget on, so only those
     move; every other row stays as it is.  Returns the new lengths
-    min(lengths, budget), int32 [sequences] (``output`` may be ``lengths`` or ``seen``).
+    min(lengths, budget), int32 [sequences] (``output`` may be ``lengths`` or ``seen``, and overlap ``lengths`` no
+    other way).
     No page may belong to two of the sequences."""
     budget, sink, recent, max_tokens = int(budget), int(sink), int(recent), int(max_tokens)
     _budget(budget, sink, recent)
@@ -331,7 +333,9 @@ def dense_decode(query, pages, block_tables, lengths, max_tokens, scale, workspa
     (or fills) output [sequences, Hq, 128] of the query dtype or float32.
     ``accumulate=True`` adds to each row's weight the softmax weights that the
     query heads of its KV head gave it (for a page that two sequences share,
-    in an order that is not fixed)."""
+    in an order that is not fixed); past 512 rows that takes 4 bytes of the
+    workspace per sequence, query head and token of max_tokens.  The workspace
+    must live as long as a graph that captured the call."""
     shape, hkv, max_tokens = query.shape, pages.heads, int(max_tokens)
     if len(shape) != 3 or shape[2] != 128 or query.dtype is not pages._dtype:
         raise ValueError("Expected a query [sequences, heads, 128] of the pages' dtype")
@@ -386,10 +390,10 @@ def prefill_weights(query, key, cu_seqlens, max_seqlen, scale, *, lse=None, wind
     ``lse`` [Hq, tokens] ``prefill_attention(..., lse=...)`` wrote, or with
     ``window=w`` over the last w queries of each sequence (lse optional; w at
     most 4096, or all with the lse).
-    Scratch of a call: with the lse and no window 4 bytes per token, query head
-    and range of queries (one up to 16384, more for a long prompt); for a window's
-    own lse up to 256 MiB (or 512 bytes per query head and 64 keys, if that is
-    more) and 4 bytes per query head and window row.
+    Scratch of a call: without a window 4 bytes per token, query head and range of
+    queries (1 to 16 of them, by the sizes); for a window's own lse up to 256 MiB
+    (or 512 bytes per query head and 64 keys, if that is more) and 4 bytes per
+    query head and window row.
     A sequence longer than max_seqlen counts as its first max_seqlen tokens.
     Tokens of no sequence, and those past max_seqlen, are not written."""
     (tokens, hq, _), qs = _token_rows(query, "query")

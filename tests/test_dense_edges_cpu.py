@@ -203,3 +203,10 @@ def test_weights_in_the_place_of_the_lse_read_a_copy(calls):
     apart = memory[80:160].view(4, 20)
     assert lse_address(lse, output=apart) == lse.data_ptr() == lse_address(lse)
     assert lse_address(apart, output=lse, window=3) == apart.data_ptr()
+
+
+@pytest.mark.parametrize("tokens,ranges", [(1000, 2), (4096, 4), (8192, 2), (16384, 2), (32768, 2), (131072, 2)])
+def test_ranges_of_a_prompts_queries(tokens, ranges):
+    """The split that the kernel's comment gives times for (28 heads): one sum per range, head and token."""
+    from inquant import _native as nat
+    assert nat.lib().iq_prefill_weights_floats(28, 1, tokens, tokens, 0, 1) == ranges * 28 * tokens
