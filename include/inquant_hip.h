@@ -603,6 +603,142 @@ typedef struct iq_dense_decode_args {
 int iq_dense_decode_from(const iq_dense_decode_args *args);
 
 /*
+ * ---------------------------------------------------------------- 4-bit pages
+ * A pool of rows at 4 bits: [pages, heads] parts of block_tokens * 144 bytes
+ * (byte strides s_page and s_head, multiples of 16; 16-byte aligned),
+ * block_tokens B in {16, 32, 64, 128, 256}.  A part holds, of a head's rows of
+ * 128 channels,
+ *   key codes [B][64 bytes], two channels a byte, the lower one in the low bits;
+ *   value codes, u16 [B / 4][channel / 8][row / 2 % 2][channel / 4 % 2][row % 2]
+ *   of four channels each, the lowest in the low bits;
+ *   key words u16 [B][4], one per group of 32 channels;
+ *   value words u16 [B / 4][4 groups][row % 4].
+ * A word is the f16 pattern of a step s whose five low bits are replaced by a
+ * zero point z (0 .. 15); code n stands for (n - z) s, which is exact in f16.
+ * Block tables as for exact pages.  No counterpart in the reference.
+ */
+typedef struct iq_int4_pages {
+    uint64_t pool;
+    int64_t s_page, s_head;
+    int64_t pages, heads, block_tokens;
+} iq_int4_pages;
+
+/*
+ * New rows into exact pages (dense, of `dtype`) or 4-bit pages (int4; the other
+ * one NULL), with the position rotation on the way.  q [tokens, Hq, 128] (NULL:
+ * none), k / v [tokens, heads, 128] of `dtype` (bf16 or f16; element strides,
+ * 16-byte aligned rows); sequences [cu_seqlens[i], cu_seqlens[i + 1]), rows from
+ * max_seqlen on left out.  Row t of sequence i goes to cache row start[i] + t
+ * (start NULL: 0) and stands at position p = positions[i] + t (NULL: start[i] +
+ * t).  rotation f32 [angles, rotary] (NULL: none, rotary 0; rotary a multiple
+ * of 16 up to 128): cos and then sin of the angles of position p; pairs of
+ * channels j and j + rotary / 2, or 2 j and 2 j + 1 if `interleaved`, of q and k
+ * turn by angle j: a cos - b sin, b cos + a sin in f32, every product and sum
+ * rounded.  A position past the table gives NaN.  factors f32 [heads, 128]
+ * (NULL: none) then multiply q (those of its KV head) and divide k.  The rotated
+ * q go to out [tokens, Hq, 128] of `dtype`, which may be q itself.  Exact pages
+ * with weights get weight 0 and position p beside a row.  4-bit pages: per group
+ * of 32 channels, over its values and 0, s = range / 15 within 2^-14 .. 2048,
+ * rounded up to six significant bits, z = rint(-lowest / s) and n = rint(x / s) +
+ * z, both within 0 .. 15; a group with an infinity or NaN is NaN.
+ */
+int iq_append_rows(const void *q, const void *k, const void *v, int dtype, int64_t q_st, int64_t q_sh, int64_t k_st,
+                   int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t Hq, const int32_t *cu_seqlens, int64_t n_seq,
+                   int64_t max_seqlen, const int32_t *start, const int32_t *positions, const float *rotation,
+                   int64_t angles, int64_t rotary, int interleaved, const float *factors, const iq_dense_pages *dense,
+                   const iq_int4_pages *int4, const int32_t *tables, int64_t bt_stride, int64_t bt_cols, void *out,
+                   int64_t o_st, int64_t o_sh, void *stream);
+
+typedef struct iq_append_rows_args {
+    uint64_t q, k, v;
+    int64_t dtype, q_st, q_sh, k_st, k_sh, v_st, v_sh, Hq;
+    uint64_t cu_seqlens;
+    int64_t n_seq, max_seqlen;
+    uint64_t start, positions, rotation;
+    int64_t angles, rotary, interleaved;
+    uint64_t factors, dense, int4, tables;
+    int64_t bt_stride, bt_cols;
+    uint64_t out;
+    int64_t o_st, o_sh;
+    uint64_t stream;
+} iq_append_rows_args;
+
+int iq_append_rows_from(const iq_append_rows_args *args);
+
+/*
+ * Rows of pages as token-major k / v [tokens, heads, 128] (element strides,
+ * 16-byte aligned rows) of `dtype`: that of exact pages, or bf16, f16 or f32
+ * (rounded once) for 4-bit pages.  Token t of sequence i takes cache row
+ * start[i] + t (start NULL: 0); rows from max_seqlen on, and those of no page
+ * of the pool, are not written.
+ */
+int iq_read_rows(const iq_dense_pages *dense, const iq_int4_pages *int4, int dtype, const int32_t *tables,
+                 int64_t bt_stride, int64_t bt_cols, const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen,
+                 const int32_t *start, void *k, int64_t k_st, int64_t k_sh, void *v, int64_t v_st, int64_t v_sh,
+                 void *stream);
+
+typedef struct iq_read_rows_args {
+    uint64_t dense, int4;
+    int64_t dtype;
+    uint64_t tables;
+    int64_t bt_stride, bt_cols;
+    uint64_t cu_seqlens;
+    int64_t n_seq, max_seqlen;
+    uint64_t start, k;
+    int64_t k_st, k_sh;
+    uint64_t v;
+    int64_t v_st, v_sh;
+    uint64_t stream;
+} iq_read_rows_args;
+
+int iq_read_rows_from(const iq_read_rows_args *args);
+
+/*
+ * Attention of the last tokens of each sequence over its 4-bit pages: q
+ * [tokens, Hq, 128] of bf16 or f16 (element strides, 16-byte aligned rows), Hq a
+ * multiple of heads with at most 16 query heads per KV head.  Sequence i holds
+ * lengths[i] cache rows (at most max_tokens) and asks for the m = cu_seqlens[i +
+ * 1] - cu_seqlens[i] tokens from cu_seqlens[i] on (at most max_seqlen; the rest
+ * is not written), the last m of its rows: token t sees the cache rows up to
+ * lengths[i] - m + t.  cu_seqlens NULL: token i is the one of sequence i
+ * (max_seqlen 1).  out [tokens, Hq, 128] of out_dtype (unit channel stride).
+ * fp32 logits, softmax and accumulation; a query is scaled by a power of two
+ * and taken as f16, softmax weights are rounded to f16 before P.V, the rows are
+ * exact.  A token that sees no row, or whose logits are all -inf, gives zeros.
+ * Rows past lengths[i], of pages outside the pool or of no page count as not
+ * there.  `tokens` bounds the query tokens (a hint for how the work is split).
+ * workspace: f32, iq_int4_workspace_floats elements, 16-byte aligned, used by
+ * one call at a time.
+ */
+int64_t iq_int4_workspace_floats(int64_t Hq, int64_t H, int64_t n_seq, int64_t tokens, int64_t max_seqlen,
+                                 int64_t max_tokens);
+
+int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t q_sh, int64_t Hq, const int32_t *cu_seqlens,
+                      int64_t n_seq, int64_t tokens, int64_t max_seqlen, const iq_int4_pages *pages,
+                      const int32_t *tables, int64_t bt_stride, int64_t bt_cols, const int32_t *lengths,
+                      int64_t max_tokens, float scale, float *workspace, int64_t workspace_floats, void *out,
+                      int64_t o_st, int64_t o_sh, int out_dtype, void *stream);
+
+typedef struct iq_int4_attention_args {
+    uint64_t q;
+    int64_t dtype, q_st, q_sh, Hq;
+    uint64_t cu_seqlens;
+    int64_t n_seq, tokens, max_seqlen;
+    uint64_t pages, tables;
+    int64_t bt_stride, bt_cols;
+    uint64_t lengths;
+    int64_t max_tokens;
+    double scale;
+    uint64_t workspace;
+    int64_t workspace_floats;
+    uint64_t out;
+    int64_t o_st, o_sh, out_dtype;
+    uint64_t stream;
+} iq_int4_attention_args;
+
+int iq_int4_attention_from(const iq_int4_attention_args *args);
+
+/*
  * Dense tail append of a cache layer.  buf holds [2 (keys, values), H,
  * capacity, D] elements of elem_bytes (element strides buf_kv, buf_h,
  * buf_t); k / v hold n_new (<= 64) rows per head (element strides: head,

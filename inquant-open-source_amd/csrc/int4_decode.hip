@@ -1,0 +1,362 @@
+// Attention of few tokens over 4-bit pages (gfx950), split over the rows and
+// joined.
+//
+// For the query tokens t and heads g that share a KV head,
+//   o_tg = sum_r p_r v_r,  p_r = exp(c q_tg.k_r) / sum,  r <= sees(t).
+// Each workgroup takes one (KV head, 16 NQ of its (token, head) columns,
+// partition of the rows, sequence) with a running maximum and sum per column.
+// Codes become f16 operands in registers, exactly: S^T = K Q^T takes 16 bytes of
+// a key row per lane (32 channels of one group), O^T = V^T P^T 16 bytes of value
+// codes (eight channels of four rows), whose column layouts agree, so neither
+// the rows nor the weights pass through LDS.
+#include "int4_attn.h"
+
+namespace {
+
+constexpr int D = 128;
+constexpr int WT = 64;                       // rows per wavefront and step
+constexpr int STEP = 4 * WT;                 // rows per workgroup of four wavefronts and step
+
+// The codes and words of a wavefront's 64 rows, as four tiles of 16.
+struct Rows {
+    u32x4 k[4], v[4];
+    u32x2 vw[4];
+    uint32_t kw[4];
+    uint32_t gone;                           // tiles of no page, which read page 0 (uniform)
+};
+
+template <int NQ, int NW>
+struct DecodeSmem {
+    float o[NW][16][D + 4];
+    float m[NQ][NW][16], l[NQ][NW][16];
+};
+
+template <bool F16, int NQ, int NW, bool DIRECT>
+__global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
+{
+    __shared__ DecodeSmem<NQ, NW> sm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4;
+    const int H = a.pool.H, h = blockIdx.x % H, col0 = (int)(blockIdx.x / H) * (16 * NQ);
+    const int part = blockIdx.y, seq = blockIdx.z;
+    const Int4Seq s = int4_seq(a, seq);
+    const int cols = int4_asked(a, s) * a.G;
+    if (col0 >= cols) return;                // uniform
+    const Int4Pool &p = a.pool;
+    const int32_t *table = p.tables + seq * p.bt_stride;
+    const int colN = col0 + 16 * NQ < cols ? col0 + 16 * NQ : cols;
+    const int sees0 = s.sees(col0 / a.G), sees1 = s.sees((colN - 1) / a.G);     // the first and last column's
+    const int t0 = part * a.span;
+    const int end = t0 + a.span < sees1 + 1 ? t0 + a.span : sees1 + 1;
+    if (!DIRECT && t0 >= end) return;        // uniform; the join does not read this partition
+    // B operand: column c16, channels 32 g4 + 8 d .. + 7; its last row and factor
+    u32x4 qb[NQ][4];
+    int sees[NQ];
+    float scale[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int col = col0 + 16 * n + c16 < colN ? col0 + 16 * n + c16 : colN - 1;
+        const int t = col / a.G, g = col - t * a.G;
+        sees[n] = s.sees(t);
+        const uint16_t *qp = a.q + (int64_t)(s.t0 + t) * a.q_st + (int64_t)(h * a.G + g) * a.q_sh + 32 * g4;
+        float x[4][8], most = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            query8<F16>(ld16(qp + 8 * d), x[d]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[d][i]));
+        }
+        const int shift = query_shift(xmax16(most));
+        const float f = __builtin_ldexpf(1.0f, shift);
+        scale[n] = __builtin_ldexpf(a.c_log2, -shift);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qb[n][d][i] = pack2<true>(x[d][i] * f, x[d][i + 4] * f);
+    }
+    float m_run[NQ], l_run[NQ], poison[NQ];  // of column c16; l_run: this lane's rows; poison: NaN or 0
+    f32x4 acc[NQ][8];                        // O^T rows 4 g4 + i of product j: channels 8 (4 g4 + i) + j, column c16
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        m_run[n] = NEG_INF;
+        l_run[n] = poison[n] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[n][j] = f32x4{0, 0, 0, 0};
+    }
+    int ids[4];
+    auto look_up = [&](int c0) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int row = c0 + 16 * t < end ? c0 + 16 * t : end - 1;
+            ids[t] = table[row >> p.shift];
+        }
+    };
+    const uint32_t kw0 = i4_key_words(p.B), v0 = i4_value_codes(p.B), vw0 = i4_value_words(p.B);
+    auto load = [&](Rows &r, int c0) {
+        r.gone = 0;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int want = c0 + 16 * t;
+            const bool ok = want < end && ids[t] >= 0 && ids[t] < p.pages;
+            if (!ok) r.gone |= 1u << t;
+            const uint32_t row = want & (p.B - 1);           // a tile lies in one page, and its rows exist
+            const uint8_t *head = p.base + (int64_t)(ok ? ids[t] : 0) * p.s_page + h * p.s_head;
+            r.k[t] = ldnt_at<u32x4>(head, 64 * row + 16 * (4 * c16 + g4));
+            r.v[t] = ldnt_at<u32x4>(head, v0 + 64 * row + 16 * (16 * g4 + c16));
+            r.kw[t] = ldnt_at<uint16_t>(head, kw0 + 8 * row + 2 * (4 * c16 + g4));
+            r.vw[t] = ldnt_at<u32x2>(head, vw0 + 8 * row + 8 * (4 * g4 + (c16 >> 2)));
+        }
+    };
+    auto take = [&](Rows &r, int c0) {
+        f32x4 sc[NQ][4];                     // S^T rows 16 t + 4 g4 + i (cache rows), column c16
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const I4Scale w = i4_scale(r.kw[t]);
+            u32x4 kf[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kf[d][i] = i4_value(i4_pair(r.k[t][d], i), lower(w.s), lower(w.c));
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                sc[n][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) sc[n][t] = mma32<true>(kf[d], qb[n][d], sc[n][t]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) sc[n][t] *= scale[n];
+        if (r.gone || c0 + WT - 1 > sees0) {                 // uniform: rows that some column does not see
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int first = c0 + 16 * t + 4 * g4;
+                const bool gone = r.gone >> t & 1;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (gone || first + i > sees[n]) sc[n][t][i] = NEG_INF;
+                // a weight of 0 does not hide a NaN: rows that no column sees become zeros, and so do
+                // NaN words of the others, which poison the columns that see them
+                uint32_t nan = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t half = 16 * (i & 1);
+                    const bool out = gone || first + i > sees1;
+                    const bool bad = !out && (r.vw[t][i >> 1] >> half & 0x7c00u) == 0x7c00u;
+                    if (out || bad) r.vw[t][i >> 1] &= ~(0xffffu << half);
+                    nan |= bad ? 1u << i : 0;
+                }
+                uint64_t lanes = __builtin_amdgcn_ballot_w64(nan != 0);
+                for (; lanes; lanes &= lanes - 1) {
+                    const int from = __builtin_ctzll(lanes);             // lane (channel block, row quad)
+                    const uint32_t which = (uint32_t)__builtin_amdgcn_readlane((int)nan, from);
+                    const int row = c0 + 16 * t + 4 * (from >> 4) + __builtin_ctz(which);
+                    if (g4 == (from & 15) >> 2)                          // the lanes whose channels are of its group
+#pragma unroll
+                        for (int n = 0; n < NQ; ++n)
+                            if (row <= sees[n]) poison[n] = __builtin_nanf("");
+                }
+            }
+        }
+        u32x4 pb[NQ][2];                     // B operand: rows 16 (2 m) + 4 g4 + i, then 16 (2 m + 1) + 4 g4 + i
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            float cmax = NEG_INF;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, sc[n][t][i]);
+            const float m_new = fmaxf(m_run[n], xmax16(cmax)), m_use = m_new == NEG_INF ? 0.0f : m_new - I4_BIAS;
+            const float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == NEG_INF ? 0.0f : m_new));
+            float lsum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = __builtin_amdgcn_exp2f(sc[n][t][i] - m_use);
+                    lsum += w[i];
+                }
+                pb[n][t >> 1][2 * (t & 1)] = pack2<true>(w[0], w[1]);
+                pb[n][t >> 1][2 * (t & 1) + 1] = pack2<true>(w[2], w[3]);
+            }
+            l_run[n] = fmaf(l_run[n], alpha, lsum);
+            m_run[n] = m_new;
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f))
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[n][j] *= alpha;
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            I4Scale w[4];                    // of row pairs 0, 1 and 2, 3 of either tile
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = i4_scale(r.vw[2 * m + (i >> 1)][i & 1]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                u32x4 vf;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    vf[i] = i4_value(i4_pair(r.v[2 * m + (i >> 1)][2 * (i & 1) + (j >> 2)], j & 3), w[i].s, w[i].c);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) acc[n][j] = mma32<true>(vf, pb[n][m], acc[n][j]);
+            }
+        }
+    };
+    // the next rows travel while these are taken
+    Rows ra, rb;
+    int c0 = t0 + WT * wave;
+    constexpr int NEXT = WT * NW;
+    if (c0 < end) {
+        look_up(c0);
+        load(ra, c0);
+        look_up(c0 + NEXT);
+        for (;;) {
+            load(rb, c0 + NEXT);
+            look_up(c0 + 2 * NEXT);
+            take(ra, c0);
+            c0 += NEXT;
+            if (c0 >= end) break;
+            load(ra, c0 + NEXT);
+            look_up(c0 + 2 * NEXT);
+            take(rb, c0);
+            c0 += NEXT;
+            if (c0 >= end) break;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        l_run[n] = xsum16(l_run[n]);
+        if (n) __syncthreads();              // the columns before have been read
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[n][4 * half + e][i] + poison[n];
+                *(f32x4 *)&sm.o[wave][c16][8 * (4 * g4 + i) + 4 * half] = x;
+            }
+        if (g4 == 0) {
+            sm.m[n][wave][c16] = m_run[n];
+            sm.l[n][wave][c16] = l_run[n];
+        }
+        __syncthreads();
+        const int here = colN - (col0 + 16 * n) < 16 ? colN - (col0 + 16 * n) : 16;
+        for (int i = tid; i < 32 * here; i += 64 * NW) {
+            const int k = i >> 5, c = 4 * (i & 31), col = col0 + 16 * n + k;
+            float M = NEG_INF;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) M = fmaxf(M, sm.m[n][w][k]);
+            const float use = M == NEG_INF ? 0.0f : M;
+            float L = 0.0f;
+            f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sm.m[n][w][k] - use);
+                L = fmaf(f, sm.l[n][w][k], L);
+                const f32x4 x = *(const f32x4 *)&sm.o[w][k][c];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+            }
+            const int t = col / a.G, hq = h * a.G + col - t * a.G;
+            if constexpr (DIRECT) {
+                const int64_t at = (int64_t)(s.t0 + t) * a.o_st + hq * a.o_sh + c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) iq_store_as(a.out, at + e, L == 0.0f ? 0.0f : o[e] / L, a.odt);
+            } else {
+                const int64_t row = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts + part;
+                *(f32x4 *)(a.part.o + row * D + c) = o;
+                if (c == 0) a.part.ml[row] = f32x2{M, L};
+            }
+        }
+    }
+}
+
+struct Split {
+    int64_t span, parts, floats;             // rows per partition, partitions, the whole workspace
+};
+
+Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seqlen, int64_t max_tokens)
+{
+    const int64_t steps = (max_tokens + STEP - 1) / STEP;
+    const int64_t cols = Hq / H * max_seqlen, groups = (cols + 31) / 32;
+    const int64_t target = n < 4 ? 1024 : 4096, per = (n * H * groups * steps + target - 1) / target;
+    Split s;
+    s.span = max_tokens <= 512 ? 512 : STEP * (per < 1 ? 1 : per);
+    s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
+    s.floats = s.parts > 1 ? tokens * Hq * s.parts * (D + 2) : 0;
+    return s;
+}
+
+template <bool F16, int NQ>
+void launch(const Int4Args &a, dim3 grid, hipStream_t stream)
+{
+    if (a.parts > 1) hipLaunchKernelGGL((int4_partials<F16, NQ, 4, false>), grid, dim3(256), 0, stream, a);
+    else if (a.max_tokens > STEP) hipLaunchKernelGGL((int4_partials<F16, NQ, 8, true>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((int4_partials<F16, NQ, 4, true>), grid, dim3(256), 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" int64_t iq_int4_workspace_floats(int64_t Hq, int64_t H, int64_t n_seq, int64_t tokens, int64_t max_seqlen,
+                                            int64_t max_tokens)
+{
+    return split_of(Hq, H, n_seq, tokens, max_seqlen, max_tokens).floats;
+}
+
+extern "C" int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t q_sh, int64_t Hq,
+                                 const int32_t *cu_seqlens, int64_t n_seq, int64_t tokens, int64_t max_seqlen,
+                                 const iq_int4_pages *pages, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
+                                 const int32_t *lengths, int64_t max_tokens, float scale, float *workspace,
+                                 int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, int out_dtype,
+                                 void *stream)
+{
+    Int4Pool pool;
+    if (const int e = int4_pool("iq_int4_attention", pages, tables, bt_stride, bt_cols, n_seq, pool)) return e;
+    IQ_CHECK_ARG(q && lengths && out, "iq_int4_attention: null pointer");
+    IQ_CHECK_ARG(dtype == IQ_BF16 || dtype == IQ_F16, "iq_int4_attention: queries must be bf16 or f16");
+    IQ_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_st | q_sh) % 8 == 0, "iq_int4_attention: query rows must be 16-byte aligned");
+    IQ_CHECK_ARG(Hq >= 1 && Hq % pool.H == 0 && Hq / pool.H <= 16, "iq_int4_attention: heads %lld / %d", (long long)Hq,
+                 pool.H);
+    IQ_CHECK_ARG(out_dtype >= IQ_F32 && out_dtype <= IQ_F16, "iq_int4_attention: bad output dtype");
+    IQ_CHECK_ARG(max_tokens >= 0 && max_tokens <= bt_cols * pool.B && max_tokens <= 0x3fffffff,
+                 "iq_int4_attention: max_tokens past the block tables");
+    IQ_CHECK_ARG(tokens >= 0 && tokens <= 0x3fffffff && max_seqlen >= 0 && max_seqlen <= 0x3fffffff &&
+                     (cu_seqlens || (max_seqlen == 1 && tokens == n_seq)), "iq_int4_attention: bad query tokens");
+    if (n_seq == 0 || tokens == 0 || max_seqlen == 0) return IQ_OK;
+    if (max_seqlen > tokens) max_seqlen = tokens;
+    const Split s = split_of(Hq, pool.H, n_seq, tokens, max_seqlen, max_tokens);
+    IQ_CHECK_ARG(s.floats == 0 || (workspace && workspace_floats >= s.floats), "iq_int4_attention: workspace too small");
+    const int64_t G = Hq / pool.H, cols = G * max_seqlen;
+    const int64_t groups = (cols + 31) / 32;
+    IQ_CHECK_ARG(s.parts <= 65535 && cols <= 0x3fffffff && groups * pool.H <= 0xffffff && Hq * max_seqlen <= 0xffffff,
+                 "iq_int4_attention: too many rows");
+    const Int4Args a{pool, (const uint16_t *)q, q_st, q_sh, cu_seqlens, lengths, (int32_t)tokens, (int32_t)max_seqlen,
+                     (int32_t)max_tokens, (int32_t)s.span, (int32_t)s.parts, (int32_t)G, (int32_t)Hq,
+                     scale * I4_LOG2E, Partials{workspace, (f32x2 *)(workspace + tokens * Hq * s.parts * D)}, out, o_st, o_sh,
+                     out_dtype};
+    const dim3 grid((unsigned)(pool.H * groups), (unsigned)s.parts, (unsigned)n_seq);
+    const hipStream_t st = (hipStream_t)stream;
+    const bool f16 = dtype == IQ_F16;
+    if (cols <= 16) f16 ? launch<true, 1>(a, grid, st) : launch<false, 1>(a, grid, st);
+    else f16 ? launch<true, 2>(a, grid, st) : launch<false, 2>(a, grid, st);
+    if (s.parts > 8)
+        hipLaunchKernelGGL(int4_join<true>, dim3((unsigned)(Hq * max_seqlen), (unsigned)n_seq), dim3(256), 0, st, a);
+    else if (s.parts > 1)
+        hipLaunchKernelGGL(int4_join<false>, dim3((unsigned)((Hq * max_seqlen + 7) / 8), (unsigned)n_seq), dim3(256), 0, st, a);
+    IQ_CHECK_LAUNCH("int4_attention");
+    return IQ_OK;
+}
+
+extern "C" int iq_int4_attention_from(const iq_int4_attention_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_int4_attention: null arguments");
+    return iq_int4_attention((const void *)a->q, (int)a->dtype, a->q_st, a->q_sh, a->Hq, (const int32_t *)a->cu_seqlens,
+                             a->n_seq, a->tokens, a->max_seqlen, (const iq_int4_pages *)a->pages,
+                             (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (const int32_t *)a->lengths,
+                             a->max_tokens, (float)a->scale, (float *)a->workspace, a->workspace_floats, (void *)a->out,
+                             a->o_st, a->o_sh, (int)a->out_dtype, (void *)a->stream);
+}

@@ -59,6 +59,13 @@ class DensePagesDesc(ctypes.Structure):
                                           "block_tokens")]
 
 
+class Int4PagesDesc(ctypes.Structure):
+    """Mirror of iq_int4_pages in include/inquant_hip.h: a pool of 4-bit pages
+    (address, byte strides of page and head, sizes)."""
+    _fields_ = [("pool", ctypes.c_uint64)] + [(name, _i64) for name in ("s_page", "s_head", "pages", "heads",
+                                                                         "block_tokens")]
+
+
 _SIGNATURES = {
     "iq_abi_version": (_int, []),
     "iq_last_error": (ctypes.c_char_p, []),
@@ -110,8 +117,15 @@ _SIGNATURES = {
     "iq_dense_workspace_floats": (_i64, [_i64, _i64, _i64, _i64, _int]),
     "iq_dense_decode": (_int, [_p, _int, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _f32, _int, _p, _i64,
                                _p, _i64, _i64, _int, _p]),
+    "iq_append_rows": (_int, [_p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p,
+                              _i64, _i64, _int, _p, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p]),
+    "iq_read_rows": (_int, [_p, _p, _int, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p]),
+    "iq_int4_workspace_floats": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "iq_int4_attention": (_int, [_p, _int, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _f32,
+                                 _p, _i64, _p, _i64, _i64, _int, _p]),
     **{name + "_from": (_int, [ctypes.c_char_p]) for name in ("iq_prefill_weights", "iq_dense_write", "iq_select_rows",
-                                                              "iq_dense_evict", "iq_dense_decode")},
+                                                              "iq_dense_evict", "iq_dense_decode", "iq_append_rows",
+                                                              "iq_read_rows", "iq_int4_attention")},
     "iq_page_bytes": (_i64, [_i64, _i64]),
     "iq_encode_pages": (_int, [_p, _p, _int, ctypes.POINTER(_i64), ctypes.POINTER(_i64), _i64, _i64, _i64, _p, _i64,
                                _p, _int, _p, _p, _p]),
