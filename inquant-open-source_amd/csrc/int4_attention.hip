@@ -1,0 +1,116 @@
+// Attention over 4-bit pages (gfx950): how a call is split, and the entry points.
+#include <cstdlib>
+#include "int4_few_dev.h"
+#include "int4_many_dev.h"
+
+namespace {
+
+constexpr int64_t MANY_COLS = QT;
+const int64_t MANY = getenv("IQ_MANY") ? atoi(getenv("IQ_MANY")) : 64;
+
+struct Split {
+    bool many;                               // the kernel for many columns
+    int64_t span, parts, floats;             // rows per partition, partitions, the whole workspace
+};
+
+int64_t few_groups(int64_t cols) { return (cols + 31) / 32; }
+
+Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seqlen, int64_t max_tokens)
+{
+    const int64_t cols = Hq / H * max_seqlen;
+    Split s;
+    s.many = cols > MANY;
+    if (s.many) {
+        const int64_t tiles = n * H * ((cols + MANY_COLS - 1) / MANY_COLS), steps = (max_tokens + KT - 1) / KT;
+        const int64_t parts = tiles >= 256 ? 1 : 512 / tiles, most = (steps + 7) / 8;
+        const int64_t want = parts < most ? parts : most;
+        s.span = KT * ((steps + (want < 1 ? 1 : want) - 1) / (want < 1 ? 1 : want));
+        if (s.span < KT) s.span = KT;
+    } else {
+        const int64_t steps = (max_tokens + STEP - 1) / STEP, groups = few_groups(cols);
+        const int64_t target = n < 4 ? 1024 : 4096, per = (n * H * groups * steps + target - 1) / target;
+        s.span = max_tokens <= 512 ? 512 : STEP * (per < 1 ? 1 : per);
+    }
+    s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
+    s.floats = s.parts > 1 ? tokens * Hq * s.parts * (D + 2) : 0;
+    return s;
+}
+
+template <bool F16, int NQ>
+void launch(const Int4Args &a, dim3 grid, hipStream_t stream)
+{
+    if (a.parts > 1) hipLaunchKernelGGL((int4_partials<F16, NQ, 4, false>), grid, dim3(256), 0, stream, a);
+    else if (a.max_tokens > STEP) hipLaunchKernelGGL((int4_partials<F16, NQ, 8, true>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((int4_partials<F16, NQ, 4, true>), grid, dim3(256), 0, stream, a);
+}
+
+template <bool F16>
+void launch_chunk(const Int4Args &a, int64_t cols, int64_t n, hipStream_t stream)
+{
+    const int tiles = (int)((cols + QT - 1) / QT), share = (tiles * a.pool.H + 7) / 8;
+    const dim3 grid((unsigned)(8 * share), (unsigned)a.parts, (unsigned)n);
+    if (a.parts > 1) hipLaunchKernelGGL((int4_chunk<F16, false>), grid, dim3(64 * NW), 0, stream, a, tiles, share);
+    else hipLaunchKernelGGL((int4_chunk<F16, true>), grid, dim3(64 * NW), 0, stream, a, tiles, share);
+}
+
+}  // namespace
+
+extern "C" int64_t iq_int4_workspace_floats(int64_t Hq, int64_t H, int64_t n_seq, int64_t tokens, int64_t max_seqlen,
+                                            int64_t max_tokens)
+{
+    return split_of(Hq, H, n_seq, tokens, max_seqlen, max_tokens).floats;
+}
+
+extern "C" int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t q_sh, int64_t Hq,
+                                 const int32_t *cu_seqlens, int64_t n_seq, int64_t tokens, int64_t max_seqlen,
+                                 const iq_int4_pages *pages, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
+                                 const int32_t *lengths, int64_t max_tokens, float scale, float *workspace,
+                                 int64_t workspace_floats, void *out, int64_t o_st, int64_t o_sh, int out_dtype,
+                                 void *stream)
+{
+    Int4Pool pool;
+    if (const int e = int4_pool("iq_int4_attention", pages, tables, bt_stride, bt_cols, n_seq, pool)) return e;
+    IQ_CHECK_ARG(q && lengths && out, "iq_int4_attention: null pointer");
+    IQ_CHECK_ARG(dtype == IQ_BF16 || dtype == IQ_F16, "iq_int4_attention: queries must be bf16 or f16");
+    IQ_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_st | q_sh) % 8 == 0, "iq_int4_attention: query rows must be 16-byte aligned");
+    IQ_CHECK_ARG(Hq >= 1 && Hq % pool.H == 0 && Hq / pool.H <= 16, "iq_int4_attention: heads %lld / %d", (long long)Hq,
+                 pool.H);
+    IQ_CHECK_ARG(out_dtype >= IQ_F32 && out_dtype <= IQ_F16, "iq_int4_attention: bad output dtype");
+    IQ_CHECK_ARG(max_tokens >= 0 && max_tokens <= bt_cols * pool.B && max_tokens <= 0x3fffffff,
+                 "iq_int4_attention: max_tokens past the block tables");
+    IQ_CHECK_ARG(tokens >= 0 && tokens <= 0x3fffffff && max_seqlen >= 0 && max_seqlen <= 0x3fffffff &&
+                     (cu_seqlens || (max_seqlen == 1 && tokens == n_seq)), "iq_int4_attention: bad query tokens");
+    if (n_seq == 0 || tokens == 0 || max_seqlen == 0) return IQ_OK;
+    if (max_seqlen > tokens) max_seqlen = tokens;
+    const Split s = split_of(Hq, pool.H, n_seq, tokens, max_seqlen, max_tokens);
+    IQ_CHECK_ARG(s.floats == 0 || (workspace && workspace_floats >= s.floats), "iq_int4_attention: workspace too small");
+    const int64_t G = Hq / pool.H, cols = G * max_seqlen, groups = few_groups(cols);
+    IQ_CHECK_ARG(s.parts <= 65535 && cols <= 0x3fffffff && groups * pool.H <= 0xffffff && Hq * max_seqlen <= 0xffffff,
+                 "iq_int4_attention: too many rows");
+    const Int4Args a{pool, (const uint16_t *)q, q_st, q_sh, cu_seqlens, lengths, (int32_t)tokens, (int32_t)max_seqlen,
+                     (int32_t)max_tokens, (int32_t)s.span, (int32_t)s.parts, (int32_t)G, (int32_t)Hq,
+                     scale * I4_LOG2E, Partials{workspace, (f32x2 *)(workspace + tokens * Hq * s.parts * D)}, out, o_st, o_sh,
+                     out_dtype};
+    const dim3 grid((unsigned)(pool.H * groups), (unsigned)s.parts, (unsigned)n_seq);
+    const hipStream_t st = (hipStream_t)stream;
+    const bool f16 = dtype == IQ_F16;
+    if (s.many) f16 ? launch_chunk<true>(a, cols, n_seq, st) : launch_chunk<false>(a, cols, n_seq, st);
+    else if (cols <= 16) f16 ? launch<true, 1>(a, grid, st) : launch<false, 1>(a, grid, st);
+    else f16 ? launch<true, 2>(a, grid, st) : launch<false, 2>(a, grid, st);
+    if (s.parts > 8)
+        hipLaunchKernelGGL(int4_join<true>, dim3((unsigned)(Hq * max_seqlen), (unsigned)n_seq), dim3(256), 0, st, a);
+    else if (s.parts > 1)
+        hipLaunchKernelGGL(int4_join<false>, dim3((unsigned)((Hq * max_seqlen + 7) / 8), (unsigned)n_seq), dim3(256), 0, st, a);
+    IQ_CHECK_LAUNCH("int4_attention");
+    return IQ_OK;
+}
+
+extern "C" int iq_int4_attention_from(const iq_int4_attention_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_int4_attention: null arguments");
+    return iq_int4_attention((const void *)a->q, (int)a->dtype, a->q_st, a->q_sh, a->Hq, (const int32_t *)a->cu_seqlens,
+                             a->n_seq, a->tokens, a->max_seqlen, (const iq_int4_pages *)a->pages,
+                             (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (const int32_t *)a->lengths,
+                             a->max_tokens, (float)a->scale, (float *)a->workspace, a->workspace_floats, (void *)a->out,
+                             a->o_st, a->o_sh, (int)a->out_dtype, (void *)a->stream);
+}

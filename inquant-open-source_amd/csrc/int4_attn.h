@@ -6,6 +6,7 @@
 
 namespace {
 
+constexpr int D = 128;
 constexpr float I4_LOG2E = 1.44269504088896341f;
 // Softmax weights are at most 1; as f16 operands (and in the sums they are
 // divided by) they are 2^14 times that, so that a weight keeps its eleven bits

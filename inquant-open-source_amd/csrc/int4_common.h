@@ -32,11 +32,23 @@ struct Int4Pool {
 
 // Eight nibbles of a dword as four pairs of f16 (16 + nibble): pair i holds
 // nibbles i and i + 4, at bits 6 .. 9 of either half, whose unit is 1 there.
-__device__ __forceinline__ uint32_t i4_pair(uint32_t x, int i)
-{
-    const uint32_t y = i == 0 ? x << 6 : i == 1 ? x << 2 : i == 2 ? x >> 2 : x >> 6;
-    return (y & 0x03c003c0u) | 0x4c004c00u;
-}
+// The masks stand in registers, so that one instruction takes both (as literals
+// they take two: no instruction of three operands holds one).
+struct I4Masks {
+    uint32_t field, unit;
+    __device__ __forceinline__ I4Masks()
+    {
+        field = 0x03c003c0u;
+        unit = 0x4c004c00u;
+        asm("" : "+s"(field));
+        asm("" : "+v"(unit));
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t x, int i) const
+    {
+        const uint32_t y = i == 0 ? x << 6 : i == 1 ? x << 2 : i == 2 ? x >> 2 : x >> 6;
+        return (y & field) | unit;
+    }
+};
 
 __device__ __forceinline__ f16x2 as_f16x2(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
 __device__ __forceinline__ uint32_t as_u32(f16x2 x) { return __builtin_bit_cast(uint32_t, x); }

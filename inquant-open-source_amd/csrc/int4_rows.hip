@@ -314,6 +314,7 @@ __global__ __launch_bounds__(NT) void read_int4_kernel(ReadArgs a)
     const Int4Pool &p = a.int4;
     const int64_t page = i4_page(p, seq, first);
     if (page < 0) return;
+    const I4Masks masks;
     const uint8_t *head = p.base + page * p.s_page + h * p.s_head;
     const uint32_t r0 = (uint32_t)first & (p.B - 1);
     uint32_t kc[4];
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(NT) void read_int4_kernel(ReadArgs a)
         const I4Scale sk = i4_scale(kw[r]);
         uint32_t pair[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pair[i] = i4_value(i4_pair(kc[r], i), lower(sk.s), lower(sk.c));
+        for (int i = 0; i < 4; ++i) pair[i] = i4_value(masks.pair(kc[r], i), lower(sk.s), lower(sk.c));
         u32x4 out;                           // pair i holds channels i and i + 4
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(NT) void read_int4_kernel(ReadArgs a)
         const I4Scale sv = i4_scale(vw[d]);
         uint32_t pair[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pair[i] = i4_value(i4_pair(vc[2 * d + (i >> 2)], i & 3), sv.s, sv.c);
+        for (int i = 0; i < 8; ++i) pair[i] = i4_value(masks.pair(vc[2 * d + (i >> 2)], i & 3), sv.s, sv.c);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int64_t t = first + 2 * d + r - start;
