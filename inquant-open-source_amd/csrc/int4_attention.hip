@@ -6,42 +6,72 @@
 namespace {
 
 constexpr int64_t MANY_COLS = QT;
-const int64_t MANY = getenv("IQ_MANY") ? atoi(getenv("IQ_MANY")) : 64;
+const int64_t WORKERS = getenv("IQ_T") ? atoi(getenv("IQ_T")) : 0;
+constexpr int64_t ONE_MOST = 512;
+const int64_t MANY = getenv("IQ_MANY") ? atoi(getenv("IQ_MANY")) : 256;
 
 struct Split {
     bool many;                               // the kernel for many columns
-    int64_t span, parts, floats;             // rows per partition, partitions, the whole workspace
+    int64_t span, parts;                     // many: rows per partition, partitions
+    int64_t groups, workers, width;          // few: groups of columns, workgroups that share a plane's rows (0: none), columns
+    int64_t floats;                          // the whole workspace
 };
 
-int64_t few_groups(int64_t cols) { return (cols + 31) / 32; }
+constexpr int64_t BATCH = 64;                // sequences of a launch that shares their rows out
 
 Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seqlen, int64_t max_tokens)
 {
     const int64_t cols = Hq / H * max_seqlen;
-    Split s;
+    Split s{};
     s.many = cols > MANY;
     if (s.many) {
         const int64_t tiles = n * H * ((cols + MANY_COLS - 1) / MANY_COLS), steps = (max_tokens + KT - 1) / KT;
-        const int64_t parts = tiles >= 256 ? 1 : 512 / tiles, most = (steps + 7) / 8;
-        const int64_t want = parts < most ? parts : most;
-        s.span = KT * ((steps + (want < 1 ? 1 : want) - 1) / (want < 1 ? 1 : want));
+        const int64_t parts = tiles >= 192 ? 1 : 256 / tiles, most = (steps + 7) / 8;
+        int64_t want = parts < most ? parts : most;
+        if (want < 1) want = 1;
+        s.span = KT * ((steps + want - 1) / want);
         if (s.span < KT) s.span = KT;
+        s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
+        s.floats = s.parts > 1 ? tokens * Hq * s.parts * (D + 2) : 0;
     } else {
-        const int64_t steps = (max_tokens + STEP - 1) / STEP, groups = few_groups(cols);
-        const int64_t target = n < 4 ? 1024 : 4096, per = (n * H * groups * steps + target - 1) / target;
-        s.span = max_tokens <= 512 ? 512 : STEP * (per < 1 ? 1 : per);
+        s.width = cols <= 16 ? 16 : 32;
+        s.groups = (cols + s.width - 1) / s.width;
+        const int64_t planes = H * s.groups, steps = (max_tokens + STEP - 1) / STEP, batch = n < BATCH ? n : BATCH;
+        if (max_tokens > ONE_MOST) {
+            s.workers = ((WORKERS ? WORKERS : batch * planes * steps > 4096 ? 512 : 256) + planes - 1) / planes;
+            if (s.workers > batch * steps) s.workers = batch * steps;
+            s.floats = planes * (s.workers + batch) * s.width * (D + 2);
+        }
     }
-    s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
-    s.floats = s.parts > 1 ? tokens * Hq * s.parts * (D + 2) : 0;
     return s;
 }
 
 template <bool F16, int NQ>
-void launch(const Int4Args &a, dim3 grid, hipStream_t stream)
+void launch_few(Int4Args a, int64_t n, hipStream_t stream)
 {
-    if (a.parts > 1) hipLaunchKernelGGL((int4_partials<F16, NQ, 4, false>), grid, dim3(256), 0, stream, a);
-    else if (a.max_tokens > STEP) hipLaunchKernelGGL((int4_partials<F16, NQ, 8, true>), grid, dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((int4_partials<F16, NQ, 4, true>), grid, dim3(256), 0, stream, a);
+    const unsigned planes = (unsigned)(a.pool.H * a.groups);
+    if (a.workers == 0) {
+        if (a.max_tokens > STEP) hipLaunchKernelGGL((int4_whole<F16, NQ, 8>), dim3(planes, 1, (unsigned)n), dim3(512), 0, stream, a);
+        else hipLaunchKernelGGL((int4_whole<F16, NQ, 4>), dim3(planes, 1, (unsigned)n), dim3(256), 0, stream, a);
+        return;
+    }
+    const int32_t *const lengths = a.lengths, *const cu = a.cu, *const tables = a.pool.tables;
+    const uint16_t *const q = a.q;
+    char *const out = (char *)a.out;
+    const int tokens = a.tokens;
+    for (int64_t s0 = 0; s0 < n; s0 += BATCH) {
+        a.n_seq = (int32_t)(n - s0 < BATCH ? n - s0 : BATCH);
+        a.lengths = lengths + s0;
+        a.pool.tables = tables + s0 * a.pool.bt_stride;
+        if (cu) a.cu = cu + s0;
+        else {                               // token i is sequence i's
+            a.q = q + s0 * a.q_st;
+            a.out = out + s0 * a.o_st * (a.odt == IQ_F32 ? 4 : 2);
+            a.tokens = tokens - (int32_t)s0;
+        }
+        hipLaunchKernelGGL((int4_shared<F16, NQ>), dim3(planes * (unsigned)a.workers), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(int4_join<true>, dim3((unsigned)(a.Hq * a.max_seqlen), (unsigned)a.n_seq), dim3(256), 0, stream, a);
+    }
 }
 
 template <bool F16>
@@ -49,7 +79,11 @@ void launch_chunk(const Int4Args &a, int64_t cols, int64_t n, hipStream_t stream
 {
     const int tiles = (int)((cols + QT - 1) / QT), share = (tiles * a.pool.H + 7) / 8;
     const dim3 grid((unsigned)(8 * share), (unsigned)a.parts, (unsigned)n);
-    if (a.parts > 1) hipLaunchKernelGGL((int4_chunk<F16, false>), grid, dim3(64 * NW), 0, stream, a, tiles, share);
+    if (a.parts > 1) {
+        hipLaunchKernelGGL((int4_chunk<F16, false>), grid, dim3(64 * NW), 0, stream, a, tiles, share);
+        hipLaunchKernelGGL(int4_join<false>, dim3((unsigned)((a.Hq * (int64_t)a.max_seqlen + 7) / 8), (unsigned)n), dim3(256), 0,
+                           stream, a);
+    }
     else hipLaunchKernelGGL((int4_chunk<F16, true>), grid, dim3(64 * NW), 0, stream, a, tiles, share);
 }
 
@@ -84,23 +118,19 @@ extern "C" int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t
     if (max_seqlen > tokens) max_seqlen = tokens;
     const Split s = split_of(Hq, pool.H, n_seq, tokens, max_seqlen, max_tokens);
     IQ_CHECK_ARG(s.floats == 0 || (workspace && workspace_floats >= s.floats), "iq_int4_attention: workspace too small");
-    const int64_t G = Hq / pool.H, cols = G * max_seqlen, groups = few_groups(cols);
-    IQ_CHECK_ARG(s.parts <= 65535 && cols <= 0x3fffffff && groups * pool.H <= 0xffffff && Hq * max_seqlen <= 0xffffff,
-                 "iq_int4_attention: too many rows");
+    const int64_t G = Hq / pool.H, cols = G * max_seqlen;
+    IQ_CHECK_ARG(s.parts <= 65535 && cols <= 0x3fffffff && s.groups * pool.H * (s.workers + 1) <= 0xffffff &&
+                     Hq * max_seqlen <= 0xffffff, "iq_int4_attention: too many rows");
+    const int64_t rows = s.floats / (D + 2);
     const Int4Args a{pool, (const uint16_t *)q, q_st, q_sh, cu_seqlens, lengths, (int32_t)tokens, (int32_t)max_seqlen,
-                     (int32_t)max_tokens, (int32_t)s.span, (int32_t)s.parts, (int32_t)G, (int32_t)Hq,
-                     scale * I4_LOG2E, Partials{workspace, (f32x2 *)(workspace + tokens * Hq * s.parts * D)}, out, o_st, o_sh,
-                     out_dtype};
-    const dim3 grid((unsigned)(pool.H * groups), (unsigned)s.parts, (unsigned)n_seq);
+                     (int32_t)max_tokens, (int32_t)G, (int32_t)Hq, (int32_t)s.span, (int32_t)s.parts, (int32_t)n_seq,
+                     (int32_t)s.groups, (int32_t)s.workers, (int32_t)s.width, scale * I4_LOG2E,
+                     Partials{workspace, (f32x2 *)(workspace + rows * D)}, out, o_st, o_sh, out_dtype};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
     if (s.many) f16 ? launch_chunk<true>(a, cols, n_seq, st) : launch_chunk<false>(a, cols, n_seq, st);
-    else if (cols <= 16) f16 ? launch<true, 1>(a, grid, st) : launch<false, 1>(a, grid, st);
-    else f16 ? launch<true, 2>(a, grid, st) : launch<false, 2>(a, grid, st);
-    if (s.parts > 8)
-        hipLaunchKernelGGL(int4_join<true>, dim3((unsigned)(Hq * max_seqlen), (unsigned)n_seq), dim3(256), 0, st, a);
-    else if (s.parts > 1)
-        hipLaunchKernelGGL(int4_join<false>, dim3((unsigned)((Hq * max_seqlen + 7) / 8), (unsigned)n_seq), dim3(256), 0, st, a);
+    else if (cols <= 16) f16 ? launch_few<true, 1>(a, n_seq, st) : launch_few<false, 1>(a, n_seq, st);
+    else f16 ? launch_few<true, 2>(a, n_seq, st) : launch_few<false, 2>(a, n_seq, st);
     IQ_CHECK_LAUNCH("int4_attention");
     return IQ_OK;
 }

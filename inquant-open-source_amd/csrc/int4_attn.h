@@ -18,9 +18,11 @@ struct Int4Args {
     const uint16_t *q;
     int64_t q_st, q_sh;                      // element strides (token, head)
     const int32_t *cu, *lengths;             // cu null: token i is the one of sequence i
-    int32_t tokens, max_seqlen, max_tokens, span, parts, G, Hq;
+    int32_t tokens, max_seqlen, max_tokens, G, Hq;
+    int32_t span, parts;                     // many columns: rows per partition, partitions
+    int32_t n_seq, groups, workers, width;   // few: see Share
     float c_log2;
-    Partials part;                           // [tokens * Hq, parts] rows
+    Partials part;                           // many: [tokens * Hq, parts] rows; few: [planes, workers + n_seq, width]
     void *out;
     int64_t o_st, o_sh;
     int odt;
@@ -72,25 +74,87 @@ __device__ __forceinline__ int query_shift(float largest)
     return e < 100 ? e : 100;
 }
 
-// Joins the partitions of a token and query head.  TEAM: one workgroup a row,
-// whose eight teams of 32 lanes split the partitions; else a team a row.
-template <bool TEAM>
+// Few columns: the rows of a launch's sequences (at most 64), in steps of 256,
+// one after the other, are shared out evenly over `workers` workgroups for each
+// plane (a KV head and `width` of its columns): every one has the same number of
+// steps, whatever the sequences' lengths (16 sequences of 2K-32K tokens, split
+// alike instead: 46 us in the best of five splits, 57 in the worst).  Lane i holds
+// sequence i.  A workgroup w leaves its part of sequence i at slot w + i of the
+// plane, which no other part has.
+constexpr int STEP = 256;
+
+struct Share {
+    Int4Seq own;                             // this lane's sequence
+    int32_t steps, upto;                     // its steps; with those before it
+    int32_t each, total;                     // of a workgroup; of all (uniform)
+    __device__ __forceinline__ Int4Seq of(int seq) const
+    {
+        return {__builtin_amdgcn_readlane(own.len, seq), __builtin_amdgcn_readlane(own.m, seq),
+                __builtin_amdgcn_readlane(own.t0, seq)};
+    }
+};
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t dpp_i(int32_t v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+
+__device__ __forceinline__ Share int4_share(const Int4Args &a)
+{
+    const int lane = threadIdx.x & 63;
+    Share r;
+    r.own = int4_seq(a, lane < a.n_seq ? lane : a.n_seq - 1);
+    r.steps = lane < a.n_seq && int4_asked(a, r.own) > 0 ? (r.own.len + STEP - 1) / STEP : 0;
+    int32_t v = r.steps;
+    v += dpp_i<0x111, 0xf>(v);               // row_shr:1
+    v += dpp_i<0x112, 0xf>(v);
+    v += dpp_i<0x114, 0xf>(v);
+    v += dpp_i<0x118, 0xf>(v);
+    v += dpp_i<0x142, 0xa>(v);               // row_bcast:15 into rows 1 and 3
+    v += dpp_i<0x143, 0xc>(v);               // row_bcast:31 into rows 2 and 3
+    r.upto = v;
+    r.total = __builtin_amdgcn_readlane(v, 63);
+    r.each = (r.total + a.workers - 1) / a.workers;
+    return r;
+}
+
+// Joins the partitions of a token and query head.  FEW: those of the workgroups
+// that shared its sequence, by one workgroup whose eight teams of 32 lanes split
+// them; else those of `span` rows, by one team.
+template <bool FEW>
 __global__ __launch_bounds__(256) void int4_join(Int4Args a)
 {
-    __shared__ float so[TEAM ? 8 : 1][TEAM ? 128 : 1], sm[8], sl[8];
+    __shared__ float so[FEW ? 8 : 1][FEW ? 128 : 1], sm[8], sl[8];
     const int tid = threadIdx.x, team = tid >> 5, c = 4 * (tid & 31), seq = blockIdx.y;
     const Int4Seq s = int4_seq(a, seq);
-    const uint32_t item = TEAM ? blockIdx.x : blockIdx.x * 8 + team;
+    const uint32_t item = FEW ? blockIdx.x : blockIdx.x * 8 + team;
     const int t = (int)(item / (uint32_t)a.Hq), hq = (int)(item - (uint32_t)t * (uint32_t)a.Hq);
-    if (t >= int4_asked(a, s)) return;       // with TEAM the whole workgroup's
-    const int last = s.sees(t), live = last < 0 ? 0 : last / a.span + 1;
-    const int64_t base = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts;
+    if (t >= int4_asked(a, s)) return;       // with FEW the whole workgroup's
+    const int last = s.sees(t);
+    int first = 0, live;                     // partitions first .. live - 1
+    int64_t base, next;                      // rows of the first of them, from one to the next
+    if constexpr (FEW) {
+        const Share r = int4_share(a);
+        const int steps = __builtin_amdgcn_readlane(r.steps, seq), from = __builtin_amdgcn_readlane(r.upto, seq) - steps;
+        const int h = hq / a.G, col = t * a.G + hq - h * a.G, group = col / a.width;
+        if (steps == 0 || last < 0) live = 0;
+        else {
+            first = from / r.each;
+            live = (from + last / STEP) / r.each + 1;
+            if (first == (from + steps - 1) / r.each) return;            // one workgroup had them all
+        }
+        next = a.width;
+        base = ((int64_t)(h + a.pool.H * group) * (a.workers + a.n_seq) + first + seq) * next + col - group * a.width;
+    } else {
+        live = last < 0 ? 0 : last / a.span + 1;
+        base = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts;
+        next = 1;
+    }
+    live -= first;
     float M = NEG_INF, L = 0.0f;
     f32x4 o = {0, 0, 0, 0};
 #pragma unroll 2
-    for (int p = TEAM ? team : 0; p < live; p += TEAM ? 8 : 1) {
-        const f32x2 ml = a.part.ml[base + p];
-        const f32x4 x = *(const f32x4 *)(a.part.o + (base + p) * 128 + c);
+    for (int p = FEW ? team : 0; p < live; p += FEW ? 8 : 1) {
+        const f32x2 ml = a.part.ml[base + p * next];
+        const f32x4 x = *(const f32x4 *)(a.part.o + (base + p * next) * 128 + c);
         const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
         const float f0 = __builtin_amdgcn_exp2f(M - use), f1 = __builtin_amdgcn_exp2f(ml[0] - use);
         L = L * f0 + ml[1] * f1;
@@ -98,7 +162,7 @@ __global__ __launch_bounds__(256) void int4_join(Int4Args a)
         for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + x[e] * f1;
         M = m;
     }
-    if constexpr (TEAM) {
+    if constexpr (FEW) {
         *(f32x4 *)&so[team][c] = o;
         if (c == 0) {
             sm[team] = M;

@@ -3,8 +3,8 @@
 //
 // For the query tokens t and heads g that share a KV head,
 //   o_tg = sum_r p_r v_r,  p_r = exp(c q_tg.k_r) / sum,  r <= sees(t).
-// Each workgroup takes one (KV head, 16 NQ of its (token, head) columns,
-// partition of the rows, sequence) with a running maximum and sum per column.
+// A workgroup takes one KV head, 16 NQ of its (token, head) columns and a share of
+// the rows, with a running maximum and sum per column.
 // Codes become f16 operands in registers, exactly: S^T = K Q^T takes 16 bytes of
 // a key row per lane (32 channels of one group), O^T = V^T P^T 16 bytes of value
 // codes (eight channels of four rows), whose column layouts agree, so neither
@@ -16,7 +16,6 @@
 namespace {
 
 constexpr int WT = 64;                       // rows per wavefront and step
-constexpr int STEP = 4 * WT;                 // rows per workgroup of four wavefronts and step
 
 // The codes and words of a wavefront's 64 rows, as four tiles of 16.
 struct Rows {
@@ -32,24 +31,37 @@ struct DecodeSmem {
     float m[NQ][NW][16], l[NQ][NW][16];
 };
 
-template <bool F16, int NQ, int NW, bool DIRECT>
-__global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
+// Rows t0 .. of a sequence up to `stop`.  DIRECT: all of its rows, and what this
+// gives are the outputs; else they are a partition's, at row `to` of the partials.
+// ONE: a wavefront has one step at most.
+template <bool F16, int NQ, int NW, bool ONE>
+__device__ __forceinline__ void few_rows(const Int4Args &a, DecodeSmem<NQ, NW> &sm, int h, int col0, int seq, const Int4Seq s,
+                                         int t0, int stop, bool direct, int64_t to)
 {
-    __shared__ DecodeSmem<NQ, NW> sm;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
-    const int H = a.pool.H, h = blockIdx.x % H, col0 = (int)(blockIdx.x / H) * (16 * NQ);
-    const int part = blockIdx.y, seq = blockIdx.z;
-    const Int4Seq s = int4_seq(a, seq);
     const int cols = int4_asked(a, s) * a.G;
     if (col0 >= cols) return;                // uniform
     const Int4Pool &p = a.pool;
     const int32_t *table = p.tables + seq * p.bt_stride;
     const int colN = col0 + 16 * NQ < cols ? col0 + 16 * NQ : cols;
     const int sees0 = s.sees(col0 / a.G), sees1 = s.sees((colN - 1) / a.G);     // the first and last column's
-    const int t0 = part * a.span;
-    const int end = t0 + a.span < sees1 + 1 ? t0 + a.span : sees1 + 1;
-    if (!DIRECT && t0 >= end) return;        // uniform; the join does not read this partition
+    const int end = stop < sees1 + 1 ? stop : sees1 + 1;
+    if (!direct && t0 >= end) return;        // uniform; the join does not read this partition
+    // The pages are looked up first, then the queries are asked for, then the first
+    // rows, so that neither waits for what it does not need.
+    constexpr int NEXT = WT * NW;
+    int c0 = t0 + WT * wave;
+    // lane l: the page of tile l % 4 of the rows that are asked for next, and of those after them
+    int id_lane = 0, id_after = 0;
+    auto look_up = [&](int c0) __attribute__((always_inline)) {
+        const int row = c0 + 16 * (lane & 3);
+        return table[(row < end ? row : end - 1) >> p.shift];
+    };
+    if (c0 < end) {
+        id_lane = look_up(c0);
+        if constexpr (!ONE) id_after = look_up(c0 + NEXT);
+    }
     // B operand: column c16, channels 32 g4 + 8 d .. + 7; its last row and factor
     u32x4 qb[NQ][4];
     int sees[NQ];
@@ -60,16 +72,44 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
         const int t = col / a.G, g = col - t * a.G;
         sees[n] = s.sees(t);
         const uint16_t *qp = a.q + (int64_t)(s.t0 + t) * a.q_st + (int64_t)(h * a.G + g) * a.q_sh + 32 * g4;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) qb[n][d] = ld16(qp + 8 * d);
+    }
+    const uint32_t kw0 = i4_key_words(p.B), v0 = i4_value_codes(p.B), vw0 = i4_value_words(p.B);
+    const uint8_t *base = p.base + h * p.s_head;
+    auto load = [&](Rows &r, int c0) __attribute__((always_inline)) {
+        const uint32_t here = (uint32_t)__builtin_amdgcn_ballot_w64(c0 + 16 * (lane & 3) < end && (uint32_t)id_lane < (uint32_t)p.pages);
+        r.gone = ~here & 15;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int id = here >> t & 1 ? __builtin_amdgcn_readlane(id_lane, t) : 0;
+            const uint32_t row = (c0 + 16 * t) & (p.B - 1);              // a tile lies in one page, and its rows exist
+            const uint8_t *head = base + (int64_t)id * p.s_page;
+            r.k[t] = ldnt_at<u32x4>(head, 64 * row + 16 * (4 * c16 + g4));
+            r.kw[t] = ldnt_at<uint16_t>(head, kw0 + 8 * row + 2 * (4 * c16 + g4));
+            r.v[t] = ldnt_at<u32x4>(head, v0 + 64 * row + 16 * (16 * g4 + c16));
+            r.vw[t] = ldnt_at<u32x2>(head, vw0 + 8 * row + 8 * (4 * g4 + (c16 >> 2)));
+        }
+    };
+    Rows ra, rb;
+    if (c0 < end) load(ra, c0);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
         float x[4][8], most = 0.0f;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            query8<F16>(ld16(qp + 8 * d), x[d]);
+            query8<F16>(qb[n][d], x[d]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[d][i]));
         }
         const int shift = query_shift(xmax16(most));
-        const float f = __builtin_ldexpf(1.0f, shift);
-        scale[n] = __builtin_ldexpf(a.c_log2, -shift);
+        // the maximum is taken before the scale, which is made positive; logits that its size rounds to 0 are 0
+        float f = __builtin_ldexpf(a.c_log2 < 0.0f ? -1.0f : 1.0f, shift);
+        scale[n] = __builtin_ldexpf(fabsf(a.c_log2), -shift);
+        if (scale[n] < 0x1p-110f) {
+            f = 0.0f;
+            scale[n] = 1.0f;
+        }
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -85,31 +125,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
         for (int j = 0; j < 8; ++j) acc[n][j] = f32x4{0, 0, 0, 0};
     }
     const I4Masks masks;
-    int ids[4];
-    auto look_up = [&](int c0) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int row = c0 + 16 * t < end ? c0 + 16 * t : end - 1;
-            ids[t] = table[row >> p.shift];
-        }
-    };
-    const uint32_t kw0 = i4_key_words(p.B), v0 = i4_value_codes(p.B), vw0 = i4_value_words(p.B);
-    auto load = [&](Rows &r, int c0) {
-        r.gone = 0;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int want = c0 + 16 * t;
-            const bool ok = want < end && ids[t] >= 0 && ids[t] < p.pages;
-            if (!ok) r.gone |= 1u << t;
-            const uint32_t row = want & (p.B - 1);           // a tile lies in one page, and its rows exist
-            const uint8_t *head = p.base + (int64_t)(ok ? ids[t] : 0) * p.s_page + h * p.s_head;
-            r.k[t] = ldnt_at<u32x4>(head, 64 * row + 16 * (4 * c16 + g4));
-            r.v[t] = ldnt_at<u32x4>(head, v0 + 64 * row + 16 * (16 * g4 + c16));
-            r.kw[t] = ldnt_at<uint16_t>(head, kw0 + 8 * row + 2 * (4 * c16 + g4));
-            r.vw[t] = ldnt_at<u32x2>(head, vw0 + 8 * row + 8 * (4 * g4 + (c16 >> 2)));
-        }
-    };
-    auto take = [&](Rows &r, int c0) {
+    auto take = [&](Rows &r, int c0) __attribute__((always_inline)) {
         f32x4 sc[NQ][4];                     // S^T rows 16 t + 4 g4 + i (cache rows), column c16
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -126,10 +142,6 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
                 for (int d = 0; d < 4; ++d) sc[n][t] = mma32<true>(kf[d], qb[n][d], sc[n][t]);
             }
         }
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) sc[n][t] *= scale[n];
         if (r.gone || c0 + WT - 1 > sees0) {                 // uniform: rows that some column does not see
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -171,14 +183,15 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, sc[n][t][i]);
-            const float m_new = fmaxf(m_run[n], xmax16(cmax)), m_use = m_new == NEG_INF ? 0.0f : m_new - I4_BIAS;
-            float alpha = __builtin_amdgcn_exp2f(m_run[n] - (m_new == NEG_INF ? 0.0f : m_new));
+            const float m_new = fmaxf(m_run[n], xmax16(cmax) * scale[n]), m_use = m_new == NEG_INF ? 0.0f : m_new;
+            float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_use);
+            const float less = I4_BIAS - m_use;
             float lsum = 0.0f;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 float w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(sc[n][t][i] - m_use);
+                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][t][i], scale[n], less));
 #pragma unroll
                 for (int i = 0; i < 2; ++i) pb[n][t >> 1][2 * (t & 1) + i] = pack2<true>(w[2 * i], w[2 * i + 1]);
                 lsum += (w[0] + w[1]) + (w[2] + w[3]);
@@ -207,22 +220,20 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
             }
         }
     };
-    // the next rows travel while these are taken
-    Rows ra, rb;
-    int c0 = t0 + WT * wave;
-    constexpr int NEXT = WT * NW;
-    if (c0 < end) {
-        look_up(c0);
-        load(ra, c0);
-        look_up(c0 + NEXT);
+    // The next rows travel while these are taken; their pages are looked up before
+    // the rows ahead of them are asked for, whose arrival they need not wait for.
+    if (ONE && c0 < end) take(ra, c0);
+    if (!ONE && c0 < end) {
         for (;;) {
+            id_lane = id_after;
+            id_after = look_up(c0 + 2 * NEXT);
             load(rb, c0 + NEXT);
-            look_up(c0 + 2 * NEXT);
             take(ra, c0);
             c0 += NEXT;
             if (c0 >= end) break;
+            id_lane = id_after;
+            id_after = look_up(c0 + 2 * NEXT);
             load(ra, c0 + NEXT);
-            look_up(c0 + 2 * NEXT);
             take(rb, c0);
             c0 += NEXT;
             if (c0 >= end) break;
@@ -231,7 +242,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         l_run[n] = xsum16(l_run[n]);
-        if (n) __syncthreads();              // the columns before have been read
+        __syncthreads();                     // what was there before has been read
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -264,16 +275,44 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_partials(Int4Args a)
                 for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
             }
             const int t = col / a.G, hq = h * a.G + col - t * a.G;
-            if constexpr (DIRECT) {
+            if (direct) {
                 const int64_t at = (int64_t)(s.t0 + t) * a.o_st + hq * a.o_sh + c;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) iq_store_as(a.out, at + e, L == 0.0f ? 0.0f : o[e] / L, a.odt);
             } else {
-                const int64_t row = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts + part;
+                const int64_t row = to + 16 * n + k;
                 *(f32x4 *)(a.part.o + row * D + c) = o;
                 if (c == 0) a.part.ml[row] = f32x2{M, L};
             }
         }
+    }
+}
+
+// One sequence (blockIdx.z) each.
+template <bool F16, int NQ, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void int4_whole(Int4Args a)
+{
+    __shared__ DecodeSmem<NQ, NW> sm;
+    const int h = blockIdx.x % a.pool.H, group = blockIdx.x / a.pool.H;
+    few_rows<F16, NQ, NW, true>(a, sm, h, group * 16 * NQ, blockIdx.z, int4_seq(a, blockIdx.z), 0, a.max_tokens, true, 0);
+}
+
+// An even share of the sequences' steps each.
+template <bool F16, int NQ>
+__global__ __launch_bounds__(256, 2) void int4_shared(Int4Args a)
+{
+    __shared__ DecodeSmem<NQ, 4> sm;
+    const int planes = a.pool.H * a.groups, plane = blockIdx.x % planes, w = blockIdx.x / planes;
+    const int h = plane % a.pool.H, group = plane / a.pool.H;
+    const Share r = int4_share(a);
+    const int x0 = w * r.each, x1 = x0 + r.each < r.total ? x0 + r.each : r.total;
+    for (int x = x0; x < x1;) {              // uniform
+        const int seq = __builtin_popcountll(__builtin_amdgcn_ballot_w64(r.upto <= x));
+        const int upto = __builtin_amdgcn_readlane(r.upto, seq), steps = __builtin_amdgcn_readlane(r.steps, seq);
+        const int from = upto - steps, stop = upto < x1 ? upto : x1;
+        few_rows<F16, NQ, 4, false>(a, sm, h, group * 16 * NQ, seq, r.of(seq), (x - from) * STEP, (stop - from) * STEP, stop - x == steps,
+                             ((int64_t)plane * (a.workers + a.n_seq) + w + seq) * (16 * NQ));
+        x = stop;
     }
 }
 
