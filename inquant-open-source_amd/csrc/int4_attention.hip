@@ -1,14 +1,17 @@
 // Attention over 4-bit pages (gfx950): how a call is split, and the entry points.
-#include <cstdlib>
 #include "int4_few_dev.h"
 #include "int4_many_dev.h"
 
 namespace {
 
-constexpr int64_t MANY_COLS = QT;
-const int64_t WORKERS = getenv("IQ_T") ? atoi(getenv("IQ_T")) : 0;
-constexpr int64_t ONE_MOST = 512;
-const int64_t MANY = getenv("IQ_MANY") ? atoi(getenv("IQ_MANY")) : 256;
+// Columns (query tokens times query heads of a KV head) from which on the kernel
+// for many takes a call: below, its workgroups of 256 columns are mostly empty
+// (8 sequences of up to 16K rows, 252 columns 104 us by the kernel for few and 126,
+// 315 columns 160 and 128; one of 32K rows 46 and 69, 67 and 53; one of 2000 rows, where
+// either ends soon, 17 and 29, 21 and 29).
+constexpr int64_t MANY = 256;
+constexpr int64_t ONE_MOST = 512;            // rows that one workgroup takes in a step, with no join
+constexpr int64_t BATCH = 64;                // sequences of a launch that shares their rows out
 
 struct Split {
     bool many;                               // the kernel for many columns
@@ -17,18 +20,16 @@ struct Split {
     int64_t floats;                          // the whole workspace
 };
 
-constexpr int64_t BATCH = 64;                // sequences of a launch that shares their rows out
-
 Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seqlen, int64_t max_tokens)
 {
     const int64_t cols = Hq / H * max_seqlen;
     Split s{};
     s.many = cols > MANY;
     if (s.many) {
-        const int64_t tiles = n * H * ((cols + MANY_COLS - 1) / MANY_COLS), steps = (max_tokens + KT - 1) / KT;
+        // as many workgroups as run at once (one per compute unit), of eight tiles of rows at least
+        const int64_t tiles = n * H * ((cols + QT - 1) / QT), steps = (max_tokens + KT - 1) / KT;
         const int64_t parts = tiles >= 192 ? 1 : 256 / tiles, most = (steps + 7) / 8;
-        int64_t want = parts < most ? parts : most;
-        if (want < 1) want = 1;
+        const int64_t want = parts < most ? parts : most < 1 ? 1 : most;
         s.span = KT * ((steps + want - 1) / want);
         if (s.span < KT) s.span = KT;
         s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
@@ -38,7 +39,11 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
         s.groups = (cols + s.width - 1) / s.width;
         const int64_t planes = H * s.groups, steps = (max_tokens + STEP - 1) / STEP, batch = n < BATCH ? n : BATCH;
         if (max_tokens > ONE_MOST) {
-            s.workers = ((WORKERS ? WORKERS : batch * planes * steps > 4096 ? 512 : 256) + planes - 1) / planes;
+            // Two workgroups per compute unit where each has enough to do, else one (one
+            // sequence of 32K rows, 28 heads over 4: 16.5 us with 512, 14.2 with 256; 16 of
+            // 2K-32K: 40.6 and 42.5, with 768 42.7, with 1024 47).
+            const int64_t all = batch * planes * steps > 4096 ? 512 : 256;
+            s.workers = (all + planes - 1) / planes;
             if (s.workers > batch * steps) s.workers = batch * steps;
             s.floats = planes * (s.workers + batch) * s.width * (D + 2);
         }

@@ -40,28 +40,29 @@ __device__ __forceinline__ void few_rows(const Int4Args &a, DecodeSmem<NQ, NW> &
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
-    const int cols = int4_asked(a, s) * a.G;
-    if (col0 >= cols) return;                // uniform
+    // The pages are looked up first (what max_tokens admits stands in the table, so a
+    // first step need not wait for the lengths), then the queries are asked for, then
+    // the first rows: neither waits for what it does not need.
     const Int4Pool &p = a.pool;
     const int32_t *table = p.tables + seq * p.bt_stride;
-    const int colN = col0 + 16 * NQ < cols ? col0 + 16 * NQ : cols;
-    const int sees0 = s.sees(col0 / a.G), sees1 = s.sees((colN - 1) / a.G);     // the first and last column's
-    const int end = stop < sees1 + 1 ? stop : sees1 + 1;
-    if (!direct && t0 >= end) return;        // uniform; the join does not read this partition
-    // The pages are looked up first, then the queries are asked for, then the first
-    // rows, so that neither waits for what it does not need.
     constexpr int NEXT = WT * NW;
     int c0 = t0 + WT * wave;
     // lane l: the page of tile l % 4 of the rows that are asked for next, and of those after them
     int id_lane = 0, id_after = 0;
     auto look_up = [&](int c0) __attribute__((always_inline)) {
         const int row = c0 + 16 * (lane & 3);
-        return table[(row < end ? row : end - 1) >> p.shift];
+        return table[(row < a.max_tokens ? row : a.max_tokens - 1) >> p.shift];
     };
-    if (c0 < end) {
+    if (a.max_tokens > 0) {
         id_lane = look_up(c0);
         if constexpr (!ONE) id_after = look_up(c0 + NEXT);
     }
+    const int cols = int4_asked(a, s) * a.G;
+    if (col0 >= cols) return;                // uniform
+    const int colN = col0 + 16 * NQ < cols ? col0 + 16 * NQ : cols;
+    const int sees0 = s.sees(col0 / a.G), sees1 = s.sees((colN - 1) / a.G);     // the first and last column's
+    const int end = stop < sees1 + 1 ? stop : sees1 + 1;
+    if (!direct && t0 >= end) return;        // uniform; the join does not read this partition
     // B operand: column c16, channels 32 g4 + 8 d .. + 7; its last row and factor
     u32x4 qb[NQ][4];
     int sees[NQ];

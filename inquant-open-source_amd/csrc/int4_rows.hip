@@ -57,10 +57,12 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8])
     return r;
 }
 
-// Rotates channels 8 c .. 8 c + 7 of the row at `row` (x).  A position that the
-// table does not hold gives NaN.
+// Rotates channels 8 c .. 8 c + 7 of a row (x, unpacked from raw); the pairs' other
+// halves come from their lane (loaded again, past what the first cache holds:
+// 274 us for 60K tokens into 4-bit pages).  A position that the table does not hold
+// gives NaN.
 template <bool F16>
-__device__ __forceinline__ void rotate8(const AppendArgs &a, const uint16_t *row, int64_t pos, int c, float (&x)[8])
+__device__ __forceinline__ void rotate8(const AppendArgs &a, u32x4 raw, int64_t pos, int c, float (&x)[8])
 {
     const int per = a.rotary >> 4;           // 16-byte chunks of a half
     if (c >= 2 * per) return;
@@ -77,8 +79,12 @@ __device__ __forceinline__ void rotate8(const AppendArgs &a, const uint16_t *row
     } else {
         const bool first = c < per;
         const int j = first ? c : c - per;
-        float y[8];                          // the pairs' other halves
-        unpack8<F16>(ld16(row + 8 * (first ? c + per : j)), y);
+        const int other = (int)(threadIdx.x & 48) + (first ? c + per : j);
+        u32x4 there;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) there[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * other, (int)raw[i]);
+        float y[8];
+        unpack8<F16>(there, y);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const f32x4 cos = *(const f32x4 *)(table + 8 * j + 4 * h);
@@ -147,74 +153,92 @@ __device__ __forceinline__ uint32_t code8(const float (&x)[8], uint32_t &word)
 
 // Bound by memory.  Sixteen lanes take a row, heads innermost, so that a
 // workgroup reads one range of a token-major batch and its rows share the
-// table's line; the partner half of a row comes out of the same lines again.
+// table's line.
 // Rows of queries and keys (and values of exact pages) go first; the values
 // of 4-bit pages follow, four cache rows of a head at a time, since their codes
 // interleave in sixteen bytes.
-template <bool F16, bool INT4>
+// A team takes R rows, sixteen apart, and asks for all of them first: with one row
+// each a workgroup is over before its latencies are paid for.
+template <bool F16, bool INT4, int R>
 __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a)
 {
     const int seq = blockIdx.y, c = threadIdx.x & 15;
     const int32_t have = a.cu[seq + 1] - a.cu[seq];
     const uint32_t len = have <= 0 ? 0 : (uint32_t)have < a.max_len ? (uint32_t)have : a.max_len;
     const int64_t t0 = a.cu[seq], start = a.start ? a.start[seq] : 0;
+    const int64_t pos0 = a.positions ? (int64_t)a.positions[seq] : start;
     const uint32_t H = (uint32_t)a.H, per_token = (uint32_t)a.Hq + (INT4 ? H : 2 * H);
-    const uint64_t item = (uint64_t)blockIdx.x * TEAMS + (threadIdx.x >> 4), rows = (uint64_t)len * per_token;
-    if (item < rows) {
-        const uint32_t t = (uint32_t)item / per_token, hs = (uint32_t)item - t * per_token;
-        const int64_t token = t0 + t;
-        const bool query = hs < (uint32_t)a.Hq, value = !INT4 && hs >= (uint32_t)a.Hq + H;
-        const uint32_t h = query ? hs / (uint32_t)a.G : value ? hs - a.Hq - H : hs - a.Hq;
-        const uint16_t *row = query ? a.q + token * a.q_st + hs * a.q_sh
-                              : value ? a.v + token * a.v_st + h * a.v_sh : a.k + token * a.k_st + h * a.k_sh;
-        u32x4 raw = ld16(row + 8 * c);
-        float x[8];
-        if (!value) {
-            unpack8<F16>(raw, x);
-            if (a.rotary) rotate8<F16>(a, row, (a.positions ? (int64_t)a.positions[seq] : start) + t, c, x);
-            if (a.factors) {
-                const float *f = a.factors + h * 128 + 8 * c;
+    const uint64_t rows = (uint64_t)len * per_token, first = (uint64_t)blockIdx.x * (TEAMS * R);
+    if (first < rows) {                      // uniform
+        u32x4 raw[R];
+        uint32_t ts[R], hss[R];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = query ? x[i] * f[i] : x[i] / f[i];
+        for (int j = 0; j < R; ++j) {
+            const uint64_t item = first + j * TEAMS + (threadIdx.x >> 4);
+            const uint32_t i = (uint32_t)(item < rows ? item : rows - 1);
+            const uint32_t t = ts[j] = i / per_token, hs = hss[j] = i - t * per_token;
+            const bool query = hs < (uint32_t)a.Hq, value = !INT4 && hs >= (uint32_t)a.Hq + H;
+            const uint16_t *row = query ? a.q + (t0 + t) * a.q_st + hs * a.q_sh
+                                  : value ? a.v + (t0 + t) * a.v_st + (hs - a.Hq - H) * a.v_sh
+                                          : a.k + (t0 + t) * a.k_st + (hs - a.Hq) * a.k_sh;
+            raw[j] = ld16(row + 8 * c);
+        }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (first + j * TEAMS + (threadIdx.x >> 4) >= rows) break;
+            const uint32_t t = ts[j], hs = hss[j];
+            const int64_t token = t0 + t;
+            const bool query = hs < (uint32_t)a.Hq, value = !INT4 && hs >= (uint32_t)a.Hq + H;
+            const uint32_t h = query ? hs / (uint32_t)a.G : value ? hs - a.Hq - H : hs - a.Hq;
+            float x[8];
+            if (!value) {
+                unpack8<F16>(raw[j], x);
+                if (a.rotary) rotate8<F16>(a, raw[j], pos0 + t, c, x);
+                if (a.factors) {
+                    const float *f = a.factors + h * 128 + 8 * c;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = query ? x[i] * f[i] : x[i] / f[i];
+                }
+                if (!INT4 || query) raw[j] = pack8<F16>(x);
             }
-            if (!INT4 || query) raw = pack8<F16>(x);
-        }
-        if (query) {
-            *(u32x4 *)(a.out + token * a.o_st + hs * a.o_sh + 8 * c) = raw;
-            return;
-        }
-        const int64_t at = start + t;
-        if constexpr (INT4) {
-            uint32_t word;
-            const uint32_t codes = code8(x, word);
-            const Int4Pool &p = a.int4;
-            const int64_t page = i4_page(p, seq, at);
-            if (page < 0) return;
-            uint8_t *head = p.base + page * p.s_page + h * p.s_head;
-            const uint32_t r = (uint32_t)at & (p.B - 1);
-            *(uint32_t *)(head + 64 * r + 4 * c) = codes;
-            if ((c & 3) == 0) *(uint16_t *)(head + i4_key_words(p.B) + 8 * r + 2 * (c >> 2)) = (uint16_t)word;
-        } else {
-            const DensePool &p = a.dense;
-            const int64_t page = dense_page(p, seq, at), r = at & (p.B - 1);
-            if (page < 0) return;
-            uint16_t *to = value ? p.value + page * p.v_sp + h * p.v_sh + r * p.v_st
-                                 : p.key + page * p.k_sp + h * p.k_sh + r * p.k_st;
-            __builtin_nontemporal_store(raw, (u32x4 *)(to + 8 * c));
-            if (!value && c == 0 && p.weights) {
-                const int64_t o = (page * p.H + h) * p.B + r;
-                p.weights[o] = 0.0f;
-                p.positions[o] = (a.positions ? a.positions[seq] : (int32_t)start) + (int32_t)t;
+            if (query) {
+                u32x4 *to = (u32x4 *)(a.out + token * a.o_st + hs * a.o_sh + 8 * c);
+                if constexpr (R > 1) __builtin_nontemporal_store(raw[j], to);
+                else *to = raw[j];
+                continue;
+            }
+            const int64_t at = start + t;
+            if constexpr (INT4) {
+                uint32_t word;
+                const uint32_t codes = code8(x, word);
+                const Int4Pool &p = a.int4;
+                const int64_t page = i4_page(p, seq, at);
+                if (page < 0) continue;
+                uint8_t *head = p.base + page * p.s_page + h * p.s_head;
+                const uint32_t r = (uint32_t)at & (p.B - 1);
+                *(uint32_t *)(head + 64 * r + 4 * c) = codes;
+                if ((c & 3) == 0) *(uint16_t *)(head + i4_key_words(p.B) + 8 * r + 2 * (c >> 2)) = (uint16_t)word;
+            } else {
+                const DensePool &p = a.dense;
+                const int64_t page = dense_page(p, seq, at), r = at & (p.B - 1);
+                if (page < 0) continue;
+                uint16_t *to = value ? p.value + page * p.v_sp + h * p.v_sh + r * p.v_st
+                                     : p.key + page * p.k_sp + h * p.k_sh + r * p.k_st;
+                __builtin_nontemporal_store(raw[j], (u32x4 *)(to + 8 * c));
+                if (!value && c == 0 && p.weights) {
+                    const int64_t o = (page * p.H + h) * p.B + r;
+                    p.weights[o] = 0.0f;
+                    p.positions[o] = (int32_t)(pos0 + t);
+                }
             }
         }
         return;
     }
     if constexpr (INT4) {
-        // whole wavefronts of either kind
-        const uint64_t from = (rows + 3) & ~3ull;
-        if (item < from || len == 0) return;
+        // whole workgroups of either kind
+        if (len == 0) return;
         const int64_t quad = start >> 2, quads = ((start + len + 3) >> 2) - quad;
-        const uint64_t i = item - from;
+        const uint64_t i = (blockIdx.x - (rows + TEAMS * R - 1) / (TEAMS * R)) * TEAMS + (threadIdx.x >> 4);
         if (i >= (uint64_t)quads * H) return;
         const uint32_t j = (uint32_t)(i / H), h = (uint32_t)(i - (uint64_t)j * H);
         const int64_t first = (quad + j) * 4;            // a cache row
@@ -381,6 +405,7 @@ __global__ __launch_bounds__(NT) void read_dense_kernel(ReadArgs a)
     __builtin_nontemporal_store(v, (u32x4 *)((uint16_t *)a.v + (t0 + t) * a.v_st + h * a.v_sh + 8 * c));
 }
 
+constexpr int64_t FEW_ROWS = 256;            // of a sequence: a row per team
 constexpr int64_t GRID_MOST = 0xffffffffLL / NT;         // workgroups of a launch's first dimension
 
 bool aligned(const void *p, int64_t strides) { return (uintptr_t)p % 16 == 0 && strides % 8 == 0; }
@@ -422,14 +447,18 @@ extern "C" int iq_append_rows(const void *q, const void *k, const void *v, int d
     a.cu = cu_seqlens, a.start = start, a.positions = positions, a.rotation = rotation, a.angles = angles;
     a.factors = factors, a.rotary = (int32_t)rotary, a.interleaved = interleaved;
     a.Hq = q ? (int32_t)Hq : 0, a.G = q ? (int32_t)(Hq / a.H) : 1, a.max_len = (uint32_t)max_seqlen;
-    // four rows may lie in two quads, and the quads' items start at a multiple of four
-    const int64_t items = max_seqlen * (a.Hq + (dense ? 2 : 1) * (int64_t)a.H) +
-                          (dense ? 0 : 3 + ((max_seqlen + 6) / 4) * (int64_t)a.H);
-    IQ_CHECK_ARG(items <= 0xffffffffLL && (items + TEAMS - 1) / TEAMS <= GRID_MOST, "iq_append_rows: too many rows");
-    const dim3 grid((unsigned)((items + TEAMS - 1) / TEAMS), (unsigned)n_seq);
+    // four rows may lie in two quads
+    const int64_t rows = max_seqlen * (a.Hq + (dense ? 2 : 1) * (int64_t)a.H);
+    const int64_t quads = dense ? 0 : (max_seqlen + 6) / 4 * a.H;
+    const bool four = rows > FEW_ROWS;
+    const int64_t each = TEAMS * (four ? 4 : 1), groups = (rows + each - 1) / each + (quads + TEAMS - 1) / TEAMS;
+    IQ_CHECK_ARG(rows <= 0xffffffffLL && groups <= GRID_MOST, "iq_append_rows: too many rows");
+    const dim3 grid((unsigned)groups, (unsigned)n_seq);
     const bool f16 = dtype == IQ_F16;
-    const auto kernel = dense ? f16 ? append_kernel<true, false> : append_kernel<false, false>
-                              : f16 ? append_kernel<true, true> : append_kernel<false, true>;
+    const auto kernel = four ? dense ? f16 ? append_kernel<true, false, 4> : append_kernel<false, false, 4>
+                                     : f16 ? append_kernel<true, true, 4> : append_kernel<false, true, 4>
+                        : dense ? f16 ? append_kernel<true, false, 1> : append_kernel<false, false, 1>
+                                : f16 ? append_kernel<true, true, 1> : append_kernel<false, true, 1>;
     hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, (hipStream_t)stream, a);
     IQ_CHECK_LAUNCH("append_rows");
     return IQ_OK;

@@ -34,8 +34,7 @@ from dataclasses import dataclass
 import torch
 
 from inquant import _native as nat
-from .dense import (DensePages, _F32, _ROWS, _apart, _call, _cu, _entry, _ints, _on_gpu, _ptr, _status, _tables,
-                    _token_rows)
+from .dense import DensePages, _F32, _ROWS, _apart, _call, _cu, _entry, _ints, _on_gpu, _ptr, _status, _tables
 from .layout import BLOCK_SIZES
 
 ROW_BYTES = 144          # of a token and head: 2 x 64 of codes, 2 x 8 of steps and zero points
@@ -87,49 +86,42 @@ def _kind(pages):
     raise ValueError("Expected DensePages or Int4Pages")
 
 
-def _span(t):
-    """The bytes from the first to the last element of token-major rows of unit channel stride."""
-    (n, h, d), (st, sh, _), size = t.shape, t.stride(), t.element_size()
-    first = t.data_ptr()
-    return first, first + size * ((n - 1) * st + (h - 1) * sh + d)
+def _rows(t, what, heads=None):
+    """(tokens, heads, token stride, head stride, address) of token-major rows."""
+    shape, stride, at = t.shape, t.stride(), t.data_ptr()
+    if len(shape) != 3 or shape[2] != 128 or heads is not None and shape[1] != heads:
+        raise ValueError(f"Expected {what} [tokens, heads, 128]")
+    n, h, _ = shape
+    # any stride will do for a dimension of one
+    st, sh = stride[0] if n > 1 else 0, stride[1] if h > 1 else 0
+    if stride[2] != 1 or (st | sh) % 8 or at % 16:
+        raise ValueError(f"{what} rows must be contiguous and 16-byte aligned")
+    return n, h, st, sh, at
 
 
-def _overlap(x, y):
-    """Whether token-major rows x and y may share memory.  Heads of one tensor
-    [tokens, heads, 128] side by side do not."""
-    (x0, x1), (y0, y1) = _span(x), _span(y)
-    if x1 <= y0 or y1 <= x0:
+def _overlap(x, y, size):
+    """Whether rows x and y (as _rows gives them, of elements of ``size`` bytes) may
+    share memory.  Heads of one tensor [tokens, heads, 128] side by side do not."""
+    n, h, st, sh, x0 = x
+    m, g, yt, yh, y0 = y
+    wx, wy = size * ((h - 1) * sh + 128), size * ((g - 1) * yh + 128)    # of a token
+    if x0 + size * (n - 1) * st + wx <= y0 or y0 + size * (m - 1) * yt + wy <= x0:
         return False
-    st = x.stride(0)
-    if x.shape[0] > 1 and (y.shape[0] == 1 or st != y.stride(0)) or x.shape[0] == 1 and y.shape[0] > 1:
+    if n != m or n < 2 or st != yt:
         return True
-    # of one token each, within a token stride of each other
-    size = x.element_size()
-    wx, wy = (size * ((t.shape[1] - 1) * t.stride(1) + t.shape[2]) for t in (x, y))
-    if x.shape[0] == 1:
-        return True                                      # their spans meet
-    at = (y0 - x0) % (size * st)
-    return at < wx or at + wy > size * st or max(wx, wy) > size * st
+    at = (y0 - x0) % (size * st) if st > 0 else 0
+    return at < wx or at + wy > size * st or wx > size * st
 
 
-def _rows_apart(t):
-    """Whether no two rows of [tokens, heads, 128] share memory."""
-    n, m = t.shape[:2]
-    a, b = t.stride()[:2]
-    if n == 0 or m * n == 1:
+def _rows_apart(n, h, st, sh):
+    """Whether no two of n x h rows of 128 elements share memory."""
+    if sh >= 128 and st >= sh * (h - 1) + 128:
         return True
-    if n == 1 or m == 1:
-        return (b if n == 1 else a) >= 128
-    return b >= 128 and a >= b * (m - 1) + 128 or a >= 128 and b >= a * (n - 1) + 128
-
-
-def _output_rows(t, what, shape, dtypes, gpu):
-    if t.shape != shape or t.dtype not in dtypes:
-        raise ValueError(f"{what} must be [tokens, heads, 128] rows of one of {', '.join(map(str, dtypes))}")
-    _, strides = _token_rows(t, what)
-    if not _rows_apart(t):
-        raise ValueError(f"the rows of {what} must not overlap")
-    return strides
+    if n * h < 2:
+        return True
+    if n == 1 or h == 1:
+        return (sh if n == 1 else st) >= 128
+    return st >= 128 and sh >= st * (n - 1) + 128
 
 
 def append_rows(query, key, value, cu_seqlens, max_seqlen, pages, block_tables, start=None, *, rotation=None,
@@ -159,13 +151,12 @@ def append_rows(query, key, value, cu_seqlens, max_seqlen, pages, block_tables, 
     no sequence, and those past max_seqlen, are not written; rows that a block
     table does not reach are left out.  The inputs must not lie in the pages."""
     dense, int4 = _kind(pages)
-    heads = pages.heads
-    shape, ks = _token_rows(key, "key", heads)
-    vshape, vs = _token_rows(value, "value", heads)
-    dtype = key.dtype
-    if shape != vshape or dtype not in _ROWS or value.dtype is not dtype or dense and dtype is not pages._dtype:
+    heads, gpu, dtype = pages.heads, pages._gpu, key.dtype
+    k, v = _rows(key, "key", heads), _rows(value, "value", heads)
+    tokens = k[0]
+    if v[0] != tokens or dtype not in _ROWS or value.dtype is not dtype or dense and dtype is not pages._dtype:
         raise ValueError("key and value must have one shape and be BF16 or FP16, of the pages' dtype for exact pages")
-    (cu, n), tokens = _cu(cu_seqlens), shape[0]
+    cu, n = _cu(cu_seqlens)
     table = _tables(block_tables, n)
     if start is not None:
         start = _ints(start, (n,), "start rows [sequences]")
@@ -173,38 +164,38 @@ def append_rows(query, key, value, cu_seqlens, max_seqlen, pages, block_tables, 
         positions = _ints(positions, (n,), "positions [sequences]")
     angles = rotary = 0
     if rotation is not None:
-        if rotation.ndim != 2 or rotation.dtype is not _F32 or not rotation.is_contiguous() or rotation.shape[0] < 1 \
-                or rotation.data_ptr() % 16 or rotation.shape[1] % 16 or not 16 <= rotation.shape[1] <= 128:
-            raise ValueError("Expected a contiguous, 16-byte aligned float32 rotation [positions, 16..128 in 16s]")
+        if rotation.ndim != 2 or rotation.dtype is not _F32 or not rotation.is_contiguous() or rotation.data_ptr() % 16:
+            raise ValueError("Expected a contiguous, 16-byte aligned float32 rotation [positions, channels]")
         angles, rotary = rotation.shape
+        if angles < 1 or rotary % 16 or not 16 <= rotary <= 128:
+            raise ValueError("A rotation has positions, and 16 to 128 channels in steps of 16")
     if factors is not None and (factors.shape != (heads, 128) or factors.dtype is not _F32
                                 or not factors.is_contiguous() or factors.data_ptr() % 16):
         raise ValueError("Expected contiguous, 16-byte aligned float32 factors [kv_heads, 128]")
     max_seqlen = int(max_seqlen)
     if max_seqlen < 0:
         raise ValueError("max_seqlen must not be negative")
-    gpu = pages._gpu
     _on_gpu(gpu, "append_rows", query, key, value, cu, block_tables, start, positions, rotation, factors, output)
-    hq, qs, os = 0, (0, 0), (0, 0)
+    q = out = (0, 0, 0, 0, 0)
     if query is not None:
-        qshape, qs = _token_rows(query, "query")
-        hq = qshape[1]
-        if qshape[0] != tokens or query.dtype is not dtype or hq < 1 or hq % heads:
+        q = _rows(query, "query")
+        if q[0] != tokens or query.dtype is not dtype or q[1] < 1 or q[1] % heads:
             raise ValueError("Expected a query [tokens, heads, 128] of the key's dtype, its heads a multiple of KV heads")
         if output is None:
-            output = torch.empty(qshape, dtype=dtype, device=query.device)
-        os = _output_rows(output, "output", qshape, (dtype,), gpu)
-        if tokens and not (output.data_ptr() == query.data_ptr() and os == qs) and _overlap(output, query) \
-                or tokens and any(_overlap(output, t) for t in (key, value)):
+            output = torch.empty(query.shape, dtype=dtype, device=query.device)
+        out = q if output is query else _rows(output, "output", q[1])
+        if out[0] != tokens or output.dtype is not dtype or not _rows_apart(*out[:4]):
+            raise ValueError("output must be [tokens, heads, 128] of the query's dtype, its rows apart")
+        if tokens and (out != q and _overlap(out, q, 2) or _overlap(out, k, 2) or _overlap(out, v, 2)):
             raise ValueError("output must be the query itself or share no memory with the inputs")
     elif output is not None:
         raise ValueError("an output needs a query")
     max_seqlen = min(max_seqlen, tokens)
     if max_seqlen == 0:
         return output
-    _call(gpu, "iq_append_rows_from", _ptr(query), key.data_ptr(), value.data_ptr(), nat.dtype_code(dtype), *qs, *ks,
-          *vs, hq, cu.data_ptr(), n, max_seqlen, _ptr(start), _ptr(positions), _ptr(rotation), angles, rotary,
-          bool(interleaved), _ptr(factors), dense, int4, *table, _ptr(output), *os)
+    _call(gpu, "iq_append_rows_from", q[4], k[4], v[4], nat.dtype_code(dtype), q[2], q[3], k[2], k[3], v[2], v[3], q[1],
+          cu.data_ptr(), n, max_seqlen, _ptr(start), _ptr(positions), _ptr(rotation), angles, rotary, bool(interleaved),
+          _ptr(factors), dense, int4, *table, out[4], out[2], out[3])
     return output
 
 
@@ -217,15 +208,14 @@ def read_rows(pages, block_tables, cu_seqlens, max_seqlen, key, value, start=Non
     on are left out) takes cache row start[i] + t (``start`` int32 [sequences], None:
     0).  Tokens of no sequence, and those whose row has no page, are not written."""
     dense, int4 = _kind(pages)
-    heads = pages.heads
-    shape, dtype = key.shape, key.dtype
-    if len(shape) != 3 or shape[1:] != (heads, 128):
-        raise ValueError("Expected key [tokens, heads, 128]")
-    gpu = pages._gpu
-    ks, vs = (_output_rows(t, what, shape, (pages._dtype,) if dense else (dtype,), gpu)
-              for t, what in ((key, "key"), (value, "value")))
-    if dtype not in (*_ROWS, _F32):
-        raise ValueError("Rows are BF16, FP16 or float32")
+    heads, gpu, dtype = pages.heads, pages._gpu, key.dtype
+    k, v = _rows(key, "key", heads), _rows(value, "value", heads)
+    tokens = k[0]
+    if v[0] != tokens or value.dtype is not dtype or (dtype is not pages._dtype if dense else dtype not in (*_ROWS, _F32)):
+        raise ValueError("key and value must have one shape and the pages' dtype (BF16, FP16 or float32 for 4-bit pages)")
+    size = 4 if dtype is _F32 else 2
+    if not _rows_apart(*k[:4]) or not _rows_apart(*v[:4]) or tokens and _overlap(k, v, size):
+        raise ValueError("the rows of key and value must not overlap")
     (cu, n), max_seqlen = _cu(cu_seqlens), int(max_seqlen)
     table = _tables(block_tables, n)
     if start is not None:
@@ -233,12 +223,10 @@ def read_rows(pages, block_tables, cu_seqlens, max_seqlen, key, value, start=Non
     if max_seqlen < 0:
         raise ValueError("max_seqlen must not be negative")
     _on_gpu(gpu, "read_rows", key, value, cu, block_tables, start)
-    if shape[0] and _overlap(key, value):
-        raise ValueError("key and value must not overlap")
-    max_seqlen = min(max_seqlen, shape[0])
+    max_seqlen = min(max_seqlen, tokens)
     if max_seqlen:
         _call(gpu, "iq_read_rows_from", dense, int4, nat.dtype_code(dtype), *table, cu.data_ptr(), n, max_seqlen,
-              _ptr(start), key.data_ptr(), *ks, value.data_ptr(), *vs)
+              _ptr(start), k[4], k[2], k[3], v[4], v[2], v[3])
     return key, value
 
 
@@ -268,7 +256,7 @@ def _attention(what, query, cu, n, max_seqlen, pages, block_tables, lengths, max
     dtype, os = output.dtype, output.stride()
     if output.shape != shape or os[2] != 1 or dtype is not query.dtype and dtype is not _F32:
         raise ValueError("output must be [tokens, heads, 128] of the query dtype or float32")
-    if not _rows_apart(output) and not _apart(tokens, hq, *os[:2]):
+    if not _rows_apart(tokens, hq, os[0], os[1]) and not _apart(tokens, hq, *os[:2]):
         raise ValueError("the output's rows must not overlap")
     if n == 0 or tokens == 0 or max_seqlen == 0:
         return output
