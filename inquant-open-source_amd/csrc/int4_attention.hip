@@ -13,8 +13,13 @@ constexpr int64_t MANY = 256;
 constexpr int64_t ONE_MOST = 512;            // rows that one workgroup takes in a step, with no join
 constexpr int64_t BATCH = 64;                // sequences of a launch that shares their rows out
 
+// A call for many that some sequences ask little of (a chunk of a prompt beside
+// single and drafted tokens) leaves sequences of at most MIXED columns to the kernel
+// for few, which shares their rows out: one workgroup would walk through each.
+constexpr int64_t MIXED = 32;
+
 struct Split {
-    bool many;                               // the kernel for many columns
+    bool many, mixed;                        // the kernel for many columns; beside the one for few
     int64_t span, parts;                     // many: rows per partition, partitions
     int64_t groups, workers, width;          // few: groups of columns, workgroups that share a plane's rows (0: none), columns
     int64_t floats;                          // the whole workspace
@@ -22,21 +27,27 @@ struct Split {
 
 Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seqlen, int64_t max_tokens)
 {
-    const int64_t cols = Hq / H * max_seqlen;
     Split s{};
+    if (max_seqlen > tokens) max_seqlen = tokens;
+    if (H < 1 || Hq < H || n < 1 || max_seqlen < 1) return s;
+    const int64_t cols = Hq / H * max_seqlen;
     s.many = cols > MANY;
+    s.mixed = s.many && n > 1 && tokens <= (n - 1) * max_seqlen + MIXED / (Hq / H);   // else no sequence asks so little
     if (s.many) {
         // as many workgroups as run at once (one per compute unit), of eight tiles of rows at least
-        const int64_t tiles = n * H * ((cols + QT - 1) / QT), steps = (max_tokens + KT - 1) / KT;
+        const int64_t each = (cols + QT - 1) / QT, all = (tokens * (Hq / H) + QT - 1) / QT;
+        const int64_t tiles = H * (n * each < all ? n * each : all), steps = (max_tokens + KT - 1) / KT;
         const int64_t parts = tiles >= 192 ? 1 : 256 / tiles, most = (steps + 7) / 8;
         const int64_t want = parts < most ? parts : most < 1 ? 1 : most;
         s.span = KT * ((steps + want - 1) / want);
         if (s.span < KT) s.span = KT;
         s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
         s.floats = s.parts > 1 ? tokens * Hq * s.parts * (D + 2) : 0;
-    } else {
-        s.width = cols <= 16 ? 16 : 32;
-        s.groups = (cols + s.width - 1) / s.width;
+    }
+    if (!s.many || s.mixed) {
+        const int64_t most = s.mixed ? MIXED : cols;
+        s.width = most <= 16 ? 16 : 32;
+        s.groups = (most + s.width - 1) / s.width;
         const int64_t planes = H * s.groups, steps = (max_tokens + STEP - 1) / STEP, batch = n < BATCH ? n : BATCH;
         if (max_tokens > ONE_MOST) {
             // Two workgroups per compute unit where each has enough to do, else one (one
@@ -45,14 +56,16 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
             const int64_t all = batch * planes * steps > 4096 ? 512 : 256;
             s.workers = (all + planes - 1) / planes;
             if (s.workers > batch * steps) s.workers = batch * steps;
-            s.floats = planes * (s.workers + batch) * s.width * (D + 2);
+            const int64_t floats = planes * (s.workers + batch) * s.width * (D + 2);
+            if (floats > s.floats) s.floats = floats;        // the two take turns with it
         }
     }
     return s;
 }
 
+// `most`: tokens of a sequence that the kernel for few answers
 template <bool F16, int NQ>
-void launch_few(Int4Args a, int64_t n, hipStream_t stream)
+void launch_few(Int4Args a, int64_t most, int64_t n, hipStream_t stream)
 {
     const unsigned planes = (unsigned)(a.pool.H * a.groups);
     if (a.workers == 0) {
@@ -75,7 +88,7 @@ void launch_few(Int4Args a, int64_t n, hipStream_t stream)
             a.tokens = tokens - (int32_t)s0;
         }
         hipLaunchKernelGGL((int4_shared<F16, NQ>), dim3(planes * (unsigned)a.workers), dim3(256), 0, stream, a);
-        hipLaunchKernelGGL(int4_join<true>, dim3((unsigned)(a.Hq * a.max_seqlen), (unsigned)a.n_seq), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(int4_join<true>, dim3((unsigned)(a.Hq * most), (unsigned)a.n_seq), dim3(256), 0, stream, a);
     }
 }
 
@@ -125,17 +138,21 @@ extern "C" int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t
     IQ_CHECK_ARG(s.floats == 0 || (workspace && workspace_floats >= s.floats), "iq_int4_attention: workspace too small");
     const int64_t G = Hq / pool.H, cols = G * max_seqlen;
     IQ_CHECK_ARG(s.parts <= 65535 && cols <= 0x3fffffff && s.groups * pool.H * (s.workers + 1) <= 0xffffff &&
-                     Hq * max_seqlen <= 0xffffff, "iq_int4_attention: too many rows");
+                     Hq * max_seqlen <= (s.many ? 0x3fffffff : 0xffffff), "iq_int4_attention: too many rows");
     const int64_t rows = s.floats / (D + 2);
     const Int4Args a{pool, (const uint16_t *)q, q_st, q_sh, cu_seqlens, lengths, (int32_t)tokens, (int32_t)max_seqlen,
                      (int32_t)max_tokens, (int32_t)G, (int32_t)Hq, (int32_t)s.span, (int32_t)s.parts, (int32_t)n_seq,
-                     (int32_t)s.groups, (int32_t)s.workers, (int32_t)s.width, scale * I4_LOG2E,
+                     (int32_t)s.groups, (int32_t)s.workers, (int32_t)s.width,
+                     (int32_t)(!s.many ? MANY : s.mixed ? MIXED : 0), scale * I4_LOG2E,
                      Partials{workspace, (f32x2 *)(workspace + rows * D)}, out, o_st, o_sh, out_dtype};
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = dtype == IQ_F16;
     if (s.many) f16 ? launch_chunk<true>(a, cols, n_seq, st) : launch_chunk<false>(a, cols, n_seq, st);
-    else if (cols <= 16) f16 ? launch_few<true, 1>(a, n_seq, st) : launch_few<false, 1>(a, n_seq, st);
-    else f16 ? launch_few<true, 2>(a, n_seq, st) : launch_few<false, 2>(a, n_seq, st);
+    if (!s.many || s.mixed) {
+        const int64_t most = s.many ? MIXED / G : max_seqlen;
+        if (s.width == 16) f16 ? launch_few<true, 1>(a, most, n_seq, st) : launch_few<false, 1>(a, most, n_seq, st);
+        else f16 ? launch_few<true, 2>(a, most, n_seq, st) : launch_few<false, 2>(a, most, n_seq, st);
+    }
     IQ_CHECK_LAUNCH("int4_attention");
     return IQ_OK;
 }

@@ -8,9 +8,9 @@ namespace {
 
 constexpr int D = 128;
 constexpr float I4_LOG2E = 1.44269504088896341f;
-// Softmax weights are at most 1; as f16 operands (and in the sums they are
-// divided by) they are 2^14 times that, so that a weight keeps its eleven bits
-// down to 2^-28 of the largest instead of 2^-14.
+// Softmax weights are at most 1; as f16 operands of the kernel for few columns
+// (and in the sums they are divided by) they are 2^14 times that, so that a weight
+// keeps its eleven bits down to 2^-28 of the largest instead of 2^-14.
 constexpr float I4_BIAS = 14.0f;
 
 struct Int4Args {
@@ -21,6 +21,7 @@ struct Int4Args {
     int32_t tokens, max_seqlen, max_tokens, G, Hq;
     int32_t span, parts;                     // many columns: rows per partition, partitions
     int32_t n_seq, groups, workers, width;   // few: see Share
+    int32_t few;                             // sequences of at most so many columns are its, the others the kernel's for many
     float c_log2;
     Partials part;                           // many: [tokens * Hq, parts] rows; few: [planes, workers + n_seq, width]
     void *out;
@@ -45,17 +46,18 @@ __device__ __forceinline__ Int4Seq int4_seq(const Int4Args &a, int seq)
     return s;
 }
 
-// Query tokens of a sequence that a call answers.
+// Query tokens of a sequence that a call answers; 0 where the other kernel does.
+template <bool FEW>
 __device__ __forceinline__ int32_t int4_asked(const Int4Args &a, const Int4Seq &s)
 {
     int32_t m = s.m < a.max_seqlen ? s.m : a.max_seqlen;
     if (s.t0 < 0) return 0;
     const int32_t rest = a.tokens - s.t0;    // no token behind the last of the tensor
-    return m < rest ? m : rest > 0 ? rest : 0;
+    m = m < rest ? m : rest > 0 ? rest : 0;
+    return (m * a.G <= a.few) == FEW ? m : 0;
 }
 
-// Eight channels of a query in f32, times f, as an f16 operand in the order of
-// i4_pair's pairs: channels 0, 4, 1, 5, 2, 6, 3, 7.
+// Eight channels of a query in f32.
 template <bool F16>
 __device__ __forceinline__ void query8(u32x4 raw, float (&x)[8])
 {
@@ -102,7 +104,7 @@ __device__ __forceinline__ Share int4_share(const Int4Args &a)
     const int lane = threadIdx.x & 63;
     Share r;
     r.own = int4_seq(a, lane < a.n_seq ? lane : a.n_seq - 1);
-    r.steps = lane < a.n_seq && int4_asked(a, r.own) > 0 ? (r.own.len + STEP - 1) / STEP : 0;
+    r.steps = lane < a.n_seq && int4_asked<true>(a, r.own) > 0 ? (r.own.len + STEP - 1) / STEP : 0;
     int32_t v = r.steps;
     v += dpp_i<0x111, 0xf>(v);               // row_shr:1
     v += dpp_i<0x112, 0xf>(v);
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(256) void int4_join(Int4Args a)
     const Int4Seq s = int4_seq(a, seq);
     const uint32_t item = FEW ? blockIdx.x : blockIdx.x * 8 + team;
     const int t = (int)(item / (uint32_t)a.Hq), hq = (int)(item - (uint32_t)t * (uint32_t)a.Hq);
-    if (t >= int4_asked(a, s)) return;       // with FEW the whole workgroup's
+    if (t >= int4_asked<FEW>(a, s)) return;       // with FEW the whole workgroup's
     const int last = s.sees(t);
     int first = 0, live;                     // partitions first .. live - 1
     int64_t base, next;                      // rows of the first of them, from one to the next

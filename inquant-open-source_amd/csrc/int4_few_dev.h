@@ -57,7 +57,7 @@ __device__ __forceinline__ void few_rows(const Int4Args &a, DecodeSmem<NQ, NW> &
         id_lane = look_up(c0);
         if constexpr (!ONE) id_after = look_up(c0 + NEXT);
     }
-    const int cols = int4_asked(a, s) * a.G;
+    const int cols = int4_asked<true>(a, s) * a.G;
     if (col0 >= cols) return;                // uniform
     const int colN = col0 + 16 * NQ < cols ? col0 + 16 * NQ : cols;
     const int sees0 = s.sees(col0 / a.G), sees1 = s.sees((colN - 1) / a.G);     // the first and last column's

@@ -1,13 +1,20 @@
 // Attention of many tokens over 4-bit pages (gfx950): a chunk of a prompt.
 //
-// One workgroup takes 32 NW of the (token, head) columns that share a KV head,
-// NW wavefronts of 32, and a partition of the rows in tiles of 64: S^T = K Q^T
+// One workgroup takes 256 of the (token, head) columns that share a KV head,
+// eight wavefronts of 32, and a partition of the rows in tiles of 64: S^T = K Q^T
 // and O^T = V^T P^T on 32x32x16 products, the weights staying in the lanes that
 // the second product reads them from.  The codes of a tile become f16 operands
-// once per workgroup, exactly, on their way into LDS, beside the products of the
-// tile before: 16 bytes of key codes are four chunks of eight channels, 16 bytes
-// of value codes are eight channels of four rows, which stand in LDS as the
-// product reads them, channel by channel, so nothing is transposed.
+// once per workgroup, exactly, on their way into LDS, beside the products: 16
+// bytes of key codes are four chunks of eight channels, 16 bytes of value codes
+// are eight channels of four rows, which stand in LDS as the product reads them,
+// channel by channel, so nothing is transposed.
+//
+// Bound by the matrix cores and the arithmetic of the weights beside them, which
+// the two wavefronts of a SIMD take in turn (below): 0.95-0.98 ms for 2048 tokens
+// behind 32K rows, 28 heads over 4, 0.95-0.98 PFLOP/s.  Workgroups of 128 columns, each
+// with its own coded rows, and every wavefront at its products at the same time:
+// 1.65 ms.  64 columns a wavefront halve what is read from LDS, but their products'
+// sums do not fit the registers that the weights' arithmetic can use.
 #pragma once
 
 #include <type_traits>
@@ -27,6 +34,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 // K: rows of 256 bytes, whose 16-byte chunk c is at slot c ^ (row % 16).  V:
 // [quad of rows][channel] 8 bytes of four rows; of the four 16-byte slots of
 // eight channels, the one of channels 2 k and 2 k + 1 is at k ^ (channel / 32).
+// A stage's address is told from the other's by one bit, hence the alignment.
 struct __attribute__((aligned(32768))) ChunkSmem {
     uint16_t k[2][KT * D], v[2][KT * D];
     // NaN words of masked tiles [tile % 4][16 rows][row % 4]: bit 16 (row / 4 % 4) + 4 group
@@ -68,7 +76,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
     const int h = item / tiles, place = tiles - 1 - (item - h * tiles);
     const int part = blockIdx.y, seq = blockIdx.z;
     const Int4Seq s = int4_seq(a, seq);
-    const int cols = int4_asked(a, s) * a.G, col0 = place * QT;
+    const int cols = int4_asked<false>(a, s) * a.G, col0 = place * QT;
     if (col0 >= cols) return;                // uniform
     const Int4Pool &p = a.pool;
     const int32_t *table = p.tables + seq * p.bt_stride;
@@ -186,8 +194,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
     f32x16 sc[2];                            // rows k0 + 32 b + 8 (i / 4) + 4 h32 + i % 4 of column c32
     u32x4 pb[2][2];                          // B operand of the 16 rows (b, c): registers 8 c .. 8 c + 7
     // Operands are read AHEAD products early: a wavefront that has the matrix cores
-    // for itself waits for nothing else (one read before each product: 1.49 ms for
-    // 2048 tokens of 32K rows).
+    // for itself waits for nothing else.
     // Addresses of this lane's first operands of the keys' and the values' stage,
     // carried from period to period (what follows from them alone is made anew in
     // each: kept, it would not fit the registers).
@@ -202,8 +209,8 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
         const u32x2 lo = *(lds_u32x2 *)from, hi = *(lds_u32x2 *)(from + 8 * D * 2);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
-    // products from .. to - 1 of a turn: 0 .. 15 of the values of stage `before`, 16 .. 31 of the keys of
-    // `st`; with `code`, the pieces beside them
+    // Products from .. to - 1 of a period: 0 .. 15 of the values, 16 .. 31 of the keys, and the pieces of
+    // what this group codes beside the last sixteen.
     u32x4 x[AHEAD];
     auto read = [&](int i) __attribute__((always_inline)) {
         x[i % AHEAD] = i < 16 ? value_operand(i) : key_operand(i - 16);
@@ -262,6 +269,8 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
                     const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[b][8 * c + 2 * w], c_log2, less));
                     const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[b][8 * c + 2 * w + 1], c_log2, less));
                     pb[b][c][w] = pack2<true>(p0, p1);
+                    // by additions: a dot product of the packed pair runs on the matrix cores here, and waits
+                    // for the other wavefront's products
                     lsum[w & 1] += p0;
                     lsum[w & 1] += p1;
                     // made here, beside the other wavefront's products, not where it is used
@@ -300,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
     // of tile i - 1 and the keys of tile i, and writes the other stages.
     auto run = [&](auto group) __attribute__((always_inline)) {
         constexpr bool K = decltype(group)::value;           // the second group, which codes the keys
-        // sixteens without a page of tile i and of the tiles after it; `ahead` tiles on is the next to be coded
+        // gone[j]: the sixteens of tile i + j that have no page; what is asked for next is of tile i + 2 + LEAD
         constexpr int LEAD = K ? 1 : 0;
         int gone[3 + LEAD];
         look_up(t0);
@@ -328,9 +337,7 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
         from_k ^= STAGE;
         for (;;) {
             if constexpr (K) meet();
-            
             weights(k0, gone[0]);
-            
             // past the last tile what is asked for and coded is not read
             arrived();
             gone[2 + LEAD] = fetch(k0 + (2 + LEAD) * KT);

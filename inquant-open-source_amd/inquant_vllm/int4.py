@@ -28,7 +28,6 @@ counterpart.
 from __future__ import annotations
 
 import ctypes
-import math
 from dataclasses import dataclass
 
 import torch
@@ -243,8 +242,8 @@ def _attention(what, query, cu, n, max_seqlen, pages, block_tables, lengths, max
     table = _tables(block_tables, n)
     if not 0 <= max_tokens <= table[2] * pages.block_size:
         raise ValueError("max_tokens must fit the block tables")
-    if not math.isfinite(scale):
-        raise ValueError("the scale must be finite")
+    if not abs(scale) <= 2.0 ** 126:
+        raise ValueError("the scale must be finite, as a float32 too")
     gpu = pages._gpu
     _on_gpu(gpu, what, query, cu, block_tables, lengths, output)
     qs = query.stride()
@@ -260,10 +259,15 @@ def _attention(what, query, cu, n, max_seqlen, pages, block_tables, lengths, max
         raise ValueError("the output's rows must not overlap")
     if n == 0 or tokens == 0 or max_seqlen == 0:
         return output
+    # a workgroup reads its queries before it writes their outputs, and no other's
+    at, to = query.data_ptr(), output.data_ptr()
+    if at < to + (4 if dtype is _F32 else 2) * ((tokens - 1) * os[0] + (hq - 1) * os[1] + 128) \
+            and to < at + 2 * ((tokens - 1) * qs[0] + (hq - 1) * qs[1] + 128) and not (at == to and dtype is query.dtype and os == qs):
+        raise ValueError("output must be the query itself or lie apart from it")
     # the scratch that is there serves most calls; the library says when it does not
     scratch, have, stream = workspace.floats(0, query.device)
-    args = [query.data_ptr(), nat.dtype_code(query.dtype), qs[0], qs[1], hq, _ptr(cu), n, tokens, max_seqlen,
-            pages._desc, *table, lengths.data_ptr(), max_tokens, scale, scratch, have, output.data_ptr(), os[0], os[1],
+    args = [at, nat.dtype_code(query.dtype), qs[0], qs[1], hq, _ptr(cu), n, tokens, max_seqlen,
+            pages._desc, *table, lengths.data_ptr(), max_tokens, scale, scratch, have, to, os[0], os[1],
             nat.IQ_F32 if dtype is _F32 else nat.dtype_code(dtype), stream]
     status = _status(gpu, "iq_int4_attention_from", *args)
     if status:

@@ -278,7 +278,10 @@ def test_decode(hq, h, B, dtype, lengths, out_dtype):
     (14, 2, 256, F16, [300, 90, 1, 0, 33], [290, 90, 1, 0, 2]),              # many, fewer rows than tiles of columns
     (16, 1, 16, BF, [1100, 20], [40, 40]),                                   # more tokens than rows
     (8, 8, 16, BF, [600], [600]),                                            # a whole prompt, one head per KV head
-    (4, 2, 16, F16, [400] + [40] * 70, [1] * 71)])                           # more than a launch's sequences
+    (4, 2, 16, F16, [400] + [40] * 70, [1] * 71),                            # more than a launch's sequences
+    (28, 4, 16, BF, [3000, 2000, 5, 700, 900], [1, 300, 0, 4, 5]),           # a chunk beside single and drafted tokens
+    (32, 4, 32, F16, [500, 310, 31, 1], [100, 1, 1, 1]),
+    (16, 1, 16, BF, [600 + 20 * i for i in range(69)] + [64], [1, 2] * 34 + [40, 64])])
 def test_attention(hq, h, B, dtype, lengths, asked):
     gen = gen_of(hq + 3 * B)
     pages = sum(-(-n // B) for n in lengths) + 2
@@ -482,6 +485,23 @@ def test_a_prompt_in_chunks_then_tokens():
     assert same(key[:total], case.stands_for(*case.coded(turned)))
     check(torch.cat(outs), torch.cat(rotated), [total], [total], key.view(-1, B, h, 128), value.view(-1, B, h, 128),
           torch.arange(-(-total // B))[None], B, 0.09, BF)
+
+
+def test_outputs_in_place_and_apart():
+    gen = gen_of(19)
+    held, _, _ = random_pool(gen, 120, 2, 16)
+    tables, workspace = tables_of(gen, [900, 700], 16, 120).cuda(), SharedDecodeWorkspace()
+    for m, lengths in ((1, [900, 700]), (1, [200, 500]), (5, [900, 30]), (60, [900, 700])):
+        rows = i32(lengths)
+        q = torch.randn((2 * m + 4, 8, 128), generator=gen).to(BF).cuda()
+        args = (i32([0, m, 2 * m]), m, held, tables, rows, max(lengths), 0.1, workspace)
+        want = int4_attention(q[:2 * m], *args)
+        with pytest.raises(ValueError, match="apart from it"):
+            int4_attention(q[:2 * m], *args, q[1:2 * m + 1])
+        own = q[:2 * m]
+        assert int4_attention(own, *args, own) is own and torch.equal(own, want)
+    with pytest.raises(ValueError, match="finite"):
+        int4_decode(q[:2], held, tables, rows, 900, 1e39, workspace)
 
 
 def test_outputs_repeat():
