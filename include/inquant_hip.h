@@ -701,7 +701,8 @@ int iq_read_rows_from(const iq_read_rows_args *args);
  * 1] - cu_seqlens[i] tokens from cu_seqlens[i] on (at most max_seqlen; the rest
  * is not written), the last m of its rows: token t sees the cache rows up to
  * lengths[i] - m + t.  cu_seqlens NULL: token i is the one of sequence i
- * (max_seqlen 1).  out [tokens, Hq, 128] of out_dtype (unit channel stride).
+ * (max_seqlen 1).  out [tokens, Hq, 128] of out_dtype (unit channel stride), q
+ * itself or apart from it.
  * fp32 logits, softmax and accumulation; a query is scaled by a power of two
  * and taken as f16, softmax weights are rounded to f16 before P.V, the rows are
  * exact.  A token that sees no row, or whose logits are all -inf, gives zeros.

@@ -151,14 +151,15 @@ __device__ __forceinline__ uint32_t code8(const float (&x)[8], uint32_t &word)
     return fine ? codes : 0;
 }
 
-// Bound by memory.  Sixteen lanes take a row, heads innermost, so that a
+// Bound by memory: seven prompts into exact pages 268 us (5.7 TB/s read and
+// written), 60K tokens into 4-bit pages 232-249 us (a kernel trace's).  Sixteen lanes take a row, heads innermost, so that a
 // workgroup reads one range of a token-major batch and its rows share the
 // table's line.
 // Rows of queries and keys (and values of exact pages) go first; the values
 // of 4-bit pages follow, four cache rows of a head at a time, since their codes
 // interleave in sixteen bytes.
 // A team takes R rows, sixteen apart, and asks for all of them first: with one row
-// each a workgroup is over before its latencies are paid for.
+// each a workgroup of a long call is over before its latencies are paid for.
 template <bool F16, bool INT4, int R>
 __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a)
 {
@@ -319,7 +320,8 @@ __device__ __forceinline__ void store8(void *base, int64_t at, u32x4 v)
 }
 
 // Four cache rows of a head by sixteen lanes, eight channels each; a row of a
-// page outside the pool or the table is not written.
+// page outside the pool or the table is not written.  Bound by memory: 124 us for
+// 662 MB (5.4 TB/s), most of them written.
 template <int ODT>
 __global__ __launch_bounds__(NT) void read_int4_kernel(ReadArgs a)
 {
@@ -405,7 +407,11 @@ __global__ __launch_bounds__(NT) void read_dense_kernel(ReadArgs a)
     __builtin_nontemporal_store(v, (u32x4 *)((uint16_t *)a.v + (t0 + t) * a.v_st + h * a.v_sh + 8 * c));
 }
 
-constexpr int64_t FEW_ROWS = 256;            // of a sequence: a row per team
+// Rows of a call (of queries, keys and exact pages' values) past which a team takes
+// four.  Exact pages: 18K rows 4.5 us by ones and 5.5 by fours, 74K rows 9.6 and 8.3, 1.2M
+// rows 126 and 112.  4-bit pages, whose groups cost more: 32 rows 3.4 and 4.3, 2K rows 6.5
+// either way, 16K rows 7.9 and 7.4, 65K rows 13.9 and 11.0.
+constexpr int64_t ONES_DENSE = 32768, ONES_INT4 = 8192;
 constexpr int64_t GRID_MOST = 0xffffffffLL / NT;         // workgroups of a launch's first dimension
 
 bool aligned(const void *p, int64_t strides) { return (uintptr_t)p % 16 == 0 && strides % 8 == 0; }
@@ -450,7 +456,7 @@ extern "C" int iq_append_rows(const void *q, const void *k, const void *v, int d
     // four rows may lie in two quads
     const int64_t rows = max_seqlen * (a.Hq + (dense ? 2 : 1) * (int64_t)a.H);
     const int64_t quads = dense ? 0 : (max_seqlen + 6) / 4 * a.H;
-    const bool four = rows > FEW_ROWS;
+    const bool four = rows > (dense ? ONES_DENSE : ONES_INT4) / n_seq;
     const int64_t each = TEAMS * (four ? 4 : 1), groups = (rows + each - 1) / each + (quads + TEAMS - 1) / TEAMS;
     IQ_CHECK_ARG(rows <= 0xffffffffLL && groups <= GRID_MOST, "iq_append_rows: too many rows");
     const dim3 grid((unsigned)groups, (unsigned)n_seq);

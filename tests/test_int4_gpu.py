@@ -71,6 +71,8 @@ CASES = [
     dict(lengths=[6, 2], starts=[2, 3], B=16, heads=2, hq=2, dtype=BF, rotary=128, interleaved=True),
     dict(lengths=[25], starts=[4], B=16, heads=2, hq=4, dtype=F16, rotary=0),
     dict(lengths=[500, 37], starts=[3, 0], B=16, heads=1, hq=7, dtype=BF, rotary=128),
+    dict(lengths=[900, 37, 901], starts=[3, 0, 6], B=16, heads=1, hq=15, dtype=BF, rotary=128),     # four rows a team
+    dict(lengths=[1400], starts=[7], B=64, heads=1, hq=24, dtype=F16, rotary=64, interleaved=True, factors=True),
 ]
 
 
