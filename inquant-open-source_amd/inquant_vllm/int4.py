@@ -205,7 +205,8 @@ def read_rows(pages, block_tables, cu_seqlens, max_seqlen, key, value, start=Non
 
     Token t of sequence i (cu_seqlens int32 [sequences + 1]; tokens from max_seqlen
     on are left out) takes cache row start[i] + t (``start`` int32 [sequences], None:
-    0).  Tokens of no sequence, and those whose row has no page, are not written."""
+    0).  Tokens of no sequence, and those whose row has no page, are not written.
+    The rows must not lie in the pages."""
     dense, int4 = _kind(pages)
     heads, gpu, dtype = pages.heads, pages._gpu, key.dtype
     k, v = _rows(key, "key", heads), _rows(value, "value", heads)

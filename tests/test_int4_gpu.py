@@ -410,6 +410,41 @@ def test_strided_pool_and_other_streams():
     check(out, q, [3], [530], *padded.view(2, 34, B, 2, 128), torch.arange(34)[None], B, 0.1, F16)
 
 
+@pytest.mark.parametrize("m", [1, 20, 90])
+def test_no_rows_at_all(m):
+    """max_tokens of 0 with empty block tables, and lengths that are all 0 or below."""
+    held = Int4Pages(torch.full((3, 2, 16 * 144), 0xff, dtype=torch.uint8, device="cuda"))
+    q = torch.ones((2 * m, 8, 128), dtype=BF, device="cuda")
+    empty = torch.zeros((2, 0), dtype=torch.int32, device="cuda")
+    wide = torch.zeros((2, 70), dtype=torch.int32, device="cuda")
+    for tables, lengths, most in ((empty, [0, 0], 0), (empty, [5, 9], 0), (wide, [0, -3], 1000), (wide, [0, 0], 300)):
+        out = int4_attention(q, i32([0, m, 2 * m]), m, held, tables, i32(lengths), most, 0.1, SharedDecodeWorkspace())
+        assert (out == 0).all()
+
+
+def test_two_streams_at_once():
+    """The operators on two streams at the same time, a workspace each, over the same pages."""
+    gen = gen_of(20)
+    held, _, _ = random_pool(gen, 700, 2, 16)
+    tables, rows = tables_of(gen, [6000, 4000], 16, 700).cuda(), i32([6000, 4000])
+    work = []
+    for m in (1, 5, 80):
+        q = torch.randn((2 * m, 8, 128), generator=gen).to(BF).cuda()
+        args = (q, i32([0, m, 2 * m]), m, held, tables, rows, 6000, 0.1)
+        work.append((args, int4_attention(*args, SharedDecodeWorkspace())))
+    torch.cuda.synchronize()
+    streams = [(torch.cuda.Stream(), SharedDecodeWorkspace(), []) for _ in range(2)]
+    for _ in range(5):
+        for args, _ in work:
+            for stream, workspace, got in streams:
+                with torch.cuda.stream(stream):
+                    got.append(int4_attention(*args, workspace))
+    torch.cuda.synchronize()
+    for _, _, got in streams:
+        for i, out in enumerate(got):
+            assert torch.equal(out, work[i % 3][1])
+
+
 def test_captured_steps_share_a_workspace():
     """A decode step and a draft step as two graphs over one workspace, replayed in turn with eager calls between."""
     gen, B, n = gen_of(16), 16, 5
