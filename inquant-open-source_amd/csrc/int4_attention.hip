@@ -16,9 +16,10 @@ constexpr int64_t BATCH = 64;                // sequences of a launch that share
 // A call for many that some sequences ask little of (a chunk of a prompt beside
 // single and drafted tokens) leaves sequences of at most MIXED columns to the kernel
 // for few, which shares their rows out: one workgroup would walk through each (2048
-// tokens beside 31 behind 2K-32K rows 434 us, 2456 without; 1024 beside 63 behind
-// 0.5K-4K 192 and 647; two launches that find nothing to do cost 10).
-constexpr int64_t MIXED = 32;
+// tokens beside 31 single ones behind 2K-32K rows 433 us, 2456 without; beside 31 times
+// five drafted ones 556 and 2630; 1024 beside 63 single ones behind 0.5K-4K 189 and 647; two launches
+// that find nothing to do cost under 10).
+constexpr int64_t MIXED = 64;
 
 struct Split {
     bool many, mixed;                        // the kernel for many columns; beside the one for few
@@ -55,8 +56,9 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
             // Two workgroups per compute unit where each has enough to do, else one (one
             // sequence of 32K rows, 28 heads over 4: 16.5 us with 512, 14.2 with 256; 16 of
             // 2K-32K: 40.6 and 42.5, with 768 42.7, with 1024 47).
-            const int64_t all = batch * planes * steps > 4096 ? 512 : 256;
-            s.workers = (all + planes - 1) / planes;
+            const int64_t busy = s.mixed ? H : planes;       // mixed: most have one group of columns, the others end at once
+            const int64_t all = batch * busy * steps > 4096 ? 512 : 256;
+            s.workers = (all + busy - 1) / busy;
             if (s.workers > batch * steps) s.workers = batch * steps;
             const int64_t floats = planes * (s.workers + batch) * s.width * (D + 2);
             if (floats > s.floats) s.floats = floats;        // the two take turns with it
@@ -65,7 +67,7 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
     return s;
 }
 
-// `most`: tokens of a sequence that the kernel for few answers
+// `most`: tokens of a sequence that have workgroups of their own in the join
 template <bool F16, int NQ>
 void launch_few(Int4Args a, int64_t most, int64_t n, hipStream_t stream)
 {
@@ -151,7 +153,7 @@ extern "C" int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t
     const bool f16 = dtype == IQ_F16;
     if (s.many) f16 ? launch_chunk<true>(a, cols, n_seq, st) : launch_chunk<false>(a, cols, n_seq, st);
     if (!s.many || s.mixed) {
-        const int64_t most = s.many ? MIXED / G : max_seqlen;
+        const int64_t most = s.many ? 1 : max_seqlen;        // mixed: most sequences have one
         if (s.width == 16) f16 ? launch_few<true, 1>(a, most, n_seq, st) : launch_few<false, 1>(a, most, n_seq, st);
         else f16 ? launch_few<true, 2>(a, most, n_seq, st) : launch_few<false, 2>(a, most, n_seq, st);
     }

@@ -99,12 +99,13 @@ struct Share {
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int32_t dpp_i(int32_t v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
 
-__device__ __forceinline__ Share int4_share(const Int4Args &a)
+// Of group `group`: sequences that ask for fewer columns have no steps there.
+__device__ __forceinline__ Share int4_share(const Int4Args &a, int group)
 {
     const int lane = threadIdx.x & 63;
     Share r;
     r.own = int4_seq(a, lane < a.n_seq ? lane : a.n_seq - 1);
-    r.steps = lane < a.n_seq && int4_asked<true>(a, r.own) > 0 ? (r.own.len + STEP - 1) / STEP : 0;
+    r.steps = lane < a.n_seq && int4_asked<true>(a, r.own) * a.G > group * a.width ? (r.own.len + STEP - 1) / STEP : 0;
     int32_t v = r.steps;
     v += dpp_i<0x111, 0xf>(v);               // row_shr:1
     v += dpp_i<0x112, 0xf>(v);
@@ -120,7 +121,8 @@ __device__ __forceinline__ Share int4_share(const Int4Args &a)
 
 // Joins the partitions of a token and query head.  FEW: those of the workgroups
 // that shared its sequence, by one workgroup whose eight teams of 32 lanes split
-// them; else those of `span` rows, by one team.
+// them, and which takes every gridDim.x / Hq th token; else those of `span` rows, by
+// one team.
 template <bool FEW>
 __global__ __launch_bounds__(256) void int4_join(Int4Args a)
 {
@@ -128,68 +130,71 @@ __global__ __launch_bounds__(256) void int4_join(Int4Args a)
     const int tid = threadIdx.x, team = tid >> 5, c = 4 * (tid & 31), seq = blockIdx.y;
     const Int4Seq s = int4_seq(a, seq);
     const uint32_t item = FEW ? blockIdx.x : blockIdx.x * 8 + team;
-    const int t = (int)(item / (uint32_t)a.Hq), hq = (int)(item - (uint32_t)t * (uint32_t)a.Hq);
-    if (t >= int4_asked<FEW>(a, s)) return;       // with FEW the whole workgroup's
-    const int last = s.sees(t);
-    int first = 0, live;                     // partitions first .. live - 1
-    int64_t base, next;                      // rows of the first of them, from one to the next
-    if constexpr (FEW) {
-        const Share r = int4_share(a);
-        const int steps = __builtin_amdgcn_readlane(r.steps, seq), from = __builtin_amdgcn_readlane(r.upto, seq) - steps;
-        const int h = hq / a.G, col = t * a.G + hq - h * a.G, group = col / a.width;
-        if (steps == 0 || last < 0) live = 0;
-        else {
-            first = from / r.each;
-            live = (from + last / STEP) / r.each + 1;
-            if (first == (from + steps - 1) / r.each) return;            // one workgroup had them all
+    const int t0 = (int)(item / (uint32_t)a.Hq), hq = (int)(item - (uint32_t)t0 * (uint32_t)a.Hq);
+    const int asked = int4_asked<FEW>(a, s);
+    for (int t = t0; t < asked; t += FEW ? (int)(gridDim.x / (uint32_t)a.Hq) : asked) {  // with FEW the whole workgroup's
+        const int last = s.sees(t);
+        int first = 0, live;                 // partitions first .. live - 1
+        int64_t base, next;                  // rows of the first of them, from one to the next
+        if constexpr (FEW) {
+            const int h = hq / a.G, col = t * a.G + hq - h * a.G, group = col / a.width;
+            const Share r = int4_share(a, group);
+            const int steps = __builtin_amdgcn_readlane(r.steps, seq), from = __builtin_amdgcn_readlane(r.upto, seq) - steps;
+            if (steps == 0 || last < 0) live = 0;
+            else {
+                first = from / r.each;
+                live = (from + last / STEP) / r.each + 1;
+                if (first == (from + steps - 1) / r.each) continue;      // one workgroup had them all
+            }
+            next = a.width;
+            base = ((int64_t)(h + a.pool.H * group) * (a.workers + a.n_seq) + first + seq) * next + col - group * a.width;
+        } else {
+            live = last < 0 ? 0 : last / a.span + 1;
+            base = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts;
+            next = 1;
         }
-        next = a.width;
-        base = ((int64_t)(h + a.pool.H * group) * (a.workers + a.n_seq) + first + seq) * next + col - group * a.width;
-    } else {
-        live = last < 0 ? 0 : last / a.span + 1;
-        base = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts;
-        next = 1;
-    }
-    live -= first;
-    float M = NEG_INF, L = 0.0f;
-    f32x4 o = {0, 0, 0, 0};
+        live -= first;
+        float M = NEG_INF, L = 0.0f;
+        f32x4 o = {0, 0, 0, 0};
 #pragma unroll 2
-    for (int p = FEW ? team : 0; p < live; p += FEW ? 8 : 1) {
-        const f32x2 ml = a.part.ml[base + p * next];
-        const f32x4 x = *(const f32x4 *)(a.part.o + (base + p * next) * 128 + c);
-        const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
-        const float f0 = __builtin_amdgcn_exp2f(M - use), f1 = __builtin_amdgcn_exp2f(ml[0] - use);
-        L = L * f0 + ml[1] * f1;
+        for (int p = FEW ? team : 0; p < live; p += FEW ? 8 : 1) {
+            const f32x2 ml = a.part.ml[base + p * next];
+            const f32x4 x = *(const f32x4 *)(a.part.o + (base + p * next) * 128 + c);
+            const float m = fmaxf(M, ml[0]), use = m == NEG_INF ? 0.0f : m;
+            const float f0 = __builtin_amdgcn_exp2f(M - use), f1 = __builtin_amdgcn_exp2f(ml[0] - use);
+            L = L * f0 + ml[1] * f1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + x[e] * f1;
-        M = m;
-    }
-    if constexpr (FEW) {
-        *(f32x4 *)&so[team][c] = o;
-        if (c == 0) {
-            sm[team] = M;
-            sl[team] = L;
+            for (int e = 0; e < 4; ++e) o[e] = o[e] * f0 + x[e] * f1;
+            M = m;
         }
-        __syncthreads();
-        if (team) return;
-        M = NEG_INF;
+        if constexpr (FEW) {
+            __syncthreads();                 // what was there before has been read
+            *(f32x4 *)&so[team][c] = o;
+            if (c == 0) {
+                sm[team] = M;
+                sl[team] = L;
+            }
+            __syncthreads();
+            if (team) continue;
+            M = NEG_INF;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) M = fmaxf(M, sm[i]);
-        const float use = M == NEG_INF ? 0.0f : M;
-        L = 0.0f;
-        o = f32x4{0, 0, 0, 0};
+            for (int i = 0; i < 8; ++i) M = fmaxf(M, sm[i]);
+            const float use = M == NEG_INF ? 0.0f : M;
+            L = 0.0f;
+            o = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float f = __builtin_amdgcn_exp2f(sm[i] - use);
-            L = fmaf(f, sl[i], L);
-            const f32x4 x = *(const f32x4 *)&so[i][c];
+            for (int i = 0; i < 8; ++i) {
+                const float f = __builtin_amdgcn_exp2f(sm[i] - use);
+                L = fmaf(f, sl[i], L);
+                const f32x4 x = *(const f32x4 *)&so[i][c];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+            }
         }
-    }
-    const int64_t at = (int64_t)(s.t0 + t) * a.o_st + hq * a.o_sh + c;
+        const int64_t at = (int64_t)(s.t0 + t) * a.o_st + hq * a.o_sh + c;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) iq_store_as(a.out, at + e, L == 0.0f ? 0.0f : o[e] / L, a.odt);
+        for (int e = 0; e < 4; ++e) iq_store_as(a.out, at + e, L == 0.0f ? 0.0f : o[e] / L, a.odt);
+    }
 }
 
 }  // namespace

@@ -308,9 +308,11 @@ template <bool F16, int NQ>
 __global__ __launch_bounds__(256, 2) void int4_shared(Int4Args a)
 {
     __shared__ DecodeSmem<NQ, 4> sm;
-    const int planes = a.pool.H * a.groups, plane = blockIdx.x % planes, w = blockIdx.x / planes;
-    const int h = plane % a.pool.H, group = plane / a.pool.H;
-    const Share r = int4_share(a);
+    // a group's workgroups one after the other: those of groups that no sequence has end
+    // at once, and must not stand on the same XCDs (each eighth workgroup is on one's)
+    const int per = a.pool.H * a.workers, group = blockIdx.x / per, rest = blockIdx.x - group * per;
+    const int h = rest % a.pool.H, w = rest / a.pool.H, plane = h + a.pool.H * group;
+    const Share r = int4_share(a, group);
     const int x0 = w * r.each, x1 = x0 + r.each < r.total ? x0 + r.each : r.total;
     for (int x = x0; x < x1;) {              // uniform
         const int seq = __builtin_popcountll(__builtin_amdgcn_ballot_w64(r.upto <= x));
