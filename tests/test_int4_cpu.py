@@ -177,8 +177,9 @@ def test_workspace_is_bounded():
     decode = [floats(28, 4, 16, 16, 1, n) for n in (513, 4096, 32768, 1 << 20)]
     assert 0 < max(decode) <= 4 * (128 + 16) * 16 * 130 * 2 and decode == sorted(decode)
     assert floats(28, 4, 0, 0, 1, 4096) == floats(28, 4, 3, 3, 0, 4096) == floats(28, 4, 3, 0, 5, 4096) == 0
-    # a chunk beside 63 single tokens: no more than its own split and theirs
-    assert floats(32, 4, 64, 2048 + 63, 2048, 1 << 17) <= 4 * (128 + 64) * 32 * 130
+    # a chunk beside 63 single tokens: 4 heads' two groups of 32 columns (64 are the most that a sequence beside a
+    # chunk may have), 512 / 4 workgroups and 64 sequences each
+    assert floats(32, 4, 64, 2048 + 63, 2048, 1 << 17) <= 4 * 2 * (128 + 64) * 32 * 130
     assert floats(28, 4, 1, 2048, 2048, 32768) == 0                                      # enough workgroups without
     assert 0 < floats(28, 4, 1, 64, 64, 32768) <= 64 * 28 * 64 * 130
 
