@@ -8,9 +8,9 @@ namespace {
 
 constexpr int D = 128;
 constexpr float I4_LOG2E = 1.44269504088896341f;
-// Softmax weights are at most 1; as f16 operands of the kernel for few columns
-// (and in the sums they are divided by) they are 2^14 times that, so that a weight
-// keeps its eleven bits down to 2^-28 of the largest instead of 2^-14.
+// Softmax weights are at most 1; as f16 operands (and in the sums they are
+// divided by) they are 2^14 times that, so that a weight keeps its eleven bits down
+// to 2^-28 of the largest instead of 2^-14.
 constexpr float I4_BIAS = 14.0f;
 
 struct Int4Args {

@@ -1,0 +1,76 @@
+"""Edges of the 4-bit pages' operators on the GPU: how far weights and outputs are from 64 bits, token by token."""
+import math
+
+import pytest
+import torch
+
+from densecase import EPS, i32
+from inquant.triton_attention import SharedDecodeWorkspace
+from inquant_vllm import Int4Pages, append_rows, int4_attention, read_rows
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def held_rows(key, value):
+    """One sequence's rows [n, heads, 128] in pages of 16: the pages, their table, and the rows that they stand for."""
+    n, h, _ = key.shape
+    count = -(-n // 16)
+    pages, table = Int4Pages.allocate(count, 16, h), torch.arange(count, dtype=torch.int32, device="cuda")[None]
+    append_rows(None, key, value, i32([0, n]), n, pages, table)
+    k, v = (torch.empty((n, h, 128), device="cuda") for _ in range(2))
+    read_rows(pages, table, i32([0, n]), n, k, v)
+    return pages, table, k.double(), v.double()
+
+
+def line(weights, dtype):
+    """Keys [n, 1, 128] whose logits with a query (1, 0, ...) are the numbers given, to three percent."""
+    key = torch.zeros((len(weights), 1, 128), dtype=dtype, device="cuda")
+    key[:, 0, 0] = weights.to(dtype)
+    return key
+
+
+@pytest.mark.parametrize("m, hq", [(80, 4), (300, 1), (3, 4), (40, 4)])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_a_row_with_most_of_the_weight_is_not_rounded(dtype, m, hq):
+    """One row has all but a 40th of the weight, 2^5.4 times that of the row that was the largest before it.  Its own
+    weight is the power of two that the others are measured by, so only they are rounded: by 2^-11 each.  The logits
+    are one product each, of at most 7: with the scale 3 roundings of 2^-24, in the weights and in their sum."""
+    n = 1000
+    logits = torch.full((n,), -20.0, device="cuda")
+    logits[0], logits[500] = 0.0, 5.3
+    gen = torch.Generator().manual_seed(m)
+    pages, table, k, v = held_rows(line(logits, dtype), torch.randn((n, 1, 128), generator=gen).to(dtype).cuda())
+    q = torch.zeros((m, hq, 128), dtype=dtype, device="cuda")
+    q[..., 0] = 1 + (torch.arange(m * hq, device="cuda").view(m, hq) % 16) / 64
+    out = int4_attention(q, i32([0, m]), m, pages, table, i32([n]), n, math.log(2), SharedDecodeWorkspace(),
+                         torch.empty(q.shape, dtype=F32, device="cuda"))
+    p = (q[..., 0, None].double() * k[:, 0, 0] * math.log(2)).masked_fill(
+        torch.arange(n, device="cuda") > n - m + torch.arange(m, device="cuda")[:, None, None], -math.inf).softmax(-1)
+    rest = 1 - p[..., 500]
+    assert rest.max() < 1 / 30
+    bound = v.abs().max() * (rest * EPS[F16] + 2 * 7 * math.log(2) * 4 * 2.0 ** -24 + 2.0 ** -20)
+    assert ((out.double() - p @ v[:, 0]).abs() <= bound[..., None]).all()
+
+
+@pytest.mark.parametrize("m, hq", [(80, 4), (300, 1), (3, 4), (40, 4)])
+@pytest.mark.parametrize("n", [500, 20000])             # one part, and several, most of which lack the largest weight
+@pytest.mark.parametrize("least", [-22.4, -26.3])
+def test_small_weights_keep_eleven_bits(m, hq, n, least):
+    """Rows of 2^-22 .. 2^-28 of the largest weight, whose values alone count: each weight is rounded by 2^-11 of its
+    own size.  The logits are one product each, of at most 28."""
+    logits = torch.full((n,), least, device="cuda")
+    logits[3] = 0.0
+    value = torch.full((n, 1, 128), 0.9375, dtype=BF, device="cuda")
+    value[3] = 0.0
+    pages, table, k, v = held_rows(line(logits, BF), value)
+    q = torch.zeros((m, hq, 128), dtype=BF, device="cuda")
+    q[..., 0] = 1.0
+    out = int4_attention(q, i32([0, m]), m, pages, table, i32([n]), n, math.log(2), SharedDecodeWorkspace(),
+                         torch.empty(q.shape, dtype=F32, device="cuda"))
+    sees = n - m + 1 + torch.arange(m, device="cuda")
+    small = torch.exp2(k[0, 0, 0])
+    assert 2.0 ** -28 < small < 2.0 ** -22
+    want = (sees - 1) * small * 0.9375 / (1 + (sees - 1) * small)
+    bound = want * (EPS[F16] + 2 * 28 * math.log(2) * 4 * 2.0 ** -24 + 2.0 ** -18)
+    assert ((out.double() - want[:, None, None]).abs() <= bound[:, None, None]).all()
