@@ -45,7 +45,9 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
         s.span = KT * ((steps + want - 1) / want);
         if (s.span < KT) s.span = KT;
         s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
-        s.floats = s.parts > 1 ? tokens * Hq * s.parts * (D + 2) : 0;
+        // a place for each token that a sequence can have (int4_place): at most 256 * QT columns, 34 MB
+        const int64_t places = n * max_seqlen < tokens ? n * max_seqlen : tokens;
+        s.floats = s.parts > 1 ? places * Hq * s.parts * (D + 2) : 0;
     }
     if (!s.many || s.mixed) {
         const int64_t most = s.mixed ? MIXED : cols;

@@ -23,7 +23,7 @@ struct Int4Args {
     int32_t n_seq, groups, workers, width;   // few: see Share
     int32_t few;                             // sequences of at most so many columns are its, the others the kernel's for many
     float c_log2;
-    Partials part;                           // many: [tokens * Hq, parts] rows; few: [planes, workers + n_seq, width]
+    Partials part;                           // many: [places * Hq, parts] rows (int4_place); few: [planes, workers + n_seq, width]
     void *out;
     int64_t o_st, o_sh;
     int odt;
@@ -55,6 +55,14 @@ __device__ __forceinline__ int32_t int4_asked(const Int4Args &a, const Int4Seq &
     const int32_t rest = a.tokens - s.t0;    // no token behind the last of the tensor
     m = m < rest ? m : rest > 0 ? rest : 0;
     return (m * a.G <= a.few) == FEW ? m : 0;
+}
+
+// Where partials of token t of a sequence stand: by the tensor's tokens, or by the
+// sequences' where those cannot be as many (a tensor may hold rows of no sequence).
+__device__ __forceinline__ int64_t int4_place(const Int4Args &a, int seq, const Int4Seq &s, int t)
+{
+    const int64_t most = (int64_t)a.n_seq * a.max_seqlen;
+    return most < a.tokens ? (int64_t)seq * a.max_seqlen + t : (int64_t)(s.t0 + t);
 }
 
 // Eight channels of a query in f32.
@@ -150,7 +158,7 @@ __global__ __launch_bounds__(256) void int4_join(Int4Args a)
             base = ((int64_t)(h + a.pool.H * group) * (a.workers + a.n_seq) + first + seq) * next + col - group * a.width;
         } else {
             live = last < 0 ? 0 : last / a.span + 1;
-            base = ((int64_t)(s.t0 + t) * a.Hq + hq) * a.parts;
+            base = (int4_place(a, seq, s, t) * a.Hq + hq) * a.parts;
             next = 1;
         }
         live -= first;

@@ -372,17 +372,16 @@ __global__ __launch_bounds__(64 * NW, 2) void int4_chunk(Int4Args a, int tiles, 
         if (poison >> db & 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[db][i] = __builtin_nanf("");
-    const int64_t token = s.t0 + t;
     if constexpr (DIRECT) {
         const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-        const int64_t o = token * a.o_st + hq * a.o_sh + 4 * h32;
+        const int64_t o = (int64_t)(s.t0 + t) * a.o_st + hq * a.o_sh + 4 * h32;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 iq_store_as(a.out, o + 32 * db + 8 * (i >> 2) + (i & 3), l_run == 0.0f ? 0.0f : acc[db][i] * inv, a.odt);
     } else {
-        const int64_t row = (token * a.Hq + hq) * a.parts + part;
+        const int64_t row = (int4_place(a, seq, s, t) * a.Hq + hq) * a.parts + part;
         float *o = a.part.o + row * D + 4 * h32;
 #pragma unroll
         for (int db = 0; db < 4; ++db)

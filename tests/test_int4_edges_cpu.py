@@ -1,0 +1,18 @@
+"""Edges of the 4-bit pages' operators on the host: scratch of padded batches."""
+import itertools
+
+from inquant import _native as nat
+
+
+def test_rows_of_no_sequence_take_no_scratch():
+    """What a call can ask for goes with the sequences' tokens: a padded tensor of queries adds none.  Many columns: 256
+    workgroups' columns at most, 256 each.  Few: parts of 32 columns by workgroup and by sequence (64 a launch) of every
+    plane, a KV head and 32 of its columns: eight planes a head, whose workgroups are 512 and one more a plane at most, or
+    two beside many columns, where a head has as many workgroups and so each of its planes."""
+    floats = nat.lib().iq_int4_workspace_floats
+    for (hq, h), n, most, tokens, rows in itertools.product([(28, 4), (32, 8), (16, 1), (8, 8)], [1, 2, 16], [64, 300, 512, 2048],
+                                                            [2048, 8192, 65536], [600, 4096, 32768, 1 << 20]):
+        few = max(512 + 65 * 8 * h, 2 * 512 + 65 * 2 * h) * 32 * 130
+        assert floats(hq, h, n, tokens, most, rows) <= max(256 * 256 * 130, few), (hq, h, n, most, tokens, rows)
+    alone = floats(28, 4, 1, 512, 512, 32768)
+    assert 0 < alone == floats(28, 4, 1, 8192, 512, 32768) == floats(28, 4, 1, 1 << 20, 512, 32768)

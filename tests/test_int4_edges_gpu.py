@@ -7,6 +7,7 @@ import torch
 from densecase import EPS, i32
 from inquant.triton_attention import SharedDecodeWorkspace
 from inquant_vllm import Int4Pages, append_rows, int4_attention, read_rows
+from test_int4_gpu import check, gen_of, random_pool, tables_of
 
 pytestmark = pytest.mark.gpu
 BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -74,3 +75,39 @@ def test_small_weights_keep_eleven_bits(m, hq, n, least):
     want = (sees - 1) * small * 0.9375 / (1 + (sees - 1) * small)
     bound = want * (EPS[F16] + 2 * 28 * math.log(2) * 4 * 2.0 ** -24 + 2.0 ** -18)
     assert ((out.double() - want[:, None, None]).abs() <= bound[:, None, None]).all()
+
+
+class Guarded:
+    """A workspace of exactly what a call asks for, and a mark behind it."""
+    def __init__(self):
+        self.size, self.tensor = 0, None
+
+    def floats(self, needed, device):
+        if needed > self.size:
+            self.size, self.tensor = needed, torch.full((needed + 65536,), 7.0, device=device)
+        return 0 if self.tensor is None else self.tensor.data_ptr(), self.size, torch.cuda.current_stream().cuda_stream
+
+    def kept(self):
+        return self.tensor is None or bool((self.tensor[self.size:] == 7).all())
+
+
+@pytest.mark.parametrize("hq, h, lengths, asked, before, behind", [
+    (28, 4, [3000], [64], 0, 1000),
+    (8, 2, [900, 700], [100, 70], 40, 400),
+    (4, 1, [2000, 0, 5], [300, 0, 5], 0, 700),
+    (28, 4, [3000, 2000, 5, 700, 900], [1, 300, 0, 4, 5], 3, 2000),          # a chunk beside single and drafted tokens
+    (28, 4, [700, 30, 5, 1300], [2, 1, 2, 0], 9, 50)])                       # few columns
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_padded_batches(dtype, hq, h, lengths, asked, before, behind):
+    """Tokens of no sequence in front of the batch and behind it, more than the sequences could have."""
+    gen, B = gen_of(hq + before), 16
+    pages = sum(-(-n // B) for n in lengths) + 2
+    held, key, value = random_pool(gen, pages, h, B)
+    tables, tokens = tables_of(gen, lengths, B, pages), sum(asked)
+    q = torch.randn((before + tokens + behind, hq, 128), generator=gen).to(dtype).cuda()
+    out, workspace = torch.full(q.shape, 6.0, dtype=F32, device="cuda"), Guarded()
+    cu = torch.tensor([0, *asked]).cumsum(0).add(before).int().cuda()
+    int4_attention(q, cu, max(asked), held, tables.cuda(), i32(lengths), max(lengths), 0.09, workspace, out)
+    own = slice(before, before + tokens)
+    check(out[own], q[own], asked, lengths, key, value, tables, B, 0.09, F32)
+    assert (out[:before] == 6).all() and (out[before + tokens:] == 6).all() and workspace.kept()
