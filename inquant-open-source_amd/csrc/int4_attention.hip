@@ -35,7 +35,6 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
     if (H < 1 || Hq < H || n < 1 || max_seqlen < 1) return s;
     const int64_t cols = Hq / H * max_seqlen;
     s.many = cols > MANY;
-    s.mixed = s.many && n > 1 && tokens <= (n - 1) * max_seqlen + MIXED / (Hq / H);   // else no sequence asks so little
     if (s.many) {
         // as many workgroups as run at once (one per compute unit), of eight tiles of rows at least
         const int64_t each = (cols + QT - 1) / QT, all = (tokens * (Hq / H) + QT - 1) / QT;
@@ -45,6 +44,11 @@ Split split_of(int64_t Hq, int64_t H, int64_t n, int64_t tokens, int64_t max_seq
         s.span = KT * ((steps + want - 1) / want);
         if (s.span < KT) s.span = KT;
         s.parts = max_tokens > 0 ? (max_tokens + s.span - 1) / s.span : 1;
+        // Whether some sequence asks little stands on the device only (the tensor may hold tokens of no sequence), so
+        // a call of more than one sequence reckons with it; but where all workgroups run at once, of eight tiles at
+        // most, a short one costs less than two launches do (64 tokens beside five behind 2000 rows 29 us, 50 with
+        // them; two of 64 31 and 34; 2048 tokens beside 31 single ones in a tensor of 67K 380, 2200 without)
+        s.mixed = n > 1 && (H * n * each * s.parts > 256 || s.span > 8 * KT);
         // a place for each token that a sequence can have (int4_place): at most 256 * QT columns, 34 MB
         const int64_t places = n * max_seqlen < tokens ? n * max_seqlen : tokens;
         s.floats = s.parts > 1 ? places * Hq * s.parts * (D + 2) : 0;

@@ -16,3 +16,11 @@ def test_rows_of_no_sequence_take_no_scratch():
         assert floats(hq, h, n, tokens, most, rows) <= max(256 * 256 * 130, few), (hq, h, n, most, tokens, rows)
     alone = floats(28, 4, 1, 512, 512, 32768)
     assert 0 < alone == floats(28, 4, 1, 8192, 512, 32768) == floats(28, 4, 1, 1 << 20, 512, 32768)
+
+
+def test_rows_of_no_sequence_do_not_change_how_short_sequences_are_answered():
+    """A chunk beside single tokens: their rows are shared out, which takes scratch, whatever stands behind the batch."""
+    floats = nat.lib().iq_int4_workspace_floats
+    alone = floats(28, 4, 32, 80000, 2048, 32768)                                        # many columns are not split there
+    for most, tokens in ((2048, 2048 + 31), (512, 512 + 31), (2048, 31 * 2048 + 9), (512, 80000)):
+        assert floats(28, 4, 32, tokens, most, 32768) >= alone > 0

@@ -96,6 +96,8 @@ class Guarded:
     (8, 2, [900, 700], [100, 70], 40, 400),
     (4, 1, [2000, 0, 5], [300, 0, 5], 0, 700),
     (28, 4, [3000, 2000, 5, 700, 900], [1, 300, 0, 4, 5], 3, 2000),          # a chunk beside single and drafted tokens
+    (32, 8, [300] * 39 + [511], [1] * 20 + [80] + [16, 17] * 9 + [3], 5, 4000),          # the same, one workgroup's rows
+    (8, 2, [900, 700], [100, 2], 0, 900),                                    # the same, all at once
     (28, 4, [700, 30, 5, 1300], [2, 1, 2, 0], 9, 50)])                       # few columns
 @pytest.mark.parametrize("dtype", [BF, F16])
 def test_padded_batches(dtype, hq, h, lengths, asked, before, behind):
