@@ -649,11 +649,14 @@ int iq_append_rows(const void *q, const void *k, const void *v, int dtype, int64
                    const iq_int4_pages *int4, const int32_t *tables, int64_t bt_stride, int64_t bt_cols, void *out,
                    int64_t o_st, int64_t o_sh, void *stream);
 
+/* With the tokens of the tensors: a sequence whose offset is negative has no
+ * rows, and none lie past them, whatever cu_seqlens says (iq_append_rows trusts
+ * it). */
 typedef struct iq_append_rows_args {
     uint64_t q, k, v;
     int64_t dtype, q_st, q_sh, k_st, k_sh, v_st, v_sh, Hq;
     uint64_t cu_seqlens;
-    int64_t n_seq, max_seqlen;
+    int64_t n_seq, max_seqlen, tokens;
     uint64_t start, positions, rotation;
     int64_t angles, rotary, interleaved;
     uint64_t factors, dense, int4, tables;
@@ -677,13 +680,14 @@ int iq_read_rows(const iq_dense_pages *dense, const iq_int4_pages *int4, int dty
                  const int32_t *start, void *k, int64_t k_st, int64_t k_sh, void *v, int64_t v_st, int64_t v_sh,
                  void *stream);
 
+/* With the tokens of the tensors, as iq_append_rows_args. */
 typedef struct iq_read_rows_args {
     uint64_t dense, int4;
     int64_t dtype;
     uint64_t tables;
     int64_t bt_stride, bt_cols;
     uint64_t cu_seqlens;
-    int64_t n_seq, max_seqlen;
+    int64_t n_seq, max_seqlen, tokens;
     uint64_t start, k;
     int64_t k_st, k_sh;
     uint64_t v;

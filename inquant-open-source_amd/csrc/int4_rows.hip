@@ -34,9 +34,24 @@ struct AppendArgs {
     const float *factors;                    // [H, 128] or null
     int32_t rotary, interleaved, Hq, H, G;
     uint32_t max_len;
+    int32_t tokens;                          // of the tensors
     DensePool dense;                         // one of the two, by the kernel
     Int4Pool int4;
 };
+
+// The first token of a sequence and how many of it a call takes: none in front of
+// the tensors or behind them, whatever the offsets say.
+struct RowSpan {
+    int64_t t0;
+    uint32_t len;
+};
+
+__device__ __forceinline__ RowSpan row_span(const int32_t *cu, int seq, uint32_t max_len, int32_t tokens)
+{
+    const int32_t t0 = cu[seq], behind = cu[seq + 1], end = behind < tokens ? behind : tokens;
+    const uint32_t n = t0 >= 0 && end > t0 ? end - t0 : 0;
+    return {t0, n < max_len ? n : max_len};
+}
 
 template <bool F16>
 __device__ __forceinline__ void unpack8(u32x4 raw, float (&x)[8])
@@ -164,9 +179,8 @@ template <bool F16, bool INT4, int R>
 __global__ __launch_bounds__(NT) void append_kernel(AppendArgs a)
 {
     const int seq = blockIdx.y, c = threadIdx.x & 15;
-    const int32_t have = a.cu[seq + 1] - a.cu[seq];
-    const uint32_t len = have <= 0 ? 0 : (uint32_t)have < a.max_len ? (uint32_t)have : a.max_len;
-    const int64_t t0 = a.cu[seq], start = a.start ? a.start[seq] : 0;
+    const auto [t0, len] = row_span(a.cu, seq, a.max_len, a.tokens);
+    const int64_t start = a.start ? a.start[seq] : 0;
     const int64_t pos0 = a.positions ? (int64_t)a.positions[seq] : start;
     const uint32_t H = (uint32_t)a.H, per_token = (uint32_t)a.Hq + (INT4 ? H : 2 * H);
     const uint64_t rows = (uint64_t)len * per_token, first = (uint64_t)blockIdx.x * (TEAMS * R);
@@ -297,6 +311,7 @@ struct ReadArgs {
     const int32_t *cu, *start;               // start may be null
     int32_t H;
     uint32_t max_len;
+    int32_t tokens;                          // of the tensors
     DensePool dense;
     Int4Pool int4;
 };
@@ -326,10 +341,9 @@ template <int ODT>
 __global__ __launch_bounds__(NT) void read_int4_kernel(ReadArgs a)
 {
     const int seq = blockIdx.y, c = threadIdx.x & 15;
-    const int32_t have = a.cu[seq + 1] - a.cu[seq];
-    const uint32_t len = have <= 0 ? 0 : (uint32_t)have < a.max_len ? (uint32_t)have : a.max_len;
+    const auto [t0, len] = row_span(a.cu, seq, a.max_len, a.tokens);
     if (len == 0) return;
-    const int64_t t0 = a.cu[seq], start = a.start ? a.start[seq] : 0;
+    const int64_t start = a.start ? a.start[seq] : 0;
     const uint32_t H = (uint32_t)a.H;
     const int64_t quad = start >> 2, quads = ((start + len + 3) >> 2) - quad;
     const uint64_t item = (uint64_t)blockIdx.x * TEAMS + (threadIdx.x >> 4);
@@ -392,9 +406,8 @@ __global__ __launch_bounds__(NT) void read_int4_kernel(ReadArgs a)
 __global__ __launch_bounds__(NT) void read_dense_kernel(ReadArgs a)
 {
     const int seq = blockIdx.y, c = threadIdx.x & 15;
-    const int32_t have = a.cu[seq + 1] - a.cu[seq];
-    const uint32_t len = have <= 0 ? 0 : (uint32_t)have < a.max_len ? (uint32_t)have : a.max_len;
-    const int64_t t0 = a.cu[seq], start = a.start ? a.start[seq] : 0;
+    const auto [t0, len] = row_span(a.cu, seq, a.max_len, a.tokens);
+    const int64_t start = a.start ? a.start[seq] : 0;
     const uint64_t item = (uint64_t)blockIdx.x * TEAMS + (threadIdx.x >> 4);
     if (item >= (uint64_t)len * (uint32_t)a.H) return;
     const uint32_t t = (uint32_t)(item / (uint32_t)a.H), h = (uint32_t)(item - (uint64_t)t * (uint32_t)a.H);
@@ -414,17 +427,16 @@ __global__ __launch_bounds__(NT) void read_dense_kernel(ReadArgs a)
 constexpr int64_t ONES_DENSE = 32768, ONES_INT4 = 8192;
 constexpr int64_t GRID_MOST = 0xffffffffLL / NT;         // workgroups of a launch's first dimension
 
+constexpr int64_t ANY_TOKENS = 0x7fffffff;   // more than offsets can tell
+
 bool aligned(const void *p, int64_t strides) { return (uintptr_t)p % 16 == 0 && strides % 8 == 0; }
 
-}  // namespace
-
-extern "C" int iq_append_rows(const void *q, const void *k, const void *v, int dtype, int64_t q_st, int64_t q_sh,
-                              int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t Hq,
-                              const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, const int32_t *start,
-                              const int32_t *positions, const float *rotation, int64_t angles, int64_t rotary,
-                              int interleaved, const float *factors, const iq_dense_pages *dense,
-                              const iq_int4_pages *int4, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
-                              void *out, int64_t o_st, int64_t o_sh, void *stream)
+int append_rows(const void *q, const void *k, const void *v, int dtype, int64_t q_st, int64_t q_sh, int64_t k_st,
+                int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t Hq, const int32_t *cu_seqlens, int64_t n_seq,
+                int64_t max_seqlen, int64_t tokens, const int32_t *start, const int32_t *positions, const float *rotation,
+                int64_t angles, int64_t rotary, int interleaved, const float *factors, const iq_dense_pages *dense,
+                const iq_int4_pages *int4, const int32_t *tables, int64_t bt_stride, int64_t bt_cols, void *out,
+                int64_t o_st, int64_t o_sh, void *stream)
 {
     IQ_CHECK_ARG((dense != nullptr) != (int4 != nullptr), "iq_append_rows: one kind of pages");
     AppendArgs a{};
@@ -446,13 +458,15 @@ extern "C" int iq_append_rows(const void *q, const void *k, const void *v, int d
                           : rotary == 0, "iq_append_rows: bad rotation");
     IQ_CHECK_ARG(!rotation || angles > 0, "iq_append_rows: an empty rotation");
     IQ_CHECK_ARG((uintptr_t)factors % 16 == 0, "iq_append_rows: factors must be 16-byte aligned");
-    IQ_CHECK_ARG(max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL, "iq_append_rows: bad length");
+    IQ_CHECK_ARG(max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL && tokens >= 0, "iq_append_rows: bad length");
+    if (max_seqlen > tokens) max_seqlen = tokens;
     if (n_seq == 0 || max_seqlen == 0) return IQ_OK;
     a.q = (const uint16_t *)q, a.k = (const uint16_t *)k, a.v = (const uint16_t *)v, a.out = (uint16_t *)out;
     a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh, a.o_st = o_st, a.o_sh = o_sh;
     a.cu = cu_seqlens, a.start = start, a.positions = positions, a.rotation = rotation, a.angles = angles;
     a.factors = factors, a.rotary = (int32_t)rotary, a.interleaved = interleaved;
     a.Hq = q ? (int32_t)Hq : 0, a.G = q ? (int32_t)(Hq / a.H) : 1, a.max_len = (uint32_t)max_seqlen;
+    a.tokens = (int32_t)(tokens < ANY_TOKENS ? tokens : ANY_TOKENS);
     // four rows may lie in two quads
     const int64_t rows = max_seqlen * (a.Hq + (dense ? 2 : 1) * (int64_t)a.H);
     const int64_t quads = dense ? 0 : (max_seqlen + 6) / 4 * a.H;
@@ -470,22 +484,9 @@ extern "C" int iq_append_rows(const void *q, const void *k, const void *v, int d
     return IQ_OK;
 }
 
-extern "C" int iq_append_rows_from(const iq_append_rows_args *a)
-{
-    IQ_CHECK_ARG(a, "iq_append_rows: null arguments");
-    return iq_append_rows((const void *)a->q, (const void *)a->k, (const void *)a->v, (int)a->dtype, a->q_st, a->q_sh,
-                          a->k_st, a->k_sh, a->v_st, a->v_sh, a->Hq, (const int32_t *)a->cu_seqlens, a->n_seq,
-                          a->max_seqlen, (const int32_t *)a->start, (const int32_t *)a->positions,
-                          (const float *)a->rotation, a->angles, a->rotary, (int)a->interleaved,
-                          (const float *)a->factors, (const iq_dense_pages *)a->dense, (const iq_int4_pages *)a->int4,
-                          (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (void *)a->out, a->o_st, a->o_sh,
-                          (void *)a->stream);
-}
-
-extern "C" int iq_read_rows(const iq_dense_pages *dense, const iq_int4_pages *int4, int dtype, const int32_t *tables,
-                            int64_t bt_stride, int64_t bt_cols, const int32_t *cu_seqlens, int64_t n_seq,
-                            int64_t max_seqlen, const int32_t *start, void *k, int64_t k_st, int64_t k_sh, void *v,
-                            int64_t v_st, int64_t v_sh, void *stream)
+int read_rows(const iq_dense_pages *dense, const iq_int4_pages *int4, int dtype, const int32_t *tables, int64_t bt_stride,
+              int64_t bt_cols, const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, int64_t tokens,
+              const int32_t *start, void *k, int64_t k_st, int64_t k_sh, void *v, int64_t v_st, int64_t v_sh, void *stream)
 {
     IQ_CHECK_ARG((dense != nullptr) != (int4 != nullptr), "iq_read_rows: one kind of pages");
     ReadArgs a{};
@@ -499,10 +500,12 @@ extern "C" int iq_read_rows(const iq_dense_pages *dense, const iq_int4_pages *in
     }
     IQ_CHECK_ARG(k && v && cu_seqlens, "iq_read_rows: null pointer");
     IQ_CHECK_ARG(aligned(k, k_st | k_sh) && aligned(v, v_st | v_sh), "iq_read_rows: rows must be 16-byte aligned");
-    IQ_CHECK_ARG(max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL, "iq_read_rows: bad length");
+    IQ_CHECK_ARG(max_seqlen >= 0 && max_seqlen <= 0x7fffffffLL && tokens >= 0, "iq_read_rows: bad length");
+    if (max_seqlen > tokens) max_seqlen = tokens;
     if (n_seq == 0 || max_seqlen == 0) return IQ_OK;
     a.k = k, a.v = v, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
     a.cu = cu_seqlens, a.start = start, a.max_len = (uint32_t)max_seqlen;
+    a.tokens = (int32_t)(tokens < ANY_TOKENS ? tokens : ANY_TOKENS);
     const int64_t items = (dense ? max_seqlen : (max_seqlen + 6) / 4) * (int64_t)a.H;
     IQ_CHECK_ARG((items + TEAMS - 1) / TEAMS <= GRID_MOST, "iq_read_rows: too many rows");
     const dim3 grid((unsigned)((items + TEAMS - 1) / TEAMS), (unsigned)n_seq);
@@ -513,11 +516,46 @@ extern "C" int iq_read_rows(const iq_dense_pages *dense, const iq_int4_pages *in
     return IQ_OK;
 }
 
+}  // namespace
+
+extern "C" int iq_append_rows(const void *q, const void *k, const void *v, int dtype, int64_t q_st, int64_t q_sh,
+                              int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t Hq,
+                              const int32_t *cu_seqlens, int64_t n_seq, int64_t max_seqlen, const int32_t *start,
+                              const int32_t *positions, const float *rotation, int64_t angles, int64_t rotary,
+                              int interleaved, const float *factors, const iq_dense_pages *dense,
+                              const iq_int4_pages *int4, const int32_t *tables, int64_t bt_stride, int64_t bt_cols,
+                              void *out, int64_t o_st, int64_t o_sh, void *stream)
+{
+    return append_rows(q, k, v, dtype, q_st, q_sh, k_st, k_sh, v_st, v_sh, Hq, cu_seqlens, n_seq, max_seqlen, ANY_TOKENS,
+                       start, positions, rotation, angles, rotary, interleaved, factors, dense, int4, tables, bt_stride,
+                       bt_cols, out, o_st, o_sh, stream);
+}
+
+extern "C" int iq_append_rows_from(const iq_append_rows_args *a)
+{
+    IQ_CHECK_ARG(a, "iq_append_rows: null arguments");
+    return append_rows((const void *)a->q, (const void *)a->k, (const void *)a->v, (int)a->dtype, a->q_st, a->q_sh, a->k_st,
+                       a->k_sh, a->v_st, a->v_sh, a->Hq, (const int32_t *)a->cu_seqlens, a->n_seq, a->max_seqlen, a->tokens,
+                       (const int32_t *)a->start, (const int32_t *)a->positions, (const float *)a->rotation, a->angles,
+                       a->rotary, (int)a->interleaved, (const float *)a->factors, (const iq_dense_pages *)a->dense,
+                       (const iq_int4_pages *)a->int4, (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (void *)a->out,
+                       a->o_st, a->o_sh, (void *)a->stream);
+}
+
+extern "C" int iq_read_rows(const iq_dense_pages *dense, const iq_int4_pages *int4, int dtype, const int32_t *tables,
+                            int64_t bt_stride, int64_t bt_cols, const int32_t *cu_seqlens, int64_t n_seq,
+                            int64_t max_seqlen, const int32_t *start, void *k, int64_t k_st, int64_t k_sh, void *v,
+                            int64_t v_st, int64_t v_sh, void *stream)
+{
+    return read_rows(dense, int4, dtype, tables, bt_stride, bt_cols, cu_seqlens, n_seq, max_seqlen, ANY_TOKENS, start, k, k_st,
+                     k_sh, v, v_st, v_sh, stream);
+}
+
 extern "C" int iq_read_rows_from(const iq_read_rows_args *a)
 {
     IQ_CHECK_ARG(a, "iq_read_rows: null arguments");
-    return iq_read_rows((const iq_dense_pages *)a->dense, (const iq_int4_pages *)a->int4, (int)a->dtype,
-                        (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (const int32_t *)a->cu_seqlens, a->n_seq,
-                        a->max_seqlen, (const int32_t *)a->start, (void *)a->k, a->k_st, a->k_sh, (void *)a->v, a->v_st,
-                        a->v_sh, (void *)a->stream);
+    return read_rows((const iq_dense_pages *)a->dense, (const iq_int4_pages *)a->int4, (int)a->dtype,
+                     (const int32_t *)a->tables, a->bt_stride, a->bt_cols, (const int32_t *)a->cu_seqlens, a->n_seq,
+                     a->max_seqlen, a->tokens, (const int32_t *)a->start, (void *)a->k, a->k_st, a->k_sh, (void *)a->v,
+                     a->v_st, a->v_sh, (void *)a->stream);
 }

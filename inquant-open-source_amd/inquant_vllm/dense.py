@@ -123,7 +123,7 @@ def _on_gpu(gpu, what, *tensors):
 _ARGUMENTS = {name: struct.Struct("=" + fields).pack for name, fields in {
     "iq_dense_write": "2Q5qQ2q3QqQq2Q2qQ", "iq_select_rows": "Q2qQ5q2Q", "iq_dense_evict": "QqQ2q2Q5q2QqQ",
     "iq_dense_decode": "Q5q2Q2qQqdqQqQ3qQ", "iq_prefill_weights": "2Q5qQ6qdQqQqQqQ",
-    "iq_append_rows": "3Q8qQ2q3Q3q4Q2qQ2qQ", "iq_read_rows": "2QqQ2qQ2q2Q2qQ2qQ",
+    "iq_append_rows": "3Q8qQ3q3Q3q4Q2qQ2qQ", "iq_read_rows": "2QqQ2qQ3q2Q2qQ2qQ",
     "iq_int4_attention": "Q4qQ3q2Q2qQqdQqQ3qQ"}.items()}
 _entries: dict = {}
 

@@ -148,7 +148,9 @@ def append_rows(query, key, value, cu_seqlens, max_seqlen, pages, block_tables, 
     Exact pages with weights get a weight of 0 and the position beside each row.
     ``output`` [tokens, Hq, 128] of the query dtype may be ``query`` itself.  Rows of
     no sequence, and those past max_seqlen, are not written; rows that a block
-    table does not reach are left out.  The inputs must not lie in the pages."""
+    table does not reach are left out.  Whatever cu_seqlens says, no row lies past
+    the tensors, and a sequence whose offset is negative has none.  The inputs must
+    not lie in the pages."""
     dense, int4 = _kind(pages)
     heads, gpu, dtype = pages.heads, pages._gpu, key.dtype
     k, v = _rows(key, "key", heads), _rows(value, "value", heads)
@@ -193,7 +195,7 @@ def append_rows(query, key, value, cu_seqlens, max_seqlen, pages, block_tables, 
     if max_seqlen == 0:
         return output
     _call(gpu, "iq_append_rows_from", q[4], k[4], v[4], nat.dtype_code(dtype), q[2], q[3], k[2], k[3], v[2], v[3], q[1],
-          cu.data_ptr(), n, max_seqlen, _ptr(start), _ptr(positions), _ptr(rotation), angles, rotary, bool(interleaved),
+          cu.data_ptr(), n, max_seqlen, tokens, _ptr(start), _ptr(positions), _ptr(rotation), angles, rotary, bool(interleaved),
           _ptr(factors), dense, int4, *table, out[4], out[2], out[3])
     return output
 
@@ -205,8 +207,9 @@ def read_rows(pages, block_tables, cu_seqlens, max_seqlen, key, value, start=Non
 
     Token t of sequence i (cu_seqlens int32 [sequences + 1]; tokens from max_seqlen
     on are left out) takes cache row start[i] + t (``start`` int32 [sequences], None:
-    0).  Tokens of no sequence, and those whose row has no page, are not written.
-    The rows must not lie in the pages."""
+    0).  Tokens of no sequence, and those whose row has no page, are not written, nor
+    is anything past the tensors, whatever cu_seqlens says.  The rows must not lie
+    in the pages."""
     dense, int4 = _kind(pages)
     heads, gpu, dtype = pages.heads, pages._gpu, key.dtype
     k, v = _rows(key, "key", heads), _rows(value, "value", heads)
@@ -226,7 +229,7 @@ def read_rows(pages, block_tables, cu_seqlens, max_seqlen, key, value, start=Non
     max_seqlen = min(max_seqlen, tokens)
     if max_seqlen:
         _call(gpu, "iq_read_rows_from", dense, int4, nat.dtype_code(dtype), *table, cu.data_ptr(), n, max_seqlen,
-              _ptr(start), k[4], k[2], k[3], v[4], v[2], v[3])
+              tokens, _ptr(start), k[4], k[2], k[3], v[4], v[2], v[3])
     return key, value
 
 

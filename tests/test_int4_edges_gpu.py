@@ -4,9 +4,10 @@ import math
 import pytest
 import torch
 
+import int4case as case
 from densecase import EPS, i32
 from inquant.triton_attention import SharedDecodeWorkspace
-from inquant_vllm import Int4Pages, append_rows, int4_attention, read_rows
+from inquant_vllm import DensePages, Int4Pages, append_rows, int4_attention, read_rows
 from test_int4_gpu import check, gen_of, random_pool, tables_of
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +114,37 @@ def test_padded_batches(dtype, hq, h, lengths, asked, before, behind):
     own = slice(before, before + tokens)
     check(out[own], q[own], asked, lengths, key, value, tables, B, 0.09, F32)
     assert (out[:before] == 6).all() and (out[before + tokens:] == 6).all() and workspace.kept()
+
+
+# offsets as they stand, and what of them lies within twenty tokens
+OFFSETS = [([0, 5, 40], [0, 5, 20]), ([18, 25, 31], [18, 20, 20]), ([-3, 4, 20], [4, 4, 20]), ([0, 20, -7], [0, 20, 20]),
+           ([2 ** 31 - 1, -2 ** 31, 12], [20, 20, 20]), ([30, 6, 19], [6, 6, 19])]
+
+
+@pytest.mark.parametrize("cu, clamped", OFFSETS)
+@pytest.mark.parametrize("kind", [Int4Pages, DensePages])
+def test_offsets_past_the_tensors(kind, cu, clamped):
+    """Offsets that run past the tensors, or start in front of them, touch nothing outside and no page: the tensors lie
+    within larger ones."""
+    gen, tokens = gen_of(3), 20
+    wide = torch.randn((3, 60, 4, 128), generator=gen).to(BF).cuda()
+    q, k, v = wide[0, 20:40], wide[1, 20:40, :2], wide[2, 20:40, :2]
+    table, start, rotation = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4), i32([3, 6]), case.angles(80, 128).cuda()
+
+    def pages():
+        if kind is Int4Pages:
+            return Int4Pages(torch.full((8, 2, 16 * 144), 0x55, dtype=torch.uint8, device="cuda"))
+        return DensePages(*(torch.full((8, 2, 16, 128), 9.0, dtype=BF, device="cuda") for _ in range(2)))
+
+    def run(offsets):
+        held, out = pages(), torch.full((60, 4, 128), 5.0, dtype=BF, device="cuda")
+        append_rows(q, k, v, i32(offsets), tokens, held, table, start, rotation=rotation, output=out[20:40])
+        rows = torch.full((2, 60, 2, 128), 4.0, dtype=BF, device="cuda")
+        read_rows(held, table, i32(offsets), tokens, rows[0, 20:40], rows[1, 20:40], start)
+        return out, rows, *([held.pool] if kind is Int4Pages else [held.key, held.value])
+
+    want = run(clamped)
+    for t, plain in zip(run(cu), want):
+        assert torch.equal(t, plain)
+    out, rows = want[:2]
+    assert (out[:20] == 5).all() and (out[40:] == 5).all() and (rows[:, :20] == 4).all() and (rows[:, 40:] == 4).all()
