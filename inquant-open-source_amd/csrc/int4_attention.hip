@@ -146,6 +146,7 @@ extern "C" int iq_int4_attention(const void *q, int dtype, int64_t q_st, int64_t
     if (max_seqlen > tokens) max_seqlen = tokens;
     const Split s = split_of(Hq, pool.H, n_seq, tokens, max_seqlen, max_tokens);
     IQ_CHECK_ARG(s.floats == 0 || (workspace && workspace_floats >= s.floats), "iq_int4_attention: workspace too small");
+    IQ_CHECK_ARG(s.floats == 0 || (uintptr_t)workspace % 16 == 0, "iq_int4_attention: the workspace must be 16-byte aligned");
     const int64_t G = Hq / pool.H, cols = G * max_seqlen;
     IQ_CHECK_ARG(s.parts <= 65535 && cols <= 0x3fffffff && s.groups * pool.H * (s.workers + 1) <= 0xffffff &&
                      Hq * max_seqlen <= (s.many ? 0x3fffffff : 0xffffff), "iq_int4_attention: too many rows");

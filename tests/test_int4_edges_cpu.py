@@ -1,4 +1,5 @@
 """Edges of the 4-bit pages' operators on the host: scratch of padded batches."""
+import ctypes
 import itertools
 
 from inquant import _native as nat
@@ -24,3 +25,15 @@ def test_rows_of_no_sequence_do_not_change_how_short_sequences_are_answered():
     alone = floats(28, 4, 32, 80000, 2048, 32768)                                        # many columns are not split there
     for most, tokens in ((2048, 2048 + 31), (512, 512 + 31), (2048, 31 * 2048 + 9), (512, 80000)):
         assert floats(28, 4, 32, tokens, most, 32768) >= alone > 0
+
+
+def test_a_workspace_off_its_alignment_is_refused():
+    """Partials are read and written sixteen bytes at a time."""
+    lib, fake = nat.lib(), 1 << 20
+    pages = nat.Int4PagesDesc(pool=fake, s_page=2 * 2304, s_head=2304, pages=4, heads=2, block_tokens=16)
+    need = lib.iq_int4_workspace_floats(4, 2, 1, 3, 3, 1000)
+    assert need > 0
+    for off in (4, 8):
+        assert lib.iq_int4_attention(fake, nat.IQ_BF16, 512, 128, 4, fake, 1, 3, 3, ctypes.addressof(pages), fake, 64, 64, fake, 1000, 0.1,
+                                     fake + off, need, fake, 512, 128, nat.IQ_BF16, None) == -1
+        assert b"aligned" in lib.iq_last_error()
