@@ -28,6 +28,7 @@ counterpart.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import torch
@@ -100,16 +101,20 @@ def _rows(t, what, heads=None):
 
 def _overlap(x, y, size):
     """Whether rows x and y (as _rows gives them, of elements of ``size`` bytes) may
-    share memory.  Heads of one tensor [tokens, heads, 128] side by side do not."""
+    share memory.  Heads of one tensor [tokens, heads, 128] side by side do not, nor
+    rows side by side within a head [tokens, heads, 3 * 128]."""
     n, h, st, sh, x0 = x
     m, g, yt, yh, y0 = y
     wx, wy = size * ((h - 1) * sh + 128), size * ((g - 1) * yh + 128)    # of a token
     if x0 + size * (n - 1) * st + wx <= y0 or y0 + size * (m - 1) * yt + wy <= x0:
         return False
-    if n != m or n < 2 or st != yt:
-        return True
-    at = (y0 - x0) % (size * st) if st > 0 else 0
-    return at < wx or at + wy > size * st or wx > size * st
+    if n == m and n > 1 and st == yt and st > 0:         # a token's rows within each stride
+        at = (y0 - x0) % (size * st)
+        if at >= wx and at + wy <= size * st and wx <= size * st:
+            return False
+    # any row of either lies whole strides from its first
+    every = size * math.gcd(st, sh, yt, yh)
+    return not every or not 128 * size <= (y0 - x0) % every <= every - 128 * size
 
 
 def _rows_apart(n, h, st, sh):

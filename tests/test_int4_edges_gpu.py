@@ -148,3 +148,22 @@ def test_offsets_past_the_tensors(kind, cu, clamped):
         assert torch.equal(t, plain)
     out, rows = want[:2]
     assert (out[:20] == 5).all() and (out[40:] == 5).all() and (rows[:, :20] == 4).all() and (rows[:, 40:] == 4).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 37])
+def test_rows_side_by_side_within_a_head(tokens):
+    """One projection [tokens, heads, 3 x 128], queries rotated in place, and rows read back beside each other."""
+    gen = gen_of(tokens)
+    fused = torch.randn((tokens, 2, 3 * 128), generator=gen).to(BF).cuda()
+    apart = [x.contiguous() for x in fused.split(128, 2)]
+    table, cu, rotation = torch.arange(4, dtype=torch.int32, device="cuda")[None], i32([0, tokens]), case.angles(64, 128).cuda()
+    held, plain = (Int4Pages(torch.zeros((4, 2, 16 * 144), dtype=torch.uint8, device="cuda")) for _ in range(2))
+    want = append_rows(*apart, cu, tokens, plain, table, rotation=rotation)
+    q, k, v = fused.split(128, 2)
+    assert append_rows(q, k, v, cu, tokens, held, table, rotation=rotation, output=q) is q
+    assert torch.equal(q, want) and torch.equal(held.pool, plain.pool)
+    assert torch.equal(k, apart[1]) and torch.equal(v, apart[2])
+    both, key, value = torch.zeros((tokens, 2, 2, 128), device="cuda"), *(torch.zeros((tokens, 2, 128), device="cuda") for _ in "kv")
+    read_rows(plain, table, cu, tokens, key, value)
+    read_rows(held, table, cu, tokens, both[:, :, 0], both[:, :, 1])
+    assert torch.equal(both[:, :, 0], key) and torch.equal(both[:, :, 1], value)
