@@ -77,11 +77,12 @@ __device__ __forceinline__ void query8(u32x4 raw, float (&x)[8])
 }
 
 // The power of two that brings a query's largest value to 2^14 .. 2^15, as an
-// exponent: below 2^-38 of that value it rounds, of bf16's range nothing is lost.
+// exponent: below 2^-38 of that value it rounds, of bf16's range nothing is lost
+// (the largest power of f32 brings its least value, 2^-133, to 2^-6).
 __device__ __forceinline__ int query_shift(float largest)
 {
     const int e = 14 + 127 - (int)(__float_as_uint(largest) >> 23);
-    return e < 100 ? e : 100;
+    return e < 127 ? e : 127;
 }
 
 // Few columns: the rows of a launch's sequences (at most 64), in steps of 256,

@@ -167,3 +167,36 @@ def test_rows_side_by_side_within_a_head(tokens):
     read_rows(plain, table, cu, tokens, key, value)
     read_rows(held, table, cu, tokens, both[:, :, 0], both[:, :, 1])
     assert torch.equal(both[:, :, 0], key) and torch.equal(both[:, :, 1], value)
+
+
+def by_token(out, q, k, v, scale, sees):
+    """Every token and head against 64 bits, each with its own bound.  q and out [m, hq, 128], k and v [n, h, 128]; token t
+    sees the first sees[t] rows.  A logit is off by 134 roundings of 2^-24 of its products' sizes at most (128 products and
+    sums, the scale), and a weight by that twice (its sum's too), 2^-11 for its rounding to f16, 2^-20 for exponentials and
+    sums; below 2^-28 of the largest a weight is off by 2^-39 of that.  The output is rounded once."""
+    n, h, hq = k.shape[0], k.shape[1], q.shape[1]
+    hidden = torch.arange(n, device="cuda") >= sees[:, None]
+    for head in range(hq):
+        x, key, value = q[:, head].double(), k[:, head // (hq // h)].double(), v[:, head // (hq // h)].double()
+        slack = (x.abs() @ key.abs().t() * abs(scale) * 134 * 2.0 ** -24).masked_fill(hidden, 0).amax(1, keepdim=True)
+        p = (x @ key.t() * scale).masked_fill(hidden, -math.inf).softmax(-1)
+        want = p @ value
+        bound = p @ value.abs() * (torch.expm1(2 * slack) + EPS[F16] + 2.0 ** -20) + n * 2.0 ** -39 * value.abs().max()
+        bound = bound * (1 + EPS[out.dtype]) + want.abs() * EPS[out.dtype]
+        worst = float(((out[:, head].double() - want).abs() / bound).max())
+        assert worst <= 1, (head, scale, worst)
+
+
+@pytest.mark.parametrize("scale, low, high", [(-0.2, -60, 4), (0.0, -60, 4), (1e-42, -60, 4), (3.0, -60, 4), (3.0, -6, -2),
+                                              (2.0 ** 100, -125, -104), (-2.0 ** 126, -132, -128)])
+@pytest.mark.parametrize("m", [1, 20, 70])
+def test_scales_token_by_token(m, scale, low, high):
+    """Queries of very different sizes side by side: a large one does not hide what becomes of the small ones."""
+    gen = gen_of(m)
+    pages, table, k, v = held_rows(*(torch.randn((700, 2, 128), generator=gen).to(BF).cuda() for _ in range(2)))
+    size = torch.exp2(torch.randint(low, high + 1, (m, 8, 1), generator=gen).double())
+    q = (torch.randn((m, 8, 128), generator=gen).double() * size).to(BF).cuda()
+    for out_dtype in (BF, F32):
+        out = int4_attention(q, i32([0, m]), m, pages, table, i32([700]), 700, scale, SharedDecodeWorkspace(),
+                             torch.empty(q.shape, dtype=out_dtype, device="cuda"))
+        by_token(out, q, k, v, scale, 700 - m + 1 + torch.arange(m, device="cuda"))
