@@ -200,3 +200,61 @@ def test_scales_token_by_token(m, scale, low, high):
         out = int4_attention(q, i32([0, m]), m, pages, table, i32([700]), 700, scale, SharedDecodeWorkspace(),
                              torch.empty(q.shape, dtype=out_dtype, device="cuda"))
         by_token(out, q, k, v, scale, 700 - m + 1 + torch.arange(m, device="cuda"))
+
+
+@pytest.mark.parametrize("hq, h", [(28, 4), (8, 2)])
+def test_a_captured_step_of_any_batch(hq, h):
+    """One graph for every batch of up to four sequences and 200 tokens: rows appended, then attended to.  What the
+    batches ask for stands on the device; replays and eager calls over one workspace in turn."""
+    gen, B, n, tokens, rows = gen_of(hq), 16, 4, 200, 1600
+    held = Int4Pages.allocate(n * rows // B, B, h)
+    table = tables_of(gen, [rows] * n, B, n * rows // B).cuda()
+    rotation, workspace, stream = case.angles(rows, 128).cuda(), SharedDecodeWorkspace(), torch.cuda.Stream()
+    fused = torch.zeros((tokens, hq + 2 * h, 128), dtype=BF, device="cuda")
+    cu, before, after = (torch.zeros(k, dtype=torch.int32, device="cuda") for k in (n + 1, n, n))
+    out = torch.zeros((tokens, hq, 128), dtype=BF, device="cuda")
+    kv = torch.randn((2, n * rows, h, 128), generator=gen).to(BF).cuda()
+
+    def step():
+        q = append_rows(fused[:, :hq], fused[:, hq:hq + h], fused[:, hq + h:], cu, tokens, held, table, before, rotation=rotation)
+        torch.add(before, cu[1:] - cu[:-1], out=after)
+        int4_attention(q, cu, tokens, held, table, after, rows, 0.09, workspace, out)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    batches = [([200, 0, 0, 0], [1400, 0, 3, 900]), ([1, 150, 5, 1], [1500, 20, 700, 0]), ([1] * 4, [900, 1, 64, 1599]),
+               ([0] * 4, [5] * 4), ([3, 2, 1, 190], [0, 511, 512, 600]), ([70, 60, 50, 20], [256, 0, 15, 1000])]
+
+    def play(run):
+        append_rows(None, kv[0], kv[1], i32([0, rows, 2 * rows, 3 * rows, 4 * rows]), rows, held, table)
+        torch.cuda.synchronize()
+        got = []
+        for seed, (asked, starts) in enumerate(batches):
+            fused.copy_(torch.randn(fused.shape, generator=gen_of(seed)).to(BF))
+            cu.copy_(torch.tensor([0, *asked]).cumsum(0).int()), before.copy_(torch.tensor(starts).int()), out.fill_(6.0)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                run()
+            torch.cuda.synchronize()
+            assert (out[sum(asked):] == 6).all()
+            got.append(out.clone())
+        return got
+
+    want = play(step)
+    for _ in range(2):
+        for a, b in zip(want, play(graph.replay)):
+            assert torch.equal(a, b)
+    # the last batch against 64 bits
+    asked, starts = batches[-1]
+    key, value = (torch.empty((n * rows, h, 128), device="cuda") for _ in range(2))
+    read_rows(held, table, i32([0, rows, 2 * rows, 3 * rows, 4 * rows]), rows, key, value)
+    x = torch.randn(fused.shape, generator=gen_of(len(batches) - 1)).to(BF)
+    at = torch.cat([torch.arange(a, a + m) for a, m in zip(starts, asked)])
+    q = case.turned(x[:, :hq], case.angles(rows, 128)[at], False).to(BF).cuda()
+    check(want[-1], q, asked, [a + m for a, m in zip(starts, asked)], key.view(-1, B, h, 128), value.view(-1, B, h, 128),
+          torch.arange(n * rows // B).view(n, -1), B, 0.09, BF)
