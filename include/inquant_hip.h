@@ -711,7 +711,7 @@ int iq_read_rows_from(const iq_read_rows_args *args);
  * and taken as f16, softmax weights are rounded to f16 before P.V, the rows are
  * exact.  A token that sees no row, or whose logits are all -inf, gives zeros.
  * Rows past lengths[i], of pages outside the pool or of no page count as not
- * there.  `tokens` bounds the query tokens (a hint for how the work is split).
+ * there.  `tokens` bounds the query tokens; those of no sequence take no scratch.
  * workspace: f32, iq_int4_workspace_floats elements, 16-byte aligned, used by
  * one call at a time.
  */

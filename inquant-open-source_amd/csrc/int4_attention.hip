@@ -17,8 +17,8 @@ constexpr int64_t BATCH = 64;                // sequences of a launch that share
 // single and drafted tokens) leaves sequences of at most MIXED columns to the kernel
 // for few, which shares their rows out: one workgroup would walk through each (2048
 // tokens beside 31 single ones behind 2K-32K rows 433 us, 2456 without; beside 31 times
-// five drafted ones 556 and 2630; 1024 beside 63 single ones behind 0.5K-4K 189 and 647; two launches
-// that find nothing to do cost under 10).
+// five drafted ones 556 and 2630; 1024 beside 63 single ones behind 0.5K-4K 189 and 647; the
+// launches cost 8-14 in batches that have none: 4 x 512 tokens 261 and 275).
 constexpr int64_t MIXED = 64;
 
 struct Split {

@@ -10,7 +10,7 @@
 // codes (eight channels of four rows), whose column layouts agree, so neither
 // the rows nor the weights pass through LDS.
 // Bound by memory and then by the decoding's VALU work: two sequences of 128K rows
-// 58-61 us (4.9-5.2 TB/s, the VALU busy for 71% of the cycles), 16 of 2K-32K 40 us with
+// 58-64 us (4.7-5.2 TB/s, the VALU busy for 71% of the cycles), 16 of 2K-32K 41 us with
 // the join, five drafted tokens of eight sequences 41 us (35 columns, two groups that
 // decode every row each; one group of 48 needs the registers of both wavefronts of a
 // SIMD and took as long).

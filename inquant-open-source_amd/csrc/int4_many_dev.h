@@ -10,8 +10,8 @@
 // channel by channel, so nothing is transposed.
 //
 // Bound by the matrix cores and the arithmetic of the weights beside them, which
-// the two wavefronts of a SIMD take in turn (below): 0.90-0.97 ms for 2048 tokens
-// behind 32K rows, 28 heads over 4, 0.97-1.04 PFLOP/s.  Workgroups of 128 columns, each
+// the two wavefronts of a SIMD take in turn (below): 0.93-1.02 ms by the card for 2048
+// tokens behind 32K rows, 28 heads over 4, 0.91-1.00 PFLOP/s.  Workgroups of 128 columns, each
 // with its own coded rows, and every wavefront at its products at the same time:
 // 1.65 ms.  64 columns a wavefront halve what is read from LDS, but their products'
 // sums do not fit the registers that the weights' arithmetic can use.
